@@ -8,6 +8,7 @@ kernels (used by the benchmark's ``gpu_launches``).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional
 
@@ -565,6 +566,181 @@ def attention_prefill(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
 def prefill_tcgen05_supported(hd: int, block_size: int, shared_kv: bool = False) -> bool:
     """``shared_kv``: keys and values are the same pages (attention over a cached latent), which opens head_dim 256."""
     return bool(_lib().kvcm_attention_tcgen05_supports_kv(int(hd), int(block_size), int(bool(shared_kv))))
+
+
+# ------------------------------------------------------------------ a cache in 4 bits (csrc/cuda/q4.cuh)
+
+def q4_page_bytes(block_size: int, hd: int) -> int:
+    """Bytes of one KV head's page in 4 bits: ``block_size`` rows of hd/2 bytes of codes, then ``block_size`` pairs (scale, zero) in
+    bfloat16, rounded up to 16 bytes.  A cache of keys (or of values) is uint8 [pages, kv heads, q4_page_bytes]."""
+    return (int(block_size) * (int(hd) // 2 + 4) + 15) // 16 * 16
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _q4_cache(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, nkv: int, hd: int, block_size: int) -> None:
+    _need(hd % 8 == 0 and 8 <= hd <= 256, f"{name}: head sizes are multiples of 8 up to 256")
+    _need(block_size > 0, f"{name}: block_size > 0")
+    want = (nkv, q4_page_bytes(block_size, hd))
+    for t in (k_cache, v_cache):
+        _need(t.dtype == torch.uint8 and t.dim() == 3 and tuple(t.shape[1:]) == want and t.shape[0] > 0 and t.is_contiguous()
+              and t.data_ptr() % 16 == 0, f"{name}: caches must be contiguous uint8 [pages, {want[0]}, {want[1]}] on 16 bytes")
+    _need(k_cache.shape[0] == v_cache.shape[0], f"{name}: k and v pools differ in their number of pages")
+
+
+def _q4_rows(name: str, what: str, t: torch.Tensor, rows: int, width: int, dtype: torch.dtype) -> None:
+    _need(t.dim() == 2 and t.shape[0] >= rows and t.shape[1] >= width and t.stride(1) == 1 and t.dtype == dtype,
+          f"{name}: {what} must be {dtype} rows [{rows}, {width}] with dense elements")
+    _need(t.data_ptr() % 16 == 0 and (t.stride(0) * t.element_size()) % 16 == 0, f"{name}: {what} rows must be 16-byte aligned")
+
+
+def _on_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]):
+    """The last check of a call and the device it launches on: that of its tensors, whatever the current one is."""
+    for t in others:
+        _need(t is None or t.device == first.device, f"{name}: tensors on different devices")
+    _cuda(first)
+    return _HERE if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+
+
+def rope_cache_q4(qkv: torch.Tensor, table: Optional[torch.Tensor], interleaved: bool, slot_mapping: torch.Tensor,
+                  k_cache: torch.Tensor, v_cache: torch.Tensor, q_out: torch.Tensor, nh: int, nkv: int, hd: int,
+                  block_size: int) -> None:
+    """Rotates the q and k heads of fused rows [T, (nh + 2 nkv) hd] with the step's angles and writes k (rotated, not rounded in
+    between) and v in 4 bits into the rows' page slots; the rotated q rows go to ``q_out`` [T, nh hd] (which may be those columns of
+    ``qkv`` itself).  The k and v columns of ``qkv`` stay as they are.  ``table``: float32 [T, rotary_dim], cosines then sines of
+    every row (``rope_table`` makes it; a table narrower than hd rotates the first elements of a head); None: no rotation.
+    rotary_dim is a multiple of 16 in rotate-half pairs, of 2 in interleaved ones.  Rows with a slot below zero (or beyond the
+    pool) are written nowhere.  A head with an element that is not finite reads back as not-a-number.  No two rows may share a slot."""
+    name = "rope_cache_q4"
+    T = qkv.shape[0]
+    suffix = _suffix(qkv)
+    _q4_cache(name, k_cache, v_cache, nkv, hd, block_size)
+    _q4_rows(name, "qkv", qkv, T, (nh + 2 * nkv) * hd, qkv.dtype)
+    _q4_rows(name, "q_out", q_out, T, nh * hd, qkv.dtype)
+    _need(slot_mapping.dtype == _I32 and slot_mapping.is_contiguous() and slot_mapping.numel() >= T, f"{name}: slot_mapping int32 [T]")
+    rotary = 0
+    if table is not None:
+        rotary = table.shape[-1]
+        _need(table.dtype == torch.float32 and table.dim() == 2 and table.shape[0] >= T and table.is_contiguous()
+              and table.data_ptr() % 16 == 0, f"{name}: table float32 [T, rotary_dim]")
+        _need(0 < rotary <= hd and rotary % (2 if interleaved else 16) == 0,
+              f"{name}: rotary_dim {rotary} (a multiple of 16 in rotate-half pairs, of 2 in interleaved ones, at most {hd})")
+    with _on_device(name, qkv, table, slot_mapping, k_cache, v_cache, q_out):
+        rc = getattr(_lib(), "kvcm_rope_cache_q4_" + suffix)(
+            _p(qkv), ctypes.c_longlong(qkv.stride(0)), _p(table), rotary, int(interleaved), _p(slot_mapping), _p(k_cache), _p(v_cache),
+            _p(q_out), ctypes.c_longlong(q_out.stride(0)), T, nh, nkv, hd, block_size, k_cache.shape[0], _stream())
+    _check(rc, name, f"(hd={hd}, rotary_dim={rotary})")
+
+
+def read_cache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor, k_rows: torch.Tensor,
+                  v_rows: torch.Tensor, nkv: int, hd: int, block_size: int) -> None:
+    """The values that the given slots of a cache in 4 bits stand for, as rows [T, nkv hd] of bfloat16 or float32 (for rows that move
+    to another cache, or to look at them).  Rows with a slot below zero (or beyond the pool) are left as they were."""
+    name = "read_cache_q4"
+    T = k_rows.shape[0]
+    suffix = _suffix(k_rows)
+    _q4_cache(name, k_cache, v_cache, nkv, hd, block_size)
+    _q4_rows(name, "k_rows", k_rows, T, nkv * hd, k_rows.dtype)
+    _q4_rows(name, "v_rows", v_rows, T, nkv * hd, k_rows.dtype)
+    _need(slot_mapping.dtype == _I32 and slot_mapping.is_contiguous() and slot_mapping.numel() >= T, f"{name}: slot_mapping int32 [T]")
+    with _on_device(name, k_cache, v_cache, slot_mapping, k_rows, v_rows):
+        rc = getattr(_lib(), "kvcm_read_cache_q4_" + suffix)(
+            _p(k_cache), _p(v_cache), _p(slot_mapping), _p(k_rows), _p(v_rows), ctypes.c_longlong(k_rows.stride(0)),
+            ctypes.c_longlong(v_rows.stride(0)), T, nkv, hd, block_size, k_cache.shape[0], _stream())
+    _check(rc, name, f"(hd={hd})")
+
+
+def _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink, *ints) -> None:
+    _need(nkv > 0 and nh > 0 and nh % nkv == 0, f"{name}: {nh} query heads are not a multiple of {nkv} KV heads")
+    _need(window >= 0 and softcap >= 0.0, f"{name}: window and softcap must not be negative")
+    _q4_cache(name, k_cache, v_cache, nkv, hd, block_size)
+    _need(q.dim() == 2 and out.dim() == 2 and q.dtype == out.dtype and q.dtype in _SUFFIX, f"{name}: q and out bfloat16 or float32 rows")
+    _need(out.shape[0] == q.shape[0] and q.shape[1] >= nh * hd and out.shape[1] >= nh * hd, f"{name}: q and out rows of {nh} heads of {hd}")
+    _need(q.stride(1) == 1 and out.stride(1) == 1, f"{name}: rows must be dense")
+    _need(block_tables.dtype == _I32 and block_tables.is_contiguous() and block_tables.dim() == 2,
+          f"{name}: block_tables int32 [S, max_blocks]")
+    _need(sink is None or (sink.dtype == torch.float32 and sink.is_contiguous() and sink.numel() == nh), f"{name}: sink float32 [heads]")
+    for t in ints:
+        _need(t is None or (t.dtype == _I32 and t.is_contiguous()), f"{name}: the step's arrays are contiguous int32")
+
+
+def attention_plain_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                       row_seq: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int, hd: int, block_size: int, scale: float,
+                       window: int = 0, softcap: float = 0.0, sink: Optional[torch.Tensor] = None) -> None:
+    """``attention_plain`` over a cache in 4 bits: one row a block, float32 arithmetic, q and out in bfloat16 or float32."""
+    name = "attention_plain_q4"
+    T = out.shape[0]
+    _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink, row_seq, positions)
+    _need(row_seq.numel() >= T and positions.numel() >= T, f"{name}: row_seq/positions int32 [T]")
+    with _on_device(name, q, out, k_cache, v_cache, block_tables, row_seq, positions, sink):
+        rc = getattr(_lib(), "kvcm_attention_plain_q4_" + _suffix(q))(
+            _p(q), ctypes.c_longlong(q.stride(0)), _p(out), ctypes.c_longlong(out.stride(0)), _p(k_cache), _p(v_cache), k_cache.shape[0],
+            _p(block_tables), block_tables.shape[1], _p(row_seq), _p(positions), T, nh, nkv, hd, block_size, ctypes.c_float(scale),
+            int(window), ctypes.c_float(softcap), _p(sink), _stream())
+    _check(rc, name, f"(hd={hd}, nh={nh}, nkv={nkv})")
+
+
+def paged_attention_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                       ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
+                       sink: Optional[torch.Tensor] = None) -> None:
+    """``paged_attention`` over a cache in 4 bits: attention of all rows of a step, rows [0, ctx.decode_seqs) single-row entries, the
+    rest the rows of longer portions; a row without keys gives zeros."""
+    attention_plain_q4(q, out, k_cache, v_cache, block_tables, ctx.row_seq, ctx.positions, nh, nkv, hd, block_size, scale, window,
+                       softcap, sink)
+
+
+# ------------------------------------------------------------------ a step's arrays from lengths
+
+STEP_TABLE_ERRORS = {1: "request {0} has a negative length", 2: "request {0} exceeds its page table",
+                     3: "{0} rows do not fit the step's arrays", 4: "{0} tiles do not fit the step's arrays",
+                     5: "{0} pages are missing from the stack of free ones", 6: "a count of {0} lies outside the stack of free pages"}
+
+
+def step_tables(seq_start: torch.Tensor, seq_q_len: torch.Tensor, block_tables: torch.Tensor, free_pages: torch.Tensor,
+                free_count: torch.Tensor, block_size: int, *, seq_q_start: torch.Tensor, seq_ctx_len: torch.Tensor,
+                positions: torch.Tensor, row_seq: torch.Tensor, slot_mapping: torch.Tensor, free_left: torch.Tensor,
+                status: torch.Tensor, tile_seq: Optional[torch.Tensor] = None, tile_q0: Optional[torch.Tensor] = None,
+                tile_rows: int = 64) -> None:
+    """A step's integer arrays on the device, from its requests' lengths (what ``core.BatchBuilder`` makes on the host), new pages
+    taken from a stack of free ones.  All int32.
+
+    In: request i holds the pages of its first ``seq_start[i]`` positions in ``block_tables[i]`` and brings ``seq_q_len[i]`` (0 or
+    more) rows behind them; ``free_pages[:free_count]`` are the free pages, taken from the top.
+    Out: ``block_tables`` with the new pages, ``free_left``, ``seq_q_start``, ``seq_ctx_len`` (start + rows), per row ``positions``,
+    ``row_seq`` and ``slot_mapping`` (rows behind the last one: -1, 0, -1), per tile of ``tile_rows`` rows of a request with more
+    than one row ``tile_seq`` and ``tile_q0`` (behind the last one -1); both may be left out.  ``seq_ctx_len`` may be ``seq_start``
+    and ``free_left`` may be ``free_count``: a step replayed from a CUDA graph then goes on from the one before.
+    ``status`` [4]: (0, 0, rows, tiles), or (code, number, 0, 0) where the step cannot be (``raise_on_step_tables``): pages, counts
+    and lengths are then as before and every row is one behind the last.  The host reads it when it likes; nothing waits here.
+    The requests stay in the caller's order: entries of one row come first where attention takes them as such."""
+    name = "step_tables"
+    outs = (seq_q_start, seq_ctx_len, positions, row_seq, slot_mapping, free_left, status, tile_seq, tile_q0)
+    for t in (seq_start, seq_q_len, block_tables, free_pages, free_count) + outs:
+        _need(t is None or (t.dtype == _I32 and t.is_contiguous()), f"{name}: contiguous int32 arrays")
+    S, T = seq_q_len.numel(), positions.numel()
+    _need(0 < S <= 8192, f"{name}: 1 to 8192 requests, not {S}")
+    _need(block_size > 0 and tile_rows > 0, f"{name}: block_size and tile_rows must be positive")
+    _need(seq_start.numel() == S and seq_q_start.numel() == S and seq_ctx_len.numel() == S, f"{name}: per-request arrays of {S}")
+    _need(block_tables.dim() == 2 and block_tables.shape[0] == S and block_tables.shape[1] > 0, f"{name}: block_tables [{S}, max_blocks]")
+    _need(row_seq.numel() == T and slot_mapping.numel() == T, f"{name}: per-row arrays of {T}")
+    _need((tile_seq is None) == (tile_q0 is None) and (tile_seq is None or tile_seq.numel() == tile_q0.numel()),
+          f"{name}: tile_seq and tile_q0 go together")
+    _need(free_count.numel() == 1 and free_left.numel() == 1 and status.numel() >= 4, f"{name}: free_count [1], free_left [1], status [4]")
+    tiles = 0 if tile_seq is None else tile_seq.numel()
+    with _on_device(name, seq_start, seq_q_len, block_tables, free_pages, free_count, *outs):
+        rc = _lib().kvcm_step_tables(
+            _p(seq_start), _p(seq_q_len), _p(block_tables), block_tables.shape[1], _p(free_pages), free_pages.numel(), _p(free_count),
+            _p(seq_q_start), _p(seq_ctx_len), _p(positions), _p(row_seq), _p(slot_mapping), _p(tile_seq), _p(tile_q0), _p(free_left),
+            _p(status), S, T, tiles, int(block_size), int(tile_rows), _stream())
+    _check(rc, name, f"({S} requests, {T} rows, {tiles} tiles)")
+
+
+def raise_on_step_tables(status) -> None:
+    """Raises ``KernelError`` where the status of a ``step_tables`` call (read to the host) names a refusal."""
+    code, number = int(status[0]), int(status[1])
+    if code:
+        raise KernelError("step_tables: " + STEP_TABLE_ERRORS.get(code, f"code {code}").format(number))
 
 
 def attention_tcgen05_error() -> int:
