@@ -681,13 +681,86 @@ def attention_plain_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor
     _check(rc, name, f"(hd={hd}, nh={nh}, nkv={nkv})")
 
 
+Q4_PART_KEYS = 128          # four warps with a step of 32 keys each
+
+
+def decode_partitions_q4(seqs: int, nh: int, nkv: int, hd: int, max_ctx: int, device, force_parts: int = 0):
+    """How ``attention_decode_q4`` splits the context: (keys per partition, number of partitions)."""
+    max_ctx = max(int(max_ctx), 1)
+    blocks = max(1, seqs * nkv * ((nh // nkv + 7) // 8))
+    most = (max_ctx + Q4_PART_KEYS - 1) // Q4_PART_KEYS
+    if force_parts > 0:
+        parts = min(int(force_parts), most)
+    else:
+        parts = max(1, min(_q4_resident_blocks(hd, device) // blocks, most))
+        if parts > CLUSTER_PARTS:
+            parts = max(CLUSTER_PARTS, min(parts, (max_ctx + 511) // 512))
+    size = ((max_ctx + parts - 1) // parts + Q4_PART_KEYS - 1) // Q4_PART_KEYS * Q4_PART_KEYS
+    return size, (max_ctx + size - 1) // size
+
+
+def _q4_resident_blocks(hd: int, device) -> int:
+    key = ("q4", int(hd), device.index)
+    if key not in _RESIDENT:
+        n = int(_lib().kvcm_attention_decode_q4_blocks_per_sm(int(hd)))
+        _RESIDENT[key] = max(n, 1) * sm_count(device)
+    return _RESIDENT[key]
+
+
+def attention_q4_supported(hd: int, dtype: torch.dtype) -> bool:
+    """True where ``attention_decode_q4`` takes these rows (bfloat16, heads of 32 to 256 elements in steps of 32)."""
+    return dtype == torch.bfloat16 and hd % 32 == 0 and 32 <= hd <= 256
+
+
+def attention_decode_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                        ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
+                        sink: Optional[torch.Tensor] = None) -> None:
+    """Single-row entries over a cache in 4 bits: q and out hold one bfloat16 row a request, in the order of the batch's entries;
+    ``ctx.seq_ctx_len`` says how many keys each sees (0: the row is zero), ``ctx.max_decode_ctx`` is at least the longest.
+    ``window``: the last ``window`` keys only; ``softcap``, ``sink`` as in ``attention_plain``."""
+    name = "attention_decode_q4"
+    S = q.shape[0]
+    _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink, ctx.seq_ctx_len)
+    _need(attention_q4_supported(hd, q.dtype), f"{name}: bfloat16 rows, heads of 32 to 256 elements in steps of 32")
+    _need(q.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0, f"{name}: q rows must be 16-byte aligned")
+    _need(out.data_ptr() % 8 == 0 and out.stride(0) % 4 == 0, f"{name}: out rows must be 8-byte aligned")
+    _need(block_tables.shape[0] >= S and ctx.seq_ctx_len.numel() >= S, f"{name}: an entry and a page table for each of {S} rows")
+    _need(ctx.max_decode_ctx <= block_tables.shape[1] * block_size or window > 0, f"{name}: max_decode_ctx exceeds the page tables")
+    with _on_device(name, q, out, k_cache, v_cache, block_tables, ctx.seq_ctx_len, sink):
+        if S == 0:
+            return
+        span = ctx.max_decode_ctx if window <= 0 else min(ctx.max_decode_ctx, int(window) + 31)
+        size, parts = decode_partitions_q4(S, nh, nkv, hd, span, q.device, int(ctx.options.get("attn_parts", 0)))
+        in_cluster = 1 < parts <= CLUSTER_PARTS and ctx.options.get("attn_merge", "cluster") == "cluster"
+        scratch = None
+        if parts > 1 and not in_cluster:
+            scratch = torch.empty(S * nh * parts * (hd + 2), dtype=torch.float32, device=q.device)
+        rc = _lib().kvcm_attention_decode_q4_bf16(
+            _p(q), ctypes.c_longlong(q.stride(0)), _p(out), ctypes.c_longlong(out.stride(0)), _p(k_cache), _p(v_cache), k_cache.shape[0],
+            _p(block_tables), block_tables.shape[1], _p(ctx.seq_ctx_len), S, nh, nkv, hd, block_size, ctypes.c_float(scale), int(window),
+            size, parts, _p(scratch), int(in_cluster), ctypes.c_float(softcap), _p(sink), _stream())
+    _check(rc, name, f"(hd={hd}, nh={nh}, nkv={nkv})")
+    if parts > 1 and not in_cluster:
+        global _launches
+        _launches += 1                      # the merge kernel
+
+
 def paged_attention_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                        ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
                        sink: Optional[torch.Tensor] = None) -> None:
     """``paged_attention`` over a cache in 4 bits: attention of all rows of a step, rows [0, ctx.decode_seqs) single-row entries, the
-    rest the rows of longer portions; a row without keys gives zeros."""
-    attention_plain_q4(q, out, k_cache, v_cache, block_tables, ctx.row_seq, ctx.positions, nh, nkv, hd, block_size, scale, window,
-                       softcap, sink)
+    rest the rows of longer portions; a row without keys gives zeros.  float32 rows, other head sizes and
+    ``ctx.options['attention'] == 'plain'``: ``attention_plain_q4`` for every row."""
+    if ctx.options.get("attention", "auto") == "plain" or not attention_q4_supported(hd, q.dtype):
+        attention_plain_q4(q, out, k_cache, v_cache, block_tables, ctx.row_seq, ctx.positions, nh, nkv, hd, block_size, scale, window,
+                           softcap, sink)
+        return
+    nd = ctx.decode_seqs
+    if nd > 0:
+        attention_decode_q4(q[:nd], out[:nd], k_cache, v_cache, block_tables, ctx, nh, nkv, hd, block_size, scale, window, softcap, sink)
+    if ctx.rows > nd:
+        attention_plain_q4(q[nd:], out[nd:], k_cache, v_cache, block_tables, ctx.row_seq[nd:], ctx.positions[nd:], nh, nkv, hd, block_size,
+                           scale, window, softcap, sink)
 
 
 # ------------------------------------------------------------------ a step's arrays from lengths

@@ -211,3 +211,60 @@ def test_plain_attention_of_more_keys_than_a_chunk():
 def test_a_step_of_single_rows_and_portions(dtype):
     for hd, B in ((16, 16), (64, 16), (128, 8)):
         run_attention(K().paged_attention_q4, [(0, 1), (30, 1), (77, 1), (0, 2), (19, 40), (0, 70)], 4, 2, hd, B, dtype)
+
+
+# ------------------------------------------------------------------------------------------- single rows on the tensor cores
+
+def decode(force=0, merge="cluster"):
+    def call(q, out, kc, vc, tables, ctx, *args, **kw):
+        ctx.options = {"attn_parts": force, "attn_merge": merge}
+        K().attention_decode_q4(q, out, kc, vc, tables, ctx, *args, **kw)
+    return call
+
+
+@pytest.mark.parametrize("nh,nkv,hd,B", [(2, 2, 32, 16), (8, 1, 64, 16), (4, 2, 96, 8), (6, 1, 128, 16), (3, 3, 160, 4), (18, 2, 192, 16), (4, 2, 224, 5),
+                                         (17, 1, 256, 32), (12, 1, 64, 1), (5, 5, 128, 100)])
+@pytest.mark.parametrize("force,merge", [(0, "cluster"), (1, "cluster"), (3, "cluster"), (3, "kernel")])
+def test_single_rows(nh, nkv, hd, B, force, merge):
+    spans = [(0, 1), (1, 1), (30, 1), (31, 1), (32, 1), (127, 1), (128, 1), (129, 1), (300, 1), (399, 1)]
+    run_attention(decode(force, merge), spans, nh, nkv, hd, B, "bfloat16", seed=hd, pad=3)
+
+
+@pytest.mark.parametrize("opts", OPTIONS[1:], ids=str)
+@pytest.mark.parametrize("nh,nkv,hd,B", [(8, 1, 64, 16), (6, 1, 128, 7), (2, 2, 96, 16), (2, 1, 256, 16)])
+@pytest.mark.parametrize("force", [0, 2])
+def test_single_rows_with_masks(opts, nh, nkv, hd, B, force):
+    run_attention(decode(force), [(0, 1), (6, 1), (7, 1), (45, 1), (200, 1), (385, 1)], nh, nkv, hd, B, "bfloat16", seed=7, pad=1, **dict(opts))
+
+
+def test_more_partitions_than_a_cluster_and_more_pages_than_the_slice():
+    run_attention(decode(12), [(1500, 1), (2, 1), (1535, 1)], 2, 1, 64, 16, "bfloat16")
+    run_attention(decode(1), [(600, 1), (1100, 1)], 2, 1, 64, 1, "bfloat16")          # 601 pages of one key each
+
+
+def test_large_scores_and_one_key_that_counts():
+    """Scores of a few hundred: one key has all the weight, and its value comes back."""
+    run_attention(decode(), [(700, 1), (65, 1)], 4, 2, 128, 16, "bfloat16", q_scale=60.0)
+    run_attention(decode(2), [(700, 1), (65, 1)], 4, 2, 64, 16, "bfloat16", q_scale=60.0)
+
+
+def test_a_key_behind_the_context_does_not_count():
+    """Pages end inside a step: what lies behind the context (not-a-number among it) is not seen; inside it is."""
+    hd, B, nh, nkv = 64, 16, 4, 1
+    tables, pages, ctx = make_step([(40, 1), (20, 1)], B, 3)
+    kc, vc = make_cache(pages, nkv, B, hd, 1), make_cache(pages, nkv, B, hd, 2)
+    q = torch.randn(2, nh * hd).to(torch.bfloat16).to(DEV)
+
+    def run(k, v):
+        out = torch.empty_like(q)
+        K().attention_decode_q4(q, out, k.to(DEV), v.to(DEV), tables.to(DEV), ctx, nh, nkv, hd, B, 0.125)
+        return out
+    clean = run(kc, vc)
+    for key, seen in ((41, False), (47, False), (40, True), (0, True)):
+        for which in (0, 1):
+            bad = [kc.clone(), vc.clone()]
+            page, off = int(tables[0, key // B]), key % B
+            bad[which][page, 0, B * hd // 2 + 4 * off:B * hd // 2 + 4 * off + 4] = torch.tensor([0xc0, 0x7f, 0xc0, 0x7f], dtype=torch.uint8)
+            got = run(*bad)
+            assert torch.equal(got[1], clean[1])
+            assert bool(got[0].isnan().all()) if seen else torch.equal(got[0], clean[0]), (key, which)
