@@ -29,9 +29,11 @@ namespace kvcm {
 constexpr int kQ4Warps = 4;
 constexpr int kQ4DecodeThreads = 32 * kQ4Warps;
 constexpr int kQ4Step = 32;                        // keys of a warp's step
+constexpr int kQ4Tile = kQ4Step * kQ4Warps;        // keys of a round of the block
 constexpr int kQ4Heads = 8;                        // query heads of a block
 constexpr int kQ4TabMax = 512;                     // page-table entries of a partition kept in shared memory
 constexpr int kQ4ClusterParts = 8;
+constexpr float kQ4Lowest = 3.402823466e38f;
 
 struct DecodeQ4Params {
   const bf16* q; long long q_stride;
@@ -40,7 +42,9 @@ struct DecodeQ4Params {
   const int* block_tables; int max_blocks;
   const int* seq_ctx_len;
   float* part_o; float* part_ml;
-  int nh, nkv, block_size, log2_block, num_pages, window, part_size, num_parts, cluster_merge;
+  int* part_first;                     // shares: [seqs * head tiles][2]
+  int seqs, nh, nkv, block_size, log2_block, num_pages, window;
+  int part_size, num_parts, cluster_merge;      // num_parts 0: equal shares of all keys
   float scale_log2;                    // what a score is multiplied by on its way into exp2
   float cap_pre;                       // > 0: s <- tanh(s * cap_pre) first
   const float* sink;
@@ -78,14 +82,39 @@ __device__ __forceinline__ void cp_async4(void* smem_dst, const void* gmem_src) 
 // The 8 x 8 matrix of 16-bit elements that the warp holds, one row a group of four lanes, transposed.
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
-// 128 + code -> code - 8, two at a time (whole numbers: exact).
-__device__ __forceinline__ uint32_t centred(uint32_t v) {
-  const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));     // 136
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
-  return *reinterpret_cast<const uint32_t*>(&r);
+// Elements of a value as float16, two keys a register: codes at bits 0..3 of the halves give 1024 + code, those at bits 4..7
+// 1024 + 16 code; less 1032 and 1152 they are code - 8 and 16 (code - 8), whole numbers and exact.
+__device__ __forceinline__ uint32_t low_codes(uint32_t v) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;\n" : "=r"(r) : "r"(v));
+  asm("sub.f16x2 %0, %0, %1;\n" : "+r"(r) : "r"(0x64086408u));
+  return r;
+}
+__device__ __forceinline__ uint32_t high_codes(uint32_t v) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;\n" : "=r"(r) : "r"(v));
+  asm("sub.f16x2 %0, %0, %1;\n" : "+r"(r) : "r"(0x64806480u));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// D(16x8, float) += A(16x16, row) * B(16x8, col), both bfloat16 or both float16.  (Not volatile: the compiler may order them
+// among the unpacking of other operands.)
+__device__ __forceinline__ void mma_codes(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 template <int HD, int STAGES> constexpr size_t q4_decode_core_smem() {
@@ -129,7 +158,7 @@ __device__ __forceinline__ void q4_cluster_tail(const DecodeQ4Params& p, int seq
       acc.x = fmaf(f, o[i].x, acc.x); acc.y = fmaf(f, o[i].y, acc.y); acc.z = fmaf(f, o[i].z, acc.z); acc.w = fmaf(f, o[i].w, acc.w);
       sum = fmaf(f, l[i], sum);
     }
-    if (p.sink && top != -INFINITY) sum += fast_exp2(p.sink[head0 + r] * 1.4426950408889634f - top);
+    if (p.sink && sum != 0.f) sum += fast_exp2(p.sink[head0 + r] * 1.4426950408889634f - top);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     bf16* dst = p.out + size_t(seq) * p.out_stride + size_t(head0 + r) * HD + d;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
@@ -137,15 +166,19 @@ __device__ __forceinline__ void q4_cluster_tail(const DecodeQ4Params& p, int seq
   cluster.sync();                                                  // nobody leaves while its memory is read
 }
 
-template <int HD, int STAGES>
-__global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 4 : 2) attn_decode_q4_kernel(DecodeQ4Params p) {
+// A block's piece of work: keys [begin, end) of one request for eight query heads of a KV head.
+struct Q4Segment {
+  int seq, kvh, head0, heads_here, begin, end;
+  int slot;                            // >= 0: where the partial result goes; < 0: the result itself
+};
+
+template <int HD, int STAGES, bool CAP>
+__global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_decode_q4_kernel(DecodeQ4Params p) {
   typedef Q4Shape<HD> S;
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  int* stab = reinterpret_cast<int*>(smem_raw + q4_decode_core_smem<HD, STAGES>());
-  const int part = blockIdx.x, G = p.nh / p.nkv, head_tiles = (G + kQ4Heads - 1) / kQ4Heads;
-  const int kvh = blockIdx.y / head_tiles, ht = blockIdx.y - kvh * head_tiles;
-  const int head0 = kvh * G + ht * kQ4Heads, heads_here = min(kQ4Heads, G - ht * kQ4Heads);
-  const int seq = blockIdx.z;
+  unsigned* stab = reinterpret_cast<unsigned*>(smem_raw + q4_decode_core_smem<HD, STAGES>());     // pages of the head, in units of 16 bytes
+  __shared__ int found[2];
+  const int G = p.nh / p.nkv, head_tiles = (G + kQ4Heads - 1) / kQ4Heads;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   float* mo = reinterpret_cast<float*>(smem_raw);                  // after the key loop: [warps][8][HD]
   float* mm = mo + kQ4Warps * kQ4Heads * HD;                       // [warps][8] maximum
@@ -153,334 +186,457 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 4 : 2) attn_deco
   float* bo = ml + kQ4Warps * kQ4Heads;                            // [8][HD] the block's result
   float* bm = bo + kQ4Heads * HD;                                  // [8]
   float* bl = bm + kQ4Heads;                                       // [8]
+  const bool shares = p.num_parts == 0;
 
   pdl_launch_dependents();
   // The step's integers are there before the step's kernels; keys, also old ones, only behind the wait: a caller may have
   // written a whole prompt by the kernel before this one.
-  const int ctx = p.seq_ctx_len[seq];
-  const int lo = ctx > 0 ? first_visible(ctx - 1, p.window, 0) : 0;
-  const int pbeg = lo / kQ4Step * kQ4Step + part * p.part_size;
-  const int begin = max(lo, pbeg), end = min(ctx, pbeg + p.part_size);
-  const bool nothing = begin >= end;
-  const int* table = p.block_tables + size_t(seq) * p.max_blocks;
-  int tab0 = 0;
-  bool staged = false;
-  if (!nothing) {
-    tab0 = begin / p.block_size;
-    const int n = (end - 1) / p.block_size - tab0 + 1;
-    staged = n <= kQ4TabMax;
-    if (staged)
-      for (int j = tid; j < n; j += kQ4DecodeThreads) stab[j] = table[tab0 + j];
-  }
-  pdl_wait();
-  if (nothing) {
-    if (p.cluster_merge) {
-      if (tid < kQ4Heads) { bm[tid] = -INFINITY; bl[tid] = 0.f; }
-      q4_cluster_tail<HD>(p, seq, head0, heads_here, bo, bm, bl);
-    } else if (p.num_parts == 1) {
-      for (int i = tid; i < heads_here * HD; i += kQ4DecodeThreads)
-        p.out[size_t(seq) * p.out_stride + size_t(head0) * HD + i] = __float2bfloat16_rn(0.f);
-    } else if (tid < heads_here) {
-      float* pair = p.part_ml + ((size_t(seq) * p.nh + head0 + tid) * p.num_parts + part) * 2;
-      pair[0] = -INFINITY;
-      pair[1] = 0.f;
+  auto first_key = [&](int ctx) { return ctx > 0 ? first_visible(ctx - 1, p.window, 0) : 0; };
+  auto tiles_of = [&](int ctx) { return (ctx - first_key(ctx) / kQ4Step * kQ4Step + kQ4Tile - 1) / kQ4Tile; };
+  const int H = p.nkv * head_tiles;
+  // ---- where the block's work starts
+  int seq, unit_h = 0, tile = 0;                                   // shares: request, head tile of it, tile of its keys
+  long long left = 0, U = 0, before = 0;                           // tiles left of the share; all tiles; those in front of `seq`, one head
+  long long takers = 0;                                            // blocks that have a share
+  if (!shares) {
+    seq = blockIdx.z;
+  } else {
+    // every block adds up all lengths; the thread whose requests hold the share's first tile says where
+    int* sums = reinterpret_cast<int*>(smem_raw);                  // [threads] (the rings are not in use yet)
+    const int per = (p.seqs + kQ4DecodeThreads - 1) / kQ4DecodeThreads;
+    const int s0 = min(tid * per, p.seqs), s1 = min(s0 + per, p.seqs);
+    int mine = 0;
+    for (int s = s0; s < s1; ++s) mine += tiles_of(p.seq_ctx_len[s]);
+    int up = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += v;
     }
-    return;
-  }
-  // ---- q of head g as the second operand: elements in the order in which a lane's codes lie
-  uint32_t qb[S::kKeyWords][4];
-  float qs[2];                                                     // sum of q over the elements, heads 2 t4 and 2 t4 + 1
-  {
-    float sum = 0.f;
-    const bf16* row = p.q + size_t(seq) * p.q_stride + size_t(head0 + g) * HD;
-#pragma unroll
-    for (int i = 0; i < S::kKeyWords; ++i) {
-      const int word = (S::kKeyWords % 4 == 0) ? (i / 4) * 16 + t4 * 4 + (i & 3) : t4 * S::kKeyWords + i;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (g < heads_here) v = *reinterpret_cast<const uint4*>(row + word * 8);
-      qb[i][0] = v.x; qb[i][1] = v.y; qb[i][2] = v.z; qb[i][3] = v.w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += __uint_as_float(qb[i][e] << 16) + __uint_as_float(qb[i][e] & 0xffff0000u);
-    }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    qs[0] = __shfl_sync(0xffffffffu, sum, t4 * 8);
-    qs[1] = __shfl_sync(0xffffffffu, sum, t4 * 8 + 4);
-  }
-  __syncthreads();                                                 // the page-table slice is there
-
-  // ---- the warp's steps: keys first + 32 (4 i + warp)
-  const int first = begin / kQ4Step * kQ4Step;
-  const int steps_all = (end - first + kQ4Step - 1) / kQ4Step;
-  const int steps = (steps_all - warp + kQ4Warps - 1) / kQ4Warps;
-  unsigned char* ring = smem_raw + size_t(warp) * STAGES * S::kStageBytes;
-  const size_t head_bytes = q4::page_bytes(p.block_size, HD);
-  const int pairs_at = p.block_size * (HD / 2);
-  auto place = [&](int key, size_t& base, int& off) {              // where a key's page and row are
-    const int pi = p.log2_block >= 0 ? key >> p.log2_block : key / p.block_size;
-    off = key - pi * p.block_size;
-    base = q4::page_base(staged ? stab[pi - tab0] : table[pi], kvh, p.nkv, p.num_pages, head_bytes);
-  };
-  auto load_step = [&](int i) {
-    if (i < steps) {
-      unsigned char* st = ring + (i % STAGES) * S::kStageBytes;
-      const int key0 = first + (i * kQ4Warps + warp) * kQ4Step;
-#pragma unroll
-      for (int c = 0; c < S::kChunks; ++c) {
-        const int piece = c * 32 + lane, r = piece / S::kChunks, ch = piece - r * S::kChunks;
-        const int key = key0 + r;
-        if (key >= begin && key < end) {
-          size_t base;
-          int off;
-          place(key, base, off);
-          base += size_t(off) * (HD / 2) + ch * 16;
-          const int at = S::at(r, ch);
-          cp_async16(st + at, p.k_cache + base);
-          cp_async16(st + S::kCodeBytes + at, p.v_cache + base);
-        }
-      }
-      unsigned char* pairs = st + 2 * S::kCodeBytes + lane * 4;
-      const int key = key0 + lane;
-      if (key >= begin && key < end) {
-        size_t base;
-        int off;
-        place(key, base, off);
-        base += pairs_at + off * 4;
-        cp_async4(pairs, p.k_cache + base);
-        cp_async4(pairs + kQ4Step * 4, p.v_cache + base);
-      } else {                                                     // zero, so that zero times it stays zero (codes are finite whatever they are)
-        *reinterpret_cast<uint32_t*>(pairs) = 0u;
-        *reinterpret_cast<uint32_t*>(pairs + kQ4Step * 4) = 0u;
-      }
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) load_step(i);
-
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, zacc[2] = {0.f, 0.f};       // heads 2 t4, 2 t4 + 1; this lane's keys
-  float o[S::kTiles][4];
-#pragma unroll
-  for (int i = 0; i < S::kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  const int row_g = S::row(g), row_a = S::row(2 * t4), row_b = S::row(2 * t4 + 1);
-
-  for (int i = 0; i < steps; ++i) {
-    load_step(i + STAGES - 1);
-    cp_async_wait<STAGES - 1>();
-    __syncwarp();
-    const unsigned char* st = ring + (i % STAGES) * S::kStageBytes;
-    const uint32_t* kpair = reinterpret_cast<const uint32_t*>(st + 2 * S::kCodeBytes);
-    const uint32_t* vpair = kpair + kQ4Step;
-    const int key0 = first + (i * kQ4Warps + warp) * kQ4Step;
-    const bool inside = key0 >= begin && key0 + kQ4Step <= end;
-
-    float x[2][4];                                                 // scores in log2 units: [16 keys][key g, head 2t | 2t+1; key g + 8]
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      uint32_t ka[S::kKeyWords], kb[S::kKeyWords];
-      const int ra = mt * 16 + row_g, rb = ra + 8;
-      if constexpr (S::kKeyWords % 4 == 0) {
-#pragma unroll
-        for (int w = 0; w < S::kKeyWords / 4; ++w) {
-          const uint4 a = *reinterpret_cast<const uint4*>(st + S::at(ra, w * 4 + t4));
-          const uint4 b = *reinterpret_cast<const uint4*>(st + S::at(rb, w * 4 + t4));
-          ka[4 * w] = a.x; ka[4 * w + 1] = a.y; ka[4 * w + 2] = a.z; ka[4 * w + 3] = a.w;
-          kb[4 * w] = b.x; kb[4 * w + 1] = b.y; kb[4 * w + 2] = b.z; kb[4 * w + 3] = b.w;
-        }
-      } else if constexpr (HD == 64) {
-        const uint2 a = *reinterpret_cast<const uint2*>(st + S::at(ra, t4 >> 1) + (t4 & 1) * 8);
-        const uint2 b = *reinterpret_cast<const uint2*>(st + S::at(rb, t4 >> 1) + (t4 & 1) * 8);
-        ka[0] = a.x; ka[1] = a.y; kb[0] = b.x; kb[1] = b.y;
-      } else {
-#pragma unroll
-        for (int w = 0; w < S::kKeyWords; ++w) {
-          ka[w] = *reinterpret_cast<const uint32_t*>(st + S::at(ra, 0) + (t4 * S::kKeyWords + w) * 4);
-          kb[w] = *reinterpret_cast<const uint32_t*>(st + S::at(rb, 0) + (t4 * S::kKeyWords + w) * 4);
-        }
-      }
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < S::kKeyWords; ++w)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t a[4] = {q4::two_codes_128(ka[w], 2 * h), q4::two_codes_128(kb[w], 2 * h), q4::two_codes_128(ka[w], 2 * h + 1),
-                                 q4::two_codes_128(kb[w], 2 * h + 1)};
-          mma_bf16(c, a, qb[w][2 * h], qb[w][2 * h + 1]);
-        }
-      const uint32_t pa = kpair[ra], pb = kpair[rb];
-      const float sa = q4::scale_of(pa), za = fmaf(-128.f, sa, q4::zero_of(pa));
-      const float sb = q4::scale_of(pb), zb = fmaf(-128.f, sb, q4::zero_of(pb));
-      x[mt][0] = fmaf(sa, c[0], za * qs[0]);
-      x[mt][1] = fmaf(sa, c[1], za * qs[1]);
-      x[mt][2] = fmaf(sb, c[2], zb * qs[0]);
-      x[mt][3] = fmaf(sb, c[3], zb * qs[1]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[mt][j] = (p.cap_pre > 0.f ? fast_tanh(x[mt][j] * p.cap_pre) : x[mt][j]) * p.scale_log2;
-      if (!inside) {
-        const bool in_a = key0 + ra >= begin && key0 + ra < end, in_b = key0 + rb >= begin && key0 + rb < end;
-        x[mt][0] = in_a ? x[mt][0] : -INFINITY; x[mt][1] = in_a ? x[mt][1] : -INFINITY;
-        x[mt][2] = in_b ? x[mt][2] : -INFINITY; x[mt][3] = in_b ? x[mt][3] : -INFINITY;
-      }
-    }
-    // ---- running maximum, sum
-    float grown[2];
-    bool moved = false;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float top = fmaxf(fmaxf(x[0][h], x[0][h + 2]), fmaxf(x[1][h], x[1][h + 2]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-      const float m_new = fmaxf(m[h], top);
-      grown[h] = m[h] == m_new ? 1.f : fast_exp2(m[h] - m_new);    // (-inf to -inf: nothing seen yet, nothing to rescale)
-      moved |= m[h] != m_new;
-      m[h] = m_new;
-    }
-    if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) { l[h] *= grown[h]; zacc[h] *= grown[h]; }
-#pragma unroll
-      for (int k = 0; k < S::kTiles; ++k) {
-        o[k][0] *= grown[0]; o[k][1] *= grown[1]; o[k][2] *= grown[0]; o[k][3] *= grown[1];
-      }
-    }
-    const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      const uint32_t pa = vpair[mt * 16 + row_g], pb = vpair[mt * 16 + row_g + 8];
-      const float sa = q4::scale_of(pa), za = fmaf(8.f, sa, q4::zero_of(pa));
-      const float sb = q4::scale_of(pb), zb = fmaf(8.f, sb, q4::zero_of(pb));
-      const float e0 = fast_exp2(x[mt][0] - m0), e1 = fast_exp2(x[mt][1] - m1);
-      const float e2 = fast_exp2(x[mt][2] - m0), e3 = fast_exp2(x[mt][3] - m1);
-      l[0] += e0 + e2;
-      l[1] += e1 + e3;
-      zacc[0] = fmaf(e0, za, fmaf(e2, zb, zacc[0]));
-      zacc[1] = fmaf(e1, za, fmaf(e3, zb, zacc[1]));
-      const float w0 = e0 * sa, w1 = e1 * sa, w2 = e2 * sb, w3 = e3 * sb;
-      uint32_t hi[2] = {pack_bf16(w0, w1), pack_bf16(w2, w3)};
-      uint32_t low[2] = {pack_bf16(w0 - __uint_as_float(hi[0] << 16), w1 - __uint_as_float(hi[0] & 0xffff0000u)),
-                         pack_bf16(w2 - __uint_as_float(hi[1] << 16), w3 - __uint_as_float(hi[1] & 0xffff0000u))};
-#pragma unroll
-      for (int k = 0; k < 2; ++k) { hi[k] = transposed(hi[k]); low[k] = transposed(low[k]); }
-      // ---- values: keys 2 t4, 2 t4 + 1 and the same eight further
-      const unsigned char* vt = st + S::kCodeBytes;
-      const int r0 = mt * 16 + row_a, r1 = mt * 16 + row_b;
-      uint32_t v[4][S::kFull > 0 ? S::kFull : 1];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = ((k & 1) ? r1 : r0) + (k >> 1) * 8;
-        if constexpr (HD == 64) {
-          v[k][0] = *reinterpret_cast<const uint32_t*>(vt + S::at(r, g >> 2) + (g & 3) * 4);
-        } else if constexpr (HD == 128) {
-          const uint2 u = *reinterpret_cast<const uint2*>(vt + S::at(r, g >> 1) + (g & 1) * 8);
-          v[k][0] = u.x; v[k][1] = u.y;
-        } else if constexpr (HD == 256) {
-          const uint4 u = *reinterpret_cast<const uint4*>(vt + S::at(r, g));
-          v[k][0] = u.x; v[k][1] = u.y; v[k][2] = u.z; v[k][3] = u.w;
-        } else {
-#pragma unroll
-          for (int w = 0; w < S::kFull; ++w) v[k][w] = *reinterpret_cast<const uint32_t*>(vt + S::at(r, 0) + (g * S::kFull + w) * 4);
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < S::kFull; ++w) {
-        const uint32_t ea = __byte_perm(v[0][w], v[1][w], 0x5410), oa = __byte_perm(v[0][w], v[1][w], 0x7632);    // even, odd elements
-        const uint32_t eb = __byte_perm(v[2][w], v[3][w], 0x5410), ob = __byte_perm(v[2][w], v[3][w], 0x7632);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t a[4] = {centred(q4::two_codes_128(ea, k)), centred(q4::two_codes_128(oa, k)), centred(q4::two_codes_128(eb, k)),
-                                 centred(q4::two_codes_128(ob, k))};
-          mma_bf16(o[4 * w + k], a, hi[0], hi[1]);
-          mma_bf16(o[4 * w + k], a, low[0], low[1]);
-        }
-      }
-      if constexpr (S::kHalf) {                                    // the last four words: lane groups 2w and 2w + 1 take the halves of word w
-        uint32_t u[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          u[k] = *reinterpret_cast<const uint32_t*>(vt + S::at(((k & 1) ? r1 : r0) + (k >> 1) * 8, 0) + (8 * S::kFull + (g >> 1)) * 4);
-        const uint32_t pick = (g & 1) ? 0x7632 : 0x5410;
-        const uint32_t a_ = __byte_perm(u[0], u[1], pick), b_ = __byte_perm(u[2], u[3], pick);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t a[4] = {centred(q4::two_codes_128(a_, 2 * k)), centred(q4::two_codes_128(a_, 2 * k + 1)),
-                                 centred(q4::two_codes_128(b_, 2 * k)), centred(q4::two_codes_128(b_, 2 * k + 1))};
-          mma_bf16(o[4 * S::kFull + k], a, hi[0], hi[1]);
-          mma_bf16(o[4 * S::kFull + k], a, low[0], low[1]);
-        }
-      }
-    }
-    __syncwarp();                                                  // the step's place is loaded again next round
-  }
-  cp_async_wait<0>();
-  __syncthreads();                                                 // the rings give way to the merge
-
-  // ---- the warp's partial result: lanes over keys joined, the zeros' part added to every element
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int off = 4; off <= 16; off *= 2) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
-      zacc[h] += __shfl_xor_sync(0xffffffffu, zacc[h], off);
-    }
-  float* row0 = mo + (warp * kQ4Heads + 2 * t4) * HD;
-  float* row1 = row0 + HD;
-#pragma unroll
-  for (int w = 0; w < S::kFull; ++w)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int d = 8 * (g * S::kFull + w) + 2 * k;
-      *reinterpret_cast<float2*>(row0 + d) = make_float2(o[4 * w + k][0] + zacc[0], o[4 * w + k][2] + zacc[0]);
-      *reinterpret_cast<float2*>(row1 + d) = make_float2(o[4 * w + k][1] + zacc[1], o[4 * w + k][3] + zacc[1]);
-    }
-  if constexpr (S::kHalf) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int d = 8 * (8 * S::kFull + (g >> 1)) + 4 * k + (g & 1);
-      const float (&c)[4] = o[4 * S::kFull + k];
-      row0[d] = c[0] + zacc[0]; row0[d + 2] = c[2] + zacc[0];
-      row1[d] = c[1] + zacc[1]; row1[d + 2] = c[3] + zacc[1];
-    }
-  }
-  if (g == 0) {
-    mm[warp * kQ4Heads + 2 * t4] = m[0]; mm[warp * kQ4Heads + 2 * t4 + 1] = m[1];
-    ml[warp * kQ4Heads + 2 * t4] = l[0]; ml[warp * kQ4Heads + 2 * t4 + 1] = l[1];
-  }
-  __syncthreads();
-  // ---- the four warps, four adjacent elements an item
-  constexpr int Q = HD / 4;
-  for (int it = tid; it < heads_here * Q; it += kQ4DecodeThreads) {
-    const int r = it / Q, d = (it - r * Q) * 4;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kQ4Warps; ++w) top = fmaxf(top, mm[w * kQ4Heads + r]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
+    if (lane == 31) sums[warp] = up;
+    __syncthreads();
+    int total = 0, in_front = up - mine;
 #pragma unroll
     for (int w = 0; w < kQ4Warps; ++w) {
-      const float lw = ml[w * kQ4Heads + r];
-      if (lw == 0.f) continue;                                     // a warp without keys
-      const float f = fast_exp2(mm[w * kQ4Heads + r] - top);
-      const float4 v = *reinterpret_cast<const float4*>(mo + (w * kQ4Heads + r) * HD + d);
-      acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
-      sum = fmaf(f, lw, sum);
+      if (w < warp) in_front += sums[w];
+      total += sums[w];
     }
-    const int head = head0 + r;
-    if (p.cluster_merge) {
-      *reinterpret_cast<float4*>(bo + r * HD + d) = acc;
-      if (d == 0) { bm[r] = top; bl[r] = sum; }
-    } else if (p.num_parts == 1) {
-      if (p.sink && top != -INFINITY) sum += fast_exp2(p.sink[head] * 1.4426950408889634f - top);
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      bf16* dst = p.out + size_t(seq) * p.out_stride + size_t(head) * HD + d;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-    } else {
-      const size_t at = (size_t(seq) * p.nh + head) * p.num_parts + part;
-      *reinterpret_cast<float4*>(p.part_o + at * HD + d) = acc;
-      if (d == 0) { p.part_ml[at * 2] = top; p.part_ml[at * 2 + 1] = sum; }
+    U = (long long)total * H;
+    takers = min((long long)gridDim.x, U);                         // (a block between two that share a request has a piece of it)
+    if (blockIdx.x >= takers) { pdl_wait(); return; }
+    const long long u0 = U * blockIdx.x / takers, u1 = U * (blockIdx.x + 1) / takers;
+    left = u1 - u0;
+    if ((long long)in_front * H <= u0 && u0 < (long long)(in_front + mine) * H) {
+      int s = s0, f = in_front, n = tiles_of(p.seq_ctx_len[s]);
+      while ((long long)(f + n) * H <= u0) { f += n; ++s; n = tiles_of(p.seq_ctx_len[s]); }
+      found[0] = s;
+      found[1] = f;
     }
+    __syncthreads();
+    seq = found[0];
+    before = found[1];
+    const int n = tiles_of(p.seq_ctx_len[seq]);
+    const long long at = u0 - before * H;
+    unit_h = int(at / n);
+    tile = int(at - (long long)unit_h * n);
   }
-  if (p.cluster_merge) q4_cluster_tail<HD>(p, seq, head0, heads_here, bo, bm, bl);
+  pdl_wait();
+
+  const size_t head_bytes = q4::page_bytes(p.block_size, HD);
+  const unsigned head_units = unsigned(head_bytes / 16);
+  const int pairs_at = p.block_size * (HD / 2);
+  const int row_g = S::row(g), row_a = S::row(2 * t4), row_b = S::row(2 * t4 + 1);
+  unsigned char* const ring = smem_raw + size_t(warp) * STAGES * S::kStageBytes;
+
+  for (;;) {
+    // ---- the next piece of work
+    Q4Segment w;
+    const int ctx = p.seq_ctx_len[seq], lo = first_key(ctx), base = lo / kQ4Step * kQ4Step;
+    w.seq = seq;
+    w.slot = -1;
+    int of_h;
+    if (!shares) {
+      of_h = blockIdx.y;
+      const int from = base + int(blockIdx.x) * p.part_size;
+      w.begin = max(lo, from);
+      w.end = min(ctx, from + p.part_size);
+      if (p.num_parts > 1 && !p.cluster_merge) w.slot = blockIdx.x;
+    } else {
+      of_h = unit_h;
+      const int n = tiles_of(ctx), take = int(min((long long)(n - tile), left));
+      w.begin = max(lo, base + tile * kQ4Tile);
+      w.end = min(ctx, base + (tile + take) * kQ4Tile);
+      if (take < n) w.slot = 2 * int(blockIdx.x) + (tile == 0 ? 1 : 0);
+      if (tile == 0 && tid == 0) {                                 // who reads the pieces of this request and head: blocks first .. last
+        const long long last_unit = before * H + (long long)unit_h * n + n - 1;
+        p.part_first[(seq * H + unit_h) * 2] = blockIdx.x;
+        p.part_first[(seq * H + unit_h) * 2 + 1] = int(((last_unit + 1) * takers - 1) / U);
+      }
+      left -= take;
+      tile += take;
+      if (tile == n) {
+        tile = 0;
+        if (++unit_h == H) {
+          unit_h = 0;
+          before += n;
+          if (left > 0)
+            do ++seq; while (p.seq_ctx_len[seq] <= 0);             // (there are more tiles, so there is such a request)
+        }
+      }
+    }
+    w.kvh = of_h / head_tiles;
+    const int ht = of_h - w.kvh * head_tiles;
+    w.head0 = w.kvh * G + ht * kQ4Heads;
+    w.heads_here = min(kQ4Heads, G - ht * kQ4Heads);
+
+    // heads 2 t4, 2 t4 + 1; sums over this lane's keys (the maximum starts finite: no difference to it is not-a-number)
+    float m[2] = {-kQ4Lowest, -kQ4Lowest}, l[2] = {0.f, 0.f}, zacc[2] = {0.f, 0.f};
+    float o[S::kTiles][4];
+#pragma unroll
+    for (int i = 0; i < S::kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    uint32_t unit = 0x00800000u;                                   // the power of two that weights are divided by, as a float's bits
+    if (w.begin < w.end) {
+      // ---- q of head g as the second operand: elements in the order in which a lane's codes lie
+      uint32_t qb[S::kKeyWords][4];
+      float qs[2];                                                 // sum of q over the elements, heads 2 t4 and 2 t4 + 1
+      {
+        float sum = 0.f;
+        const bf16* row = p.q + size_t(w.seq) * p.q_stride + size_t(w.head0 + g) * HD;
+#pragma unroll
+        for (int i = 0; i < S::kKeyWords; ++i) {
+          const int word = (S::kKeyWords % 4 == 0) ? (i / 4) * 16 + t4 * 4 + (i & 3) : t4 * S::kKeyWords + i;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (g < w.heads_here) v = *reinterpret_cast<const uint4*>(row + word * 8);
+          qb[i][0] = v.x; qb[i][1] = v.y; qb[i][2] = v.z; qb[i][3] = v.w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum += __uint_as_float(qb[i][e] << 16) + __uint_as_float(qb[i][e] & 0xffff0000u);
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const float unit_of_scores = CAP ? 1.f : p.scale_log2;
+        qs[0] = __shfl_sync(0xffffffffu, sum, t4 * 8) * unit_of_scores;
+        qs[1] = __shfl_sync(0xffffffffu, sum, t4 * 8 + 4) * unit_of_scores;
+      }
+      const int* table = p.block_tables + size_t(w.seq) * p.max_blocks;
+      // rounds of 128 keys; as many at a time as the table slice has pages for
+      const int first = w.begin / kQ4Step * kQ4Step;
+      const int rounds_at_once = max(1, (kQ4TabMax - 1) * p.block_size / kQ4Tile);
+      for (int at = first; at < w.end; at += rounds_at_once * kQ4Tile) {
+        const int stop = min(w.end, at + rounds_at_once * kQ4Tile);
+        const int tab0 = max(at, w.begin) / p.block_size, pages = (stop - 1) / p.block_size - tab0 + 1;
+        if (at != first) __syncthreads();                          // the slice before is read
+        for (int j = tid; j < pages; j += kQ4DecodeThreads)
+          stab[j] = (unsigned(min(max(table[tab0 + j], 0), p.num_pages - 1)) * unsigned(p.nkv) + unsigned(w.kvh)) * head_units;
+        __syncthreads();
+
+        // the warp's steps of 32 keys: at + 32 (4 i + warp)
+        const int steps = ((stop - at + kQ4Step - 1) / kQ4Step - warp + kQ4Warps - 1) / kQ4Warps;
+        unsigned char* load_to = ring;
+        int load_key = at + warp * kQ4Step, loads = steps;
+        auto load_step = [&]() {
+          if (loads > 0) {
+            unsigned char* const pairs = load_to + 2 * S::kCodeBytes + lane * 4;
+            const unsigned* const tab = stab - tab0;
+            if (p.log2_block >= 0 && load_key >= w.begin && load_key + kQ4Step <= w.end) {      // the usual step
+              const int lb = p.log2_block, in_page = p.block_size - 1;
+#pragma unroll
+              for (int c = 0; c < S::kChunks; ++c) {
+                const int piece = c * 32 + lane, r = piece / S::kChunks, ch = piece - r * S::kChunks;
+                const int key = load_key + r, to = S::at(r, ch);
+                const unsigned u = tab[key >> lb] + unsigned((key & in_page) * S::kChunks + ch);
+                cp_async16(load_to + to, p.k_cache + size_t(u) * 16);
+                cp_async16(load_to + S::kCodeBytes + to, p.v_cache + size_t(u) * 16);
+              }
+              const int key = load_key + lane;
+              const size_t u = size_t(tab[key >> lb]) * 16 + unsigned(pairs_at + (key & in_page) * 4);
+              cp_async4(pairs, p.k_cache + u);
+              cp_async4(pairs + kQ4Step * 4, p.v_cache + u);
+            } else {                                               // pages of any size, keys outside the piece of work
+#pragma unroll 1
+              for (int piece = lane; piece < kQ4Step * S::kChunks; piece += 32) {
+                const int r = piece / S::kChunks, ch = piece - r * S::kChunks, key = load_key + r;
+                if (key < w.begin || key >= w.end) continue;
+                const int pi = key / p.block_size, off = key - pi * p.block_size;
+                const size_t u = size_t(tab[pi] + unsigned(off * S::kChunks + ch)) * 16;
+                const int to = S::at(r, ch);
+                cp_async16(load_to + to, p.k_cache + u);
+                cp_async16(load_to + S::kCodeBytes + to, p.v_cache + u);
+              }
+              const int key = load_key + lane;
+              if (key >= w.begin && key < w.end) {
+                const int pi = key / p.block_size, off = key - pi * p.block_size;
+                const size_t u = size_t(tab[pi]) * 16 + unsigned(pairs_at + off * 4);
+                cp_async4(pairs, p.k_cache + u);
+                cp_async4(pairs + kQ4Step * 4, p.v_cache + u);
+              } else {                                             // zero, so that zero times it stays zero (codes are finite whatever they are)
+                *reinterpret_cast<uint32_t*>(pairs) = 0u;
+                *reinterpret_cast<uint32_t*>(pairs + kQ4Step * 4) = 0u;
+              }
+            }
+            --loads;
+            load_key += kQ4Tile;
+            load_to = load_to + S::kStageBytes == ring + STAGES * S::kStageBytes ? ring : load_to + S::kStageBytes;
+          }
+          cp_async_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) load_step();
+
+        // scores of a step in log2 units: x[16 keys][key g, head 2 t4 | 2 t4 + 1; key g + 8]
+        auto scores = [&](const unsigned char* st, float (&x)[2][4]) {
+          const uint32_t* kpair = reinterpret_cast<const uint32_t*>(st + 2 * S::kCodeBytes);
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            uint32_t ka[S::kKeyWords], kb[S::kKeyWords];
+            const int ra = mt * 16 + row_g, rb = ra + 8;
+            if constexpr (S::kKeyWords % 4 == 0) {
+#pragma unroll
+              for (int j = 0; j < S::kKeyWords / 4; ++j) {
+                const uint4 a = *reinterpret_cast<const uint4*>(st + S::at(ra, j * 4 + t4));
+                const uint4 b = *reinterpret_cast<const uint4*>(st + S::at(rb, j * 4 + t4));
+                ka[4 * j] = a.x; ka[4 * j + 1] = a.y; ka[4 * j + 2] = a.z; ka[4 * j + 3] = a.w;
+                kb[4 * j] = b.x; kb[4 * j + 1] = b.y; kb[4 * j + 2] = b.z; kb[4 * j + 3] = b.w;
+              }
+            } else if constexpr (HD == 64) {
+              const uint2 a = *reinterpret_cast<const uint2*>(st + S::at(ra, t4 >> 1) + (t4 & 1) * 8);
+              const uint2 b = *reinterpret_cast<const uint2*>(st + S::at(rb, t4 >> 1) + (t4 & 1) * 8);
+              ka[0] = a.x; ka[1] = a.y; kb[0] = b.x; kb[1] = b.y;
+            } else {
+#pragma unroll
+              for (int j = 0; j < S::kKeyWords; ++j) {
+                ka[j] = *reinterpret_cast<const uint32_t*>(st + S::at(ra, 0) + (t4 * S::kKeyWords + j) * 4);
+                kb[j] = *reinterpret_cast<const uint32_t*>(st + S::at(rb, 0) + (t4 * S::kKeyWords + j) * 4);
+              }
+            }
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < S::kKeyWords; ++j)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t a[4] = {q4::two_codes_128(ka[j], 2 * h), q4::two_codes_128(kb[j], 2 * h), q4::two_codes_128(ka[j], 2 * h + 1),
+                                       q4::two_codes_128(kb[j], 2 * h + 1)};
+                mma_codes(c, a, qb[j][2 * h], qb[j][2 * h + 1]);
+              }
+            const uint32_t pa = kpair[ra], pb = kpair[rb];
+            float sa = q4::scale_of(pa), sb = q4::scale_of(pb);
+            const float za = fmaf(-128.f, sa, q4::zero_of(pa)), zb = fmaf(-128.f, sb, q4::zero_of(pb));
+            if constexpr (!CAP) { sa *= p.scale_log2; sb *= p.scale_log2; }
+            x[mt][0] = fmaf(sa, c[0], za * qs[0]);
+            x[mt][1] = fmaf(sa, c[1], za * qs[1]);
+            x[mt][2] = fmaf(sb, c[2], zb * qs[0]);
+            x[mt][3] = fmaf(sb, c[3], zb * qs[1]);
+            if constexpr (CAP) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[mt][j] = fast_tanh(x[mt][j] * p.cap_pre) * p.scale_log2;
+            }
+          }
+        };
+        // The scores of step i + 1 are formed while the softmax of step i, whose steps wait for one another, is under way.
+        const unsigned char* st = ring;
+        int key0 = at + warp * kQ4Step;
+        float x[2][4], ahead[2][4];
+        if (steps > 0) {
+          cp_async_wait<STAGES - 2>();
+          __syncwarp();
+          scores(st, ahead);
+        }
+        for (int i = 0; i < steps; ++i) {
+          load_step();
+          cp_async_wait<STAGES - 2>();
+          __syncwarp();
+          const uint32_t* vpair = reinterpret_cast<const uint32_t*>(st + 2 * S::kCodeBytes) + kQ4Step;
+          const unsigned char* const next = st + S::kStageBytes == ring + STAGES * S::kStageBytes ? ring : st + S::kStageBytes;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[mt][j] = ahead[mt][j];
+          if (key0 < w.begin || key0 + kQ4Step > w.end) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int key = key0 + mt * 16 + row_g + (j >> 1) * 8;
+                x[mt][j] = key >= w.begin && key < w.end ? x[mt][j] : -INFINITY;
+              }
+          }
+          scores(next, ahead);                                     // (behind the last step: of what lies there, and nobody reads it)
+          // ---- running maximum; and the unit of the weights: the power of two above the largest scale so far
+          float top[2], grown[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            top[h] = fmaxf(fmaxf(x[0][h], x[0][h + 2]), fmaxf(x[1][h], x[1][h + 2]));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 4));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 8));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 16));
+          }
+          const uint32_t largest = __reduce_max_sync(0xffffffffu, vpair[lane] << 16);
+          if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1] || largest >= unit)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float m_new = fmaxf(m[h], top[h]);
+              grown[h] = fast_exp2(m[h] - m_new);                  // (zero where nothing was seen yet)
+              m[h] = m_new;
+              l[h] *= grown[h];
+              zacc[h] *= grown[h];
+            }
+            if (largest >= unit) {
+              const uint32_t unit_new = min((largest & 0x7f800000u) + 0x00800000u, 0x7f000000u);
+              const float f = __uint_as_float(unit) / __uint_as_float(unit_new);
+              grown[0] *= f;
+              grown[1] *= f;
+              unit = unit_new;
+            }
+#pragma unroll
+            for (int k = 0; k < S::kTiles; ++k) {
+              o[k][0] *= grown[0]; o[k][1] *= grown[1]; o[k][2] *= grown[0]; o[k][3] *= grown[1];
+            }
+          }
+          const float per_unit = __uint_as_float(0x7f000000u - unit);         // 1 / unit
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            const uint32_t pa = vpair[mt * 16 + row_g], pb = vpair[mt * 16 + row_g + 8];
+            const float sa = q4::scale_of(pa), za = fmaf(8.f, sa, q4::zero_of(pa));
+            const float sb = q4::scale_of(pb), zb = fmaf(8.f, sb, q4::zero_of(pb));
+            const float e0 = fast_exp2(x[mt][0] - m[0]), e1 = fast_exp2(x[mt][1] - m[1]);
+            const float e2 = fast_exp2(x[mt][2] - m[0]), e3 = fast_exp2(x[mt][3] - m[1]);
+            l[0] += e0 + e2;
+            l[1] += e1 + e3;
+            zacc[0] = fmaf(e0, za, fmaf(e2, zb, zacc[0]));
+            zacc[1] = fmaf(e1, za, fmaf(e3, zb, zacc[1]));
+            const float ua = sa * per_unit, ub = sb * per_unit;
+            const uint32_t b0 = transposed(pack_half(e0 * ua, e1 * ua)), b1 = transposed(pack_half(e2 * ub, e3 * ub));
+            // ---- values: keys 2 t4, 2 t4 + 1 and the same eight further
+            const unsigned char* vt = st + S::kCodeBytes;
+            const int r0 = mt * 16 + row_a, r1 = mt * 16 + row_b;
+            uint32_t v[4][S::kFull > 0 ? S::kFull : 1];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int r = ((k & 1) ? r1 : r0) + (k >> 1) * 8;
+              if constexpr (HD == 64) {
+                v[k][0] = *reinterpret_cast<const uint32_t*>(vt + S::at(r, g >> 2) + (g & 3) * 4);
+              } else if constexpr (HD == 128) {
+                const uint2 u = *reinterpret_cast<const uint2*>(vt + S::at(r, g >> 1) + (g & 1) * 8);
+                v[k][0] = u.x; v[k][1] = u.y;
+              } else if constexpr (HD == 256) {
+                const uint4 u = *reinterpret_cast<const uint4*>(vt + S::at(r, g));
+                v[k][0] = u.x; v[k][1] = u.y; v[k][2] = u.z; v[k][3] = u.w;
+              } else {
+#pragma unroll
+                for (int j = 0; j < S::kFull; ++j) v[k][j] = *reinterpret_cast<const uint32_t*>(vt + S::at(r, 0) + (g * S::kFull + j) * 4);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < S::kFull; ++j) {
+              uint32_t ea = __byte_perm(v[0][j], v[1][j], 0x5410), oa = __byte_perm(v[0][j], v[1][j], 0x7632);    // even, odd elements
+              uint32_t eb = __byte_perm(v[2][j], v[3][j], 0x5410), ob = __byte_perm(v[2][j], v[3][j], 0x7632);
+#pragma unroll
+              for (int k = 0; k < 4; k += 2) {
+                const uint32_t a[4] = {low_codes(ea), low_codes(oa), low_codes(eb), low_codes(ob)};
+                mma_half(o[4 * j + k], a, b0, b1);
+                const uint32_t c[4] = {high_codes(ea), high_codes(oa), high_codes(eb), high_codes(ob)};
+                mma_half(o[4 * j + k + 1], c, b0, b1);
+                ea >>= 8; oa >>= 8; eb >>= 8; ob >>= 8;
+              }
+            }
+            if constexpr (S::kHalf) {                              // the last four words: lane groups 2w and 2w + 1 take the halves of word w
+              uint32_t u[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                u[k] = *reinterpret_cast<const uint32_t*>(vt + S::at(((k & 1) ? r1 : r0) + (k >> 1) * 8, 0) + (8 * S::kFull + (g >> 1)) * 4);
+              const uint32_t pick = (g & 1) ? 0x7632 : 0x5410;
+              uint32_t a_ = __byte_perm(u[0], u[1], pick), b_ = __byte_perm(u[2], u[3], pick);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const uint32_t a[4] = {low_codes(a_), high_codes(a_), low_codes(b_), high_codes(b_)};
+                mma_half(o[4 * S::kFull + k], a, b0, b1);
+                a_ >>= 8; b_ >>= 8;
+              }
+            }
+          }
+          __syncwarp();                                            // the step's place is loaded again next round
+          key0 += kQ4Tile;
+          st = next;
+        }
+        cp_async_wait<0>();
+      }
+    }
+    __syncthreads();                                               // the rings give way to the merge
+
+    // ---- the warp's partial result: lanes over keys joined, units taken out, the zeros' part added to every element
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int off = 4; off <= 16; off *= 2) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
+        zacc[h] += __shfl_xor_sync(0xffffffffu, zacc[h], off);
+      }
+    const float f_low = __uint_as_float(unit), f_high = f_low * 0.0625f;
+    float* row0 = mo + (warp * kQ4Heads + 2 * t4) * HD;
+    float* row1 = row0 + HD;
+#pragma unroll
+    for (int j = 0; j < S::kFull; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int d = 8 * (g * S::kFull + j) + 2 * k;
+        const float f = (k & 1) ? f_high : f_low;
+        const float (&c)[4] = o[4 * j + k];
+        *reinterpret_cast<float2*>(row0 + d) = make_float2(fmaf(c[0], f, zacc[0]), fmaf(c[2], f, zacc[0]));
+        *reinterpret_cast<float2*>(row1 + d) = make_float2(fmaf(c[1], f, zacc[1]), fmaf(c[3], f, zacc[1]));
+      }
+    if constexpr (S::kHalf) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int d = 8 * (8 * S::kFull + (g >> 1)) + 4 * k + (g & 1);
+        const float (&c)[4] = o[4 * S::kFull + k];
+        row0[d] = fmaf(c[0], f_low, zacc[0]); row0[d + 2] = fmaf(c[2], f_high, zacc[0]);
+        row1[d] = fmaf(c[1], f_low, zacc[1]); row1[d + 2] = fmaf(c[3], f_high, zacc[1]);
+      }
+    }
+    if (g == 0) {
+      mm[warp * kQ4Heads + 2 * t4] = m[0]; mm[warp * kQ4Heads + 2 * t4 + 1] = m[1];
+      ml[warp * kQ4Heads + 2 * t4] = l[0]; ml[warp * kQ4Heads + 2 * t4 + 1] = l[1];
+    }
+    __syncthreads();
+    // ---- the four warps, four adjacent elements an item
+    constexpr int Q = HD / 4;
+    for (int it = tid; it < w.heads_here * Q; it += kQ4DecodeThreads) {
+      const int r = it / Q, d = (it - r * Q) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kQ4Warps; ++k) top = fmaxf(top, mm[k * kQ4Heads + r]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kQ4Warps; ++k) {
+        const float lk = ml[k * kQ4Heads + r];
+        if (lk == 0.f) continue;                                   // a warp without keys
+        const float f = fast_exp2(mm[k * kQ4Heads + r] - top);
+        const float4 v = *reinterpret_cast<const float4*>(mo + (k * kQ4Heads + r) * HD + d);
+        acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+        sum = fmaf(f, lk, sum);
+      }
+      const int head = w.head0 + r;
+      if (p.cluster_merge) {
+        *reinterpret_cast<float4*>(bo + r * HD + d) = acc;
+        if (d == 0) { bm[r] = top; bl[r] = sum; }
+      } else if (w.slot < 0) {
+        if (p.sink && sum != 0.f) sum += fast_exp2(p.sink[head] * 1.4426950408889634f - top);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        bf16* dst = p.out + size_t(w.seq) * p.out_stride + size_t(head) * HD + d;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+      } else {
+        const size_t at = shares ? size_t(w.slot) * kQ4Heads + r : (size_t(w.seq) * p.nh + head) * p.num_parts + w.slot;
+        *reinterpret_cast<float4*>(p.part_o + at * HD + d) = acc;
+        if (d == 0) { p.part_ml[at * 2] = top; p.part_ml[at * 2 + 1] = sum; }
+      }
+    }
+    if (!shares) {
+      if (p.cluster_merge) q4_cluster_tail<HD>(p, w.seq, w.head0, w.heads_here, bo, bm, bl);
+      return;
+    }
+    if (left <= 0) return;
+    __syncthreads();                                               // the merge gives way to the rings
+  }
 }
 
 // More partitions than a cluster merges, out of scratch memory, in their order.
@@ -501,17 +657,54 @@ __global__ void attn_decode_q4_merge_kernel(const float* part_o, const float* pa
       acc = fmaf(f, part_o[(base + i) * hd + d], acc);
       sum = fmaf(f, li, sum);
     }
-    if (sink && top != -INFINITY) sum += exp2f(sink[head] * 1.4426950408889634f - top);
+    if (sink && sum != 0.f) sum += exp2f(sink[head] * 1.4426950408889634f - top);
     out[size_t(seq) * out_stride + size_t(head) * hd + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
   }
 }
 
-template <int HD> constexpr int q4_decode_stages() { return HD <= 128 ? 3 : 2; }
+// The pieces of a request and eight heads that blocks part_first[0] .. part_first[1] have left, in their order: the first block's
+// lies in its second place, the others' in their first.
+__global__ void __launch_bounds__(128) attn_decode_q4_shares_kernel(const float* part_o, const float* part_ml, const int* part_first,
+                                                                    const int* __restrict__ seq_ctx_len, bf16* __restrict__ out,
+                                                                    long long out_stride, int nh, int nkv, int hd, const float* __restrict__ sink) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int G = nh / nkv, head_tiles = (G + kQ4Heads - 1) / kQ4Heads, H = nkv * head_tiles;
+  const int seq = blockIdx.x, h = blockIdx.y, kvh = h / head_tiles, ht = h - kvh * head_tiles;
+  const int head0 = kvh * G + ht * kQ4Heads, heads_here = min(kQ4Heads, G - ht * kQ4Heads);
+  const bool empty = seq_ctx_len[seq] <= 0;
+  const int first = empty ? 0 : part_first[(seq * H + h) * 2], last = empty ? 0 : part_first[(seq * H + h) * 2 + 1];
+  if (!empty && first == last) return;                             // one block had it all
+  const int quads = hd / 4;
+  for (int it = threadIdx.x; it < heads_here * quads; it += 128) {
+    const int r = it / quads, d = (it - r * quads) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f, top = -INFINITY;
+    if (!empty) {
+      for (int b = first; b <= last; ++b) top = fmaxf(top, part_ml[(size_t(2 * b + (b == first)) * kQ4Heads + r) * 2]);
+      for (int b = first; b <= last; ++b) {
+        const size_t at = size_t(2 * b + (b == first)) * kQ4Heads + r;
+        const float lb = part_ml[at * 2 + 1];
+        if (lb == 0.f) continue;
+        const float f = fast_exp2(part_ml[at * 2] - top);
+        const float4 v = *reinterpret_cast<const float4*>(part_o + at * hd + d);
+        acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+        sum = fmaf(f, lb, sum);
+      }
+      if (sink && sum != 0.f) sum += fast_exp2(sink[head0 + r] * 1.4426950408889634f - top);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    bf16* dst = out + size_t(seq) * out_stride + size_t(head0 + r) * hd + d;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  }
+}
 
-template <int HD>
-int launch_decode_q4(const DecodeQ4Params& p, int seqs, cudaStream_t s) {
+template <int HD> constexpr int q4_decode_stages() { return HD <= 128 ? 4 : 3; }
+
+template <int HD, bool CAP>
+int launch_decode_q4(const DecodeQ4Params& p, int shares, cudaStream_t s) {
   constexpr int STAGES = q4_decode_stages<HD>();
-  auto kernel = attn_decode_q4_kernel<HD, STAGES>;
+  auto kernel = attn_decode_q4_kernel<HD, STAGES, CAP>;
   constexpr size_t smem = q4_decode_smem<HD, STAGES>();
   static OncePerDevice once;
   if (smem > 48 * 1024) {
@@ -519,14 +712,14 @@ int launch_decode_q4(const DecodeQ4Params& p, int seqs, cudaStream_t s) {
     if (rc != 0) return rc;
   }
   const int G = p.nh / p.nkv;
-  const dim3 grid(p.num_parts, p.nkv * ((G + kQ4Heads - 1) / kQ4Heads), seqs);
+  const dim3 grid = p.num_parts == 0 ? dim3(shares) : dim3(p.num_parts, p.nkv * ((G + kQ4Heads - 1) / kQ4Heads), p.seqs);
   if (p.cluster_merge) return pdl_launch_cluster(kernel, grid, dim3(kQ4DecodeThreads), smem, s, p.num_parts, p);
   return pdl_launch(kernel, grid, dim3(kQ4DecodeThreads), smem, s, p);
 }
 
 template <int HD> int q4_blocks_per_sm() {
   constexpr int STAGES = q4_decode_stages<HD>();
-  auto kernel = attn_decode_q4_kernel<HD, STAGES>;
+  auto kernel = attn_decode_q4_kernel<HD, STAGES, false>;
   constexpr size_t smem = q4_decode_smem<HD, STAGES>();
   int n = 0;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return 0;
@@ -551,27 +744,35 @@ KVCM_API int kvcm_attention_decode_q4_blocks_per_sm(int hd) {
   return 0;
 }
 
-// num_parts partitions of part_size keys (a multiple of 128) cover [first visible key rounded down to 32, context).  More than 8 of
-// them, or cluster_merge == 0, want scratch: seqs * nh * num_parts * (hd + 2) floats.
+// num_parts > 0: that many partitions of part_size keys (a multiple of 128) cover [first visible key rounded down to 32, context).
+// More than 8 of them, or cluster_merge == 0, want scratch: seqs * nh * num_parts * (hd + 2) floats.
+// num_parts == 0: `shares` blocks take equal shares of all requests' and heads' tiles of 128 keys, and a second kernel joins what
+// was cut; scratch: shares * 16 * (hd + 2) floats, then seqs * nkv * ceil(nh / nkv / 8) * 2 ints.
 KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, void* out, long long out_stride, const void* k_cache,
                                            const void* v_cache, int num_pages, const int* block_tables, int max_blocks,
                                            const int* seq_ctx_len, int seqs, int nh, int nkv, int hd, int block_size, float scale,
-                                           int window, int part_size, int num_parts, float* scratch, int cluster_merge, float softcap,
-                                           const float* sink, void* stream) {
+                                           int window, int part_size, int num_parts, int shares, float* scratch, int cluster_merge,
+                                           float softcap, const float* sink, void* stream) {
   if (seqs == 0) return 0;
-  if (nkv <= 0 || nh <= 0 || nh % nkv || block_size <= 0 || num_pages <= 0 || part_size <= 0 || part_size % (kQ4Step * kQ4Warps) ||
-      num_parts < 1 || seqs > 65535 || nh > 65535)
+  if (nkv <= 0 || nh <= 0 || nh % nkv || block_size <= 0 || num_pages <= 0 || num_parts < 0 || seqs > 65535 || nh > 65535 ||
+      !kvcm_attention_q4_decode_supports(hd))
     return KVCM_ERR_UNSUPPORTED;
+  if (num_parts > 0 ? (part_size <= 0 || part_size % kQ4Tile) : (shares <= 0 || shares > (1 << 20))) return KVCM_ERR_UNSUPPORTED;
   if (((reinterpret_cast<uintptr_t>(q) | uintptr_t(q_stride * 2) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15) ||
       ((reinterpret_cast<uintptr_t>(out) | uintptr_t(out_stride * 2)) & 7))
     return KVCM_ERR_UNSUPPORTED;
-  if (cluster_merge && (num_parts < 2 || num_parts > kQ4ClusterParts)) cluster_merge = 0;
-  if (num_parts > 1 && !cluster_merge && scratch == nullptr) return KVCM_ERR_UNSUPPORTED;
+  // pages are found by 32-bit counts of 16 bytes
+  if (q4::page_bytes(block_size, hd) / 16 * (unsigned long long)num_pages * nkv > 0xffffffffull) return KVCM_ERR_UNSUPPORTED;
+  if (num_parts == 0 || num_parts > kQ4ClusterParts || num_parts < 2) cluster_merge = 0;
+  if (num_parts != 1 && !cluster_merge && (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15))) return KVCM_ERR_UNSUPPORTED;
+  const int head_tiles = (nh / nkv + kQ4Heads - 1) / kQ4Heads;
+  const size_t pieces = num_parts == 0 ? size_t(shares) * 2 * kQ4Heads : size_t(seqs) * nh * num_parts;
   DecodeQ4Params p;
   p.q = (const bf16*)q; p.q_stride = q_stride; p.out = (bf16*)out; p.out_stride = out_stride;
   p.k_cache = (const uint8_t*)k_cache; p.v_cache = (const uint8_t*)v_cache; p.num_pages = num_pages;
-  p.block_tables = block_tables; p.max_blocks = max_blocks; p.seq_ctx_len = seq_ctx_len;
-  p.part_o = scratch; p.part_ml = scratch ? scratch + (size_t)seqs * nh * num_parts * hd : nullptr;
+  p.block_tables = block_tables; p.max_blocks = max_blocks; p.seq_ctx_len = seq_ctx_len; p.seqs = seqs;
+  p.part_o = scratch; p.part_ml = scratch ? scratch + pieces * hd : nullptr;
+  p.part_first = scratch ? reinterpret_cast<int*>(scratch + pieces * (hd + 2)) : nullptr;
   p.nh = nh; p.nkv = nkv; p.block_size = block_size; p.window = window;
   p.part_size = part_size; p.num_parts = num_parts; p.cluster_merge = cluster_merge;
   p.scale_log2 = (softcap > 0.f ? softcap : scale) * 1.4426950408889634f;
@@ -580,10 +781,13 @@ KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, vo
   p.log2_block = -1;
   for (int b = 0; b < 31; ++b) if ((1 << b) == block_size) p.log2_block = b;
   int rc = KVCM_ERR_UNSUPPORTED;
-#define X(N) if (hd == N) rc = launch_decode_q4<N>(p, seqs, (cudaStream_t)stream);
+#define X(N) if (hd == N) rc = softcap > 0.f ? launch_decode_q4<N, true>(p, shares, (cudaStream_t)stream) : launch_decode_q4<N, false>(p, shares, (cudaStream_t)stream);
   KVCM_FOR_Q4_HEAD_DIMS(X)
 #undef X
   if (rc != 0 || num_parts == 1 || cluster_merge) return rc;
+  if (num_parts == 0)
+    return pdl_launch(attn_decode_q4_shares_kernel, dim3(seqs, nkv * head_tiles), dim3(128), 0, (cudaStream_t)stream, (const float*)p.part_o,
+                      (const float*)p.part_ml, (const int*)p.part_first, seq_ctx_len, p.out, out_stride, nh, nkv, hd, sink);
   return pdl_launch(attn_decode_q4_merge_kernel, dim3(seqs, nh), dim3(hd < 64 ? 32 : 64), 0, (cudaStream_t)stream, (const float*)p.part_o,
                     (const float*)p.part_ml, p.out, out_stride, nh, hd, num_parts, p.sink);
 }

@@ -689,6 +689,8 @@ def decode_partitions_q4(seqs: int, nh: int, nkv: int, hd: int, max_ctx: int, de
     max_ctx = max(int(max_ctx), 1)
     blocks = max(1, seqs * nkv * ((nh // nkv + 7) // 8))
     most = (max_ctx + Q4_PART_KEYS - 1) // Q4_PART_KEYS
+    if force_parts < 0:
+        return Q4_PART_KEYS, 0
     if force_parts > 0:
         parts = min(int(force_parts), most)
     else:
@@ -732,15 +734,18 @@ def attention_decode_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tenso
         span = ctx.max_decode_ctx if window <= 0 else min(ctx.max_decode_ctx, int(window) + 31)
         size, parts = decode_partitions_q4(S, nh, nkv, hd, span, q.device, int(ctx.options.get("attn_parts", 0)))
         in_cluster = 1 < parts <= CLUSTER_PARTS and ctx.options.get("attn_merge", "cluster") == "cluster"
-        scratch = None
-        if parts > 1 and not in_cluster:
+        scratch, shares = None, 0
+        if parts == 0:
+            shares = _q4_resident_blocks(hd, q.device)
+            scratch = torch.empty(shares * 16 * (hd + 2) + S * nkv * ((nh // nkv + 7) // 8) * 2, dtype=torch.float32, device=q.device)
+        elif parts > 1 and not in_cluster:
             scratch = torch.empty(S * nh * parts * (hd + 2), dtype=torch.float32, device=q.device)
         rc = _lib().kvcm_attention_decode_q4_bf16(
             _p(q), ctypes.c_longlong(q.stride(0)), _p(out), ctypes.c_longlong(out.stride(0)), _p(k_cache), _p(v_cache), k_cache.shape[0],
             _p(block_tables), block_tables.shape[1], _p(ctx.seq_ctx_len), S, nh, nkv, hd, block_size, ctypes.c_float(scale), int(window),
-            size, parts, _p(scratch), int(in_cluster), ctypes.c_float(softcap), _p(sink), _stream())
+            size, parts, shares, _p(scratch), int(in_cluster), ctypes.c_float(softcap), _p(sink), _stream())
     _check(rc, name, f"(hd={hd}, nh={nh}, nkv={nkv})")
-    if parts > 1 and not in_cluster:
+    if parts != 1 and not in_cluster:
         global _launches
         _launches += 1                      # the merge kernel
 
@@ -759,8 +764,36 @@ def paged_attention_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor
     if nd > 0:
         attention_decode_q4(q[:nd], out[:nd], k_cache, v_cache, block_tables, ctx, nh, nkv, hd, block_size, scale, window, softcap, sink)
     if ctx.rows > nd:
-        attention_plain_q4(q[nd:], out[nd:], k_cache, v_cache, block_tables, ctx.row_seq[nd:], ctx.positions[nd:], nh, nkv, hd, block_size,
-                           scale, window, softcap, sink)
+        attention_prefill_q4(q, out, k_cache, v_cache, block_tables, ctx, nh, nkv, hd, block_size, scale, window, softcap, sink)
+
+
+def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                         ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
+                         sink: Optional[torch.Tensor] = None) -> None:
+    """Rows of portions longer than one token over a cache in 4 bits; q and out are the step's full bfloat16 row arrays, ``ctx`` has
+    the step's arrays with tiles of 64 rows.  The pages that the portions see are first laid out in bfloat16 (in scratch of the
+    call) and then read by ``attention_prefill``."""
+    name = "attention_prefill_q4"
+    _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink, ctx.seq_q_start,
+                  ctx.seq_q_len, ctx.seq_ctx_len, ctx.tile_seq, ctx.tile_q0)
+    _need(attention_q4_supported(hd, q.dtype), f"{name}: bfloat16 rows, heads of 32 to 256 elements in steps of 32")
+    _need(q.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0, f"{name}: q rows must be 16-byte aligned")
+    _need(out.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0, f"{name}: out rows must be 16-byte aligned")
+    _need(ctx.tile_rows == 64, f"{name}: the batch must be tiled in 64 query rows")
+    S = ctx.seq_ctx_len.numel()
+    _need(block_tables.shape[0] >= S, f"{name}: a page table for each of {S} entries")
+    with _on_device(name, q, out, k_cache, v_cache, block_tables, sink, ctx.seq_q_start, ctx.seq_q_len, ctx.seq_ctx_len, ctx.tile_seq, ctx.tile_q0):
+        first, seqs = ctx.decode_seqs, S - ctx.decode_seqs
+        if seqs <= 0 or ctx.prefill_tiles == 0:
+            return
+        blocks = min(block_tables.shape[1], (ctx.max_ctx + block_size - 1) // block_size)
+        pages = torch.empty((2, seqs * blocks, nkv, block_size, hd), dtype=torch.bfloat16, device=q.device)
+        rc = _lib().kvcm_unpack_pages_q4_bf16(_p(k_cache), _p(v_cache), _p(block_tables), block_tables.shape[1], _p(ctx.seq_q_len),
+                                              _p(ctx.seq_ctx_len), _p(pages[0]), _p(pages[1]), first, seqs, blocks, nkv, hd, block_size,
+                                              k_cache.shape[0], int(window), _stream())
+        _check(rc, name, f"(hd={hd}, nkv={nkv})")
+        tables = torch.arange(-first * blocks, seqs * blocks, dtype=torch.int32, device=q.device).view(S, blocks)
+        attention_prefill(q, out, pages[0], pages[1], tables, ctx, nh, nkv, hd, scale, window, softcap, sink)
 
 
 # ------------------------------------------------------------------ a step's arrays from lengths

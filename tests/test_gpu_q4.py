@@ -224,7 +224,7 @@ def decode(force=0, merge="cluster"):
 
 @pytest.mark.parametrize("nh,nkv,hd,B", [(2, 2, 32, 16), (8, 1, 64, 16), (4, 2, 96, 8), (6, 1, 128, 16), (3, 3, 160, 4), (18, 2, 192, 16), (4, 2, 224, 5),
                                          (17, 1, 256, 32), (12, 1, 64, 1), (5, 5, 128, 100)])
-@pytest.mark.parametrize("force,merge", [(0, "cluster"), (1, "cluster"), (3, "cluster"), (3, "kernel")])
+@pytest.mark.parametrize("force,merge", [(0, "cluster"), (1, "cluster"), (3, "cluster"), (3, "kernel"), (-1, "kernel")])
 def test_single_rows(nh, nkv, hd, B, force, merge):
     spans = [(0, 1), (1, 1), (30, 1), (31, 1), (32, 1), (127, 1), (128, 1), (129, 1), (300, 1), (399, 1)]
     run_attention(decode(force, merge), spans, nh, nkv, hd, B, "bfloat16", seed=hd, pad=3)
@@ -232,14 +232,22 @@ def test_single_rows(nh, nkv, hd, B, force, merge):
 
 @pytest.mark.parametrize("opts", OPTIONS[1:], ids=str)
 @pytest.mark.parametrize("nh,nkv,hd,B", [(8, 1, 64, 16), (6, 1, 128, 7), (2, 2, 96, 16), (2, 1, 256, 16)])
-@pytest.mark.parametrize("force", [0, 2])
+@pytest.mark.parametrize("force", [0, 2, -1])
 def test_single_rows_with_masks(opts, nh, nkv, hd, B, force):
     run_attention(decode(force), [(0, 1), (6, 1), (7, 1), (45, 1), (200, 1), (385, 1)], nh, nkv, hd, B, "bfloat16", seed=7, pad=1, **dict(opts))
 
 
 def test_more_partitions_than_a_cluster_and_more_pages_than_the_slice():
     run_attention(decode(12), [(1500, 1), (2, 1), (1535, 1)], 2, 1, 64, 16, "bfloat16")
-    run_attention(decode(1), [(600, 1), (1100, 1)], 2, 1, 64, 1, "bfloat16")          # 601 pages of one key each
+    for force in (1, -1):
+        run_attention(decode(force), [(600, 1), (1100, 1)], 2, 1, 64, 1, "bfloat16")      # 601 pages of one key each
+
+
+def test_shares_of_many_requests():
+    """More tiles than blocks at once, shares that begin and end inside requests, empty requests among them."""
+    spans = [(int(700 * abs(math.sin(3 * i))), 1) for i in range(40)]
+    run_attention(decode(-1), spans, 16, 8, 64, 16, "bfloat16", pad=7)
+    run_attention(decode(-1), [(5000, 1), (0, 1), (3, 1)], 12, 4, 128, 16, "bfloat16")
 
 
 def test_large_scores_and_one_key_that_counts():
@@ -268,3 +276,18 @@ def test_a_key_behind_the_context_does_not_count():
             got = run(*bad)
             assert torch.equal(got[1], clean[1])
             assert bool(got[0].isnan().all()) if seen else torch.equal(got[0], clean[0]), (key, which)
+
+
+# ------------------------------------------------------------------------------------------- portions
+
+@pytest.mark.parametrize("opts", OPTIONS, ids=str)
+@pytest.mark.parametrize("nh,nkv,hd,B", [(4, 2, 32, 16), (8, 1, 64, 16), (2, 2, 96, 8), (6, 1, 128, 16), (4, 2, 64, 64), (4, 4, 128, 8), (2, 1, 256, 16),
+                                         (3, 1, 64, 7)])
+def test_portions(opts, nh, nkv, hd, B):
+    spans = [(0, 2), (0, 65), (7, 64), (131, 130), (64, 3), (0, 300)]
+    run_attention(K().attention_prefill_q4, spans, nh, nkv, hd, B, "bfloat16", seed=hd + B, **dict(opts))
+
+
+def test_single_rows_before_portions():
+    for hd, B in ((64, 16), (128, 32)):
+        run_attention(K().paged_attention_q4, [(200, 1), (0, 1), (5, 1), (90, 140), (0, 20)], 8, 2, hd, B, "bfloat16", seed=hd)
