@@ -8,7 +8,6 @@ kernels (used by the benchmark's ``gpu_launches``).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional
 
@@ -568,6 +567,51 @@ def prefill_tcgen05_supported(hd: int, block_size: int, shared_kv: bool = False)
     return bool(_lib().kvcm_attention_tcgen05_supports_kv(int(hd), int(block_size), int(bool(shared_kv))))
 
 
+class _Entry:
+    """One C entry point: argument types set once (p address, l 64-bit, i 32-bit, f float), called with plain numbers on a given
+    device's current stream.  A launch of a small kernel costs more on the host than on the GPU, and most of that was wrapping."""
+    _TYPES = {"p": ctypes.c_void_p, "l": ctypes.c_longlong, "i": ctypes.c_int, "f": ctypes.c_float}
+
+    def __init__(self, symbol: str, types: str) -> None:
+        self.symbol, self.types, self.fn = symbol, types, None
+
+    def __call__(self, device: int, *args) -> int:
+        if self.fn is None:
+            fn = getattr(_lib(), self.symbol)
+            fn.argtypes = [self._TYPES[c] for c in self.types] + [ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+            self.fn = fn
+        if device == torch._C._cuda_getDevice():
+            return self.fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        with torch.cuda.device(device):
+            return self.fn(*args, torch._C._cuda_getCurrentRawStream(device))
+
+
+def _one_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The last check of a call: the device that all its tensors are on, which it launches on whatever the current one is."""
+    d = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != d:
+            raise KernelError(f"{name}: tensors on different devices")
+    if d < 0:
+        _cuda(first)
+    return d
+
+
+def _launched(rc: int, name: str, detail: str, *numbers) -> None:
+    """``_check`` that puts its text together only for a failed launch."""
+    if rc:
+        _check(rc, name, detail.format(*numbers))
+    global _launches
+    _launches += 1
+    if _profile is not None:
+        profile_mark(name)
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
 # ------------------------------------------------------------------ a cache in 4 bits (csrc/cuda/q4.cuh)
 
 def q4_page_bytes(block_size: int, hd: int) -> int:
@@ -576,31 +620,40 @@ def q4_page_bytes(block_size: int, hd: int) -> int:
     return (int(block_size) * (int(hd) // 2 + 4) + 15) // 16 * 16
 
 
-_HERE = contextlib.nullcontext()
-
 
 def _q4_cache(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, nkv: int, hd: int, block_size: int) -> None:
-    _need(hd % 8 == 0 and 8 <= hd <= 256, f"{name}: head sizes are multiples of 8 up to 256")
-    _need(block_size > 0, f"{name}: block_size > 0")
-    want = (nkv, q4_page_bytes(block_size, hd))
+    if hd % 8 or not 8 <= hd <= 256:
+        raise KernelError(f"{name}: head sizes are multiples of 8 up to 256")
+    if block_size <= 0:
+        raise KernelError(f"{name}: block_size > 0")
+    pages = k_cache.shape[0]
+    want = (pages, nkv, q4_page_bytes(block_size, hd))
     for t in (k_cache, v_cache):
-        _need(t.dtype == torch.uint8 and t.dim() == 3 and tuple(t.shape[1:]) == want and t.shape[0] > 0 and t.is_contiguous()
-              and t.data_ptr() % 16 == 0, f"{name}: caches must be contiguous uint8 [pages, {want[0]}, {want[1]}] on 16 bytes")
-    _need(k_cache.shape[0] == v_cache.shape[0], f"{name}: k and v pools differ in their number of pages")
+        if t.dtype != torch.uint8 or t.dim() != 3 or t.shape[1:] != want[1:] or not t.is_contiguous() or t.data_ptr() % 16:
+            raise KernelError(f"{name}: caches must be contiguous uint8 [pages, {want[1]}, {want[2]}] on 16 bytes")
+    if pages == 0 or v_cache.shape[0] != pages:
+        raise KernelError(f"{name}: k and v pools differ in their number of pages")
 
 
 def _q4_rows(name: str, what: str, t: torch.Tensor, rows: int, width: int, dtype: torch.dtype) -> None:
-    _need(t.dim() == 2 and t.shape[0] >= rows and t.shape[1] >= width and t.stride(1) == 1 and t.dtype == dtype,
-          f"{name}: {what} must be {dtype} rows [{rows}, {width}] with dense elements")
-    _need(t.data_ptr() % 16 == 0 and (t.stride(0) * t.element_size()) % 16 == 0, f"{name}: {what} rows must be 16-byte aligned")
+    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < width or t.stride(1) != 1 or t.dtype != dtype:
+        raise KernelError(f"{name}: {what} must be {dtype} rows [{rows}, {width}] with dense elements")
+    if t.data_ptr() % 16 or t.stride(0) * (2 if dtype == torch.bfloat16 else 4) % 16:
+        raise KernelError(f"{name}: {what} rows must be 16-byte aligned")
 
 
-def _on_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]):
-    """The last check of a call and the device it launches on: that of its tensors, whatever the current one is."""
-    for t in others:
-        _need(t is None or t.device == first.device, f"{name}: tensors on different devices")
-    _cuda(first)
-    return _HERE if first.device.index == torch.cuda.current_device() else torch.cuda.device(first.device)
+def _ints(name: str, what: str, t: torch.Tensor, least: int) -> None:
+    if t.dtype != _I32 or not t.is_contiguous() or t.numel() < least:
+        raise KernelError(f"{name}: {what} must be contiguous int32 of at least {least}")
+
+
+_STORE_Q4 = {s: _Entry("kvcm_rope_cache_q4_" + s, "plpiippppliiiiii") for s in ("f32", "bf16")}
+_READ_Q4 = {s: _Entry("kvcm_read_cache_q4_" + s, "pppppll" + "iiiii") for s in ("f32", "bf16")}
+_PLAIN_Q4 = {s: _Entry("kvcm_attention_plain_q4_" + s, "plplpp" + "ipipp" + "iiiii" + "fifp") for s in ("f32", "bf16")}
+_UNPACK_Q4 = _Entry("kvcm_unpack_pages_q4_bf16", "pppi" + "pppp" + "iiiiiiii")
+_PREFILL_Q4 = _Entry("kvcm_attention_prefill_q4_bf16", "plipl" + "ppipi" + "ppppp" + "iiiii" + "fifp")
+_DECODE_Q4 = _Entry("kvcm_attention_decode_q4_bf16", "plplpp" + "ipip" + "iiiii" + "fiiiipifp")
+_STEP_TABLES = _Entry("kvcm_step_tables", "pppipip" + "ppppppppp" + "iiiii")
 
 
 def rope_cache_q4(qkv: torch.Tensor, table: Optional[torch.Tensor], interleaved: bool, slot_mapping: torch.Tensor,
@@ -613,24 +666,23 @@ def rope_cache_q4(qkv: torch.Tensor, table: Optional[torch.Tensor], interleaved:
     rotary_dim is a multiple of 16 in rotate-half pairs, of 2 in interleaved ones.  Rows with a slot below zero (or beyond the
     pool) are written nowhere.  A head with an element that is not finite reads back as not-a-number.  No two rows may share a slot."""
     name = "rope_cache_q4"
-    T = qkv.shape[0]
-    suffix = _suffix(qkv)
+    T, suffix = qkv.shape[0], _suffix(qkv)
     _q4_cache(name, k_cache, v_cache, nkv, hd, block_size)
     _q4_rows(name, "qkv", qkv, T, (nh + 2 * nkv) * hd, qkv.dtype)
     _q4_rows(name, "q_out", q_out, T, nh * hd, qkv.dtype)
-    _need(slot_mapping.dtype == _I32 and slot_mapping.is_contiguous() and slot_mapping.numel() >= T, f"{name}: slot_mapping int32 [T]")
+    _ints(name, "slot_mapping", slot_mapping, T)
     rotary = 0
     if table is not None:
         rotary = table.shape[-1]
-        _need(table.dtype == torch.float32 and table.dim() == 2 and table.shape[0] >= T and table.is_contiguous()
-              and table.data_ptr() % 16 == 0, f"{name}: table float32 [T, rotary_dim]")
-        _need(0 < rotary <= hd and rotary % (2 if interleaved else 16) == 0,
-              f"{name}: rotary_dim {rotary} (a multiple of 16 in rotate-half pairs, of 2 in interleaved ones, at most {hd})")
-    with _on_device(name, qkv, table, slot_mapping, k_cache, v_cache, q_out):
-        rc = getattr(_lib(), "kvcm_rope_cache_q4_" + suffix)(
-            _p(qkv), ctypes.c_longlong(qkv.stride(0)), _p(table), rotary, int(interleaved), _p(slot_mapping), _p(k_cache), _p(v_cache),
-            _p(q_out), ctypes.c_longlong(q_out.stride(0)), T, nh, nkv, hd, block_size, k_cache.shape[0], _stream())
-    _check(rc, name, f"(hd={hd}, rotary_dim={rotary})")
+        if table.dtype != torch.float32 or table.dim() != 2 or table.shape[0] < T or not table.is_contiguous() or table.data_ptr() % 16:
+            raise KernelError(f"{name}: table float32 [T, rotary_dim]")
+        if not 0 < rotary <= hd or rotary % (2 if interleaved else 16):
+            raise KernelError(f"{name}: rotary_dim {rotary} (a multiple of 16 in rotate-half pairs, of 2 in interleaved ones, at most {hd})")
+    device = _one_device(name, qkv, table, slot_mapping, k_cache, v_cache, q_out)
+    rc = _STORE_Q4[suffix](device, qkv.data_ptr(), qkv.stride(0), _at(table), rotary, int(interleaved), slot_mapping.data_ptr(),
+                           k_cache.data_ptr(), v_cache.data_ptr(), q_out.data_ptr(), q_out.stride(0), T, nh, nkv, hd, block_size,
+                           k_cache.shape[0])
+    _launched(rc, name, "(hd={}, rotary_dim={})", hd, rotary)
 
 
 def read_cache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor, k_rows: torch.Tensor,
@@ -638,31 +690,34 @@ def read_cache_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: to
     """The values that the given slots of a cache in 4 bits stand for, as rows [T, nkv hd] of bfloat16 or float32 (for rows that move
     to another cache, or to look at them).  Rows with a slot below zero (or beyond the pool) are left as they were."""
     name = "read_cache_q4"
-    T = k_rows.shape[0]
-    suffix = _suffix(k_rows)
+    T, suffix = k_rows.shape[0], _suffix(k_rows)
     _q4_cache(name, k_cache, v_cache, nkv, hd, block_size)
     _q4_rows(name, "k_rows", k_rows, T, nkv * hd, k_rows.dtype)
     _q4_rows(name, "v_rows", v_rows, T, nkv * hd, k_rows.dtype)
-    _need(slot_mapping.dtype == _I32 and slot_mapping.is_contiguous() and slot_mapping.numel() >= T, f"{name}: slot_mapping int32 [T]")
-    with _on_device(name, k_cache, v_cache, slot_mapping, k_rows, v_rows):
-        rc = getattr(_lib(), "kvcm_read_cache_q4_" + suffix)(
-            _p(k_cache), _p(v_cache), _p(slot_mapping), _p(k_rows), _p(v_rows), ctypes.c_longlong(k_rows.stride(0)),
-            ctypes.c_longlong(v_rows.stride(0)), T, nkv, hd, block_size, k_cache.shape[0], _stream())
-    _check(rc, name, f"(hd={hd})")
+    _ints(name, "slot_mapping", slot_mapping, T)
+    device = _one_device(name, k_cache, v_cache, slot_mapping, k_rows, v_rows)
+    rc = _READ_Q4[suffix](device, k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), k_rows.data_ptr(), v_rows.data_ptr(),
+                          k_rows.stride(0), v_rows.stride(0), T, nkv, hd, block_size, k_cache.shape[0])
+    _launched(rc, name, "(hd={})", hd)
 
 
-def _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink, *ints) -> None:
-    _need(nkv > 0 and nh > 0 and nh % nkv == 0, f"{name}: {nh} query heads are not a multiple of {nkv} KV heads")
-    _need(window >= 0 and softcap >= 0.0, f"{name}: window and softcap must not be negative")
+def _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink) -> None:
+    if nkv <= 0 or nh <= 0 or nh % nkv:
+        raise KernelError(f"{name}: {nh} query heads are not a multiple of {nkv} KV heads")
+    if window < 0 or softcap < 0.0:
+        raise KernelError(f"{name}: window and softcap must not be negative")
     _q4_cache(name, k_cache, v_cache, nkv, hd, block_size)
-    _need(q.dim() == 2 and out.dim() == 2 and q.dtype == out.dtype and q.dtype in _SUFFIX, f"{name}: q and out bfloat16 or float32 rows")
-    _need(out.shape[0] == q.shape[0] and q.shape[1] >= nh * hd and out.shape[1] >= nh * hd, f"{name}: q and out rows of {nh} heads of {hd}")
-    _need(q.stride(1) == 1 and out.stride(1) == 1, f"{name}: rows must be dense")
-    _need(block_tables.dtype == _I32 and block_tables.is_contiguous() and block_tables.dim() == 2,
-          f"{name}: block_tables int32 [S, max_blocks]")
-    _need(sink is None or (sink.dtype == torch.float32 and sink.is_contiguous() and sink.numel() == nh), f"{name}: sink float32 [heads]")
-    for t in ints:
-        _need(t is None or (t.dtype == _I32 and t.is_contiguous()), f"{name}: the step's arrays are contiguous int32")
+    if q.dtype != out.dtype or q.dtype not in _SUFFIX:
+        raise KernelError(f"{name}: q and out must be bfloat16 or float32 rows of one type")
+    width = nh * hd
+    if q.dim() != 2 or out.dim() != 2 or out.shape[0] != q.shape[0] or q.shape[1] < width or out.shape[1] < width:
+        raise KernelError(f"{name}: q and out must be rows of {nh} heads of {hd}")
+    if q.stride(1) != 1 or out.stride(1) != 1:
+        raise KernelError(f"{name}: rows must be dense")
+    if block_tables.dtype != _I32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+        raise KernelError(f"{name}: block_tables must be contiguous int32 [S, max_blocks]")
+    if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nh or not sink.is_contiguous()):
+        raise KernelError(f"{name}: sink must be float32 [heads]")
 
 
 def attention_plain_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -671,28 +726,29 @@ def attention_plain_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor
     """``attention_plain`` over a cache in 4 bits: one row a block, float32 arithmetic, q and out in bfloat16 or float32."""
     name = "attention_plain_q4"
     T = out.shape[0]
-    _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink, row_seq, positions)
-    _need(row_seq.numel() >= T and positions.numel() >= T, f"{name}: row_seq/positions int32 [T]")
-    with _on_device(name, q, out, k_cache, v_cache, block_tables, row_seq, positions, sink):
-        rc = getattr(_lib(), "kvcm_attention_plain_q4_" + _suffix(q))(
-            _p(q), ctypes.c_longlong(q.stride(0)), _p(out), ctypes.c_longlong(out.stride(0)), _p(k_cache), _p(v_cache), k_cache.shape[0],
-            _p(block_tables), block_tables.shape[1], _p(row_seq), _p(positions), T, nh, nkv, hd, block_size, ctypes.c_float(scale),
-            int(window), ctypes.c_float(softcap), _p(sink), _stream())
-    _check(rc, name, f"(hd={hd}, nh={nh}, nkv={nkv})")
+    _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink)
+    _ints(name, "row_seq", row_seq, T)
+    _ints(name, "positions", positions, T)
+    device = _one_device(name, q, out, k_cache, v_cache, block_tables, row_seq, positions, sink)
+    rc = _PLAIN_Q4[_SUFFIX[q.dtype]](
+        device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
+        block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), T, nh, nkv, hd, block_size, scale, window,
+        softcap, _at(sink))
+    _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
 
 
 Q4_PART_KEYS = 128          # four warps with a step of 32 keys each
 
 
-def decode_partitions_q4(seqs: int, nh: int, nkv: int, hd: int, max_ctx: int, device, force_parts: int = 0):
-    """How ``attention_decode_q4`` splits the context: (keys per partition, number of partitions)."""
-    max_ctx = max(int(max_ctx), 1)
+def decode_partitions_q4(seqs: int, nh: int, nkv: int, hd: int, max_ctx: int, device: int, force_parts: int = 0):
+    """How ``attention_decode_q4`` splits the context: (keys per partition, number of partitions), no partitions for equal shares."""
+    max_ctx = max(max_ctx, 1)
     blocks = max(1, seqs * nkv * ((nh // nkv + 7) // 8))
     most = (max_ctx + Q4_PART_KEYS - 1) // Q4_PART_KEYS
     if force_parts < 0:
         return Q4_PART_KEYS, 0
     if force_parts > 0:
-        parts = min(int(force_parts), most)
+        parts = min(force_parts, most)
     else:
         parts = max(1, min(_q4_resident_blocks(hd, device) // blocks, most))
         if parts > CLUSTER_PARTS:
@@ -701,12 +757,14 @@ def decode_partitions_q4(seqs: int, nh: int, nkv: int, hd: int, max_ctx: int, de
     return size, (max_ctx + size - 1) // size
 
 
-def _q4_resident_blocks(hd: int, device) -> int:
-    key = ("q4", int(hd), device.index)
-    if key not in _RESIDENT:
-        n = int(_lib().kvcm_attention_decode_q4_blocks_per_sm(int(hd)))
-        _RESIDENT[key] = max(n, 1) * sm_count(device)
-    return _RESIDENT[key]
+def _q4_resident_blocks(hd: int, device: int) -> int:
+    key = ("q4", hd, device)
+    n = _RESIDENT.get(key)
+    if n is None:
+        with torch.cuda.device(device):
+            n = max(int(_lib().kvcm_attention_decode_q4_blocks_per_sm(int(hd))), 1) * sm_count(torch.device("cuda", device))
+        _RESIDENT[key] = n
+    return n
 
 
 def attention_q4_supported(hd: int, dtype: torch.dtype) -> bool:
@@ -721,33 +779,33 @@ def attention_decode_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tenso
     ``ctx.seq_ctx_len`` says how many keys each sees (0: the row is zero), ``ctx.max_decode_ctx`` is at least the longest.
     ``window``: the last ``window`` keys only; ``softcap``, ``sink`` as in ``attention_plain``."""
     name = "attention_decode_q4"
-    S = q.shape[0]
-    _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink, ctx.seq_ctx_len)
-    _need(attention_q4_supported(hd, q.dtype), f"{name}: bfloat16 rows, heads of 32 to 256 elements in steps of 32")
-    _need(q.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0, f"{name}: q rows must be 16-byte aligned")
-    _need(out.data_ptr() % 8 == 0 and out.stride(0) % 4 == 0, f"{name}: out rows must be 8-byte aligned")
-    _need(block_tables.shape[0] >= S and ctx.seq_ctx_len.numel() >= S, f"{name}: an entry and a page table for each of {S} rows")
-    _need(ctx.max_decode_ctx <= block_tables.shape[1] * block_size or window > 0, f"{name}: max_decode_ctx exceeds the page tables")
-    with _on_device(name, q, out, k_cache, v_cache, block_tables, ctx.seq_ctx_len, sink):
-        if S == 0:
-            return
-        span = ctx.max_decode_ctx if window <= 0 else min(ctx.max_decode_ctx, int(window) + 31)
-        size, parts = decode_partitions_q4(S, nh, nkv, hd, span, q.device, int(ctx.options.get("attn_parts", 0)))
-        in_cluster = 1 < parts <= CLUSTER_PARTS and ctx.options.get("attn_merge", "cluster") == "cluster"
-        scratch, shares = None, 0
-        if parts == 0:
-            shares = _q4_resident_blocks(hd, q.device)
-            scratch = torch.empty(shares * 16 * (hd + 2) + S * nkv * ((nh // nkv + 7) // 8) * 2, dtype=torch.float32, device=q.device)
-        elif parts > 1 and not in_cluster:
-            scratch = torch.empty(S * nh * parts * (hd + 2), dtype=torch.float32, device=q.device)
-        rc = _lib().kvcm_attention_decode_q4_bf16(
-            _p(q), ctypes.c_longlong(q.stride(0)), _p(out), ctypes.c_longlong(out.stride(0)), _p(k_cache), _p(v_cache), k_cache.shape[0],
-            _p(block_tables), block_tables.shape[1], _p(ctx.seq_ctx_len), S, nh, nkv, hd, block_size, ctypes.c_float(scale), int(window),
-            size, parts, shares, _p(scratch), int(in_cluster), ctypes.c_float(softcap), _p(sink), _stream())
-    _check(rc, name, f"(hd={hd}, nh={nh}, nkv={nkv})")
-    if parts != 1 and not in_cluster:
-        global _launches
-        _launches += 1                      # the merge kernel
+    S, lengths = q.shape[0], ctx.seq_ctx_len
+    _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink)
+    _ints(name, "seq_ctx_len", lengths, S)
+    if not attention_q4_supported(hd, q.dtype):
+        raise KernelError(f"{name}: bfloat16 rows, heads of 32 to 256 elements in steps of 32")
+    if q.data_ptr() % 16 or q.stride(0) % 8 or out.data_ptr() % 8 or out.stride(0) % 4:
+        raise KernelError(f"{name}: q rows must be 16-byte aligned, out rows 8-byte aligned")
+    if block_tables.shape[0] < S:
+        raise KernelError(f"{name}: a page table for each of {S} rows")
+    device = _one_device(name, q, out, k_cache, v_cache, block_tables, lengths, sink)
+    if S == 0:
+        return
+    span = ctx.max_decode_ctx if window <= 0 else min(ctx.max_decode_ctx, window + 31)
+    size, parts = decode_partitions_q4(S, nh, nkv, hd, span, device, ctx.options.get("attn_parts", 0))
+    in_cluster = 1 < parts <= CLUSTER_PARTS and ctx.options.get("attn_merge", "cluster") == "cluster"
+    scratch, shares = None, 0
+    if parts == 0:
+        shares = _q4_resident_blocks(hd, device)
+        scratch = torch.empty(shares * 16 * (hd + 2) + S * nkv * ((nh // nkv + 7) // 8) * 2, dtype=torch.float32, device=q.device)
+    elif parts > 1 and not in_cluster:
+        scratch = torch.empty(S * nh * parts * (hd + 2), dtype=torch.float32, device=q.device)
+    rc = _DECODE_Q4(device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
+                    block_tables.data_ptr(), block_tables.shape[1], lengths.data_ptr(), S, nh, nkv, hd, block_size, scale, window,
+                    size, parts, shares, _at(scratch), int(in_cluster), softcap, _at(sink))
+    _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
+    if scratch is not None:
+        add_launches(1)                     # the merge kernel
 
 
 def paged_attention_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -762,7 +820,9 @@ def paged_attention_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor
         return
     nd = ctx.decode_seqs
     if nd > 0:
-        attention_decode_q4(q[:nd], out[:nd], k_cache, v_cache, block_tables, ctx, nh, nkv, hd, block_size, scale, window, softcap, sink)
+        all_single = nd == q.shape[0]
+        attention_decode_q4(q if all_single else q[:nd], out if all_single else out[:nd], k_cache, v_cache, block_tables, ctx, nh, nkv, hd,
+                            block_size, scale, window, softcap, sink)
     if ctx.rows > nd:
         attention_prefill_q4(q, out, k_cache, v_cache, block_tables, ctx, nh, nkv, hd, block_size, scale, window, softcap, sink)
 
@@ -771,28 +831,43 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                          ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
                          sink: Optional[torch.Tensor] = None) -> None:
     """Rows of portions longer than one token over a cache in 4 bits; q and out are the step's full bfloat16 row arrays, ``ctx`` has
-    the step's arrays with tiles of 64 rows.  The pages that the portions see are first laid out in bfloat16 (in scratch of the
-    call) and then read by ``attention_prefill``."""
+    the step's arrays with tiles of 64 rows (tiles of request -1 are none).  Heads of 64 and 128 elements: one kernel that unpacks
+    pages beside the products.  Other heads, or ``ctx.options['attn_prefill'] == 'unpack'``: the pages that the portions see are
+    laid out in bfloat16 (in scratch of the call) and read by ``attention_prefill``."""
     name = "attention_prefill_q4"
-    _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink, ctx.seq_q_start,
-                  ctx.seq_q_len, ctx.seq_ctx_len, ctx.tile_seq, ctx.tile_q0)
-    _need(attention_q4_supported(hd, q.dtype), f"{name}: bfloat16 rows, heads of 32 to 256 elements in steps of 32")
-    _need(q.data_ptr() % 16 == 0 and q.stride(0) % 8 == 0, f"{name}: q rows must be 16-byte aligned")
-    _need(out.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0, f"{name}: out rows must be 16-byte aligned")
-    _need(ctx.tile_rows == 64, f"{name}: the batch must be tiled in 64 query rows")
+    _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink)
     S = ctx.seq_ctx_len.numel()
-    _need(block_tables.shape[0] >= S, f"{name}: a page table for each of {S} entries")
-    with _on_device(name, q, out, k_cache, v_cache, block_tables, sink, ctx.seq_q_start, ctx.seq_q_len, ctx.seq_ctx_len, ctx.tile_seq, ctx.tile_q0):
-        first, seqs = ctx.decode_seqs, S - ctx.decode_seqs
-        if seqs <= 0 or ctx.prefill_tiles == 0:
-            return
-        blocks = min(block_tables.shape[1], (ctx.max_ctx + block_size - 1) // block_size)
-        pages = torch.empty((2, seqs * blocks, nkv, block_size, hd), dtype=torch.bfloat16, device=q.device)
-        rc = _lib().kvcm_unpack_pages_q4_bf16(_p(k_cache), _p(v_cache), _p(block_tables), block_tables.shape[1], _p(ctx.seq_q_len),
-                                              _p(ctx.seq_ctx_len), _p(pages[0]), _p(pages[1]), first, seqs, blocks, nkv, hd, block_size,
-                                              k_cache.shape[0], int(window), _stream())
-        _check(rc, name, f"(hd={hd}, nkv={nkv})")
-        tables = torch.arange(-first * blocks, seqs * blocks, dtype=torch.int32, device=q.device).view(S, blocks)
+    for what in ("seq_q_start", "seq_q_len", "seq_ctx_len"):
+        _ints(name, what, getattr(ctx, what), S)
+    _ints(name, "tile_seq", ctx.tile_seq, ctx.prefill_tiles)
+    _ints(name, "tile_q0", ctx.tile_q0, ctx.prefill_tiles)
+    if not attention_q4_supported(hd, q.dtype):
+        raise KernelError(f"{name}: bfloat16 rows, heads of 32 to 256 elements in steps of 32")
+    if q.data_ptr() % 16 or q.stride(0) % 8 or out.data_ptr() % 16 or out.stride(0) % 8:
+        raise KernelError(f"{name}: q and out rows must be 16-byte aligned")
+    if ctx.tile_rows != 64:
+        raise KernelError(f"{name}: the batch must be tiled in 64 query rows")
+    if block_tables.shape[0] < S:
+        raise KernelError(f"{name}: a page table for each of {S} entries")
+    device = _one_device(name, q, out, k_cache, v_cache, block_tables, sink, ctx.seq_q_start, ctx.seq_q_len, ctx.seq_ctx_len, ctx.tile_seq, ctx.tile_q0)
+    first, seqs = ctx.decode_seqs, S - ctx.decode_seqs
+    if seqs <= 0 or ctx.prefill_tiles == 0:
+        return
+    if hd in (64, 128) and ctx.options.get("attn_prefill", "auto") != "unpack":
+        rc = _PREFILL_Q4(device, q.data_ptr(), q.stride(0), q.shape[0], out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+                         k_cache.shape[0], block_tables.data_ptr(), block_tables.shape[1], ctx.tile_seq.data_ptr(), ctx.tile_q0.data_ptr(),
+                         ctx.seq_q_start.data_ptr(), ctx.seq_q_len.data_ptr(), ctx.seq_ctx_len.data_ptr(), ctx.prefill_tiles, nh, nkv, hd,
+                         block_size, scale, window, softcap, _at(sink))
+        _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
+        return
+    blocks = min(block_tables.shape[1], (ctx.max_ctx + block_size - 1) // block_size)
+    pages = torch.empty((2, seqs * blocks, nkv, block_size, hd), dtype=torch.bfloat16, device=q.device)
+    rc = _UNPACK_Q4(device, k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], ctx.seq_q_len.data_ptr(),
+                    ctx.seq_ctx_len.data_ptr(), pages[0].data_ptr(), pages[1].data_ptr(), first, seqs, blocks, nkv, hd, block_size,
+                    k_cache.shape[0], window)
+    _launched(rc, name, "(hd={}, nkv={})", hd, nkv)
+    tables = torch.arange(-first * blocks, seqs * blocks, dtype=torch.int32, device=q.device).view(S, blocks)
+    with torch.cuda.device(device):
         attention_prefill(q, out, pages[0], pages[1], tables, ctx, nh, nkv, hd, scale, window, softcap, sink)
 
 
@@ -821,25 +896,33 @@ def step_tables(seq_start: torch.Tensor, seq_q_len: torch.Tensor, block_tables: 
     and lengths are then as before and every row is one behind the last.  The host reads it when it likes; nothing waits here.
     The requests stay in the caller's order: entries of one row come first where attention takes them as such."""
     name = "step_tables"
-    outs = (seq_q_start, seq_ctx_len, positions, row_seq, slot_mapping, free_left, status, tile_seq, tile_q0)
-    for t in (seq_start, seq_q_len, block_tables, free_pages, free_count) + outs:
-        _need(t is None or (t.dtype == _I32 and t.is_contiguous()), f"{name}: contiguous int32 arrays")
     S, T = seq_q_len.numel(), positions.numel()
-    _need(0 < S <= 8192, f"{name}: 1 to 8192 requests, not {S}")
-    _need(block_size > 0 and tile_rows > 0, f"{name}: block_size and tile_rows must be positive")
-    _need(seq_start.numel() == S and seq_q_start.numel() == S and seq_ctx_len.numel() == S, f"{name}: per-request arrays of {S}")
-    _need(block_tables.dim() == 2 and block_tables.shape[0] == S and block_tables.shape[1] > 0, f"{name}: block_tables [{S}, max_blocks]")
-    _need(row_seq.numel() == T and slot_mapping.numel() == T, f"{name}: per-row arrays of {T}")
-    _need((tile_seq is None) == (tile_q0 is None) and (tile_seq is None or tile_seq.numel() == tile_q0.numel()),
-          f"{name}: tile_seq and tile_q0 go together")
-    _need(free_count.numel() == 1 and free_left.numel() == 1 and status.numel() >= 4, f"{name}: free_count [1], free_left [1], status [4]")
+    if not 0 < S <= 8192:
+        raise KernelError(f"{name}: 1 to 8192 requests, not {S}")
+    if block_size <= 0 or tile_rows <= 0:
+        raise KernelError(f"{name}: block_size and tile_rows must be positive")
+    for t in (seq_start, seq_q_len, block_tables, free_pages, free_count, seq_q_start, seq_ctx_len, positions, row_seq, slot_mapping, free_left,
+              status, tile_seq, tile_q0):
+        if t is not None and (t.dtype != _I32 or not t.is_contiguous()):
+            raise KernelError(f"{name}: contiguous int32 arrays")
+    if seq_start.numel() != S or seq_q_start.numel() != S or seq_ctx_len.numel() != S:
+        raise KernelError(f"{name}: per-request arrays of {S}")
+    if block_tables.dim() != 2 or block_tables.shape[0] != S or block_tables.shape[1] == 0:
+        raise KernelError(f"{name}: block_tables [{S}, max_blocks]")
+    if row_seq.numel() != T or slot_mapping.numel() != T:
+        raise KernelError(f"{name}: per-row arrays of {T}")
+    if (tile_seq is None) != (tile_q0 is None) or (tile_seq is not None and tile_seq.numel() != tile_q0.numel()):
+        raise KernelError(f"{name}: tile_seq and tile_q0 go together")
+    if free_count.numel() != 1 or free_left.numel() != 1 or status.numel() < 4:
+        raise KernelError(f"{name}: free_count [1], free_left [1], status [4]")
     tiles = 0 if tile_seq is None else tile_seq.numel()
-    with _on_device(name, seq_start, seq_q_len, block_tables, free_pages, free_count, *outs):
-        rc = _lib().kvcm_step_tables(
-            _p(seq_start), _p(seq_q_len), _p(block_tables), block_tables.shape[1], _p(free_pages), free_pages.numel(), _p(free_count),
-            _p(seq_q_start), _p(seq_ctx_len), _p(positions), _p(row_seq), _p(slot_mapping), _p(tile_seq), _p(tile_q0), _p(free_left),
-            _p(status), S, T, tiles, int(block_size), int(tile_rows), _stream())
-    _check(rc, name, f"({S} requests, {T} rows, {tiles} tiles)")
+    device = _one_device(name, seq_start, seq_q_len, block_tables, free_pages, free_count, seq_q_start, seq_ctx_len, positions, row_seq,
+                         slot_mapping, free_left, status, tile_seq, tile_q0)
+    rc = _STEP_TABLES(device, seq_start.data_ptr(), seq_q_len.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], free_pages.data_ptr(),
+                      free_pages.numel(), free_count.data_ptr(), seq_q_start.data_ptr(), seq_ctx_len.data_ptr(), positions.data_ptr(),
+                      row_seq.data_ptr(), slot_mapping.data_ptr(), _at(tile_seq), _at(tile_q0), free_left.data_ptr(), status.data_ptr(),
+                      S, T, tiles, block_size, tile_rows)
+    _launched(rc, name, "({} requests, {} rows, {} tiles)", S, T, tiles)
 
 
 def raise_on_step_tables(status) -> None:

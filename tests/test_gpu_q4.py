@@ -283,9 +283,33 @@ def test_a_key_behind_the_context_does_not_count():
 @pytest.mark.parametrize("opts", OPTIONS, ids=str)
 @pytest.mark.parametrize("nh,nkv,hd,B", [(4, 2, 32, 16), (8, 1, 64, 16), (2, 2, 96, 8), (6, 1, 128, 16), (4, 2, 64, 64), (4, 4, 128, 8), (2, 1, 256, 16),
                                          (3, 1, 64, 7)])
-def test_portions(opts, nh, nkv, hd, B):
+@pytest.mark.parametrize("how", ["auto", "unpack"])
+def test_portions(opts, nh, nkv, hd, B, how):
+    if how == "unpack" and hd not in (64, 128):
+        pytest.skip("the only way for this head size")
+
+    def call(q, out, kc, vc, tables, ctx, *args, **kw):
+        ctx.options = {"attn_prefill": how}
+        K().attention_prefill_q4(q, out, kc, vc, tables, ctx, *args, **kw)
     spans = [(0, 2), (0, 65), (7, 64), (131, 130), (64, 3), (0, 300)]
-    run_attention(K().attention_prefill_q4, spans, nh, nkv, hd, B, "bfloat16", seed=hd + B, **dict(opts))
+    run_attention(call, spans, nh, nkv, hd, B, "bfloat16", seed=hd + B, **dict(opts))
+
+
+@pytest.mark.parametrize("spans", [[(0, 127)], [(0, 128)], [(1, 129)], [(63, 255)], [(64, 256)], [(0, 257)], [(700, 513)], [(2, 2), (900, 30), (0, 600)]],
+                         ids=str)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_groups_and_tiles_of_portions(spans, hd):
+    run_attention(K().attention_prefill_q4, spans, 2, 1, hd, 16, "bfloat16", seed=len(spans))
+
+
+def test_portions_with_large_scores_and_tiles_that_are_none():
+    def call(q, out, kc, vc, tables, ctx, *args, **kw):
+        none = torch.full((3,), -1, dtype=torch.int32, device=DEV)
+        ctx.tile_seq, ctx.tile_q0 = torch.cat((ctx.tile_seq, none)), torch.cat((ctx.tile_q0, none))
+        ctx.prefill_tiles += 3
+        K().attention_prefill_q4(q, out, kc, vc, tables, ctx, *args, **kw)
+    for hd in (64, 128):
+        run_attention(call, [(300, 90), (0, 200)], 4, 2, hd, 16, "bfloat16", q_scale=40.0)
 
 
 def test_single_rows_before_portions():
