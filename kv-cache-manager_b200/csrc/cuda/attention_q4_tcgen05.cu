@@ -2,20 +2,25 @@
 // head_dim 64 or 128.
 //
 // One block per (256 query rows of a request, query head), as two groups of 128 rows that share every tile of keys and values.  Per
-// tile of 64 keys and group:
-//     S = Q C^T   C = 128 + the key's codes (bfloat16, exact), accumulator in tensor memory, two buffers
-//     softmax     one thread a row:  x = scale_k S + (zero_k - 128 scale_k) sum(q),  p = 2^(x - m),  P = bfloat16(p scale_v)
-//     O += P W    W = the value's codes - 8 (exact), MN-major operand, O in tensor memory for the whole block
-// and at the end  o = (O + sum p (zero_v + 8 scale_v)) / sum p.  Keys and values are never rounded: what is rounded is P, to bfloat16.
-// Reference maximum renewed only when it is 2^8 behind, as in attention_tcgen05.cu.
+// tile of 128 keys and group:
+//     S = Q C^T   C = 128 + the key's codes (bfloat16, exact), accumulator in tensor memory
+//     softmax     one thread a row:  x = scale S + (zero - 128 scale) sum(q),  P = bfloat16(2^(x - m))
+//     O += P V    V = bfloat16(zero + scale code), MN-major operand, O in tensor memory for the whole block
+// A key is never rounded: its scale and zero meet the score, which costs two packed multiply-adds for two scores.  A value is, once, to
+// bfloat16, as P is: applied to P instead, its scale and zero were three more instructions for two scores in the loop that
+// bounds the kernel (four portions behind long prefixes: 1,270 us against DONE_US).
+// A row takes its tile relative to the maximum that it knew before, without looking for the tile's own: where the tile's sum comes
+// out above 2^12 (or the row has seen nothing yet) the tile's maximum is found, sums and O are rescaled, and the tile is taken
+// again, S being still there.  The largest probability therefore lies between 1 and 2^12 times 1, which float32 sums and the
+// exponents of bfloat16 do not mind.
 //
-// Roles (12 warps): 0-3 and 4-7 softmax and output of the two groups; 8-10 turn pages into operands: a thread takes 16 bytes of
-// codes (32 elements of a key), writes four 16-byte pieces of a 128-byte swizzled row, and asks for the next tile's codes before
-// it waits; one thread of warp 11 brings Q and issues the products, S one tile ahead of O.
-// Two groups to a tile because unpacking is then paid once for 256 rows, and because the softmax of one covers the products of
-// the other: the exponentials of a tile and a group (128 x 64 at 16 a cycle) take as long as its two products at head_dim 128.
-// Scales and zeros lie in a ring of five tiles beside the operands: a thread of the softmax may still read those of tile n while
-// tile n + 4 is unpacked, but not n + 5 (its products ask for S_(n+3), which wants every row's S_(n+1) read).
+// Roles (16 warps, 128 registers a thread): 0-3 and 4-7 softmax and output of the two groups; 8-11 turn keys into operands and
+// pairs into scales, 12-14 values; one thread of warp 15 brings Q and issues the products, S of a group's next tile before O += P W
+// of this one, the groups in turn, so that the products of one run under the softmax of the other.
+// What bounds it: at head_dim 128 a tile's exponentials (256 x 128 at 16 a cycle) and its products each take 2,048 cycles, and the
+// handshakes between roles, some 150 cycles each, come on top where they are not hidden: tiles of 64 keys, with twice as many
+// of them, took 4,100 cycles for half the work.
+// A thread of warps 8-14 copies what it unpacks itself (cp.async into shared memory, a tile ahead) and so waits for nobody else's.
 // Masks: key <= position, optional window.  Every wait is bounded; one that runs out sets the error word of the tcgen05 attention
 // family (codes 17 and up) and ends the block.
 #include "pdl.cuh"
@@ -26,16 +31,13 @@ extern "C" const int* kvcm_attention_tcgen05_error_address(void);
 
 namespace kvcm {
 
-constexpr int kQfThreads = 384;                   // (twelve warps, three to a scheduler: 168 registers a thread)
-constexpr int kQfUnpackWarps = 3;
+constexpr int kQfThreads = 512;
 constexpr int kQfGroupRows = 128, kQfRows = 256;
-constexpr int kQfKeys = 64;
-constexpr int kQfStages = 2;                       // tiles of K operands, and of V operands
-constexpr int kQfScaleRing = 5;
-constexpr int kQfTile = 128 * 128;                 // [128 rows][64 bf16]
-constexpr int kQfBlock = kQfKeys * 128;            // [64 keys][64 bf16]
-constexpr float kQfRescaleStep = 8.f;              // in log2 units
-// tensor memory: S of group g in buffer b at column (2 g + b) * 64; O of group g at 256 + g * head_dim
+constexpr int kQfKeys = 128;
+constexpr int kQfKeyWarps = 4, kQfValueWarps = 3;
+constexpr int kQfTile = 128 * 128;                 // [128 rows][64 bf16]: also a 64-wide block of a tile of keys or values
+constexpr float kQfMost = 4096.f;                  // a row's sum of one tile from which its maximum is renewed
+// tensor memory: S of group g at column g * 128; O of group g at 256 + g * head_dim
 
 struct PrefillQ4Params {
   bf16* out; long long out_stride;
@@ -59,28 +61,17 @@ __device__ __forceinline__ float qf_tanh(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(qf_exp2(x * 2.8853900817779268f) + 1.f));
   return fmaf(-2.f, r, 1.f);
 }
-__device__ __forceinline__ float qf_max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
+__device__ __forceinline__ void qf_copy16(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(tc5::s32(smem)), "l"(gmem) : "memory");
 }
-// 128 + code -> code - 8, two at a time.
-__device__ __forceinline__ uint32_t qf_centred(uint32_t v) {
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(v), "r"(0x43084308u));
-  return r;
+__device__ __forceinline__ void qf_copy4(void* smem, const void* gmem) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(tc5::s32(smem)), "l"(gmem) : "memory");
 }
 // a * b + c of two floats at once
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
   asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}\n"
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}\n"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -90,28 +81,136 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-struct QfScales { float2 k_scale, k_zero, v_scale, v_zero; };      // of two neighbouring keys
+struct QfScales { float2 scale, zero; };           // of two neighbouring keys, as they meet a score
+
+// The scores of two keys, less m, from their products.
+template <bool CAP>
+__device__ __forceinline__ float2 qf_scores(uint32_t s0, uint32_t s1, const QfScales* sc, float2 qs2, float2 less_m, float cap_pre, float scale_log2) {
+  const float4 f = *reinterpret_cast<const float4*>(sc);
+  float2 t = fma2(make_float2(__uint_as_float(s0), __uint_as_float(s1)), make_float2(f.x, f.y), fma2(make_float2(f.z, f.w), qs2, CAP ? make_float2(0.f, 0.f) : less_m));
+  if constexpr (CAP) {
+    t.x = fmaf(qf_tanh(t.x * cap_pre), scale_log2, less_m.x);
+    t.y = fmaf(qf_tanh(t.y * cap_pre), scale_log2, less_m.y);
+  }
+  return t;
+}
+
+// A row's 128 products into probabilities in P (128-byte swizzled, two blocks of 64 keys); returns their sum.  MASK: only keys
+// [a, b) count.
+template <bool CAP, bool MASK>
+__device__ __forceinline__ float qf_softmax_tile(uint32_t s_addr, const QfScales* sc, unsigned char* rowp, int r, float qs, float m, float cap_pre,
+                                                 float scale_log2, int a, int b) {
+  const float2 qs2 = make_float2(qs, qs), less_m = make_float2(-m, -m);
+  float2 l0 = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t s[32];
+    tc5::ld32(s_addr + uint32_t(c * 32), s);
+    tc5::ld_wait();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {                                  // 16-byte pieces of the row of P
+      uint32_t packed[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = e * 4 + i;
+        float2 t = qf_scores<CAP>(s[2 * k], s[2 * k + 1], &sc[c * 16 + k], qs2, less_m, cap_pre, scale_log2);
+        if constexpr (MASK) {
+          const int j = c * 32 + 2 * k;
+          t.x = (j >= a && j < b) ? t.x : -INFINITY;
+          t.y = (j + 1 >= a && j + 1 < b) ? t.y : -INFINITY;
+        }
+        const float2 ex = make_float2(qf_exp2(t.x), qf_exp2(t.y));
+        if (i & 1) l1 = add2(l1, ex); else l0 = add2(l0, ex);
+        const __nv_bfloat162 pk = __floats2bfloat162_rn(ex.x, ex.y);
+        packed[i] = *reinterpret_cast<const uint32_t*>(&pk);
+      }
+      const int piece = c * 4 + e;
+      *reinterpret_cast<uint4*>(rowp + (piece >> 3) * kQfTile + (((piece & 7) ^ (r & 7)) * 16)) =
+          make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    }
+  }
+  l0 = add2(l0, l1);
+  return l0.x + l0.y;
+}
+
+// The largest score of a row's 128 products, keys [a, b).
+template <bool CAP>
+__device__ __noinline__ float qf_largest(uint32_t s_addr, const QfScales* sc, float qs, float cap_pre, float scale_log2, int a, int b) {
+  const float2 qs2 = make_float2(qs, qs), none = make_float2(0.f, 0.f);
+  float mx = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t s[32];
+    tc5::ld32(s_addr + uint32_t(c * 32), s);
+    tc5::ld_wait();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float2 t = qf_scores<CAP>(s[2 * k], s[2 * k + 1], &sc[c * 16 + k], qs2, none, cap_pre, scale_log2);
+      const int j = c * 32 + 2 * k;
+      mx = (j >= a && j < b) ? fmaxf(mx, t.x) : mx;
+      mx = (j + 1 >= a && j + 1 < b) ? fmaxf(mx, t.y) : mx;
+    }
+  }
+  return mx;
+}
+
+// 16 bytes of codes (elements 32 ch .. 32 ch + 31 of row r) as bfloat16 into a 128-byte swizzled tile [HD/64][128 rows][64]:
+// 128 + code, or the values.
+template <bool VALUES>
+__device__ __forceinline__ void qf_spread(unsigned char* tile, const unsigned char* from, int r, int ch, float scale, float zero_128) {
+  const uint4 u = *reinterpret_cast<const uint4*>(from);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  unsigned char* row = tile + (ch >> 1) * kQfTile + r * 128;
+  const float2 s2 = make_float2(scale, scale), z2 = make_float2(zero_128, zero_128);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      e[i] = q4::two_codes_128(w[j], i);
+      if (VALUES) {
+        const float2 v = fma2(make_float2(__uint_as_float(e[i] << 16), __uint_as_float(e[i] & 0xffff0000u)), s2, z2);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+        e[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(row + ((((ch & 1) * 4 + j) ^ (r & 7)) * 16)) = make_uint4(e[0], e[1], e[2], e[3]);
+  }
+}
+
+// The codes of a tile's keys (or values) on their way through shared memory into operands: WARPS warps, each lane its own pieces.
+// Neighbouring lanes take neighbouring keys, whose swizzled rows differ in every bank.
+template <int HD, int WARPS>
+struct QfUnpacker {
+  static constexpr int kPieces = HD / 32;                          // 16-byte pieces of a row
+  static constexpr int kGroups8 = kQfKeys * kPieces / 8;           // groups of eight pieces
+  static constexpr int kPerThread = (kGroups8 + 4 * WARPS - 1) / (4 * WARPS);
+  int wq, lane;
+  __device__ __forceinline__ bool piece(int i, int& r, int& ch) const {
+    const int group = (i * WARPS + wq) * 4 + (lane >> 3);
+    r = (group / kPieces) * 8 + (lane & 7);
+    ch = group % kPieces;
+    return group < kGroups8;
+  }
+};
 
 template <int HD> constexpr size_t qf_smem() {
   constexpr int KB = HD / 64;
-  return size_t(2) * KB * kQfTile + size_t(2) * kQfStages * KB * kQfBlock + size_t(4) * kQfTile + size_t(kQfScaleRing) * (kQfKeys / 2) * sizeof(QfScales);
+  return size_t(2 + 1 + 1) * KB * kQfTile + size_t(4) * kQfTile + size_t(2) * (kQfKeys / 2) * sizeof(QfScales) + kQfKeys * HD + kQfKeys * 4 +
+         QfUnpacker<HD, kQfValueWarps>::kPerThread * kQfValueWarps * 32 * 4;
 }
 
 template <int HD, bool CAP>
 __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __grid_constant__ CUtensorMap map_q, PrefillQ4Params p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   constexpr int KB = HD / 64;                                      // 64-wide blocks of head_dim
-  constexpr int kStage = KB * kQfBlock;
-  constexpr int kPieces = HD / 32;                                 // 16-byte pieces of a row of codes
-  constexpr int kGroups8 = kQfKeys * kPieces / 8;                  // groups of eight pieces of K (and of V)
-  constexpr int kPerThread = (kGroups8 + 4 * kQfUnpackWarps - 1) / (4 * kQfUnpackWarps);
   unsigned char* q_s = smem_raw;                                   // [2][KB][128 rows][64]
-  unsigned char* k_s = q_s + 2 * KB * kQfTile;                     // [stages][KB][64 keys][64]
-  unsigned char* v_s = k_s + kQfStages * kStage;
-  unsigned char* p_s = v_s + kQfStages * kStage;                   // [2 groups][2][128 rows][64 keys]
-  QfScales* scales = reinterpret_cast<QfScales*>(p_s + 4 * kQfTile);       // [ring][32 pairs of keys]
-  __shared__ __align__(8) uint64_t q_full, k_full[kQfStages], k_empty[kQfStages], v_full[kQfStages], v_empty[kQfStages], sc_full[kQfScaleRing],
-      s_full[2][2], s_free[2][2], p_full[2][2], p_free[2][2], o_full;
+  unsigned char* k_s = q_s + 2 * KB * kQfTile;                     // [KB][128 keys][64]
+  unsigned char* v_s = k_s + KB * kQfTile;
+  unsigned char* p_s = v_s + KB * kQfTile;                         // [2 groups][2][128 rows][64 keys]
+  QfScales* scales = reinterpret_cast<QfScales*>(p_s + 4 * kQfTile);       // [2][64 pairs of keys]
+  unsigned char* raw = reinterpret_cast<unsigned char*>(scales + 2 * (kQfKeys / 2));      // codes [2][128][HD/2]; the keys' pairs [128]; of each value piece
+  __shared__ __align__(8) uint64_t q_full, k_full, v_full, sc_full[2], s_full[2], s_free[2], p_full[2], p_free[2], o_full;
   __shared__ uint32_t tmem_base;
   __shared__ volatile int abort_flag;
 
@@ -140,24 +239,19 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
   if (threadIdx.x == 0) {
     abort_flag = 0;
     tc5::mbar_init(&q_full, 1);
-    for (int i = 0; i < kQfStages; ++i) {
-      tc5::mbar_init(&k_full[i], kQfUnpackWarps);
-      tc5::mbar_init(&v_full[i], kQfUnpackWarps);
-      tc5::mbar_init(&k_empty[i], 1);
-      tc5::mbar_init(&v_empty[i], 1);
+    tc5::mbar_init(&k_full, kQfKeyWarps);
+    tc5::mbar_init(&v_full, kQfValueWarps);
+    for (int i = 0; i < 2; ++i) {
+      tc5::mbar_init(&sc_full[i], kQfKeyWarps);
+      tc5::mbar_init(&s_full[i], 1);
+      tc5::mbar_init(&s_free[i], 4);                               // a group's four warps
+      tc5::mbar_init(&p_full[i], 4);
+      tc5::mbar_init(&p_free[i], 1);
     }
-    for (int i = 0; i < kQfScaleRing; ++i) tc5::mbar_init(&sc_full[i], kQfUnpackWarps);
-    for (int g = 0; g < 2; ++g)
-      for (int i = 0; i < 2; ++i) {
-        tc5::mbar_init(&s_full[g][i], 1);
-        tc5::mbar_init(&s_free[g][i], 4);                          // a group's four warps
-        tc5::mbar_init(&p_full[g][i], 4);
-        tc5::mbar_init(&p_free[g][i], 1);
-      }
     tc5::mbar_init(&o_full, 1);
     tc5::mbar_init_fence();
   }
-  if (warp == 11) {
+  if (warp == 15) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5::s32(&tmem_base)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
   }
@@ -173,7 +267,22 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
     abort_flag = 1;
   };
 
-  if (warp == 11) {
+  auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {  // the warp stays together whatever a lane saw
+    const bool ok = !abort_flag && tc5::mbar_wait(bar, parity);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    if (!abort_flag && lane == 0) fail(code);
+    return false;
+  };
+  const size_t bytes = q4::page_bytes(p.block_size, HD);
+  const int* table = p.block_tables + size_t(seq) * p.max_blocks;
+  auto page_of = [&](int key, int& off) {
+    const int pi = p.log2_block >= 0 ? key >> p.log2_block : key / p.block_size;
+    off = key - pi * p.block_size;
+    return q4::page_base(table[pi], kvh, p.nkv, p.num_pages, bytes);
+  };
+  const int pairs_at = p.block_size * (HD / 2);
+
+  if (warp == 15) {
     // ---- one thread: Q once, then the products
     if (lane == 0) {
       tc5::mbar_expect_tx(&q_full, groups * KB * kQfTile);
@@ -181,170 +290,141 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
         for (int kb = 0; kb < KB; ++kb)
           tc5::tma_load_2d(q_s + (g * KB + kb) * kQfTile, &map_q, &q_full, head * HD + kb * 64, q_start + q0 + g * kQfGroupRows);
       constexpr uint32_t idesc_s = tc5::idesc(kQfGroupRows, kQfKeys, false);
-      constexpr uint32_t idesc_o = tc5::idesc(kQfGroupRows, 64, true);
+      constexpr uint32_t idesc_o = tc5::idesc(kQfGroupRows, HD, true);
+      const uint64_t dk = tc5::smem_desc(tc5::s32(k_s));
+      // values, MN-major: 64-wide blocks a leading offset apart
+      const uint64_t dv = (tc5::smem_desc(tc5::s32(v_s)) & ~(uint64_t(0x3fff) << 16)) | (uint64_t(kQfTile >> 4) << 16);
       bool ok = tc5::mbar_wait(&q_full, 0);
       if (!ok) fail(18);
       for (int n = 0; ok && n <= n_tiles && !abort_flag; ++n) {
-        if (n < n_tiles) {                                         // S_n of both groups
-          const int st = n % kQfStages;
-          if (!tc5::mbar_wait(&k_full[st], (n / kQfStages) & 1)) { fail(19); break; }
-          const uint64_t dk = tc5::smem_desc(tc5::s32(k_s + st * kStage));
-          for (int g = 0; g < groups; ++g) {
-            if (g == 0 && n >= n_first) continue;
-            if (!tc5::mbar_wait(&s_free[g][n & 1], ((n >> 1) & 1) ^ 1)) { fail(20); ok = false; break; }
+        if (n < n_tiles && !tc5::mbar_wait(&k_full, n & 1)) { fail(19); break; }
+        for (int g = 0; ok && g < groups; ++g) {
+          const int mine = g == 0 ? n_first : n_tiles;
+          if (n < mine) {                                          // S_n
+            if (!tc5::mbar_wait(&s_free[g], (n & 1) ^ 1)) { fail(20); ok = false; break; }
             tc5::fence_after();
             const uint64_t dq = tc5::smem_desc(tc5::s32(q_s + g * KB * kQfTile));
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                tc5::mma(tmem + uint32_t((2 * g + (n & 1)) * kQfKeys), dq + uint64_t(kb * (kQfTile >> 4) + 2 * j),
-                         dk + uint64_t(kb * (kQfBlock >> 4) + 2 * j), idesc_s, (kb > 0 || j > 0) ? 1u : 0u);
-            tc5::commit(&s_full[g][n & 1]);
+                tc5::mma(tmem + uint32_t(g * kQfKeys), dq + uint64_t(kb * (kQfTile >> 4) + 2 * j), dk + uint64_t(kb * (kQfTile >> 4) + 2 * j),
+                         idesc_s, (kb > 0 || j > 0) ? 1u : 0u);
+            tc5::commit(&s_full[g]);
           }
-          if (!ok) break;
-          tc5::commit(&k_empty[st]);
-        }
-        if (n >= 1) {                                              // O += P_m W_m of both groups
-          const int m = n - 1, st = m % kQfStages;
-          if (!tc5::mbar_wait(&v_full[st], (m / kQfStages) & 1)) { fail(21); break; }
-          const uint32_t v_addr = tc5::s32(v_s + st * kStage);
-          for (int g = 0; g < groups; ++g) {
-            if (g == 0 && m >= n_first) continue;
-            if (!tc5::mbar_wait(&p_full[g][m & 1], (m >> 1) & 1)) { fail(22); ok = false; break; }
+          if (n >= 1 && n <= mine) {                               // O += P_(n-1) W_(n-1)
+            const int m = n - 1;
+            if (!tc5::mbar_wait(&p_full[g], m & 1)) { fail(22); ok = false; break; }
+            if (!tc5::mbar_wait(&v_full, m & 1)) { fail(21); ok = false; break; }
             tc5::fence_after();
-            const uint64_t dp = tc5::smem_desc(tc5::s32(p_s + (2 * g + (m & 1)) * kQfTile));
+            const uint64_t dp = tc5::smem_desc(tc5::s32(p_s + 2 * g * kQfTile));
 #pragma unroll
-            for (int j = 0; j < kQfKeys / 16; ++j)
-#pragma unroll
-              for (int nb = 0; nb < KB; ++nb)
-                tc5::mma(tmem + 256 + g * HD + nb * 64, dp + uint64_t(2 * j), tc5::smem_desc(v_addr + nb * kQfBlock + j * 16 * 128), idesc_o,
-                         (m > 0 || j > 0) ? 1u : 0u);
-            tc5::commit(&p_free[g][m & 1]);
+            for (int j = 0; j < kQfKeys / 16; ++j)                 // 16 keys: 32 bytes along a row of P, 16 rows down W
+              tc5::mma(tmem + 256 + g * HD, dp + uint64_t((j >> 2) * (kQfTile >> 4) + 2 * (j & 3)), dv + uint64_t(j * (16 * 128 >> 4)), idesc_o,
+                       (m > 0 || j > 0) ? 1u : 0u);
+            tc5::commit(&p_free[g]);
           }
-          if (!ok) break;
-          tc5::commit(&v_empty[st]);
         }
       }
       tc5::commit(&o_full);
     }
-  } else if (warp >= 8) {
-    // ---- pages into operands
-    const int t = threadIdx.x - 256, wq = warp - 8;
-    const size_t bytes = q4::page_bytes(p.block_size, HD);
-    const int pairs_at = p.block_size * (HD / 2);
-    const int* table = p.block_tables + size_t(seq) * p.max_blocks;
-    auto page_of = [&](int key, int& off) {
-      const int pi = p.log2_block >= 0 ? key >> p.log2_block : key / p.block_size;
-      off = key - pi * p.block_size;
-      return q4::page_base(table[pi], kvh, p.nkv, p.num_pages, bytes);
-    };
-    // this thread's pieces: neighbouring lanes take neighbouring keys (their swizzled rows differ in every bank)
-    int key_of[kPerThread], ch_of[kPerThread];
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      const int group = (i * kQfUnpackWarps + wq) * 4 + (lane >> 3);       // eight lanes: eight keys, one piece
-      key_of[i] = group < kGroups8 ? (group / kPieces) * 8 + (lane & 7) : -1;
-      ch_of[i] = group % kPieces;
-    }
-    uint4 kc[kPerThread], vc[kPerThread];
-    uint32_t kp = 0, vp = 0;                                       // the pair of key t (t < 64)
+  } else if (warp >= 8 && warp < 8 + kQfKeyWarps) {
+    // ---- keys into operands, pairs of both into scales.  S of the last group is the last to read a tile of keys; and where it
+    // is asked for, every row has taken the tile before, so two places for scales are enough.
+    const QfUnpacker<HD, kQfKeyWarps> unpack{warp - 8, lane};
+    const int t = threadIdx.x - 256;                               // this thread's key of the tile
+    unsigned char* pair = raw + kQfKeys * HD + t * 4;
     auto ask = [&](int n) {
       const int key0 = (j0 + n) * kQfKeys;
 #pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        const int key = key0 + key_of[i];
-        kc[i] = vc[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (key_of[i] >= 0 && key >= lo && key < hi) {
-          int off;
-          size_t at = page_of(key, off);
-          at += size_t(off) * (HD / 2) + ch_of[i] * 16;
-          kc[i] = *reinterpret_cast<const uint4*>(p.k_cache + at);
-          vc[i] = *reinterpret_cast<const uint4*>(p.v_cache + at);
+      for (int i = 0; i < unpack.kPerThread; ++i) {
+        int r, ch, off;
+        if (unpack.piece(i, r, ch) && key0 + r >= lo && key0 + r < hi) {
+          const size_t at = page_of(key0 + r, off);
+          qf_copy16(raw + r * (HD / 2) + ch * 16, p.k_cache + at + size_t(off) * (HD / 2) + ch * 16);
         }
       }
-      if (t < kQfKeys) {
-        const int key = key0 + t;
-        kp = vp = 0u;                                              // zero: zero times it stays zero
-        if (key >= lo && key < hi) {
-          int off;
-          size_t at = page_of(key, off);
-          at += pairs_at + off * 4;
-          kp = *reinterpret_cast<const uint32_t*>(p.k_cache + at);
-          vp = *reinterpret_cast<const uint32_t*>(p.v_cache + at);
-        }
+      if (key0 + t >= lo && key0 + t < hi) {
+        int off;
+        const size_t at = page_of(key0 + t, off);
+        qf_copy4(pair, p.k_cache + at + pairs_at + off * 4);
+      } else {
+        *reinterpret_cast<uint32_t*>(pair) = 0u;                   // (a masked score, finite whatever the codes are)
       }
-    };
-    // element 32 ch + 8 j of key r: 16 bytes at swizzled piece (32 ch + 8 j) % 64 / 8 of row r of block ch / 2
-    auto spread = [&](unsigned char* base, const uint4& codes, int r, int ch, bool centre) {
-      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-      unsigned char* row = base + (ch >> 1) * kQfBlock + r * 128;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[i] = q4::two_codes_128(w[j], i);
-          if (centre) e[i] = qf_centred(e[i]);
-        }
-        *reinterpret_cast<uint4*>(row + ((((ch & 1) * 4 + j) ^ (r & 7)) * 16)) = make_uint4(e[0], e[1], e[2], e[3]);
-      }
-    };
-    auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
-      const bool ok = !abort_flag && tc5::mbar_wait(bar, parity);
-      if (__all_sync(0xffffffffu, ok)) return true;
-      if (!abort_flag && lane == 0) fail(code);
-      return false;
     };
     ask(0);
     for (int n = 0; n < n_tiles; ++n) {
-      const int st = n % kQfStages;
-      const uint32_t round = ((n / kQfStages) & 1) ^ 1;
-      if (!wait_all(&k_empty[st], round, 23)) break;
-      if (t < kQfKeys) {
-        float* f = reinterpret_cast<float*>(scales + (n % kQfScaleRing) * (kQfKeys / 2) + (t >> 1)) + (t & 1);
-        const float unit = CAP ? 1.f : p.scale_log2;
-        const float ks = q4::scale_of(kp), vs = q4::scale_of(vp);
-        f[0] = ks * unit;
-        f[2] = fmaf(-128.f, ks, q4::zero_of(kp)) * unit;
-        f[4] = vs;
-        f[6] = fmaf(8.f, vs, q4::zero_of(vp));
-      }
+      asm volatile("cp.async.wait_all;\n" ::: "memory");
+      if (n > 0 && !wait_all(&s_full[groups - 1], (n - 1) & 1, 23)) break;
+      const uint32_t two = *reinterpret_cast<const uint32_t*>(pair);
+      float* f = reinterpret_cast<float*>(scales + (n & 1) * (kQfKeys / 2) + (t >> 1)) + (t & 1);
+      const float unit = CAP ? 1.f : p.scale_log2, scale = q4::scale_of(two);
+      f[0] = scale * unit;
+      f[2] = fmaf(-128.f, scale, q4::zero_of(two)) * unit;
 #pragma unroll
-      for (int i = 0; i < kPerThread; ++i)
-        if (key_of[i] >= 0) spread(k_s + st * kStage, kc[i], key_of[i], ch_of[i], false);
+      for (int i = 0; i < unpack.kPerThread; ++i) {
+        int r, ch;
+        if (unpack.piece(i, r, ch)) qf_spread<false>(k_s, raw + r * (HD / 2) + ch * 16, r, ch, 0.f, 0.f);
+      }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
       if (lane == 0) {
-        tc5::mbar_arrive(&sc_full[n % kQfScaleRing]);
-        tc5::mbar_arrive(&k_full[st]);
+        tc5::mbar_arrive(&sc_full[n & 1]);
+        tc5::mbar_arrive(&k_full);
       }
-      if (!wait_all(&v_empty[st], round, 24)) break;
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i)
-        if (key_of[i] >= 0) spread(v_s + st * kStage, vc[i], key_of[i], ch_of[i], true);
       if (n + 1 < n_tiles) ask(n + 1);
+    }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+  } else if (warp >= 8 && warp < 8 + kQfKeyWarps + kQfValueWarps) {
+    // ---- values into operands; each piece with its own copy of its row's pair
+    const QfUnpacker<HD, kQfValueWarps> unpack{warp - 8 - kQfKeyWarps, lane};
+    unsigned char* codes = raw + kQfKeys * (HD / 2);
+    unsigned char* pair = raw + kQfKeys * HD + kQfKeys * 4 + (threadIdx.x - 32 * (8 + kQfKeyWarps)) * 4;
+    constexpr int kPairStep = kQfValueWarps * 32 * 4;
+    auto ask = [&](int n) {
+      const int key0 = (j0 + n) * kQfKeys;
+#pragma unroll
+      for (int i = 0; i < unpack.kPerThread; ++i) {
+        int r, ch, off;
+        if (!unpack.piece(i, r, ch)) continue;
+        if (key0 + r >= lo && key0 + r < hi) {
+          const size_t at = page_of(key0 + r, off);
+          qf_copy16(codes + r * (HD / 2) + ch * 16, p.v_cache + at + size_t(off) * (HD / 2) + ch * 16);
+          qf_copy4(pair + i * kPairStep, p.v_cache + at + pairs_at + off * 4);
+        } else {
+          *reinterpret_cast<uint32_t*>(pair + i * kPairStep) = 0u; // a value of zero: zero times it stays zero
+        }
+      }
+    };
+    ask(0);
+    for (int n = 0; n < n_tiles; ++n) {
+      asm volatile("cp.async.wait_all;\n" ::: "memory");
+      if (n > 0 && !wait_all(&p_free[groups - 1], (n - 1) & 1, 24)) break;
+#pragma unroll
+      for (int i = 0; i < unpack.kPerThread; ++i) {
+        int r, ch;
+        if (!unpack.piece(i, r, ch)) continue;
+        const uint32_t two = *reinterpret_cast<const uint32_t*>(pair + i * kPairStep);
+        const float scale = q4::scale_of(two);
+        qf_spread<true>(v_s, codes + r * (HD / 2) + ch * 16, r, ch, scale, fmaf(-128.f, scale, q4::zero_of(two)));
+      }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
-      if (lane == 0) tc5::mbar_arrive(&v_full[st]);
+      if (lane == 0) tc5::mbar_arrive(&v_full);
+      if (n + 1 < n_tiles) ask(n + 1);
     }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
   } else {
     // ---- softmax and output: this thread owns row r of its group (lane r of tensor memory)
     const int g = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const int mine = g == 0 ? n_first : n_tiles;
     const int row = g * kQfGroupRows + r, pos = pos0 + row;        // rows beyond rows_here compute and store nothing
     const uint32_t lane_addr = tmem + (uint32_t(quarter * 32) << 16);
-    const uint32_t o_addr = lane_addr + 256 + g * HD;
+    const uint32_t s_addr = lane_addr + g * kQfKeys, o_addr = lane_addr + 256 + g * HD;
     if (g < groups) {
       const int first = first_visible(pos, p.window, 0);
       const int group_pos = pos0 + g * kQfGroupRows;               // of the group's first row
       const int last_first = first_visible(group_pos + kQfGroupRows - 1, p.window, 0);
-      auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
-        const bool ok = !abort_flag && tc5::mbar_wait(bar, parity);
-        if (__all_sync(0xffffffffu, ok)) return true;
-        if (!abort_flag && lane == 0) fail(code);
-        return false;
-      };
       bool alive = wait_all(&q_full, 0, 25);
       float qs = 0.f;                                              // sum of q over the row
       if (alive) {
@@ -356,104 +436,59 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
           for (int i = 0; i < 4; ++i) qs += __uint_as_float(w[i] << 16) + __uint_as_float(w[i] & 0xffff0000u);
         }
       }
-      const float2 qs2 = make_float2(qs, qs);
       float m = -INFINITY;                                         // the maximum the row currently scales by
-      float2 l2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);
+      float l = 0.f;
+      unsigned char* const rowp = p_s + 2 * g * kQfTile + r * 128;
       for (int n = 0; alive && n < mine; ++n) {
-        if (!wait_all(&s_full[g][n & 1], (n >> 1) & 1, 26)) { alive = false; break; }
+        if (!wait_all(&s_full[g], n & 1, 26) || !wait_all(&sc_full[n & 1], (n >> 1) & 1, 27)) { alive = false; break; }
+        // P's buffer was last read by O += P_(n-1) W_(n-1); O must hold that tile where it is rescaled
+        if (n > 0 && !wait_all(&p_free[g], (n - 1) & 1, 28)) { alive = false; break; }
         tc5::fence_after();
-        uint32_t v[2][32];                                         // the row's 64 products
-#pragma unroll
-        for (int c = 0; c < 2; ++c) tc5::ld32(lane_addr + uint32_t((2 * g + (n & 1)) * kQfKeys + c * 32), v[c]);
-        tc5::ld_wait();
-        tc5::fence_before();
-        __syncwarp();
-        if (lane == 0) tc5::mbar_arrive(&s_free[g][n & 1]);        // S_(n+2) may be written
-        if (!wait_all(&sc_full[n % kQfScaleRing], (n / kQfScaleRing) & 1, 27)) { alive = false; break; }
-        const QfScales* sc = scales + (n % kQfScaleRing) * (kQfKeys / 2);
-        float* x = reinterpret_cast<float*>(&v[0][0]);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float4 s = *reinterpret_cast<const float4*>(&sc[i]);       // scales, then zeros, of keys 2i and 2i + 1
-          float2 t = fma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(s.x, s.y), mul2(make_float2(s.z, s.w), qs2));
-          if constexpr (CAP) {
-            t.x = qf_tanh(t.x * p.cap_pre) * p.scale_log2;
-            t.y = qf_tanh(t.y * p.cap_pre) * p.scale_log2;
-          }
-          x[2 * i] = t.x;
-          x[2 * i + 1] = t.y;
-        }
+        const QfScales* sc = scales + (n & 1) * (kQfKeys / 2);
         const int key0 = (j0 + n) * kQfKeys;
         // the keys of this tile that the row may see: [a, b) relative to it; masks only where some row of the group needs one
         const int a = max(first, lo) - key0, b = min(pos + 1, hi) - key0;
         const bool full = key0 + kQfKeys - 1 <= group_pos && key0 >= last_first;
-        if (!full) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) x[i] = (i >= a && i < b) ? x[i] : -INFINITY;
-        }
-        float part[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float t = qf_max3(x[8 * e], x[8 * e + 1], x[8 * e + 2]);
-          t = qf_max3(t, x[8 * e + 3], x[8 * e + 4]);
-          t = qf_max3(t, x[8 * e + 5], x[8 * e + 6]);
-          part[e] = fmaxf(t, x[8 * e + 7]);
-        }
-        const float m_tile = fmaxf(qf_max3(qf_max3(part[0], part[1], part[2]), part[3], part[4]), qf_max3(part[5], part[6], part[7]));
-        float alpha = 1.f;
-        bool rescale = false;
-        if (m == -INFINITY) {
-          m = m_tile;                                              // nothing was added yet
-        } else if (m_tile > m + kQfRescaleStep) {
-          alpha = qf_exp2(m - m_tile);
-          m = m_tile;
-          rescale = true;
-        }
-        if (__any_sync(0xffffffffu, rescale)) {
-          // O must hold tile n - 1 completely; nothing newer is issued before this warp has delivered P_n
-          if (n > 0 && !wait_all(&p_free[g][(n - 1) & 1], ((n - 1) >> 1) & 1, 28)) { alive = false; break; }
-          tc5::fence_after();
-          uint32_t ov[32];
+        float sum = 0.f;
+        bool again = m == -INFINITY;                               // nothing seen yet: the maximum first
+        for (int pass = 0; pass < 2; ++pass) {
+          if (__any_sync(0xffffffffu, again)) {
+            const float mx = qf_largest<CAP>(s_addr, sc, qs, p.cap_pre, p.scale_log2, a, b);
+            const bool renew = again && mx > m;
+            const float alpha = renew && m != -INFINITY ? qf_exp2(m - mx) : 1.f;
+            if (renew) m = mx;
+            l *= alpha;
+            if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+              uint32_t ov[32];
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            tc5::ld32(o_addr + uint32_t(c * 32), ov);
-            tc5::ld_wait();
+              for (int c = 0; c < HD / 32; ++c) {
+                tc5::ld32(o_addr + uint32_t(c * 32), ov);
+                tc5::ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-            tc5::st32(o_addr + uint32_t(c * 32), ov);
+                for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+                tc5::st32(o_addr + uint32_t(c * 32), ov);
+              }
+              tc5::st_wait();
+            }
           }
-          tc5::st_wait();
-          l2.x *= alpha; l2.y *= alpha; z2.x *= alpha; z2.y *= alpha;
+          const float m_use = (m == -INFINITY) ? 0.f : m;
+          sum = full ? qf_softmax_tile<CAP, false>(s_addr, sc, rowp, r, qs, m_use, p.cap_pre, p.scale_log2, a, b)
+                     : qf_softmax_tile<CAP, true>(s_addr, sc, rowp, r, qs, m_use, p.cap_pre, p.scale_log2, a, b);
+          again = !again && sum > kQfMost;                         // (after a look at the maximum it is at most 128)
+          if (!__any_sync(0xffffffffu, again)) break;
         }
-        // P_n's buffer was last read by O += P_(n-2) W_(n-2), issued before S_n: having seen S_n, it may be written
-        const float m_use = (m == -INFINITY) ? 0.f : m;
-        unsigned char* rowp = p_s + (2 * g + (n & 1)) * kQfTile + r * 128;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t packed[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = c * 4 + i;
-            const float4 s = *(reinterpret_cast<const float4*>(&sc[k]) + 1);
-            const float2 e = make_float2(qf_exp2(x[2 * k] - m_use), qf_exp2(x[2 * k + 1] - m_use));
-            l2 = add2(l2, e);
-            z2 = fma2(e, make_float2(s.z, s.w), z2);
-            const float2 w = mul2(e, make_float2(s.x, s.y));
-            const __nv_bfloat162 h = __floats2bfloat162_rn(w.x, w.y);
-            packed[i] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-          *reinterpret_cast<uint4*>(rowp + ((c ^ (r & 7)) * 16)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-        }
+        l += sum;
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         tc5::fence_before();
         __syncwarp();
-        if (lane == 0) tc5::mbar_arrive(&p_full[g][n & 1]);
+        if (lane == 0) {
+          tc5::mbar_arrive(&s_free[g]);                            // S_(n+1) may be written
+          tc5::mbar_arrive(&p_full[g]);
+        }
       }
       if (alive) alive = wait_all(&o_full, 0, 29);
       tc5::fence_after();
       if (alive) {
-        float l = l2.x + l2.y;
-        const float z = z2.x + z2.y;
         if (p.sink && m != -INFINITY) l += qf_exp2(p.sink[head] * 1.4426950408889634f - m);
         const float inv = l == 0.f ? 0.f : 1.f / l;
         bf16* dst = p.out + size_t(q_start + q0 + row) * p.out_stride + size_t(head) * HD;
@@ -468,7 +503,7 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
               __nv_bfloat162 h[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                h[i] = __floats2bfloat162_rn((__uint_as_float(ov[e * 8 + 2 * i]) + z) * inv, (__uint_as_float(ov[e * 8 + 2 * i + 1]) + z) * inv);
+                h[i] = __floats2bfloat162_rn(__uint_as_float(ov[e * 8 + 2 * i]) * inv, __uint_as_float(ov[e * 8 + 2 * i + 1]) * inv);
               *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = *reinterpret_cast<const uint4*>(h);
             }
           }
@@ -484,7 +519,7 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
   }
   tc5::fence_before();
   __syncthreads();
-  if (warp == 11) {
+  if (warp == 15) {
     tc5::fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512));
   }
