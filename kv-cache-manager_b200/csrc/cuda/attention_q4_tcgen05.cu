@@ -9,17 +9,19 @@
 // A key is never rounded: its scale and zero meet the score, which costs two packed multiply-adds for two scores.  A value is, once, to
 // bfloat16, as P is: applied to P instead, its scale and zero were three more instructions for two scores in the loop that
 // bounds the kernel (four portions behind long prefixes: 1,270 us against DONE_US).
-// A row takes its tile relative to the maximum that it knew before, without looking for the tile's own: where the tile's sum comes
-// out above 2^12 (or the row has seen nothing yet) the tile's maximum is found, sums and O are rescaled, and the tile is taken
-// again, S being still there.  The largest probability therefore lies between 1 and 2^12 times 1, which float32 sums and the
-// exponents of bfloat16 do not mind.
+// A row takes its products 32 at a time, relative to the maximum that it knows, without looking for theirs: where 32 probabilities
+// add up to more than 2^12 (or the row has seen nothing yet) their maximum is found, sums, O and the tile's earlier probabilities
+// are rescaled, and the 32 are taken again, which after the first tiles hardly ever happens.  The largest probability then lies
+// between 1 and 2^12, which float32 sums and the exponents of bfloat16 do not mind.
+// P lies in tensor memory over the products that it was made of (32 columns of S become 16 of P), as the first operand of O += P V.
+// The products of a group run in order: S of the next tile behind O += P V of this one, so one barrier says that S is there, that
+// O holds the tile before, and that P has been read.
 //
 // Roles (16 warps, 128 registers a thread): 0-3 and 4-7 softmax and output of the two groups; 8-11 turn keys into operands and
-// pairs into scales, 12-14 values; one thread of warp 15 brings Q and issues the products, S of a group's next tile before O += P W
-// of this one, the groups in turn, so that the products of one run under the softmax of the other.
-// What bounds it: at head_dim 128 a tile's exponentials (256 x 128 at 16 a cycle) and its products each take 2,048 cycles, and the
-// handshakes between roles, some 150 cycles each, come on top where they are not hidden: tiles of 64 keys, with twice as many
-// of them, took 4,100 cycles for half the work.
+// their pairs into scales, 12-14 values; one thread of warp 15 brings Q and issues the products, the groups in turn, so that the
+// products of one run under the softmax of the other.
+// What bounds it: at head_dim 128 a tile's exponentials (256 x 128 at 16 a cycle) and its products each take 2,048 cycles; a
+// handshake between roles takes some 250 cycles, and four of them lie between two softmaxes of a group.
 // A thread of warps 8-14 copies what it unpacks itself (cp.async into shared memory, a tile ahead) and so waits for nobody else's.
 // Masks: key <= position, optional window.  Every wait is bounded; one that runs out sets the error word of the tcgen05 attention
 // family (codes 17 and up) and ends the block.
@@ -36,8 +38,10 @@ constexpr int kQfGroupRows = 128, kQfRows = 256;
 constexpr int kQfKeys = 128;
 constexpr int kQfKeyWarps = 4, kQfValueWarps = 3;
 constexpr int kQfTile = 128 * 128;                 // [128 rows][64 bf16]: also a 64-wide block of a tile of keys or values
-constexpr float kQfMost = 4096.f;                  // a row's sum of one tile from which its maximum is renewed
-// tensor memory: S of group g at column g * 128; O of group g at 256 + g * head_dim
+constexpr int kQfStages = 2;                       // tiles of keys, and of values, as operands
+constexpr int kQfScaleRing = 4;
+constexpr float kQfMost = 4096.f;                  // a row's sum of 32 probabilities from which its maximum is renewed
+// tensor memory: S of group g at column g * 128 (and P in its first 64 columns); O of group g at 256 + g * head_dim
 
 struct PrefillQ4Params {
   bf16* out; long long out_stride;
@@ -67,6 +71,25 @@ __device__ __forceinline__ void qf_copy16(void* smem, const void* gmem) {
 __device__ __forceinline__ void qf_copy4(void* smem, const void* gmem) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(tc5::s32(smem)), "l"(gmem) : "memory");
 }
+// 16 consecutive columns of this thread's lane of tensor memory (no wait).
+__device__ __forceinline__ void qf_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                 "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void qf_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n"
+               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+                 "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
+// The product with its first operand in tensor memory: 16-bit elements, two neighbours of a row to a column.
+__device__ __forceinline__ void qf_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t db, uint32_t instr, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(d_tmem), "r"(a_tmem), "l"(db), "r"(instr), "r"(accumulate) : "memory");
+}
 // a * b + c of two floats at once
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -95,63 +118,66 @@ __device__ __forceinline__ float2 qf_scores(uint32_t s0, uint32_t s1, const QfSc
   return t;
 }
 
-// A row's 128 products into probabilities in P (128-byte swizzled, two blocks of 64 keys); returns their sum.  MASK: only keys
-// [a, b) count.
+// 32 products of a row into probabilities, as bfloat16 pairs; returns their sum.  MASK: only keys [a, b) of the 32 count.
 template <bool CAP, bool MASK>
-__device__ __forceinline__ float qf_softmax_tile(uint32_t s_addr, const QfScales* sc, unsigned char* rowp, int r, float qs, float m, float cap_pre,
-                                                 float scale_log2, int a, int b) {
+__device__ __forceinline__ float qf_exponentials(const uint32_t (&s)[32], const QfScales* sc, uint32_t (&packed)[16], float qs, float m,
+                                                 float cap_pre, float scale_log2, int a, int b) {
   const float2 qs2 = make_float2(qs, qs), less_m = make_float2(-m, -m);
   float2 l0 = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    uint32_t s[32];
-    tc5::ld32(s_addr + uint32_t(c * 32), s);
-    tc5::ld_wait();
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {                                  // 16-byte pieces of the row of P
-      uint32_t packed[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = e * 4 + i;
-        float2 t = qf_scores<CAP>(s[2 * k], s[2 * k + 1], &sc[c * 16 + k], qs2, less_m, cap_pre, scale_log2);
-        if constexpr (MASK) {
-          const int j = c * 32 + 2 * k;
-          t.x = (j >= a && j < b) ? t.x : -INFINITY;
-          t.y = (j + 1 >= a && j + 1 < b) ? t.y : -INFINITY;
-        }
-        const float2 ex = make_float2(qf_exp2(t.x), qf_exp2(t.y));
-        if (i & 1) l1 = add2(l1, ex); else l0 = add2(l0, ex);
-        const __nv_bfloat162 pk = __floats2bfloat162_rn(ex.x, ex.y);
-        packed[i] = *reinterpret_cast<const uint32_t*>(&pk);
-      }
-      const int piece = c * 4 + e;
-      *reinterpret_cast<uint4*>(rowp + (piece >> 3) * kQfTile + (((piece & 7) ^ (r & 7)) * 16)) =
-          make_uint4(packed[0], packed[1], packed[2], packed[3]);
+  for (int k = 0; k < 16; ++k) {
+    float2 t = qf_scores<CAP>(s[2 * k], s[2 * k + 1], &sc[k], qs2, less_m, cap_pre, scale_log2);
+    if constexpr (MASK) {
+      t.x = (2 * k >= a && 2 * k < b) ? t.x : -INFINITY;
+      t.y = (2 * k + 1 >= a && 2 * k + 1 < b) ? t.y : -INFINITY;
     }
+    const float2 ex = make_float2(qf_exp2(t.x), qf_exp2(t.y));
+    if (k & 1) l1 = add2(l1, ex); else l0 = add2(l0, ex);
+    const __nv_bfloat162 pk = __floats2bfloat162_rn(ex.x, ex.y);
+    packed[k] = *reinterpret_cast<const uint32_t*>(&pk);
   }
   l0 = add2(l0, l1);
   return l0.x + l0.y;
 }
 
-// The largest score of a row's 128 products, keys [a, b).
+// The largest score, less m, of the 32.
 template <bool CAP>
-__device__ __noinline__ float qf_largest(uint32_t s_addr, const QfScales* sc, float qs, float cap_pre, float scale_log2, int a, int b) {
-  const float2 qs2 = make_float2(qs, qs), none = make_float2(0.f, 0.f);
+__device__ __forceinline__ float qf_largest(const uint32_t (&s)[32], const QfScales* sc, float qs, float m, float cap_pre, float scale_log2, int a, int b) {
+  const float2 qs2 = make_float2(qs, qs), less_m = make_float2(-m, -m);
   float mx = -INFINITY;
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    uint32_t s[32];
-    tc5::ld32(s_addr + uint32_t(c * 32), s);
-    tc5::ld_wait();
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float2 t = qf_scores<CAP>(s[2 * k], s[2 * k + 1], &sc[c * 16 + k], qs2, none, cap_pre, scale_log2);
-      const int j = c * 32 + 2 * k;
-      mx = (j >= a && j < b) ? fmaxf(mx, t.x) : mx;
-      mx = (j + 1 >= a && j + 1 < b) ? fmaxf(mx, t.y) : mx;
-    }
+  for (int k = 0; k < 16; ++k) {
+    const float2 t = qf_scores<CAP>(s[2 * k], s[2 * k + 1], &sc[k], qs2, less_m, cap_pre, scale_log2);
+    mx = (2 * k >= a && 2 * k < b) ? fmaxf(mx, t.x) : mx;
+    mx = (2 * k + 1 >= a && 2 * k + 1 < b) ? fmaxf(mx, t.y) : mx;
   }
   return mx;
+}
+
+// What a row has in tensor memory times alpha: O, and the first `chunks` pieces of 32 probabilities.  (The whole warp takes part.)
+template <int HD>
+__device__ __noinline__ void qf_rescale(uint32_t o_addr, bool has_o, uint32_t p_addr, int chunks, float alpha) {
+  uint32_t v[16];
+#pragma unroll 1
+  for (int c = 0; has_o && c < HD / 16; ++c) {
+    qf_ld16(o_addr + uint32_t(c * 16), v);
+    tc5::ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+    qf_st16(o_addr + uint32_t(c * 16), v);
+  }
+#pragma unroll 1
+  for (int c = 0; c < chunks; ++c) {
+    qf_ld16(p_addr + uint32_t(c * 16), v);
+    tc5::ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(v[i] << 16) * alpha, __uint_as_float(v[i] & 0xffff0000u) * alpha);
+      v[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    qf_st16(p_addr + uint32_t(c * 16), v);
+  }
+  tc5::st_wait();
 }
 
 // 16 bytes of codes (elements 32 ch .. 32 ch + 31 of row r) as bfloat16 into a 128-byte swizzled tile [HD/64][128 rows][64]:
@@ -196,7 +222,7 @@ struct QfUnpacker {
 
 template <int HD> constexpr size_t qf_smem() {
   constexpr int KB = HD / 64;
-  return size_t(2 + 1 + 1) * KB * kQfTile + size_t(4) * kQfTile + size_t(2) * (kQfKeys / 2) * sizeof(QfScales) + kQfKeys * HD + kQfKeys * 4 +
+  return size_t(2 + 2 * kQfStages) * KB * kQfTile + size_t(kQfScaleRing) * (kQfKeys / 2) * sizeof(QfScales) + kQfKeys * HD + kQfKeys * 4 +
          QfUnpacker<HD, kQfValueWarps>::kPerThread * kQfValueWarps * 32 * 4;
 }
 
@@ -205,12 +231,11 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   constexpr int KB = HD / 64;                                      // 64-wide blocks of head_dim
   unsigned char* q_s = smem_raw;                                   // [2][KB][128 rows][64]
-  unsigned char* k_s = q_s + 2 * KB * kQfTile;                     // [KB][128 keys][64]
-  unsigned char* v_s = k_s + KB * kQfTile;
-  unsigned char* p_s = v_s + KB * kQfTile;                         // [2 groups][2][128 rows][64 keys]
-  QfScales* scales = reinterpret_cast<QfScales*>(p_s + 4 * kQfTile);       // [2][64 pairs of keys]
-  unsigned char* raw = reinterpret_cast<unsigned char*>(scales + 2 * (kQfKeys / 2));      // codes [2][128][HD/2]; the keys' pairs [128]; of each value piece
-  __shared__ __align__(8) uint64_t q_full, k_full, v_full, sc_full[2], s_full[2], s_free[2], p_full[2], p_free[2], o_full;
+  unsigned char* k_s = q_s + 2 * KB * kQfTile;                     // [stages][KB][128 keys][64]
+  unsigned char* v_s = k_s + kQfStages * KB * kQfTile;
+  QfScales* scales = reinterpret_cast<QfScales*>(v_s + kQfStages * KB * kQfTile);          // [ring][64 pairs of keys]
+  unsigned char* raw = reinterpret_cast<unsigned char*>(scales + kQfScaleRing * (kQfKeys / 2));     // codes [2][128][HD/2]; the keys' pairs [128]; of each value piece
+  __shared__ __align__(8) uint64_t q_full, k_full[kQfStages], v_full[kQfStages], sc_full[kQfScaleRing], s_full[2], p_full[2], done[kQfStages], o_full;
   __shared__ uint32_t tmem_base;
   __shared__ volatile int abort_flag;
 
@@ -239,14 +264,15 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
   if (threadIdx.x == 0) {
     abort_flag = 0;
     tc5::mbar_init(&q_full, 1);
-    tc5::mbar_init(&k_full, kQfKeyWarps);
-    tc5::mbar_init(&v_full, kQfValueWarps);
-    for (int i = 0; i < 2; ++i) {
-      tc5::mbar_init(&sc_full[i], kQfKeyWarps);
-      tc5::mbar_init(&s_full[i], 1);
-      tc5::mbar_init(&s_free[i], 4);                               // a group's four warps
-      tc5::mbar_init(&p_full[i], 4);
-      tc5::mbar_init(&p_free[i], 1);
+    for (int i = 0; i < kQfStages; ++i) {
+      tc5::mbar_init(&k_full[i], kQfKeyWarps);
+      tc5::mbar_init(&v_full[i], kQfValueWarps);
+      tc5::mbar_init(&done[i], 1);
+    }
+    for (int i = 0; i < kQfScaleRing; ++i) tc5::mbar_init(&sc_full[i], kQfKeyWarps);
+    for (int g = 0; g < 2; ++g) {
+      tc5::mbar_init(&s_full[g], 1);
+      tc5::mbar_init(&p_full[g], 4);                               // a group's four warps
     }
     tc5::mbar_init(&o_full, 1);
     tc5::mbar_init_fence();
@@ -268,9 +294,8 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
   };
 
   auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {  // the warp stays together whatever a lane saw
-    const bool ok = !abort_flag && tc5::mbar_wait(bar, parity);
-    if (__all_sync(0xffffffffu, ok)) return true;
-    if (!abort_flag && lane == 0) fail(code);
+    if (__all_sync(0xffffffffu, tc5::mbar_wait(bar, parity))) return true;
+    if (!abort_flag && lane == 0) fail(code);                      // (the first to give up says so; the others' waits run out too)
     return false;
   };
   const size_t bytes = q4::page_bytes(p.block_size, HD);
@@ -291,46 +316,46 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
           tc5::tma_load_2d(q_s + (g * KB + kb) * kQfTile, &map_q, &q_full, head * HD + kb * 64, q_start + q0 + g * kQfGroupRows);
       constexpr uint32_t idesc_s = tc5::idesc(kQfGroupRows, kQfKeys, false);
       constexpr uint32_t idesc_o = tc5::idesc(kQfGroupRows, HD, true);
+      constexpr uint64_t kStageStep = (KB * kQfTile) >> 4;          // (descriptor addresses count units of 16 bytes)
       const uint64_t dk = tc5::smem_desc(tc5::s32(k_s));
       // values, MN-major: 64-wide blocks a leading offset apart
       const uint64_t dv = (tc5::smem_desc(tc5::s32(v_s)) & ~(uint64_t(0x3fff) << 16)) | (uint64_t(kQfTile >> 4) << 16);
       bool ok = tc5::mbar_wait(&q_full, 0);
       if (!ok) fail(18);
-      for (int n = 0; ok && n <= n_tiles && !abort_flag; ++n) {
-        if (n < n_tiles && !tc5::mbar_wait(&k_full, n & 1)) { fail(19); break; }
-        for (int g = 0; ok && g < groups; ++g) {
+      for (int n = 0; ok && n <= n_tiles; ++n) {
+        for (int g = 0; g < groups; ++g) {
           const int mine = g == 0 ? n_first : n_tiles;
-          if (n < mine) {                                          // S_n
-            if (!tc5::mbar_wait(&s_free[g], (n & 1) ^ 1)) { fail(20); ok = false; break; }
+          if (n >= 1 && n <= mine) {                               // O += P_(n-1) V_(n-1)
+            const int m = n - 1, st = m % kQfStages;
+            if (!tc5::mbar_wait(&v_full[st], (m / kQfStages) & 1)) { fail(21); ok = false; break; }
+            if (!tc5::mbar_wait(&p_full[g], m & 1)) { fail(22); ok = false; break; }
+            tc5::fence_after();
+#pragma unroll
+            for (int j = 0; j < kQfKeys / 16; ++j)                 // 16 keys: 8 columns of P, 16 rows down V
+              qf_mma_ts(tmem + 256 + g * HD, tmem + g * kQfKeys + j * 8, dv + st * kStageStep + uint64_t(j * (16 * 128 >> 4)), idesc_o,
+                        (m > 0 || j > 0) ? 1u : 0u);
+          }
+          if (n < mine) {                                          // S_n, over P_(n-1)
+            const int st = n % kQfStages;
+            if (!tc5::mbar_wait(&k_full[st], (n / kQfStages) & 1)) { fail(19); ok = false; break; }
             tc5::fence_after();
             const uint64_t dq = tc5::smem_desc(tc5::s32(q_s + g * KB * kQfTile));
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                tc5::mma(tmem + uint32_t(g * kQfKeys), dq + uint64_t(kb * (kQfTile >> 4) + 2 * j), dk + uint64_t(kb * (kQfTile >> 4) + 2 * j),
-                         idesc_s, (kb > 0 || j > 0) ? 1u : 0u);
-            tc5::commit(&s_full[g]);
-          }
-          if (n >= 1 && n <= mine) {                               // O += P_(n-1) W_(n-1)
-            const int m = n - 1;
-            if (!tc5::mbar_wait(&p_full[g], m & 1)) { fail(22); ok = false; break; }
-            if (!tc5::mbar_wait(&v_full, m & 1)) { fail(21); ok = false; break; }
-            tc5::fence_after();
-            const uint64_t dp = tc5::smem_desc(tc5::s32(p_s + 2 * g * kQfTile));
-#pragma unroll
-            for (int j = 0; j < kQfKeys / 16; ++j)                 // 16 keys: 32 bytes along a row of P, 16 rows down W
-              tc5::mma(tmem + 256 + g * HD, dp + uint64_t((j >> 2) * (kQfTile >> 4) + 2 * (j & 3)), dv + uint64_t(j * (16 * 128 >> 4)), idesc_o,
-                       (m > 0 || j > 0) ? 1u : 0u);
-            tc5::commit(&p_free[g]);
+                tc5::mma(tmem + uint32_t(g * kQfKeys), dq + uint64_t(kb * (kQfTile >> 4) + 2 * j),
+                         dk + st * kStageStep + uint64_t(kb * (kQfTile >> 4) + 2 * j), idesc_s, (kb > 0 || j > 0) ? 1u : 0u);
+            tc5::commit(&s_full[g]);                               // and O += P_(n-1) V_(n-1) before it
+            if (g == groups - 1) tc5::commit(&done[st]);           // tile n of the keys and n - 1 of the values are read
           }
         }
       }
       tc5::commit(&o_full);
     }
   } else if (warp >= 8 && warp < 8 + kQfKeyWarps) {
-    // ---- keys into operands, pairs of both into scales.  S of the last group is the last to read a tile of keys; and where it
-    // is asked for, every row has taken the tile before, so two places for scales are enough.
+    // ---- keys into operands, their pairs into scales.  Where S_n of the last group is issued, both groups are done with the
+    // scales of tile n - 1: three places would do.
     const QfUnpacker<HD, kQfKeyWarps> unpack{warp - 8, lane};
     const int t = threadIdx.x - 256;                               // this thread's key of the tile
     unsigned char* pair = raw + kQfKeys * HD + t * 4;
@@ -355,22 +380,22 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
     ask(0);
     for (int n = 0; n < n_tiles; ++n) {
       asm volatile("cp.async.wait_all;\n" ::: "memory");
-      if (n > 0 && !wait_all(&s_full[groups - 1], (n - 1) & 1, 23)) break;
+      if (n >= kQfStages && !wait_all(&done[n % kQfStages], ((n - kQfStages) / kQfStages) & 1, 23)) break;
       const uint32_t two = *reinterpret_cast<const uint32_t*>(pair);
-      float* f = reinterpret_cast<float*>(scales + (n & 1) * (kQfKeys / 2) + (t >> 1)) + (t & 1);
+      float* f = reinterpret_cast<float*>(scales + (n % kQfScaleRing) * (kQfKeys / 2) + (t >> 1)) + (t & 1);
       const float unit = CAP ? 1.f : p.scale_log2, scale = q4::scale_of(two);
       f[0] = scale * unit;
       f[2] = fmaf(-128.f, scale, q4::zero_of(two)) * unit;
 #pragma unroll
       for (int i = 0; i < unpack.kPerThread; ++i) {
         int r, ch;
-        if (unpack.piece(i, r, ch)) qf_spread<false>(k_s, raw + r * (HD / 2) + ch * 16, r, ch, 0.f, 0.f);
+        if (unpack.piece(i, r, ch)) qf_spread<false>(k_s + (n % kQfStages) * KB * kQfTile, raw + r * (HD / 2) + ch * 16, r, ch, 0.f, 0.f);
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
       if (lane == 0) {
-        tc5::mbar_arrive(&sc_full[n & 1]);
-        tc5::mbar_arrive(&k_full);
+        tc5::mbar_arrive(&sc_full[n % kQfScaleRing]);
+        tc5::mbar_arrive(&k_full[n % kQfStages]);
       }
       if (n + 1 < n_tiles) ask(n + 1);
     }
@@ -399,18 +424,18 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
     ask(0);
     for (int n = 0; n < n_tiles; ++n) {
       asm volatile("cp.async.wait_all;\n" ::: "memory");
-      if (n > 0 && !wait_all(&p_free[groups - 1], (n - 1) & 1, 24)) break;
+      if (n >= kQfStages && !wait_all(&done[(n - 1) % kQfStages], ((n - 1) / kQfStages) & 1, 24)) break;
 #pragma unroll
       for (int i = 0; i < unpack.kPerThread; ++i) {
         int r, ch;
         if (!unpack.piece(i, r, ch)) continue;
         const uint32_t two = *reinterpret_cast<const uint32_t*>(pair + i * kPairStep);
         const float scale = q4::scale_of(two);
-        qf_spread<true>(v_s, codes + r * (HD / 2) + ch * 16, r, ch, scale, fmaf(-128.f, scale, q4::zero_of(two)));
+        qf_spread<true>(v_s + (n % kQfStages) * KB * kQfTile, codes + r * (HD / 2) + ch * 16, r, ch, scale, fmaf(-128.f, scale, q4::zero_of(two)));
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
-      if (lane == 0) tc5::mbar_arrive(&v_full);
+      if (lane == 0) tc5::mbar_arrive(&v_full[n % kQfStages]);
       if (n + 1 < n_tiles) ask(n + 1);
     }
     asm volatile("cp.async.wait_all;\n" ::: "memory");
@@ -437,54 +462,56 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
         }
       }
       float m = -INFINITY;                                         // the maximum the row currently scales by
+      bool fresh = true;                                           // some row of the warp has none
       float l = 0.f;
-      unsigned char* const rowp = p_s + 2 * g * kQfTile + r * 128;
-      for (int n = 0; alive && n < mine; ++n) {
-        if (!wait_all(&s_full[g], n & 1, 26) || !wait_all(&sc_full[n & 1], (n >> 1) & 1, 27)) { alive = false; break; }
-        // P's buffer was last read by O += P_(n-1) W_(n-1); O must hold that tile where it is rescaled
-        if (n > 0 && !wait_all(&p_free[g], (n - 1) & 1, 28)) { alive = false; break; }
+      for (int n = 0; n < mine; ++n) {
+        alive = alive && wait_all(&s_full[g], n & 1, 26) && wait_all(&sc_full[n % kQfScaleRing], (n / kQfScaleRing) & 1, 27);
+        if (!alive) break;
         tc5::fence_after();
-        const QfScales* sc = scales + (n & 1) * (kQfKeys / 2);
+        const QfScales* sc = scales + (n % kQfScaleRing) * (kQfKeys / 2);
         const int key0 = (j0 + n) * kQfKeys;
         // the keys of this tile that the row may see: [a, b) relative to it; masks only where some row of the group needs one
         const int a = max(first, lo) - key0, b = min(pos + 1, hi) - key0;
         const bool full = key0 + kQfKeys - 1 <= group_pos && key0 >= last_first;
         float sum = 0.f;
-        bool again = m == -INFINITY;                               // nothing seen yet: the maximum first
-        for (int pass = 0; pass < 2; ++pass) {
-          if (__any_sync(0xffffffffu, again)) {
-            const float mx = qf_largest<CAP>(s_addr, sc, qs, p.cap_pre, p.scale_log2, a, b);
-            const bool renew = again && mx > m;
-            const float alpha = renew && m != -INFINITY ? qf_exp2(m - mx) : 1.f;
-            if (renew) m = mx;
-            l *= alpha;
-            if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-              uint32_t ov[32];
 #pragma unroll 1
-              for (int c = 0; c < HD / 32; ++c) {
-                tc5::ld32(o_addr + uint32_t(c * 32), ov);
-                tc5::ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-                tc5::st32(o_addr + uint32_t(c * 32), ov);
-              }
-              tc5::st_wait();
+        for (int c = 0; c < 4; ++c) {
+          uint32_t s[32], packed[16];
+          tc5::ld32(s_addr + uint32_t(c * 32), s);
+          tc5::ld_wait();
+          const QfScales* scc = sc + c * 16;
+          const int ac = a - c * 32, bc = b - c * 32;
+          float part;
+          for (int pass = 0;; ++pass) {
+            const float m_use = (m == -INFINITY) ? 0.f : m;
+            bool renew = fresh;                                    // some row of the warp has seen nothing yet
+            if (!fresh) {
+              part = full ? qf_exponentials<CAP, false>(s, scc, packed, qs, m_use, p.cap_pre, p.scale_log2, ac, bc)
+                          : qf_exponentials<CAP, true>(s, scc, packed, qs, m_use, p.cap_pre, p.scale_log2, ac, bc);
+              renew = pass == 0 && part > kQfMost;                 // (behind a renewal a part is at most 32)
+            }
+            if (!__any_sync(0xffffffffu, renew)) break;
+            const float mx = qf_largest<CAP>(s, scc, qs, m_use, p.cap_pre, p.scale_log2, ac, bc);
+            const bool grows = renew && mx != -INFINITY && (m == -INFINITY || mx > 0.f);
+            const float alpha = grows && m != -INFINITY ? qf_exp2(-mx) : 1.f;
+            if (grows) m = m_use + mx;
+            sum *= alpha;
+            l *= alpha;
+            if (__any_sync(0xffffffffu, alpha != 1.f)) qf_rescale<HD>(o_addr, n > 0, s_addr, c, alpha);
+            if (fresh) {
+              part = qf_exponentials<CAP, true>(s, scc, packed, qs, (m == -INFINITY) ? 0.f : m, p.cap_pre, p.scale_log2, ac, bc);
+              fresh = __any_sync(0xffffffffu, m == -INFINITY);
+              break;
             }
           }
-          const float m_use = (m == -INFINITY) ? 0.f : m;
-          sum = full ? qf_softmax_tile<CAP, false>(s_addr, sc, rowp, r, qs, m_use, p.cap_pre, p.scale_log2, a, b)
-                     : qf_softmax_tile<CAP, true>(s_addr, sc, rowp, r, qs, m_use, p.cap_pre, p.scale_log2, a, b);
-          again = !again && sum > kQfMost;                         // (after a look at the maximum it is at most 128)
-          if (!__any_sync(0xffffffffu, again)) break;
+          sum += part;
+          qf_st16(s_addr + uint32_t(c * 16), packed);              // over products that are read
         }
         l += sum;
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        tc5::st_wait();
         tc5::fence_before();
         __syncwarp();
-        if (lane == 0) {
-          tc5::mbar_arrive(&s_free[g]);                            // S_(n+1) may be written
-          tc5::mbar_arrive(&p_full[g]);
-        }
+        if (lane == 0) tc5::mbar_arrive(&p_full[g]);
       }
       if (alive) alive = wait_all(&o_full, 0, 29);
       tc5::fence_after();
