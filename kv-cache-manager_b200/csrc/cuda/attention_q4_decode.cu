@@ -1,23 +1,25 @@
 // Decode attention over a paged cache in 4 bits (layout and formulas: q4.cuh): one query row a request, bfloat16 rows.
 //
-// One block per (context partition, KV head x 8 query heads, request), four warps; a warp takes every fourth step of 32 keys of the
-// partition and needs no other warp until the end.  The products are transposed, so that the query heads are the 8 columns of an
-// m16n8k16 product and a group of at most eight heads wastes nothing of the 16 rows, which are keys (S^T = K Q^T) and then
-// elements of the head (O^T = V^T P^T):
-//   S^T: a lane's codes of a key are hd/4 elements in a row, any order of the contraction being as good as another if q is read
-//        in the same one; they enter as 128 + code (bfloat16, exact), and  q.k = scale (q.(128 + code)) + (zero - 128 scale) sum(q).
-//        In float32 the offset costs four bits of 24, in an error of a score of about 2e-5 at hd 128.
-//   O^T: an element of two neighbouring keys is one register (the words of the two keys, half by half), as code - 8 (exact), and
-//        sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters as the sum of two bfloat16 (16 bits): with one,
-//        its rounding would meet the offset zero, which the exact sum of p does not share, and double the error of the result.
+// One block per piece of work (keys of one request, KV head x 4 or 8 query heads), four warps; a warp takes every fourth step of 32
+// keys and needs no other warp until the end.  The products are transposed, so that the query heads are the columns of the
+// products and the rows are keys (S^T = K Q^T) and then elements of the head (O^T = V^T P^T): a group of few heads wastes little.
+//   S^T  in whole numbers, m16n8k32: a lane's codes of a key are hd/4 elements in a row (any order of the contraction is as good as
+//        another if q is read in the same one) and enter as they are, four to a register for one shift and two ands a word; q enters
+//        as 16-bit fixed point relative to its head's largest element, in two 8-bit halves that are two columns: four heads to a
+//        product.  Exact but for q's rounding, 2^-17 of its largest element, which moves a score by less than float32 sums of
+//        larger products would.   q.k = scale (q.code) + zero sum(q)  follows in float32.
+//   O^T  in float16, m16n8k16: an element of two neighbouring keys is one register (the words of the two keys, half by half), as
+//        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of the power of two
+//        above the largest scale that the warp has seen (a float16 below one), so a weight is rounded by 2^-12 of itself, and by
+//        2^-25 of the largest where it is smaller than 2^-14.
 //   P goes from accumulators to operands by a transposing register move (movmatrix): no shared memory in between.
-// Pages come by 16-byte asynchronous copies into a ring of steps per warp: no barriers between warps, pages of any size.
+// The scores of the next step are formed under the softmax of this one.  Pages come by 16-byte asynchronous copies into a ring of
+// steps per warp: no barriers between warps, pages of any size.
 //
-// What bounds it: a step of 32 keys at hd 128 is 4.25 KB of memory and about 480 warp instructions, 120 cycles of an SM's four
-// schedulers against 190 that the memory takes for it: memory, if enough warps are there to cover each other's latencies.
-// More than eight heads on one KV head: a block for each eight, which read the same pages from L2.
-// Partitions of a request: at most 8 are the blocks of one cluster and merge through distributed shared memory; more go
-// through scratch memory and a second kernel (as in attention_fast.cu).
+// Pieces of work: partitions of every request (of the grid), of which up to 8 are the blocks of a cluster that merges through
+// distributed shared memory, or equal shares of all requests' tiles of 128 keys, for batches of ragged or many requests: a share
+// begins and ends inside a request, the two pieces go through scratch memory, and a second kernel joins them.
+//
 #include <cooperative_groups.h>
 
 #include "attention_mma.cuh"
@@ -30,10 +32,13 @@ constexpr int kQ4Warps = 4;
 constexpr int kQ4DecodeThreads = 32 * kQ4Warps;
 constexpr int kQ4Step = 32;                        // keys of a warp's step
 constexpr int kQ4Tile = kQ4Step * kQ4Warps;        // keys of a round of the block
-constexpr int kQ4Heads = 8;                        // query heads of a block
+constexpr int kQ4Heads = 8;                        // most query heads of a block
 constexpr int kQ4TabMax = 512;                     // page-table entries of a partition kept in shared memory
 constexpr int kQ4ClusterParts = 8;
 constexpr float kQ4Lowest = 3.402823466e38f;
+// What it costs to start on a request and head, in tiles of 128 keys, for the shares: its table, its q, an empty ring.  (64 ragged
+// requests: 54 us without it, 47, 44 and 41 with 2, 4 and 6.)
+constexpr int kQ4Start = 6;
 
 struct DecodeQ4Params {
   const bf16* q; long long q_stride;
@@ -104,12 +109,16 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// D(16x8, float) += A(16x16, row) * B(16x8, col), both bfloat16 or both float16.  (Not volatile: the compiler may order them
-// among the unpacking of other operands.)
-__device__ __forceinline__ void mma_codes(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// D(16x8) += A(16x32 or 16x16, row) * B(.. x8, col): codes times 8-bit halves of q, float16 weights.  (Not volatile: the compiler may
+// order them among the unpacking of other operands.)
+__device__ __forceinline__ void mma_codes(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four 8-bit numbers as a register.
+__device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
+  return uint32_t(a & 255) | (uint32_t(b & 255) << 8) | (uint32_t(c & 255) << 16) | (uint32_t(d) << 24);
 }
 __device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -172,13 +181,14 @@ struct Q4Segment {
   int slot;                            // >= 0: where the partial result goes; < 0: the result itself
 };
 
-template <int HD, int STAGES, bool CAP>
-__global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_decode_q4_kernel(DecodeQ4Params p) {
+// HG: heads come in groups of four, one or two.  A lane of a warp has the sums of heads t4 and (second group) t4 + 4.
+template <int HD, int STAGES, bool CAP, int HG>
+__global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 : 3) attn_decode_q4_kernel(DecodeQ4Params p) {
   typedef Q4Shape<HD> S;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned* stab = reinterpret_cast<unsigned*>(smem_raw + q4_decode_core_smem<HD, STAGES>());     // pages of the head, in units of 16 bytes
   __shared__ int found[2];
-  const int G = p.nh / p.nkv, head_tiles = (G + kQ4Heads - 1) / kQ4Heads;
+  const int G = p.nh / p.nkv, head_tiles = (G + 4 * HG - 1) / (4 * HG);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   float* mo = reinterpret_cast<float*>(smem_raw);                  // after the key loop: [warps][8][HD]
   float* mm = mo + kQ4Warps * kQ4Heads * HD;                       // [warps][8] maximum
@@ -192,11 +202,12 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
   // The step's integers are there before the step's kernels; keys, also old ones, only behind the wait: a caller may have
   // written a whole prompt by the kernel before this one.
   auto first_key = [&](int ctx) { return ctx > 0 ? first_visible(ctx - 1, p.window, 0) : 0; };
-  auto tiles_of = [&](int ctx) { return (ctx - first_key(ctx) / kQ4Step * kQ4Step + kQ4Tile - 1) / kQ4Tile; };
+  // a request's cost for each head: its tiles of keys behind the start
+  auto cost_of = [&](int ctx) { return ctx > 0 ? kQ4Start + (ctx - first_key(ctx) / kQ4Step * kQ4Step + kQ4Tile - 1) / kQ4Tile : 0; };
   const int H = p.nkv * head_tiles;
   // ---- where the block's work starts
-  int seq, unit_h = 0, tile = 0;                                   // shares: request, head tile of it, tile of its keys
-  long long left = 0, U = 0, before = 0;                           // tiles left of the share; all tiles; those in front of `seq`, one head
+  int seq, unit_h = 0, at_cost = 0;                                // shares: request, head tile of it, how far in
+  long long left = 0, U = 0, before = 0;                           // cost left of the share; of all; of one head of the requests before
   long long takers = 0;                                            // blocks that have a share
   if (!shares) {
     seq = blockIdx.z;
@@ -206,7 +217,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
     const int per = (p.seqs + kQ4DecodeThreads - 1) / kQ4DecodeThreads;
     const int s0 = min(tid * per, p.seqs), s1 = min(s0 + per, p.seqs);
     int mine = 0;
-    for (int s = s0; s < s1; ++s) mine += tiles_of(p.seq_ctx_len[s]);
+    for (int s = s0; s < s1; ++s) mine += cost_of(p.seq_ctx_len[s]);
     int up = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -222,23 +233,23 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
       total += sums[w];
     }
     U = (long long)total * H;
-    takers = min((long long)gridDim.x, U);                         // (a block between two that share a request has a piece of it)
+    takers = min((long long)gridDim.x, U);                         // (a block between two that share a request then has a piece of it)
     if (blockIdx.x >= takers) { pdl_wait(); return; }
     const long long u0 = U * blockIdx.x / takers, u1 = U * (blockIdx.x + 1) / takers;
     left = u1 - u0;
     if ((long long)in_front * H <= u0 && u0 < (long long)(in_front + mine) * H) {
-      int s = s0, f = in_front, n = tiles_of(p.seq_ctx_len[s]);
-      while ((long long)(f + n) * H <= u0) { f += n; ++s; n = tiles_of(p.seq_ctx_len[s]); }
+      int s = s0, f = in_front, n = cost_of(p.seq_ctx_len[s]);
+      while ((long long)(f + n) * H <= u0) { f += n; ++s; n = cost_of(p.seq_ctx_len[s]); }
       found[0] = s;
       found[1] = f;
     }
     __syncthreads();
     seq = found[0];
     before = found[1];
-    const int n = tiles_of(p.seq_ctx_len[seq]);
+    const int n = cost_of(p.seq_ctx_len[seq]);
     const long long at = u0 - before * H;
     unit_h = int(at / n);
-    tile = int(at - (long long)unit_h * n);
+    at_cost = int(at - (long long)unit_h * n);
   }
   pdl_wait();
 
@@ -255,6 +266,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
     w.seq = seq;
     w.slot = -1;
     int of_h;
+    bool empty;
     if (!shares) {
       of_h = blockIdx.y;
       const int from = base + int(blockIdx.x) * p.part_size;
@@ -263,59 +275,99 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
       if (p.num_parts > 1 && !p.cluster_merge) w.slot = blockIdx.x;
     } else {
       of_h = unit_h;
-      const int n = tiles_of(ctx), take = int(min((long long)(n - tile), left));
-      w.begin = max(lo, base + tile * kQ4Tile);
-      w.end = min(ctx, base + (tile + take) * kQ4Tile);
-      if (take < n) w.slot = 2 * int(blockIdx.x) + (tile == 0 ? 1 : 0);
-      if (tile == 0 && tid == 0) {                                 // who reads the pieces of this request and head: blocks first .. last
+      const int n = cost_of(ctx), take = int(min((long long)(n - at_cost), left));
+      const int tile0 = max(0, at_cost - kQ4Start), tile1 = max(0, at_cost + take - kQ4Start);
+      w.begin = max(lo, base + tile0 * kQ4Tile);
+      w.end = min(ctx, base + tile1 * kQ4Tile);
+      empty = tile1 <= tile0;                                      // the start alone: the next block takes it
+      if (tile0 > 0 || tile1 < n - kQ4Start) w.slot = 2 * int(blockIdx.x) + (tile0 == 0 ? 1 : 0);
+      if (!empty && tile0 == 0 && tid == 0) {                      // who reads the pieces of this request and head: blocks first .. last
         const long long last_unit = before * H + (long long)unit_h * n + n - 1;
         p.part_first[(seq * H + unit_h) * 2] = blockIdx.x;
         p.part_first[(seq * H + unit_h) * 2 + 1] = int(((last_unit + 1) * takers - 1) / U);
       }
       left -= take;
-      tile += take;
-      if (tile == n) {
-        tile = 0;
+      at_cost += take;
+      if (at_cost == n) {
+        at_cost = 0;
         if (++unit_h == H) {
           unit_h = 0;
           before += n;
           if (left > 0)
-            do ++seq; while (p.seq_ctx_len[seq] <= 0);             // (there are more tiles, so there is such a request)
+            do ++seq; while (p.seq_ctx_len[seq] <= 0);             // (there is more, so there is such a request)
         }
+      }
+      if (empty) {
+        if (left <= 0) return;
+        continue;
       }
     }
     w.kvh = of_h / head_tiles;
     const int ht = of_h - w.kvh * head_tiles;
-    w.head0 = w.kvh * G + ht * kQ4Heads;
-    w.heads_here = min(kQ4Heads, G - ht * kQ4Heads);
+    w.head0 = w.kvh * G + ht * 4 * HG;
+    w.heads_here = min(4 * HG, G - ht * 4 * HG);
 
-    // heads 2 t4, 2 t4 + 1; sums over this lane's keys (the maximum starts finite: no difference to it is not-a-number)
+    // heads t4, t4 + 4; sums over this lane's keys (the maximum starts finite: no difference to it is not-a-number)
     float m[2] = {-kQ4Lowest, -kQ4Lowest}, l[2] = {0.f, 0.f}, zacc[2] = {0.f, 0.f};
     float o[S::kTiles][4];
 #pragma unroll
     for (int i = 0; i < S::kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     uint32_t unit = 0x00800000u;                                   // the power of two that weights are divided by, as a float's bits
     if (w.begin < w.end) {
-      // ---- q of head g as the second operand: elements in the order in which a lane's codes lie
-      uint32_t qb[S::kKeyWords][4];
-      float qs[2];                                                 // sum of q over the elements, heads 2 t4 and 2 t4 + 1
-      {
-        float sum = 0.f;
-        const bf16* row = p.q + size_t(w.seq) * p.q_stride + size_t(w.head0 + g) * HD;
+      // ---- q as the second operand: column g of group h is half g % 2 of head 4 h + g / 2, elements in the order in which a lane's
+      // codes lie (of a word's eight, bytes 0, 4, 1, 5 and 2, 6, 3, 7)
+      uint32_t qb[HG][S::kKeyWords][2];
+      float step[HG], qs[HG];                                      // of heads t4 (+ 4): what q's whole numbers count, sum of q; times scale
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        const int head = 4 * h + (g >> 1);
+        const bf16* row = p.q + size_t(w.seq) * p.q_stride + size_t(w.head0 + head) * HD;
+        uint4 v[S::kKeyWords];
+        float sum = 0.f, largest = 0.f;
+        int bad = 0;
 #pragma unroll
         for (int i = 0; i < S::kKeyWords; ++i) {
           const int word = (S::kKeyWords % 4 == 0) ? (i / 4) * 16 + t4 * 4 + (i & 3) : t4 * S::kKeyWords + i;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (g < w.heads_here) v = *reinterpret_cast<const uint4*>(row + word * 8);
-          qb[i][0] = v.x; qb[i][1] = v.y; qb[i][2] = v.z; qb[i][3] = v.w;
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (head < w.heads_here) v[i] = *reinterpret_cast<const uint4*>(row + word * 8);
+          const uint32_t e[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum += __uint_as_float(qb[i][e] << 16) + __uint_as_float(qb[i][e] & 0xffff0000u);
+          for (int j = 0; j < 4; ++j) {
+            const float lo16 = __uint_as_float(e[j] << 16), hi16 = __uint_as_float(e[j] & 0xffff0000u);
+            sum += lo16 + hi16;
+            largest = fmaxf(largest, fmaxf(fabsf(lo16), fabsf(hi16)));
+            bad |= !(fabsf(lo16) <= kQ4Lowest) || !(fabsf(hi16) <= kQ4Lowest);
+          }
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int off = 1; off <= 2; off *= 2) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, off);
+          largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, off));
+          bad |= __shfl_xor_sync(0xffffffffu, bad, off);
+        }
+        // whole numbers up to 127 * 256 in size; halves of -128 .. 127
+        const float unit_q = fmaxf(largest * (1.f / 32512.f), 1.17549435e-38f), per = 1.f / unit_q;
+#pragma unroll
+        for (int i = 0; i < S::kKeyWords; ++i) {
+          const uint32_t e[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          int n[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            n[2 * j] = __float2int_rn(__uint_as_float(e[j] << 16) * per);
+            n[2 * j + 1] = __float2int_rn(__uint_as_float(e[j] & 0xffff0000u) * per);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int high = (n[j] + 128) >> 8;
+            n[j] = (g & 1) ? n[j] - high * 256 : high;
+          }
+          qb[h][i][0] = bytes4(n[0], n[4], n[1], n[5]);
+          qb[h][i][1] = bytes4(n[2], n[6], n[3], n[7]);
+        }
         const float unit_of_scores = CAP ? 1.f : p.scale_log2;
-        qs[0] = __shfl_sync(0xffffffffu, sum, t4 * 8) * unit_of_scores;
-        qs[1] = __shfl_sync(0xffffffffu, sum, t4 * 8 + 4) * unit_of_scores;
+        const float mine = bad ? __int_as_float(0x7fffffff) : unit_q;      // an element that is not finite: no score is
+        step[h] = __shfl_sync(0xffffffffu, mine, t4 * 8) * unit_of_scores;
+        qs[h] = __shfl_sync(0xffffffffu, sum, t4 * 8) * unit_of_scores;
       }
       const int* table = p.block_tables + size_t(w.seq) * p.max_blocks;
       // rounds of 128 keys; as many at a time as the table slice has pages for
@@ -382,8 +434,8 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
 #pragma unroll
         for (int i = 0; i < STAGES - 1; ++i) load_step();
 
-        // scores of a step in log2 units: x[16 keys][key g, head 2 t4 | 2 t4 + 1; key g + 8]
-        auto scores = [&](const unsigned char* st, float (&x)[2][4]) {
+        // scores of a step in log2 units: x[16 keys][key g, key g + 8][head t4, t4 + 4]
+        auto scores = [&](const unsigned char* st, float (&x)[2][2][HG]) {
           const uint32_t* kpair = reinterpret_cast<const uint32_t*>(st + 2 * S::kCodeBytes);
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
@@ -408,33 +460,35 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
                 kb[j] = *reinterpret_cast<const uint32_t*>(st + S::at(rb, 0) + (t4 * S::kKeyWords + j) * 4);
               }
             }
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            // sums start at 1.5 * 2^23 as a float's bits: a float again without a conversion (they stay below 2^22)
+            int c[HG][4];
 #pragma unroll
-            for (int j = 0; j < S::kKeyWords; ++j)
+            for (int h = 0; h < HG; ++h) c[h][0] = c[h][1] = c[h][2] = c[h][3] = 0x4b400000;
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t a[4] = {q4::two_codes_128(ka[j], 2 * h), q4::two_codes_128(kb[j], 2 * h), q4::two_codes_128(ka[j], 2 * h + 1),
-                                       q4::two_codes_128(kb[j], 2 * h + 1)};
-                mma_codes(c, a, qb[j][2 * h], qb[j][2 * h + 1]);
-              }
+            for (int j = 0; j < S::kKeyWords; ++j) {
+              const uint32_t a0 = ka[j] & 0x0f0f0f0fu, a1 = kb[j] & 0x0f0f0f0fu, a2 = (ka[j] >> 4) & 0x0f0f0f0fu, a3 = (kb[j] >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+              for (int h = 0; h < HG; ++h) mma_codes(c[h], a0, a1, a2, a3, qb[h][j][0], qb[h][j][1]);
+            }
             const uint32_t pa = kpair[ra], pb = kpair[rb];
-            float sa = q4::scale_of(pa), sb = q4::scale_of(pb);
-            const float za = fmaf(-128.f, sa, q4::zero_of(pa)), zb = fmaf(-128.f, sb, q4::zero_of(pb));
-            if constexpr (!CAP) { sa *= p.scale_log2; sb *= p.scale_log2; }
-            x[mt][0] = fmaf(sa, c[0], za * qs[0]);
-            x[mt][1] = fmaf(sa, c[1], za * qs[1]);
-            x[mt][2] = fmaf(sb, c[2], zb * qs[0]);
-            x[mt][3] = fmaf(sb, c[3], zb * qs[1]);
-            if constexpr (CAP) {
+            const float sa = q4::scale_of(pa), sb = q4::scale_of(pb), za = q4::zero_of(pa), zb = q4::zero_of(pb);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) x[mt][j] = fast_tanh(x[mt][j] * p.cap_pre) * p.scale_log2;
+            for (int h = 0; h < HG; ++h) {
+              const float na = fmaf(256.f, __int_as_float(c[h][0]) - 12582912.f, __int_as_float(c[h][1]) - 12582912.f);
+              const float nb = fmaf(256.f, __int_as_float(c[h][2]) - 12582912.f, __int_as_float(c[h][3]) - 12582912.f);
+              x[mt][0][h] = fmaf(sa * na, step[h], za * qs[h]);
+              x[mt][1][h] = fmaf(sb * nb, step[h], zb * qs[h]);
+              if constexpr (CAP) {
+                x[mt][0][h] = fast_tanh(x[mt][0][h] * p.cap_pre) * p.scale_log2;
+                x[mt][1][h] = fast_tanh(x[mt][1][h] * p.cap_pre) * p.scale_log2;
+              }
             }
           }
         };
         // The scores of step i + 1 are formed while the softmax of step i, whose steps wait for one another, is under way.
         const unsigned char* st = ring;
         int key0 = at + warp * kQ4Step;
-        float x[2][4], ahead[2][4];
+        float x[2][2][HG], ahead[2][2][HG];
         if (steps > 0) {
           cp_async_wait<STAGES - 2>();
           __syncwarp();
@@ -449,46 +503,52 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[mt][j] = ahead[mt][j];
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int h = 0; h < HG; ++h) x[mt][k][h] = ahead[mt][k][h];
           if (key0 < w.begin || key0 + kQ4Step > w.end) {
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int key = key0 + mt * 16 + row_g + (j >> 1) * 8;
-                x[mt][j] = key >= w.begin && key < w.end ? x[mt][j] : -INFINITY;
+              for (int k = 0; k < 2; ++k) {
+                const int key = key0 + mt * 16 + row_g + k * 8;
+#pragma unroll
+                for (int h = 0; h < HG; ++h) x[mt][k][h] = key >= w.begin && key < w.end ? x[mt][k][h] : -INFINITY;
               }
           }
           scores(next, ahead);                                     // (behind the last step: of what lies there, and nobody reads it)
           // ---- running maximum; and the unit of the weights: the power of two above the largest scale so far
-          float top[2], grown[2];
+          float top[HG];
+          bool moved = false;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            top[h] = fmaxf(fmaxf(x[0][h], x[0][h + 2]), fmaxf(x[1][h], x[1][h + 2]));
+          for (int h = 0; h < HG; ++h) {
+            top[h] = fmaxf(fmaxf(x[0][0][h], x[0][1][h]), fmaxf(x[1][0][h], x[1][1][h]));
             top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 4));
             top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 8));
             top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 16));
+            moved |= top[h] > m[h];
           }
           const uint32_t largest = __reduce_max_sync(0xffffffffu, vpair[lane] << 16);
-          if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1] || largest >= unit)) {
+          if (__any_sync(0xffffffffu, moved || largest >= unit)) {
+            float grown[HG], f = 1.f;
+            if (largest >= unit) {
+              const uint32_t unit_new = min((largest & 0x7f800000u) + 0x00800000u, 0x7f000000u);
+              f = __uint_as_float(unit) / __uint_as_float(unit_new);
+              unit = unit_new;
+            }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < HG; ++h) {
               const float m_new = fmaxf(m[h], top[h]);
               grown[h] = fast_exp2(m[h] - m_new);                  // (zero where nothing was seen yet)
               m[h] = m_new;
               l[h] *= grown[h];
               zacc[h] *= grown[h];
-            }
-            if (largest >= unit) {
-              const uint32_t unit_new = min((largest & 0x7f800000u) + 0x00800000u, 0x7f000000u);
-              const float f = __uint_as_float(unit) / __uint_as_float(unit_new);
-              grown[0] *= f;
-              grown[1] *= f;
-              unit = unit_new;
+              grown[h] *= f;
             }
 #pragma unroll
             for (int k = 0; k < S::kTiles; ++k) {
-              o[k][0] *= grown[0]; o[k][1] *= grown[1]; o[k][2] *= grown[0]; o[k][3] *= grown[1];
+              o[k][0] *= grown[0]; o[k][2] *= grown[0];
+              if constexpr (HG == 2) { o[k][1] *= grown[1]; o[k][3] *= grown[1]; }
             }
           }
           const float per_unit = __uint_as_float(0x7f000000u - unit);         // 1 / unit
@@ -497,14 +557,18 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
             const uint32_t pa = vpair[mt * 16 + row_g], pb = vpair[mt * 16 + row_g + 8];
             const float sa = q4::scale_of(pa), za = fmaf(8.f, sa, q4::zero_of(pa));
             const float sb = q4::scale_of(pb), zb = fmaf(8.f, sb, q4::zero_of(pb));
-            const float e0 = fast_exp2(x[mt][0] - m[0]), e1 = fast_exp2(x[mt][1] - m[1]);
-            const float e2 = fast_exp2(x[mt][2] - m[0]), e3 = fast_exp2(x[mt][3] - m[1]);
-            l[0] += e0 + e2;
-            l[1] += e1 + e3;
-            zacc[0] = fmaf(e0, za, fmaf(e2, zb, zacc[0]));
-            zacc[1] = fmaf(e1, za, fmaf(e3, zb, zacc[1]));
             const float ua = sa * per_unit, ub = sb * per_unit;
-            const uint32_t b0 = transposed(pack_half(e0 * ua, e1 * ua)), b1 = transposed(pack_half(e2 * ub, e3 * ub));
+            float wa[2] = {0.f, 0.f}, wb[2] = {0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+              const float ea = fast_exp2(x[mt][0][h] - m[h]), eb = fast_exp2(x[mt][1][h] - m[h]);
+              l[h] += ea + eb;
+              zacc[h] = fmaf(ea, za, fmaf(eb, zb, zacc[h]));
+              wa[h] = ea * ua;
+              wb[h] = eb * ub;
+            }
+            // columns of O: 2 t4 is head t4, 2 t4 + 1 head t4 + 4 (of one group: nobody)
+            const uint32_t b0 = transposed(pack_half(wa[0], wa[1])), b1 = transposed(pack_half(wb[0], wb[1]));
             // ---- values: keys 2 t4, 2 t4 + 1 and the same eight further
             const unsigned char* vt = st + S::kCodeBytes;
             const int r0 = mt * 16 + row_a, r1 = mt * 16 + row_b;
@@ -571,8 +635,8 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
         zacc[h] += __shfl_xor_sync(0xffffffffu, zacc[h], off);
       }
     const float f_low = __uint_as_float(unit), f_high = f_low * 0.0625f;
-    float* row0 = mo + (warp * kQ4Heads + 2 * t4) * HD;
-    float* row1 = row0 + HD;
+    float* row0 = mo + (warp * kQ4Heads + t4) * HD;
+    float* row1 = row0 + 4 * HD;
 #pragma unroll
     for (int j = 0; j < S::kFull; ++j)
 #pragma unroll
@@ -581,7 +645,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
         const float f = (k & 1) ? f_high : f_low;
         const float (&c)[4] = o[4 * j + k];
         *reinterpret_cast<float2*>(row0 + d) = make_float2(fmaf(c[0], f, zacc[0]), fmaf(c[2], f, zacc[0]));
-        *reinterpret_cast<float2*>(row1 + d) = make_float2(fmaf(c[1], f, zacc[1]), fmaf(c[3], f, zacc[1]));
+        if constexpr (HG == 2) *reinterpret_cast<float2*>(row1 + d) = make_float2(fmaf(c[1], f, zacc[1]), fmaf(c[3], f, zacc[1]));
       }
     if constexpr (S::kHalf) {
 #pragma unroll
@@ -589,12 +653,12 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD <= 128 ? 3 : 2) attn_deco
         const int d = 8 * (8 * S::kFull + (g >> 1)) + 4 * k + (g & 1);
         const float (&c)[4] = o[4 * S::kFull + k];
         row0[d] = fmaf(c[0], f_low, zacc[0]); row0[d + 2] = fmaf(c[2], f_high, zacc[0]);
-        row1[d] = fmaf(c[1], f_low, zacc[1]); row1[d + 2] = fmaf(c[3], f_high, zacc[1]);
+        if constexpr (HG == 2) { row1[d] = fmaf(c[1], f_low, zacc[1]); row1[d + 2] = fmaf(c[3], f_high, zacc[1]); }
       }
     }
     if (g == 0) {
-      mm[warp * kQ4Heads + 2 * t4] = m[0]; mm[warp * kQ4Heads + 2 * t4 + 1] = m[1];
-      ml[warp * kQ4Heads + 2 * t4] = l[0]; ml[warp * kQ4Heads + 2 * t4 + 1] = l[1];
+      mm[warp * kQ4Heads + t4] = m[0]; mm[warp * kQ4Heads + t4 + 4] = m[1];
+      ml[warp * kQ4Heads + t4] = l[0]; ml[warp * kQ4Heads + t4 + 4] = l[1];
     }
     __syncthreads();
     // ---- the four warps, four adjacent elements an item
@@ -662,70 +726,134 @@ __global__ void attn_decode_q4_merge_kernel(const float* part_o, const float* pa
   }
 }
 
-// The pieces of a request and eight heads that blocks part_first[0] .. part_first[1] have left, in their order: the first block's
-// lies in its second place, the others' in their first.
+// The pieces of a request and its four or eight heads that blocks part_first[0] .. part_first[1] have left, in their order: the first
+// block's lies in its second place, the others' in their first.  A long request has many: the weights of 128 of them at a time are
+// formed side by side, so that what follows one another is additions.
+constexpr int kQ4JoinAtOnce = 128;
 __global__ void __launch_bounds__(128) attn_decode_q4_shares_kernel(const float* part_o, const float* part_ml, const int* part_first,
                                                                     const int* __restrict__ seq_ctx_len, bf16* __restrict__ out,
-                                                                    long long out_stride, int nh, int nkv, int hd, const float* __restrict__ sink) {
+                                                                    long long out_stride, int nh, int nkv, int hd, int tile_heads,
+                                                                    const float* __restrict__ sink) {
+  __shared__ float weight[kQ4JoinAtOnce][kQ4Heads];
+  __shared__ float tops[4][kQ4Heads], all_top[kQ4Heads], all_sum[kQ4Heads];
   pdl_launch_dependents();
   pdl_wait();
-  const int G = nh / nkv, head_tiles = (G + kQ4Heads - 1) / kQ4Heads, H = nkv * head_tiles;
+  const int G = nh / nkv, head_tiles = (G + tile_heads - 1) / tile_heads, H = nkv * head_tiles;
   const int seq = blockIdx.x, h = blockIdx.y, kvh = h / head_tiles, ht = h - kvh * head_tiles;
-  const int head0 = kvh * G + ht * kQ4Heads, heads_here = min(kQ4Heads, G - ht * kQ4Heads);
-  const bool empty = seq_ctx_len[seq] <= 0;
-  const int first = empty ? 0 : part_first[(seq * H + h) * 2], last = empty ? 0 : part_first[(seq * H + h) * 2 + 1];
-  if (!empty && first == last) return;                             // one block had it all
-  const int quads = hd / 4;
-  for (int it = threadIdx.x; it < heads_here * quads; it += 128) {
-    const int r = it / quads, d = (it - r * quads) * 4;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f, top = -INFINITY;
-    if (!empty) {
-      for (int b = first; b <= last; ++b) top = fmaxf(top, part_ml[(size_t(2 * b + (b == first)) * kQ4Heads + r) * 2]);
-      for (int b = first; b <= last; ++b) {
-        const size_t at = size_t(2 * b + (b == first)) * kQ4Heads + r;
-        const float lb = part_ml[at * 2 + 1];
-        if (lb == 0.f) continue;
-        const float f = fast_exp2(part_ml[at * 2] - top);
-        const float4 v = *reinterpret_cast<const float4*>(part_o + at * hd + d);
-        acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
-        sum = fmaf(f, lb, sum);
-      }
-      if (sink && sum != 0.f) sum += fast_exp2(sink[head0 + r] * 1.4426950408889634f - top);
+  const int head0 = kvh * G + ht * tile_heads, heads_here = min(tile_heads, G - ht * tile_heads);
+  const int tid = threadIdx.x, quads = hd / 4, items = heads_here * quads;
+  if (seq_ctx_len[seq] <= 0) {
+    for (int it = tid; it < items; it += 128) {
+      const int r = it / quads, d = (it - r * quads) * 4;
+      *reinterpret_cast<uint2*>(out + size_t(seq) * out_stride + size_t(head0 + r) * hd + d) = make_uint2(0u, 0u);
     }
+    return;
+  }
+  const int first = part_first[(seq * H + h) * 2], pieces = part_first[(seq * H + h) * 2 + 1] - first + 1;
+  if (pieces == 1) return;                                         // one block had it all
+  auto at = [&](int i, int r) { return size_t(2 * (first + i) + (i == 0)) * kQ4Heads + r; };
+  // the largest maximum of every head
+  {
+    const int r = tid & 7;
+    float top = -INFINITY;
+    if (r < heads_here)
+      for (int i = tid >> 3; i < pieces; i += 16) top = fmaxf(top, part_ml[at(i, r) * 2]);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    if ((tid & 31) < 8) tops[tid >> 5][r] = top;
+    __syncthreads();
+    if (tid < 8) {
+      all_top[tid] = fmaxf(fmaxf(tops[0][tid], tops[1][tid]), fmaxf(tops[2][tid], tops[3][tid]));
+      all_sum[tid] = 0.f;
+    }
+    __syncthreads();
+  }
+  constexpr int kMost = kQ4Heads * 256 / 4 / 128;                  // items of a thread
+  float4 acc[kMost];
+#pragma unroll
+  for (int k = 0; k < kMost; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < pieces; i0 += kQ4JoinAtOnce) {
+    const int n = min(kQ4JoinAtOnce, pieces - i0);
+    for (int j = tid; j < n * kQ4Heads; j += 128) {
+      const int i = j >> 3, r = j & 7;
+      float w = 0.f;
+      if (r < heads_here) {
+        const float l = part_ml[at(i0 + i, r) * 2 + 1];
+        w = l == 0.f ? 0.f : fast_exp2(part_ml[at(i0 + i, r) * 2] - all_top[r]);
+      }
+      weight[i][r] = w;
+    }
+    __syncthreads();
+    if (tid < heads_here) {                                        // (one thread a head: the sums keep their order)
+      float sum = all_sum[tid];
+      for (int i = 0; i < n; ++i) sum = fmaf(weight[i][tid], part_ml[at(i0 + i, tid) * 2 + 1], sum);
+      all_sum[tid] = sum;
+    }
+#pragma unroll
+    for (int k = 0; k < kMost; ++k) {
+      const int it = tid + k * 128;
+      if (it >= items) break;
+      const int r = it / quads, d = (it - r * quads) * 4;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float f = weight[i][r];
+        const float4 v = *reinterpret_cast<const float4*>(part_o + at(i0 + i, r) * hd + d);
+        acc[k].x = fmaf(f, v.x, acc[k].x); acc[k].y = fmaf(f, v.y, acc[k].y); acc[k].z = fmaf(f, v.z, acc[k].z); acc[k].w = fmaf(f, v.w, acc[k].w);
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < kMost; ++k) {
+    const int it = tid + k * 128;
+    if (it >= items) break;
+    const int r = it / quads, d = (it - r * quads) * 4;
+    float sum = all_sum[r];
+    if (sink && sum != 0.f) sum += fast_exp2(sink[head0 + r] * 1.4426950408889634f - all_top[r]);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    bf16* dst = out + size_t(seq) * out_stride + size_t(head0 + r) * hd + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(out + size_t(seq) * out_stride + size_t(head0 + r) * hd + d) =
+        make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv), pack_bf16(acc[k].z * inv, acc[k].w * inv));
   }
 }
 
-template <int HD> constexpr int q4_decode_stages() { return HD <= 128 ? 4 : 3; }
+// Steps in flight.  Four blocks of three an SM for one group of heads at 128 registers a thread; two groups want 168, and then
+// three blocks of four steps.  (64 requests of 8,192 keys, 8 KV heads of 128: 112 us with four blocks, 121 with three; 8 requests of
+// 1,536, 4 KV heads of 64 with eight query heads each: 8.6 and 7.9.)
+template <int HD, int HG> constexpr int q4_decode_stages() { return HD > 128 || HG == 1 ? 3 : 4; }
 
-template <int HD, bool CAP>
-int launch_decode_q4(const DecodeQ4Params& p, int shares, cudaStream_t s) {
-  constexpr int STAGES = q4_decode_stages<HD>();
-  auto kernel = attn_decode_q4_kernel<HD, STAGES, CAP>;
+// Query heads of a block: four where a KV head has no more, else eight.
+inline int q4_tile_heads(int nh, int nkv) { return nh / nkv <= 4 ? 4 : 8; }
+
+template <int HD, bool CAP, int HG>
+int launch_decode_q4_as(const DecodeQ4Params& p, int shares, cudaStream_t s) {
+  constexpr int STAGES = q4_decode_stages<HD, HG>();
+  auto kernel = attn_decode_q4_kernel<HD, STAGES, CAP, HG>;
   constexpr size_t smem = q4_decode_smem<HD, STAGES>();
   static OncePerDevice once;
   if (smem > 48 * 1024) {
     const int rc = allow_shared_memory(once, kernel, smem);
     if (rc != 0) return rc;
   }
-  const int G = p.nh / p.nkv;
-  const dim3 grid = p.num_parts == 0 ? dim3(shares) : dim3(p.num_parts, p.nkv * ((G + kQ4Heads - 1) / kQ4Heads), p.seqs);
+  const int tiles = (p.nh / p.nkv + 4 * HG - 1) / (4 * HG);
+  const dim3 grid = p.num_parts == 0 ? dim3(shares) : dim3(p.num_parts, p.nkv * tiles, p.seqs);
   if (p.cluster_merge) return pdl_launch_cluster(kernel, grid, dim3(kQ4DecodeThreads), smem, s, p.num_parts, p);
   return pdl_launch(kernel, grid, dim3(kQ4DecodeThreads), smem, s, p);
 }
+template <int HD, bool CAP>
+int launch_decode_q4(const DecodeQ4Params& p, int shares, cudaStream_t s) {
+  return q4_tile_heads(p.nh, p.nkv) == 4 ? launch_decode_q4_as<HD, CAP, 1>(p, shares, s) : launch_decode_q4_as<HD, CAP, 2>(p, shares, s);
+}
 
-template <int HD> int q4_blocks_per_sm() {
-  constexpr int STAGES = q4_decode_stages<HD>();
-  auto kernel = attn_decode_q4_kernel<HD, STAGES, false>;
+template <int HD, int HG> int q4_blocks_per_sm_of() {
+  constexpr int STAGES = q4_decode_stages<HD, HG>();
+  auto kernel = attn_decode_q4_kernel<HD, STAGES, false, HG>;
   constexpr size_t smem = q4_decode_smem<HD, STAGES>();
   int n = 0;
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess) return 0;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kQ4DecodeThreads, smem) != cudaSuccess) return 0;
   return n;
 }
+template <int HD> int q4_blocks_per_sm(int groups) { return groups == 1 ? q4_blocks_per_sm_of<HD, 1>() : q4_blocks_per_sm_of<HD, 2>(); }
 
 #define KVCM_FOR_Q4_HEAD_DIMS(X) X(32) X(64) X(96) X(128) X(160) X(192) X(224) X(256)
 
@@ -736,9 +864,9 @@ using namespace kvcm;
 // 1 if the tensor-core kernels take this head size.
 KVCM_API int kvcm_attention_q4_decode_supports(int hd) { return hd > 0 && hd <= 256 && hd % 32 == 0; }
 
-// Blocks of the kernel that an SM of the current device holds at once (0: it cannot say).
-KVCM_API int kvcm_attention_decode_q4_blocks_per_sm(int hd) {
-#define X(N) if (hd == N) return q4_blocks_per_sm<N>();
+// Blocks of the kernel that an SM of the current device holds at once (0: it cannot say), for heads in one or two groups of four.
+KVCM_API int kvcm_attention_decode_q4_blocks_per_sm(int hd, int groups) {
+#define X(N) if (hd == N) return q4_blocks_per_sm<N>(groups);
   KVCM_FOR_Q4_HEAD_DIMS(X)
 #undef X
   return 0;
@@ -747,7 +875,7 @@ KVCM_API int kvcm_attention_decode_q4_blocks_per_sm(int hd) {
 // num_parts > 0: that many partitions of part_size keys (a multiple of 128) cover [first visible key rounded down to 32, context).
 // More than 8 of them, or cluster_merge == 0, want scratch: seqs * nh * num_parts * (hd + 2) floats.
 // num_parts == 0: `shares` blocks take equal shares of all requests' and heads' tiles of 128 keys, and a second kernel joins what
-// was cut; scratch: shares * 16 * (hd + 2) floats, then seqs * nkv * ceil(nh / nkv / 8) * 2 ints.
+// was cut; scratch: shares * 16 * (hd + 2) floats, then seqs * nh * 2 ints.
 KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, void* out, long long out_stride, const void* k_cache,
                                            const void* v_cache, int num_pages, const int* block_tables, int max_blocks,
                                            const int* seq_ctx_len, int seqs, int nh, int nkv, int hd, int block_size, float scale,
@@ -765,7 +893,7 @@ KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, vo
   if (q4::page_bytes(block_size, hd) / 16 * (unsigned long long)num_pages * nkv > 0xffffffffull) return KVCM_ERR_UNSUPPORTED;
   if (num_parts == 0 || num_parts > kQ4ClusterParts || num_parts < 2) cluster_merge = 0;
   if (num_parts != 1 && !cluster_merge && (scratch == nullptr || (reinterpret_cast<uintptr_t>(scratch) & 15))) return KVCM_ERR_UNSUPPORTED;
-  const int head_tiles = (nh / nkv + kQ4Heads - 1) / kQ4Heads;
+  const int tile_heads = q4_tile_heads(nh, nkv), head_tiles = (nh / nkv + tile_heads - 1) / tile_heads;
   const size_t pieces = num_parts == 0 ? size_t(shares) * 2 * kQ4Heads : size_t(seqs) * nh * num_parts;
   DecodeQ4Params p;
   p.q = (const bf16*)q; p.q_stride = q_stride; p.out = (bf16*)out; p.out_stride = out_stride;
@@ -787,7 +915,7 @@ KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, vo
   if (rc != 0 || num_parts == 1 || cluster_merge) return rc;
   if (num_parts == 0)
     return pdl_launch(attn_decode_q4_shares_kernel, dim3(seqs, nkv * head_tiles), dim3(128), 0, (cudaStream_t)stream, (const float*)p.part_o,
-                      (const float*)p.part_ml, (const int*)p.part_first, seq_ctx_len, p.out, out_stride, nh, nkv, hd, sink);
+                      (const float*)p.part_ml, (const int*)p.part_first, seq_ctx_len, p.out, out_stride, nh, nkv, hd, tile_heads, sink);
   return pdl_launch(attn_decode_q4_merge_kernel, dim3(seqs, nh), dim3(hd < 64 ? 32 : 64), 0, (cudaStream_t)stream, (const float*)p.part_o,
                     (const float*)p.part_ml, p.out, out_stride, nh, hd, num_parts, p.sink);
 }

@@ -741,28 +741,35 @@ Q4_PART_KEYS = 128          # four warps with a step of 32 keys each
 
 
 def decode_partitions_q4(seqs: int, nh: int, nkv: int, hd: int, max_ctx: int, device: int, force_parts: int = 0):
-    """How ``attention_decode_q4`` splits the context: (keys per partition, number of partitions), no partitions for equal shares."""
+    """How ``attention_decode_q4`` splits the context: (keys per partition, number of partitions), no partitions for equal shares.
+
+    As many partitions as a cluster merges and the GPU holds at once (an eighth more: not all are full), none for up to 256 keys;
+    where they would be longer than 1,024 keys, equal shares of all requests' keys.  B200, microseconds, heads of 128, 8 KV heads,
+    partitions | shares: 4 requests up to 2,048 keys 8.7 | 14, 32 of 1,024 15 | 23, 16 ragged ones up to 8,192 34 | 30, 64 of them
+    62 | 41, 64 of 8,192 117 | 112; 148 keys of one request: one partition 4.8, two 5.5."""
     max_ctx = max(max_ctx, 1)
-    blocks = max(1, seqs * nkv * ((nh // nkv + 7) // 8))
+    heads = 4 if nh <= 4 * nkv else 8
+    blocks = max(1, seqs * nkv * ((nh // nkv + heads - 1) // heads))
     most = (max_ctx + Q4_PART_KEYS - 1) // Q4_PART_KEYS
     if force_parts < 0:
         return Q4_PART_KEYS, 0
     if force_parts > 0:
         parts = min(force_parts, most)
     else:
-        parts = max(1, min(_q4_resident_blocks(hd, device) // blocks, most))
-        if parts > CLUSTER_PARTS:
-            parts = max(CLUSTER_PARTS, min(parts, (max_ctx + 511) // 512))
+        room = _q4_resident_blocks(hd, heads // 4, device) * 9 // 8 // blocks
+        parts = max(1, min(CLUSTER_PARTS, room, most if max_ctx > 2 * Q4_PART_KEYS else 1))
     size = ((max_ctx + parts - 1) // parts + Q4_PART_KEYS - 1) // Q4_PART_KEYS * Q4_PART_KEYS
+    if force_parts == 0 and size > 1024:
+        return Q4_PART_KEYS, 0
     return size, (max_ctx + size - 1) // size
 
 
-def _q4_resident_blocks(hd: int, device: int) -> int:
-    key = ("q4", hd, device)
+def _q4_resident_blocks(hd: int, groups: int, device: int) -> int:
+    key = ("q4", hd, groups, device)
     n = _RESIDENT.get(key)
     if n is None:
         with torch.cuda.device(device):
-            n = max(int(_lib().kvcm_attention_decode_q4_blocks_per_sm(int(hd))), 1) * sm_count(torch.device("cuda", device))
+            n = max(int(_lib().kvcm_attention_decode_q4_blocks_per_sm(int(hd), int(groups))), 1) * sm_count(torch.device("cuda", device))
         _RESIDENT[key] = n
     return n
 
@@ -796,8 +803,8 @@ def attention_decode_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tenso
     in_cluster = 1 < parts <= CLUSTER_PARTS and ctx.options.get("attn_merge", "cluster") == "cluster"
     scratch, shares = None, 0
     if parts == 0:
-        shares = _q4_resident_blocks(hd, device)
-        scratch = torch.empty(shares * 16 * (hd + 2) + S * nkv * ((nh // nkv + 7) // 8) * 2, dtype=torch.float32, device=q.device)
+        shares = _q4_resident_blocks(hd, 1 if nh <= 4 * nkv else 2, device)
+        scratch = torch.empty(shares * 16 * (hd + 2) + S * nh * 2, dtype=torch.float32, device=q.device)
     elif parts > 1 and not in_cluster:
         scratch = torch.empty(S * nh * parts * (hd + 2), dtype=torch.float32, device=q.device)
     rc = _DECODE_Q4(device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
@@ -831,9 +838,9 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                          ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
                          sink: Optional[torch.Tensor] = None) -> None:
     """Rows of portions longer than one token over a cache in 4 bits; q and out are the step's full bfloat16 row arrays, ``ctx`` has
-    the step's arrays with tiles of 64 rows (tiles of request -1 are none).  Heads of 64 and 128 elements: one kernel that unpacks
-    pages beside the products.  Other heads, or ``ctx.options['attn_prefill'] == 'unpack'``: the pages that the portions see are
-    laid out in bfloat16 (in scratch of the call) and read by ``attention_prefill``."""
+    the step's arrays with tiles of 64 rows (tiles of request -1 are none).  Heads of 128 elements, and of 64 with up to 2,048 keys: one
+    kernel that unpacks pages beside the products.  Else, or where ``ctx.options['attn_prefill']`` is 'unpack', the pages that the
+    portions see are laid out in bfloat16 (in scratch of the call) and read by ``attention_prefill``.  ('fused' forces the one kernel.)"""
     name = "attention_prefill_q4"
     _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink)
     S = ctx.seq_ctx_len.numel()
@@ -853,7 +860,11 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
     first, seqs = ctx.decode_seqs, S - ctx.decode_seqs
     if seqs <= 0 or ctx.prefill_tiles == 0:
         return
-    if hd in (64, 128) and ctx.options.get("attn_prefill", "auto") != "unpack":
+    # At 64 elements a head the products are half as long and the kernel over bfloat16 pages runs two blocks an SM: behind long
+    # contexts laying out the pages pays (four portions behind 3,000 keys: 219 us against 255; 2,048 rows of one request: 57 both;
+    # 148 rows: 12 against 10).  At 128 elements it never did (100 rows behind 2,000 keys, three requests: 93 against 57).
+    how = ctx.options.get("attn_prefill", "auto")
+    if hd in (64, 128) and (how == "fused" or (how == "auto" and (hd == 128 or ctx.max_ctx <= 2048))):
         rc = _PREFILL_Q4(device, q.data_ptr(), q.stride(0), q.shape[0], out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
                          k_cache.shape[0], block_tables.data_ptr(), block_tables.shape[1], ctx.tile_seq.data_ptr(), ctx.tile_q0.data_ptr(),
                          ctx.seq_q_start.data_ptr(), ctx.seq_q_len.data_ptr(), ctx.seq_ctx_len.data_ptr(), ctx.prefill_tiles, nh, nkv, hd,
