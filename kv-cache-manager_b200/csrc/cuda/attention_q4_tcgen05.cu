@@ -4,11 +4,11 @@
 // One block per (256 query rows of a request, query head), as two groups of 128 rows that share every tile of keys and values.  Per
 // tile of 128 keys and group:
 //     S = Q C^T   C = 128 + the key's codes (bfloat16, exact), accumulator in tensor memory
-//     softmax     one thread a row:  x = scale S + (zero - 128 scale) sum(q),  P = bfloat16(2^(x - m))
-//     O += P V    V = bfloat16(zero + scale code), MN-major operand, O in tensor memory for the whole block
-// A key is never rounded: its scale and zero meet the score, which costs two packed multiply-adds for two scores.  A value is, once, to
-// bfloat16, as P is: applied to P instead, its scale and zero were three more instructions for two scores in the loop that
-// bounds the kernel (four portions behind long prefixes: 1,270 us against DONE_US).
+//     softmax     one thread a row:  x = scale_k S + (zero_k - 128 scale_k) sum(q),  p = 2^(x - m),  P = bfloat16(p scale_v)
+//     O += P W    W = the value's codes - 8 (exact), MN-major operand, O in tensor memory for the whole block
+// and at the end  o = (O + sum p (zero_v + 8 scale_v)) / sum p.
+// Keys and values are never rounded; P is, to bfloat16.  (With V = bfloat16(zero + scale code) as the operand three instructions for two
+// scores fall away, 1,045 us instead of 1,098 for four portions behind long prefixes; but the result is then 1.7 times as far off as its own rounding, with P's alone 1.4 times.)
 // A row takes its products 32 at a time, relative to the maximum that it knows, without looking for theirs: where 32 probabilities
 // add up to more than 2^12 (or the row has seen nothing yet) their maximum is found, sums, O and the tile's earlier probabilities
 // are rescaled, and the 32 are taken again, which after the first tiles hardly ever happens.  The largest probability then lies
@@ -90,6 +90,12 @@ __device__ __forceinline__ void qf_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
                ::"r"(d_tmem), "r"(a_tmem), "l"(db), "r"(instr), "r"(accumulate) : "memory");
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 // a * b + c of two floats at once
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -104,7 +110,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-struct QfScales { float2 scale, zero; };           // of two neighbouring keys, as they meet a score
+struct QfScales { float2 k_scale, k_zero, v_scale, v_zero; };      // of two neighbouring keys, as they meet scores and probabilities
 
 // The scores of two keys, less m, from their products.
 template <bool CAP>
@@ -118,10 +124,11 @@ __device__ __forceinline__ float2 qf_scores(uint32_t s0, uint32_t s1, const QfSc
   return t;
 }
 
-// 32 products of a row into probabilities, as bfloat16 pairs; returns their sum.  MASK: only keys [a, b) of the 32 count.
+// 32 products of a row into probabilities times the values' scales, as bfloat16 pairs; returns the probabilities' sum and adds what
+// the values' zeros come to to z2.  MASK: only keys [a, b) of the 32 count.
 template <bool CAP, bool MASK>
 __device__ __forceinline__ float qf_exponentials(const uint32_t (&s)[32], const QfScales* sc, uint32_t (&packed)[16], float qs, float m,
-                                                 float cap_pre, float scale_log2, int a, int b) {
+                                                 float cap_pre, float scale_log2, int a, int b, float2& z2) {
   const float2 qs2 = make_float2(qs, qs), less_m = make_float2(-m, -m);
   float2 l0 = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -132,8 +139,11 @@ __device__ __forceinline__ float qf_exponentials(const uint32_t (&s)[32], const 
       t.y = (2 * k + 1 >= a && 2 * k + 1 < b) ? t.y : -INFINITY;
     }
     const float2 ex = make_float2(qf_exp2(t.x), qf_exp2(t.y));
+    const float4 f = *(reinterpret_cast<const float4*>(&sc[k]) + 1);
     if (k & 1) l1 = add2(l1, ex); else l0 = add2(l0, ex);
-    const __nv_bfloat162 pk = __floats2bfloat162_rn(ex.x, ex.y);
+    z2 = fma2(ex, make_float2(f.z, f.w), z2);
+    const float2 w = mul2(ex, make_float2(f.x, f.y));
+    const __nv_bfloat162 pk = __floats2bfloat162_rn(w.x, w.y);
     packed[k] = *reinterpret_cast<const uint32_t*>(&pk);
   }
   l0 = add2(l0, l1);
@@ -181,24 +191,19 @@ __device__ __noinline__ void qf_rescale(uint32_t o_addr, bool has_o, uint32_t p_
 }
 
 // 16 bytes of codes (elements 32 ch .. 32 ch + 31 of row r) as bfloat16 into a 128-byte swizzled tile [HD/64][128 rows][64]:
-// 128 + code, or the values.
-template <bool VALUES>
-__device__ __forceinline__ void qf_spread(unsigned char* tile, const unsigned char* from, int r, int ch, float scale, float zero_128) {
+// 128 + code, or code - 8.
+template <bool CENTRE>
+__device__ __forceinline__ void qf_spread(unsigned char* tile, const unsigned char* from, int r, int ch) {
   const uint4 u = *reinterpret_cast<const uint4*>(from);
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
   unsigned char* row = tile + (ch >> 1) * kQfTile + r * 128;
-  const float2 s2 = make_float2(scale, scale), z2 = make_float2(zero_128, zero_128);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     uint32_t e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       e[i] = q4::two_codes_128(w[j], i);
-      if (VALUES) {
-        const float2 v = fma2(make_float2(__uint_as_float(e[i] << 16), __uint_as_float(e[i] & 0xffff0000u)), s2, z2);
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
-        e[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
+      if (CENTRE) asm("sub.rn.bf16x2 %0, %0, %1;\n" : "+r"(e[i]) : "r"(0x43084308u));
     }
     *reinterpret_cast<uint4*>(row + ((((ch & 1) * 4 + j) ^ (r & 7)) * 16)) = make_uint4(e[0], e[1], e[2], e[3]);
   }
@@ -222,8 +227,7 @@ struct QfUnpacker {
 
 template <int HD> constexpr size_t qf_smem() {
   constexpr int KB = HD / 64;
-  return size_t(2 + 2 * kQfStages) * KB * kQfTile + size_t(kQfScaleRing) * (kQfKeys / 2) * sizeof(QfScales) + kQfKeys * HD + kQfKeys * 4 +
-         QfUnpacker<HD, kQfValueWarps>::kPerThread * kQfValueWarps * 32 * 4;
+  return size_t(2 + 2 * kQfStages) * KB * kQfTile + size_t(kQfScaleRing) * (kQfKeys / 2) * sizeof(QfScales) + kQfKeys * HD + 2 * kQfKeys * 4;
 }
 
 template <int HD, bool CAP>
@@ -234,7 +238,7 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
   unsigned char* k_s = q_s + 2 * KB * kQfTile;                     // [stages][KB][128 keys][64]
   unsigned char* v_s = k_s + kQfStages * KB * kQfTile;
   QfScales* scales = reinterpret_cast<QfScales*>(v_s + kQfStages * KB * kQfTile);          // [ring][64 pairs of keys]
-  unsigned char* raw = reinterpret_cast<unsigned char*>(scales + kQfScaleRing * (kQfKeys / 2));     // codes [2][128][HD/2]; the keys' pairs [128]; of each value piece
+  unsigned char* raw = reinterpret_cast<unsigned char*>(scales + kQfScaleRing * (kQfKeys / 2));     // codes [2][128][HD/2], pairs [2][128]
   __shared__ __align__(8) uint64_t q_full, k_full[kQfStages], v_full[kQfStages], sc_full[kQfScaleRing], s_full[2], p_full[2], done[kQfStages], o_full;
   __shared__ uint32_t tmem_base;
   __shared__ volatile int abort_flag;
@@ -373,23 +377,27 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
         int off;
         const size_t at = page_of(key0 + t, off);
         qf_copy4(pair, p.k_cache + at + pairs_at + off * 4);
-      } else {
-        *reinterpret_cast<uint32_t*>(pair) = 0u;                   // (a masked score, finite whatever the codes are)
+        qf_copy4(pair + kQfKeys * 4, p.v_cache + at + pairs_at + off * 4);
+      } else {                                                     // zero: zero times it stays zero (codes are finite whatever they are)
+        *reinterpret_cast<uint32_t*>(pair) = 0u;
+        *reinterpret_cast<uint32_t*>(pair + kQfKeys * 4) = 0u;
       }
     };
     ask(0);
     for (int n = 0; n < n_tiles; ++n) {
       asm volatile("cp.async.wait_all;\n" ::: "memory");
       if (n >= kQfStages && !wait_all(&done[n % kQfStages], ((n - kQfStages) / kQfStages) & 1, 23)) break;
-      const uint32_t two = *reinterpret_cast<const uint32_t*>(pair);
+      const uint32_t kp = *reinterpret_cast<const uint32_t*>(pair), vp = *reinterpret_cast<const uint32_t*>(pair + kQfKeys * 4);
       float* f = reinterpret_cast<float*>(scales + (n % kQfScaleRing) * (kQfKeys / 2) + (t >> 1)) + (t & 1);
-      const float unit = CAP ? 1.f : p.scale_log2, scale = q4::scale_of(two);
-      f[0] = scale * unit;
-      f[2] = fmaf(-128.f, scale, q4::zero_of(two)) * unit;
+      const float unit = CAP ? 1.f : p.scale_log2, ks = q4::scale_of(kp), vs = q4::scale_of(vp);
+      f[0] = ks * unit;
+      f[2] = fmaf(-128.f, ks, q4::zero_of(kp)) * unit;
+      f[4] = vs;
+      f[6] = fmaf(8.f, vs, q4::zero_of(vp));
 #pragma unroll
       for (int i = 0; i < unpack.kPerThread; ++i) {
         int r, ch;
-        if (unpack.piece(i, r, ch)) qf_spread<false>(k_s + (n % kQfStages) * KB * kQfTile, raw + r * (HD / 2) + ch * 16, r, ch, 0.f, 0.f);
+        if (unpack.piece(i, r, ch)) qf_spread<false>(k_s + (n % kQfStages) * KB * kQfTile, raw + r * (HD / 2) + ch * 16, r, ch);
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
@@ -401,23 +409,17 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
     }
     asm volatile("cp.async.wait_all;\n" ::: "memory");
   } else if (warp >= 8 && warp < 8 + kQfKeyWarps + kQfValueWarps) {
-    // ---- values into operands; each piece with its own copy of its row's pair
+    // ---- values into operands
     const QfUnpacker<HD, kQfValueWarps> unpack{warp - 8 - kQfKeyWarps, lane};
     unsigned char* codes = raw + kQfKeys * (HD / 2);
-    unsigned char* pair = raw + kQfKeys * HD + kQfKeys * 4 + (threadIdx.x - 32 * (8 + kQfKeyWarps)) * 4;
-    constexpr int kPairStep = kQfValueWarps * 32 * 4;
     auto ask = [&](int n) {
       const int key0 = (j0 + n) * kQfKeys;
 #pragma unroll
       for (int i = 0; i < unpack.kPerThread; ++i) {
         int r, ch, off;
-        if (!unpack.piece(i, r, ch)) continue;
-        if (key0 + r >= lo && key0 + r < hi) {
+        if (unpack.piece(i, r, ch) && key0 + r >= lo && key0 + r < hi) {
           const size_t at = page_of(key0 + r, off);
           qf_copy16(codes + r * (HD / 2) + ch * 16, p.v_cache + at + size_t(off) * (HD / 2) + ch * 16);
-          qf_copy4(pair + i * kPairStep, p.v_cache + at + pairs_at + off * 4);
-        } else {
-          *reinterpret_cast<uint32_t*>(pair + i * kPairStep) = 0u; // a value of zero: zero times it stays zero
         }
       }
     };
@@ -428,10 +430,7 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
 #pragma unroll
       for (int i = 0; i < unpack.kPerThread; ++i) {
         int r, ch;
-        if (!unpack.piece(i, r, ch)) continue;
-        const uint32_t two = *reinterpret_cast<const uint32_t*>(pair + i * kPairStep);
-        const float scale = q4::scale_of(two);
-        qf_spread<true>(v_s + (n % kQfStages) * KB * kQfTile, codes + r * (HD / 2) + ch * 16, r, ch, scale, fmaf(-128.f, scale, q4::zero_of(two)));
+        if (unpack.piece(i, r, ch)) qf_spread<true>(v_s + (n % kQfStages) * KB * kQfTile, codes + r * (HD / 2) + ch * 16, r, ch);
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
@@ -464,6 +463,7 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
       float m = -INFINITY;                                         // the maximum the row currently scales by
       bool fresh = true;                                           // some row of the warp has none
       float l = 0.f;
+      float2 z2 = make_float2(0.f, 0.f);                           // what the values' zeros come to
       for (int n = 0; n < mine; ++n) {
         alive = alive && wait_all(&s_full[g], n & 1, 26) && wait_all(&sc_full[n % kQfScaleRing], (n / kQfScaleRing) & 1, 27);
         if (!alive) break;
@@ -482,12 +482,14 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
           const QfScales* scc = sc + c * 16;
           const int ac = a - c * 32, bc = b - c * 32;
           float part;
+          float2 z_part;
           for (int pass = 0;; ++pass) {
+            z_part = make_float2(0.f, 0.f);
             const float m_use = (m == -INFINITY) ? 0.f : m;
             bool renew = fresh;                                    // some row of the warp has seen nothing yet
             if (!fresh) {
-              part = full ? qf_exponentials<CAP, false>(s, scc, packed, qs, m_use, p.cap_pre, p.scale_log2, ac, bc)
-                          : qf_exponentials<CAP, true>(s, scc, packed, qs, m_use, p.cap_pre, p.scale_log2, ac, bc);
+              part = full ? qf_exponentials<CAP, false>(s, scc, packed, qs, m_use, p.cap_pre, p.scale_log2, ac, bc, z_part)
+                          : qf_exponentials<CAP, true>(s, scc, packed, qs, m_use, p.cap_pre, p.scale_log2, ac, bc, z_part);
               renew = pass == 0 && part > kQfMost;                 // (behind a renewal a part is at most 32)
             }
             if (!__any_sync(0xffffffffu, renew)) break;
@@ -497,14 +499,17 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
             if (grows) m = m_use + mx;
             sum *= alpha;
             l *= alpha;
+            z2.x *= alpha;
+            z2.y *= alpha;
             if (__any_sync(0xffffffffu, alpha != 1.f)) qf_rescale<HD>(o_addr, n > 0, s_addr, c, alpha);
             if (fresh) {
-              part = qf_exponentials<CAP, true>(s, scc, packed, qs, (m == -INFINITY) ? 0.f : m, p.cap_pre, p.scale_log2, ac, bc);
+              part = qf_exponentials<CAP, true>(s, scc, packed, qs, (m == -INFINITY) ? 0.f : m, p.cap_pre, p.scale_log2, ac, bc, z_part);
               fresh = __any_sync(0xffffffffu, m == -INFINITY);
               break;
             }
           }
           sum += part;
+          z2 = add2(z2, z_part);
           qf_st16(s_addr + uint32_t(c * 16), packed);              // over products that are read
         }
         l += sum;
@@ -517,7 +522,7 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
       tc5::fence_after();
       if (alive) {
         if (p.sink && m != -INFINITY) l += qf_exp2(p.sink[head] * 1.4426950408889634f - m);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l, z = z2.x + z2.y;
         bf16* dst = p.out + size_t(q_start + q0 + row) * p.out_stride + size_t(head) * HD;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
               __nv_bfloat162 h[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                h[i] = __floats2bfloat162_rn(__uint_as_float(ov[e * 8 + 2 * i]) * inv, __uint_as_float(ov[e * 8 + 2 * i + 1]) * inv);
+                h[i] = __floats2bfloat162_rn((__uint_as_float(ov[e * 8 + 2 * i]) + z) * inv, (__uint_as_float(ov[e * 8 + 2 * i + 1]) + z) * inv);
               *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = *reinterpret_cast<const uint4*>(h);
             }
           }

@@ -838,9 +838,11 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                          ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
                          sink: Optional[torch.Tensor] = None) -> None:
     """Rows of portions longer than one token over a cache in 4 bits; q and out are the step's full bfloat16 row arrays, ``ctx`` has
-    the step's arrays with tiles of 64 rows (tiles of request -1 are none).  Heads of 128 elements, and of 64 with up to 2,048 keys: one
-    kernel that unpacks pages beside the products.  Else, or where ``ctx.options['attn_prefill']`` is 'unpack', the pages that the
-    portions see are laid out in bfloat16 (in scratch of the call) and read by ``attention_prefill``.  ('fused' forces the one kernel.)"""
+    the step's arrays with tiles of 64 rows (tiles of request -1 are none).  Heads of 64 and 128 elements: one kernel that unpacks pages
+    beside the products.  Other heads, or ``ctx.options['attn_prefill'] == 'unpack'``: the pages that the portions see are laid out
+    in bfloat16, in scratch of the call, and read by ``attention_prefill`` (keys and values rounded once more).  B200, heads of 128,
+    one kernel | laid out: 148 rows 10 | 12 us, 2,048 rows 73 | 109, 100 rows behind 2,000 keys, three requests, 57 | 93; heads of 64, four
+    portions of 500 rows behind 3,000 keys, 255 | 219, which the second rounding does not buy."""
     name = "attention_prefill_q4"
     _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink)
     S = ctx.seq_ctx_len.numel()
@@ -860,11 +862,7 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
     first, seqs = ctx.decode_seqs, S - ctx.decode_seqs
     if seqs <= 0 or ctx.prefill_tiles == 0:
         return
-    # At 64 elements a head the products are half as long and the kernel over bfloat16 pages runs two blocks an SM: behind long
-    # contexts laying out the pages pays (four portions behind 3,000 keys: 219 us against 255; 2,048 rows of one request: 57 both;
-    # 148 rows: 12 against 10).  At 128 elements it never did (100 rows behind 2,000 keys, three requests: 93 against 57).
-    how = ctx.options.get("attn_prefill", "auto")
-    if hd in (64, 128) and (how == "fused" or (how == "auto" and (hd == 128 or ctx.max_ctx <= 2048))):
+    if hd in (64, 128) and ctx.options.get("attn_prefill", "auto") != "unpack":
         rc = _PREFILL_Q4(device, q.data_ptr(), q.stride(0), q.shape[0], out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
                          k_cache.shape[0], block_tables.data_ptr(), block_tables.shape[1], ctx.tile_seq.data_ptr(), ctx.tile_q0.data_ptr(),
                          ctx.seq_q_start.data_ptr(), ctx.seq_q_len.data_ptr(), ctx.seq_ctx_len.data_ptr(), ctx.prefill_tiles, nh, nkv, hd,
