@@ -7,9 +7,12 @@
 // code 0.  A row with an element that is not finite, or whose range is beyond float32, reads back as not-a-number everywhere: loud,
 // not wrong.
 //
-// What bounds it: memory.  A lane has one word of a row (eight elements: one 16-byte load, one 4-byte store of codes); the lanes
-// of a head (hd / 8, rounded up to a power of two) sit in one warp and find minimum and maximum by shuffles, and so does a
-// rotate-half partner, hd / 16 lanes away.
+// What bounds it: memory, if little is done for each element.  A lane has two words of a head (eight elements each: a 16-byte load
+// and a 4-byte store of codes), in rotate-half pairs the two that turn with one another, so that angles are read once for both and
+// nothing is exchanged; the lanes of a head (hd / 16, rounded up to a power of two) sit in one warp and find minimum and
+// maximum by shuffles.  A block has 256 such pairs of one row (grid: rows x pieces of a row), so nothing is divided to find one's
+// place.  8,192 rows of 48 heads of 128 (180 MB): STORE_US us; 71 with one word a lane and partners exchanged by shuffles, 96 with
+// places counted through and taken apart by 64-bit divisions.  Reading the 8 + 8 KV heads back: READ_US us.
 #include "pdl.cuh"
 #include "q4.cuh"
 
@@ -50,74 +53,76 @@ struct StoreQ4Params {
   uint8_t* k_out; uint8_t* v_out;      // caches
   void* q_out; long long q_stride;
   int rows, nh, nkv, hd, block_size, num_pages;
-  int lanes;                           // lanes of a head: hd / 8 rounded up to a power of two
+  int log2_lanes;                      // lanes of a head: hd / 16 rounded up to a power of two
 };
 
-// One lane a word; item = (row, head, word).
+// One lane two words.
 template <typename T>
 __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(StoreQ4Params p) {
   pdl_launch_dependents();
   pdl_wait();
-  const long long item = (long long)blockIdx.x * kQ4Threads + threadIdx.x;
-  const int heads = p.nh + 2 * p.nkv;
-  const int word = int(item) & (p.lanes - 1);                     // (lanes divides 32 and the block)
-  const long long rh = item / p.lanes;
-  const int row = int(rh / heads), head = int(rh - (long long)row * heads);
-  const bool live = row < p.rows && word * 8 < p.hd;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (live) load8(static_cast<const T*>(p.qkv) + size_t(row) * p.row_stride + size_t(head) * p.hd + word * 8, x);
-  // ---- rotation of q and k heads.  Partner lanes take part whether or not they are live.
-  if (p.angles != nullptr) {
+  const int item = blockIdx.y * kQ4Threads + threadIdx.x;
+  const int heads = p.nh + 2 * p.nkv, lanes = 1 << p.log2_lanes, words = p.hd / 8;
+  const int i = item & (lanes - 1);                                // (a head's lanes lie in one warp)
+  const int row = blockIdx.x, head = item >> p.log2_lanes;
+  // words i and i + away turn with one another; the words behind the rotation, and all where pairs are neighbours, by twos
+  const int away = p.angles != nullptr && !p.interleaved ? p.rotary_dim / 16 : 0;
+  const int word[2] = {i < away ? i : 2 * i, i < away ? i + away : 2 * i + 1};
+  const bool live[2] = {head < heads && word[0] < words, head < heads && word[1] < words};
+  float x[2][8];
+  const T* from = static_cast<const T*>(p.qkv) + size_t(row) * p.row_stride + size_t(head) * p.hd;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[k][e] = 0.f;
+    if (live[k]) load8(from + word[k] * 8, x[k]);
+  }
+  // ---- rotation of q and k heads
+  if (p.angles != nullptr && live[0] && head < p.nh + p.nkv) {
     const int half = p.rotary_dim / 2;
-    const float* cs = p.angles + size_t(live ? row : 0) * p.rotary_dim;
+    const float* cs = p.angles + size_t(row) * p.rotary_dim;
     if (p.interleaved) {
-      if (live && head < p.nh + p.nkv) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int pair = word * 4 + i;
-          if (pair < half) rotate_pair(x[2 * i], x[2 * i + 1], cs[pair], cs[half + pair], x[2 * i], x[2 * i + 1]);
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int pair = word[k] * 4 + e;
+          if (pair < half) rotate_pair(x[k][2 * e], x[k][2 * e + 1], cs[pair], cs[half + pair], x[k][2 * e], x[k][2 * e + 1]);
         }
-      }
-    } else {
-      const int away = half / 8;                                   // words between partners
-      const bool first = word < away;
-      const int lane = threadIdx.x & 31;
-      const int partner = word < 2 * away ? (first ? lane + away : lane - away) : lane;
-      float y[8];
+    } else if (i < away) {
+      float c[8], s[8];
+      load8(cs + i * 8, c);
+      load8(cs + half + i * 8, s);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], partner);
-      if (live && head < p.nh + p.nkv && word < 2 * away) {
-        const int j0 = (first ? word : word - away) * 8;
-        float c[8], s[8];
-        load8(cs + j0, c);
-        load8(cs + half + j0, s);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float ra, rb;
-          rotate_pair(first ? x[e] : y[e], first ? y[e] : x[e], c[e], s[e], ra, rb);
-          x[e] = first ? ra : rb;
-        }
-      }
+      for (int e = 0; e < 8; ++e) rotate_pair(x[0][e], x[1][e], c[e], s[e], x[0][e], x[1][e]);
     }
   }
-  if (live && head < p.nh) store8(static_cast<T*>(p.q_out) + size_t(row) * p.q_stride + size_t(head) * p.hd + word * 8, x);
+  if (head < p.nh) {
+    T* to = static_cast<T*>(p.q_out) + size_t(row) * p.q_stride + size_t(head) * p.hd;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (live[k]) store8(to + word[k] * 8, x[k]);
+  }
+  if (__all_sync(0xffffffffu, !live[0] || head < p.nh)) return;    // q heads alone
   // ---- the row's range (lanes of q heads and dead lanes go along)
   float low = INFINITY, high = -INFINITY;
   int bad = 0;
-  if (live) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      low = fminf(low, x[e]);
-      high = fmaxf(high, x[e]);
-      bad |= !(fabsf(x[e]) <= 3.402823466e38f);
+  for (int k = 0; k < 2; ++k)
+    if (live[k]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        low = fminf(low, x[k][e]);
+        high = fmaxf(high, x[k][e]);
+        bad |= !(fabsf(x[k][e]) <= 3.402823466e38f);
+      }
     }
-  }
-  for (int o = p.lanes >> 1; o > 0; o >>= 1) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
     low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
     bad |= __shfl_xor_sync(0xffffffffu, bad, o);
   }
-  if (!live || head < p.nh) return;
+  if (!live[0] || head < p.nh) return;
   const int slot = p.slot_mapping[row];
   if (slot < 0) return;
   const int page = slot / p.block_size, off = slot - page * p.block_size;
@@ -127,17 +132,21 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(StoreQ4Params p) {
   bf16 scale = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(high, low), 15.f)), zero = __float2bfloat16_rn(low);
   const float s = __bfloat162float(scale), z = __bfloat162float(zero);
   bad |= !(s <= 3.402823466e38f);
-  uint32_t code[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float t = s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[e], z), s)) : 0.f;
-    code[e] = bad ? 0u : uint32_t(fminf(fmaxf(t, 0.f), 15.f));
-  }
-  if (bad) scale = zero = __ushort_as_bfloat16(0x7fc0);
   const size_t bytes = q4::page_bytes(p.block_size, p.hd);
   uint8_t* base = (is_k ? p.k_out : p.v_out) + (size_t(page) * p.nkv + kvh) * bytes;
-  *reinterpret_cast<uint32_t*>(base + size_t(off) * (p.hd / 2) + word * 4) = q4::pack_codes(code);
-  if (word == 0)
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (!live[k]) continue;
+    uint32_t code[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float t = s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[k][e], z), s)) : 0.f;
+      code[e] = bad ? 0u : uint32_t(fminf(fmaxf(t, 0.f), 15.f));
+    }
+    *reinterpret_cast<uint32_t*>(base + size_t(off) * (p.hd / 2) + word[k] * 4) = q4::pack_codes(code);
+  }
+  if (bad) scale = zero = __ushort_as_bfloat16(0x7fc0);
+  if (i == 0)
     *reinterpret_cast<uint32_t*>(base + size_t(p.block_size) * (p.hd / 2) + off * 4) =
         uint32_t(__bfloat16_as_ushort(scale)) | (uint32_t(__bfloat16_as_ushort(zero)) << 16);
 }
@@ -152,15 +161,12 @@ __device__ __forceinline__ void values8(uint32_t word, uint32_t pair, float (&x)
 template <typename T>
 __global__ void __launch_bounds__(kQ4Threads)
 read_q4_kernel(const uint8_t* k_cache, const uint8_t* v_cache, const int* __restrict__ slot_mapping, T* __restrict__ k_rows,
-               T* __restrict__ v_rows, long long k_stride, long long v_stride, int rows, int nkv, int hd, int block_size, int num_pages) {
+               T* __restrict__ v_rows, long long k_stride, long long v_stride, int nkv, int hd, int block_size, int num_pages) {
   pdl_launch_dependents();
   pdl_wait();
-  const int words = hd / 8;
-  const long long item = (long long)blockIdx.x * kQ4Threads + threadIdx.x;
-  const long long rh = item / words;
-  const int word = int(item - rh * words);
-  const int row = int(rh / (2 * nkv)), head = int(rh - (long long)row * 2 * nkv);
-  if (row >= rows) return;
+  const int words = hd / 8, item = blockIdx.y * kQ4Threads + threadIdx.x;
+  const int row = blockIdx.x, head = item / words, word = item - head * words;
+  if (head >= 2 * nkv) return;
   const int slot = slot_mapping[row];
   if (slot < 0) return;
   const int page = slot / block_size, off = slot - page * block_size;
@@ -209,24 +215,22 @@ unpack_pages_q4_kernel(const uint8_t* k_cache, const uint8_t* v_cache, const int
 
 template <typename T>
 int launch_store_q4(const StoreQ4Params& p, cudaStream_t s) {
-  const long long items = (long long)p.rows * (p.nh + 2 * p.nkv) * p.lanes;
-  return pdl_launch(store_q4_kernel<T>, dim3(unsigned((items + kQ4Threads - 1) / kQ4Threads)), dim3(kQ4Threads), 0, s, p);
+  const int items = (p.nh + 2 * p.nkv) << p.log2_lanes;
+  return pdl_launch(store_q4_kernel<T>, dim3(p.rows, (items + kQ4Threads - 1) / kQ4Threads), dim3(kQ4Threads), 0, s, p);
 }
 
 template <typename T>
 int launch_read_q4(const void* k_cache, const void* v_cache, const int* slots, void* k_rows, void* v_rows, long long k_stride,
                    long long v_stride, int rows, int nkv, int hd, int block_size, int num_pages, cudaStream_t s) {
-  const long long items = (long long)rows * 2 * nkv * (hd / 8);
-  return pdl_launch(read_q4_kernel<T>, dim3(unsigned((items + kQ4Threads - 1) / kQ4Threads)), dim3(kQ4Threads), 0, s,
-                    (const uint8_t*)k_cache, (const uint8_t*)v_cache, slots, (T*)k_rows, (T*)v_rows, k_stride, v_stride, rows, nkv, hd,
+  const int items = 2 * nkv * (hd / 8);
+  return pdl_launch(read_q4_kernel<T>, dim3(rows, (items + kQ4Threads - 1) / kQ4Threads), dim3(kQ4Threads), 0, s,
+                    (const uint8_t*)k_cache, (const uint8_t*)v_cache, slots, (T*)k_rows, (T*)v_rows, k_stride, v_stride, nkv, hd,
                     block_size, num_pages);
 }
 
 bool q4_sizes_ok(int nkv, int hd, int block_size, int num_pages) {
-  return nkv > 0 && hd >= 8 && hd <= 256 && hd % 8 == 0 && block_size > 0 && num_pages > 0;
+  return nkv > 0 && nkv <= 8192 && hd >= 8 && hd <= 256 && hd % 8 == 0 && block_size > 0 && num_pages > 0;
 }
-
-bool items_fit(long long items) { return (items + kQ4Threads - 1) / kQ4Threads <= 0x7fffffffll; }
 
 }  // namespace kvcm
 
@@ -243,7 +247,7 @@ KVCM_API long long kvcm_q4_page_bytes(int block_size, int hd) { return (long lon
                                            long long q_stride, int rows, int nh, int nkv, int hd, int block_size, int num_pages, \
                                            void* stream) {                                                                    \
     if (rows == 0) return 0;                                                                                                   \
-    if (!q4_sizes_ok(nkv, hd, block_size, num_pages) || nh < 0) return KVCM_ERR_UNSUPPORTED;                                   \
+    if (!q4_sizes_ok(nkv, hd, block_size, num_pages) || nh < 0 || nh > 32768) return KVCM_ERR_UNSUPPORTED;                     \
     if (angles != nullptr && (rotary_dim < 2 || rotary_dim > hd || rotary_dim % (interleaved ? 2 : 16)))                       \
       return KVCM_ERR_UNSUPPORTED;                                                                                             \
     const uintptr_t places = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) |                           \
@@ -256,9 +260,8 @@ KVCM_API long long kvcm_q4_page_bytes(int block_size, int hd) { return (long lon
     p.slot_mapping = slot_mapping; p.k_out = (uint8_t*)k_cache; p.v_out = (uint8_t*)v_cache; p.q_out = q_out;                  \
     p.q_stride = q_stride; p.rows = rows; p.nh = nh; p.nkv = nkv; p.hd = hd; p.block_size = block_size;                        \
     p.num_pages = num_pages;                                                                                                   \
-    p.lanes = 1;                                                                                                               \
-    while (p.lanes * 8 < hd) p.lanes *= 2;                                                                                     \
-    if (!items_fit((long long)rows * (nh + 2 * nkv) * p.lanes)) return KVCM_ERR_UNSUPPORTED;                                   \
+    p.log2_lanes = 0;                                                                                                          \
+    while ((16 << p.log2_lanes) < hd) ++p.log2_lanes;                                                                           \
     return launch_store_q4<T>(p, (cudaStream_t)stream);                                                                        \
   }                                                                                                                           \
   KVCM_API int kvcm_read_cache_q4_##SUFFIX(const void* k_cache, const void* v_cache, const int* slot_mapping, void* k_rows,    \
@@ -267,7 +270,7 @@ KVCM_API long long kvcm_q4_page_bytes(int block_size, int hd) { return (long lon
     if (rows == 0) return 0;                                                                                                   \
     const uintptr_t places = reinterpret_cast<uintptr_t>(k_rows) | reinterpret_cast<uintptr_t>(v_rows) |                       \
                              uintptr_t(k_stride * sizeof(T)) | uintptr_t(v_stride * sizeof(T));                                \
-    if (!q4_sizes_ok(nkv, hd, block_size, num_pages) || (places & 15) || !items_fit((long long)rows * 2 * nkv * (hd / 8)))     \
+    if (!q4_sizes_ok(nkv, hd, block_size, num_pages) || (places & 15))                                                         \
       return KVCM_ERR_UNSUPPORTED;                                                                                             \
     return launch_read_q4<T>(k_cache, v_cache, slot_mapping, k_rows, v_rows, k_stride, v_stride, rows, nkv, hd, block_size,    \
                              num_pages, (cudaStream_t)stream);                                                                 \
