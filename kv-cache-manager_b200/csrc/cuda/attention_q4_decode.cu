@@ -44,7 +44,7 @@ struct DecodeQ4Params {
   const bf16* q; long long q_stride;
   bf16* out; long long out_stride;
   const uint8_t* k_cache; const uint8_t* v_cache;
-  const int* block_tables; int max_blocks;
+  const int* block_tables; int max_blocks, max_keys;      // keys that a request's table has pages for
   const int* seq_ctx_len;
   float* part_o; float* part_ml;
   int* part_first;                     // shares: [seqs * head tiles][2]
@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
   pdl_launch_dependents();
   // The step's integers are there before the step's kernels; keys, also old ones, only behind the wait: a caller may have
   // written a whole prompt by the kernel before this one.
+  auto length = [&](int s) { return min(p.seq_ctx_len[s], p.max_keys); };     // (a context ends with its table)
   auto first_key = [&](int ctx) { return ctx > 0 ? first_visible(ctx - 1, p.window, 0) : 0; };
   // a request's cost for each head: its tiles of keys behind the start
   auto cost_of = [&](int ctx) { return ctx > 0 ? kQ4Start + (ctx - first_key(ctx) / kQ4Step * kQ4Step + kQ4Tile - 1) / kQ4Tile : 0; };
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
     const int per = (p.seqs + kQ4DecodeThreads - 1) / kQ4DecodeThreads;
     const int s0 = min(tid * per, p.seqs), s1 = min(s0 + per, p.seqs);
     int mine = 0;
-    for (int s = s0; s < s1; ++s) mine += cost_of(p.seq_ctx_len[s]);
+    for (int s = s0; s < s1; ++s) mine += cost_of(length(s));
     int up = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -238,15 +239,15 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
     const long long u0 = U * blockIdx.x / takers, u1 = U * (blockIdx.x + 1) / takers;
     left = u1 - u0;
     if ((long long)in_front * H <= u0 && u0 < (long long)(in_front + mine) * H) {
-      int s = s0, f = in_front, n = cost_of(p.seq_ctx_len[s]);
-      while ((long long)(f + n) * H <= u0) { f += n; ++s; n = cost_of(p.seq_ctx_len[s]); }
+      int s = s0, f = in_front, n = cost_of(length(s));
+      while ((long long)(f + n) * H <= u0) { f += n; ++s; n = cost_of(length(s)); }
       found[0] = s;
       found[1] = f;
     }
     __syncthreads();
     seq = found[0];
     before = found[1];
-    const int n = cost_of(p.seq_ctx_len[seq]);
+    const int n = cost_of(length(seq));
     const long long at = u0 - before * H;
     unit_h = int(at / n);
     at_cost = int(at - (long long)unit_h * n);
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
   for (;;) {
     // ---- the next piece of work
     Q4Segment w;
-    const int ctx = p.seq_ctx_len[seq], lo = first_key(ctx), base = lo / kQ4Step * kQ4Step;
+    const int ctx = length(seq), lo = first_key(ctx), base = lo / kQ4Step * kQ4Step;
     w.seq = seq;
     w.slot = -1;
     int of_h;
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
           unit_h = 0;
           before += n;
           if (left > 0)
-            do ++seq; while (p.seq_ctx_len[seq] <= 0);             // (there is more, so there is such a request)
+            do ++seq; while (length(seq) <= 0);             // (there is more, so there is such a request)
         }
       }
       if (empty) {
@@ -882,7 +883,7 @@ KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, vo
                                            int window, int part_size, int num_parts, int shares, float* scratch, int cluster_merge,
                                            float softcap, const float* sink, void* stream) {
   if (seqs == 0) return 0;
-  if (nkv <= 0 || nh <= 0 || nh % nkv || block_size <= 0 || num_pages <= 0 || num_parts < 0 || seqs > 65535 || nh > 65535 ||
+  if (nkv <= 0 || nh <= 0 || nh % nkv || block_size <= 0 || block_size > q4::kMaxBlock || max_blocks <= 0 || num_pages <= 0 || num_parts < 0 || seqs > 65535 || nh > 65535 ||
       !kvcm_attention_q4_decode_supports(hd))
     return KVCM_ERR_UNSUPPORTED;
   if (num_parts > 0 ? (part_size <= 0 || part_size % kQ4Tile) : (shares <= 0 || shares > (1 << 20))) return KVCM_ERR_UNSUPPORTED;
@@ -898,7 +899,9 @@ KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, vo
   DecodeQ4Params p;
   p.q = (const bf16*)q; p.q_stride = q_stride; p.out = (bf16*)out; p.out_stride = out_stride;
   p.k_cache = (const uint8_t*)k_cache; p.v_cache = (const uint8_t*)v_cache; p.num_pages = num_pages;
-  p.block_tables = block_tables; p.max_blocks = max_blocks; p.seq_ctx_len = seq_ctx_len; p.seqs = seqs;
+  p.block_tables = block_tables; p.max_blocks = max_blocks; p.seq_ctx_len = seq_ctx_len;
+  p.max_keys = q4::max_keys(max_blocks, block_size);
+  p.seqs = seqs;
   p.part_o = scratch; p.part_ml = scratch ? scratch + pieces * hd : nullptr;
   p.part_first = scratch ? reinterpret_cast<int*>(scratch + pieces * (hd + 2)) : nullptr;
   p.nh = nh; p.nkv = nkv; p.block_size = block_size; p.window = window;

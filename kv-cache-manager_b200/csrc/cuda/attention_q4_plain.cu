@@ -18,7 +18,7 @@ struct PlainQ4Params {
   const void* q; long long q_stride;
   void* out; long long out_stride;
   const uint8_t* k_cache; const uint8_t* v_cache;
-  const int* block_tables; int max_blocks;
+  const int* block_tables; int max_blocks, max_keys;      // keys that a request's table has pages for
   const int* row_seq; const int* positions;
   int nh, nkv, hd, block_size, num_pages, window;
   float scale, softcap;
@@ -37,8 +37,8 @@ __global__ void __launch_bounds__(kQ4PlainThreads) attention_q4_plain_kernel(Pla
   pdl_wait();
   const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
   const int kvh = h / (p.nh / p.nkv);
-  const int ctx = p.positions[row] + 1;
-  const int lo = first_visible(ctx - 1, p.window, 0);
+  const int position = p.positions[row], ctx = min(position, p.max_keys - 1) + 1;      // (a context ends with its table)
+  const int lo = first_visible(position, p.window, 0);
   const int words = p.hd / 8, row_bytes = p.hd / 2;
   const size_t bytes = q4::page_bytes(p.block_size, p.hd);
   const int* table = p.block_tables + size_t(p.row_seq[row]) * p.max_blocks;
@@ -134,12 +134,12 @@ using namespace kvcm;
       const int* block_tables, int max_blocks, const int* row_seq, const int* positions, int rows, int nh, int nkv, int hd,    \
       int block_size, float scale, int window, float softcap, const float* sink, void* stream) {                               \
     if (rows == 0) return 0;                                                                                                   \
-    if (nkv <= 0 || nh % nkv || hd < 8 || hd > 256 || hd % 8 || block_size <= 0 || num_pages <= 0 || nh > 65535)               \
+    if (nkv <= 0 || nh % nkv || hd < 8 || hd > 256 || hd % 8 || block_size <= 0 || block_size > q4::kMaxBlock || max_blocks <= 0 || num_pages <= 0 || nh > 65535)               \
       return KVCM_ERR_UNSUPPORTED;                                                                                             \
     PlainQ4Params p;                                                                                                           \
     p.q = q; p.q_stride = q_stride; p.out = out; p.out_stride = out_stride;                                                    \
     p.k_cache = (const uint8_t*)k_cache; p.v_cache = (const uint8_t*)v_cache; p.num_pages = num_pages;                         \
-    p.block_tables = block_tables; p.max_blocks = max_blocks; p.row_seq = row_seq; p.positions = positions;                    \
+    p.block_tables = block_tables; p.max_blocks = max_blocks; p.max_keys = q4::max_keys(max_blocks, block_size); p.row_seq = row_seq; p.positions = positions;                    \
     p.nh = nh; p.nkv = nkv; p.hd = hd; p.block_size = block_size; p.window = window;                                           \
     p.scale = scale; p.softcap = softcap; p.sink = sink;                                                                       \
     return launch_plain_q4<T>(p, rows, (cudaStream_t)stream);                                                                  \

@@ -46,7 +46,7 @@ constexpr float kQfMost = 4096.f;                  // a row's sum of 32 probabil
 struct PrefillQ4Params {
   bf16* out; long long out_stride;
   const uint8_t* k_cache; const uint8_t* v_cache;
-  const int* block_tables; int max_blocks;
+  const int* block_tables; int max_blocks, max_keys;      // keys that a request's table has pages for
   const int* tile_seq; const int* tile_q0;         // tiles of 64 rows; a block takes every fourth and its three successors
   const int* seq_q_start; const int* seq_q_len; const int* seq_ctx_len;
   int nh, nkv, block_size, log2_block, num_pages, window;
@@ -134,12 +134,13 @@ __device__ __forceinline__ float qf_exponentials(const uint32_t (&s)[32], const 
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
     float2 t = qf_scores<CAP>(s[2 * k], s[2 * k + 1], &sc[k], qs2, less_m, cap_pre, scale_log2);
-    if constexpr (MASK) {
-      t.x = (2 * k >= a && 2 * k < b) ? t.x : -INFINITY;
-      t.y = (2 * k + 1 >= a && 2 * k + 1 < b) ? t.y : -INFINITY;
+    float4 f = *(reinterpret_cast<const float4*>(&sc[k]) + 1);
+    if constexpr (MASK) {                                          // (a masked value may be no number: zero times it has to be zero)
+      const bool x = 2 * k >= a && 2 * k < b, y = 2 * k + 1 >= a && 2 * k + 1 < b;
+      t.x = x ? t.x : -INFINITY; f.x = x ? f.x : 0.f; f.z = x ? f.z : 0.f;
+      t.y = y ? t.y : -INFINITY; f.y = y ? f.y : 0.f; f.w = y ? f.w : 0.f;
     }
     const float2 ex = make_float2(qf_exp2(t.x), qf_exp2(t.y));
-    const float4 f = *(reinterpret_cast<const float4*>(&sc[k]) + 1);
     if (k & 1) l1 = add2(l1, ex); else l0 = add2(l0, ex);
     z2 = fma2(ex, make_float2(f.z, f.w), z2);
     const float2 w = mul2(ex, make_float2(f.x, f.y));
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
     return;
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int q_start = p.seq_q_start[seq], q_len = p.seq_q_len[seq], ctx = p.seq_ctx_len[seq];
+  const int q_start = p.seq_q_start[seq], q_len = p.seq_q_len[seq], ctx = min(p.seq_ctx_len[seq], p.max_keys);     // (a context ends with its table)
   const int rows_here = min(kQfRows, q_len - q0);
   const int pos0 = ctx - q_len + q0;                               // position of the block's first row
   const int hi = pos0 + rows_here;                                 // keys [lo, hi) matter to the block
@@ -579,7 +580,7 @@ KVCM_API int kvcm_attention_prefill_q4_bf16(const void* q, long long q_stride, i
                                             const int* seq_ctx_len, int tiles, int nh, int nkv, int hd, int block_size, float scale,
                                             int window, float softcap, const float* sink, void* stream) {
   if (tiles <= 0) return 0;
-  if (!kvcm_attention_prefill_q4_supports(hd) || nkv <= 0 || nh <= 0 || nh % nkv || block_size <= 0 || num_pages <= 0 || total_rows <= 0 ||
+  if (!kvcm_attention_prefill_q4_supports(hd) || nkv <= 0 || nh <= 0 || nh % nkv || block_size <= 0 || block_size > q4::kMaxBlock || max_blocks <= 0 || num_pages <= 0 || total_rows <= 0 ||
       tiles > 65535)
     return KVCM_ERR_UNSUPPORTED;
   if ((q_stride % 8) || (out_stride % 8) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
@@ -591,7 +592,7 @@ KVCM_API int kvcm_attention_prefill_q4_bf16(const void* q, long long q_stride, i
   PrefillQ4Params p;
   p.out = (bf16*)out; p.out_stride = out_stride;
   p.k_cache = (const uint8_t*)k_cache; p.v_cache = (const uint8_t*)v_cache; p.num_pages = num_pages;
-  p.block_tables = block_tables; p.max_blocks = max_blocks; p.tile_seq = tile_seq; p.tile_q0 = tile_q0;
+  p.block_tables = block_tables; p.max_blocks = max_blocks; p.max_keys = q4::max_keys(max_blocks, block_size); p.tile_seq = tile_seq; p.tile_q0 = tile_q0;
   p.seq_q_start = seq_q_start; p.seq_q_len = seq_q_len; p.seq_ctx_len = seq_ctx_len;
   p.nh = nh; p.nkv = nkv; p.block_size = block_size; p.window = window;
   p.scale_log2 = (softcap > 0.f ? softcap : scale) * 1.4426950408889634f;

@@ -11,8 +11,8 @@
 // and a 4-byte store of codes), in rotate-half pairs the two that turn with one another, so that angles are read once for both and
 // nothing is exchanged; the lanes of a head (hd / 16, rounded up to a power of two) sit in one warp and find minimum and
 // maximum by shuffles.  A block has 256 such pairs of one row (grid: rows x pieces of a row), so nothing is divided to find one's
-// place.  8,192 rows of 48 heads of 128 (180 MB): STORE_US us; 71 with one word a lane and partners exchanged by shuffles, 96 with
-// places counted through and taken apart by 64-bit divisions.  Reading the 8 + 8 KV heads back: READ_US us.
+// place.  8,192 rows of 48 heads of 128 (180 MB): 55 us; 71 with one word a lane and partners exchanged by shuffles, 96 with
+// places counted through and taken apart by 64-bit divisions.  Reading the 8 + 8 KV heads back: 16.7 us.
 #include "pdl.cuh"
 #include "q4.cuh"
 
@@ -229,7 +229,7 @@ int launch_read_q4(const void* k_cache, const void* v_cache, const int* slots, v
 }
 
 bool q4_sizes_ok(int nkv, int hd, int block_size, int num_pages) {
-  return nkv > 0 && nkv <= 8192 && hd >= 8 && hd <= 256 && hd % 8 == 0 && block_size > 0 && num_pages > 0;
+  return nkv > 0 && nkv <= 8192 && hd >= 8 && hd <= 256 && hd % 8 == 0 && block_size > 0 && block_size <= q4::kMaxBlock && num_pages > 0;
 }
 
 }  // namespace kvcm

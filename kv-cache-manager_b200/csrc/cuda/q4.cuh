@@ -15,8 +15,16 @@
 namespace kvcm {
 namespace q4 {
 
+constexpr int kMaxBlock = 1 << 16;               // largest page, in rows: counts of keys stay far from 2^31
+
 __host__ __device__ inline size_t page_bytes(int block_size, int hd) {
   return (size_t(block_size) * (hd / 2 + 4) + 15) & ~size_t(15);
+}
+
+// Keys that a request's row of the page table has room for: contexts end there (a step that was refused may leave a longer one).
+inline int max_keys(int max_blocks, int block_size) {
+  const long long n = (long long)max_blocks * block_size;
+  return n < (1 << 30) ? int(n) : 1 << 30;
 }
 
 // The page of head `kvh`.  Page ids outside the pool are taken into it: a wrong table reads a wrong page, not foreign memory.

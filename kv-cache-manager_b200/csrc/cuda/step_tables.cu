@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(TabParams p) {
     *p.free_left = count - total.pages;
     p.status[0] = code; p.status[1] = detail; p.status[2] = total.rows; p.status[3] = total.tiles;
   }
+  __threadfence();                                 // (whoever starts at this kernel's end may read before its dependency wait)
 }
 
 }  // namespace kvcm

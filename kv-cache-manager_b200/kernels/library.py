@@ -9,6 +9,7 @@ kernels (used by the benchmark's ``gpu_launches``).
 from __future__ import annotations
 
 import ctypes
+import types
 from typing import Optional
 
 import torch
@@ -620,12 +621,11 @@ def q4_page_bytes(block_size: int, hd: int) -> int:
     return (int(block_size) * (int(hd) // 2 + 4) + 15) // 16 * 16
 
 
-
 def _q4_cache(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, nkv: int, hd: int, block_size: int) -> None:
     if hd % 8 or not 8 <= hd <= 256:
         raise KernelError(f"{name}: head sizes are multiples of 8 up to 256")
-    if block_size <= 0:
-        raise KernelError(f"{name}: block_size > 0")
+    if not 0 < block_size <= 65536:
+        raise KernelError(f"{name}: block_size of 1 to 65536 rows")
     pages = k_cache.shape[0]
     want = (pages, nkv, q4_page_bytes(block_size, hd))
     for t in (k_cache, v_cache):
@@ -714,7 +714,7 @@ def _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, blo
         raise KernelError(f"{name}: q and out must be rows of {nh} heads of {hd}")
     if q.stride(1) != 1 or out.stride(1) != 1:
         raise KernelError(f"{name}: rows must be dense")
-    if block_tables.dtype != _I32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+    if block_tables.dtype != _I32 or block_tables.dim() != 2 or not block_tables.is_contiguous() or block_tables.shape[1] == 0:
         raise KernelError(f"{name}: block_tables must be contiguous int32 [S, max_blocks]")
     if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nh or not sink.is_contiguous()):
         raise KernelError(f"{name}: sink must be float32 [heads]")
@@ -838,11 +838,13 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                          ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
                          sink: Optional[torch.Tensor] = None) -> None:
     """Rows of portions longer than one token over a cache in 4 bits; q and out are the step's full bfloat16 row arrays, ``ctx`` has
-    the step's arrays with tiles of 64 rows (tiles of request -1 are none).  Heads of 64 and 128 elements: one kernel that unpacks pages
-    beside the products.  Other heads, or ``ctx.options['attn_prefill'] == 'unpack'``: the pages that the portions see are laid out
-    in bfloat16, in scratch of the call, and read by ``attention_prefill`` (keys and values rounded once more).  B200, heads of 128,
-    one kernel | laid out: 148 rows 10 | 12 us, 2,048 rows 73 | 109, 100 rows behind 2,000 keys, three requests, 57 | 93; heads of 64, four
-    portions of 500 rows behind 3,000 keys, 255 | 219, which the second rounding does not buy."""
+    the step's arrays with tiles of 64 rows (tiles of request -1 are none; ``ctx.max_ctx`` is at least the longest context; a context
+    ends with its page table).  Heads of 64 and 128 elements: one kernel that unpacks pages beside the products.  Other heads, or
+    ``ctx.options['attn_prefill'] == 'unpack'``: the pages that the portions see are laid out in bfloat16, in scratch of the call,
+    and read by ``attention_prefill`` (keys and values rounded once more, and a value that is not a number also reaches rows of its
+    tile that do not see it).  B200, heads of 128, one kernel | laid out: 148 rows 10 | 12 us, 2,048 rows 73 | 109, 100 rows behind
+    2,000 keys, three requests, 57 | 93; heads of 64, four portions of 500 rows behind 3,000 keys, 255 | 219, which the second
+    rounding does not buy."""
     name = "attention_prefill_q4"
     _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink)
     S = ctx.seq_ctx_len.numel()
@@ -875,9 +877,16 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                     ctx.seq_ctx_len.data_ptr(), pages[0].data_ptr(), pages[1].data_ptr(), first, seqs, blocks, nkv, hd, block_size,
                     k_cache.shape[0], window)
     _launched(rc, name, "(hd={}, nkv={})", hd, nkv)
-    tables = torch.arange(-first * blocks, seqs * blocks, dtype=torch.int32, device=q.device).view(S, blocks)
     with torch.cuda.device(device):
-        attention_prefill(q, out, pages[0], pages[1], tables, ctx, nh, nkv, hd, scale, window, softcap, sink)
+        # tiles of no request become those of one more, which has no row and sees one key
+        pad = lambda t, v: torch.nn.functional.pad(t[:S], (0, 1), value=v)
+        tables = torch.arange(-first * blocks, (seqs + 1) * blocks, dtype=torch.int32, device=q.device).view(S + 1, blocks)
+        tables[S].zero_()
+        step = types.SimpleNamespace(
+            seq_q_start=pad(ctx.seq_q_start, 0), seq_q_len=pad(ctx.seq_q_len, 0), seq_ctx_len=pad(ctx.seq_ctx_len, 1).clamp_(max=blocks * block_size),
+            tile_seq=torch.where(ctx.tile_seq < 0, S, ctx.tile_seq), tile_q0=ctx.tile_q0.clamp(min=0), prefill_tiles=ctx.prefill_tiles,
+            tile_rows=ctx.tile_rows, options=ctx.options)
+        attention_prefill(q, out, pages[0], pages[1], tables, step, nh, nkv, hd, scale, window, softcap, sink)
 
 
 # ------------------------------------------------------------------ a step's arrays from lengths

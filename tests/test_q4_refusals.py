@@ -97,7 +97,7 @@ def test_rows_that_cannot_be_read(change, match):
     (dict(nh=3), "multiple"), (dict(dtype=torch.float16), "bfloat16 or float32"), (dict(out=torch.zeros(T, NH * HD)), "q and out"),
     (dict(out=torch.zeros((T - 1, NH * HD), dtype=torch.bfloat16)), "q and out"), (dict(window=-1), "negative"), (dict(softcap=-2.0), "negative"),
     (dict(sink=torch.zeros(NH - 1)), "sink"), (dict(sink=torch.zeros(NH, dtype=torch.bfloat16)), "sink"), (dict(block_tables=i32(T * 4)), "block_tables"),
-    (dict(block_tables=torch.zeros((T, 4), dtype=torch.int64)), "block_tables")])
+    (dict(block_tables=torch.zeros((T, 4), dtype=torch.int64)), "block_tables"), (dict(block_tables=i32(T, 0)), "block_tables")])
 def test_attention_that_cannot_be(change, match):
     refused(attend, match, **change)
 
