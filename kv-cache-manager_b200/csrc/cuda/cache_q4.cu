@@ -10,15 +10,21 @@
 // What bounds it: memory, if little is done for each element.  A lane has two words of a head (eight elements each: a 16-byte load
 // and a 4-byte store of codes), in rotate-half pairs the two that turn with one another, so that angles are read once for both and
 // nothing is exchanged; the lanes of a head (hd / 16, rounded up to a power of two) sit in one warp and find minimum and
-// maximum by shuffles.  A block has 256 such pairs of one row (grid: rows x pieces of a row), so nothing is divided to find one's
-// place.  8,192 rows of 48 heads of 128 (180 MB): 55 us; 71 with one word a lane and partners exchanged by shuffles, 96 with
-// places counted through and taken apart by 64-bit divisions.  Reading the 8 + 8 KV heads back: 16.7 us.
+// maximum by shuffles.  A block has up to 256 such pairs of one row (grid: rows x equal pieces of a row), so nothing is divided to
+// find one's place, and codes are found without divisions too (see there).  8,192 rows of 48 heads of 128 (180 MB): 44 us, 4.1 TB/s
+// (28 us at the rate of a copy); 55 with 16 divisions a lane, 71 with one word a lane and partners exchanged by shuffles, 96 with
+// places counted through and taken apart by 64-bit divisions.  What is left is waiting: a block is one load, a few hundred
+// instructions and a store; packed pairs of float32 (50 us), other block sizes and cache hints (no change) do not help.  Reading the
+// 8 + 8 KV heads back: 11.5 us (43 MB), 16.7 with a word a lane and codes converted from whole numbers.
 #include "pdl.cuh"
 #include "q4.cuh"
 
 namespace kvcm {
 
-constexpr int kQ4Threads = 256;
+constexpr int kQ4Threads = 256;                    // most threads of a block
+constexpr float kQ4Finite = 3.402823466e38f;
+constexpr float kQ4Magic = 12582912.f;             // 1.5 * 2^23: what is added to it is rounded to a whole number, ties to even
+constexpr uint32_t kQ4MagicWord = 0x3f400000u;     // eight words of its bits (0x4b400000) under the shifts of pack_codes, added up
 
 __device__ __forceinline__ void load8(const bf16* p, float (&x)[8]) {
   const uint4 v = *reinterpret_cast<const uint4*>(p);
@@ -58,10 +64,10 @@ struct StoreQ4Params {
 
 // One lane two words.
 template <typename T>
-__global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(StoreQ4Params p) {
+__global__ void __launch_bounds__(kQ4Threads, 5) store_q4_kernel(StoreQ4Params p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int item = blockIdx.y * kQ4Threads + threadIdx.x;
+  const int item = blockIdx.y * blockDim.x + threadIdx.x;
   const int heads = p.nh + 2 * p.nkv, lanes = 1 << p.log2_lanes, words = p.hd / 8;
   const int i = item & (lanes - 1);                                // (a head's lanes lie in one warp)
   const int row = blockIdx.x, head = item >> p.log2_lanes;
@@ -69,7 +75,14 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(StoreQ4Params p) {
   const int away = p.angles != nullptr && !p.interleaved ? p.rotary_dim / 16 : 0;
   const int word[2] = {i < away ? i : 2 * i, i < away ? i + away : 2 * i + 1};
   const bool live[2] = {head < heads && word[0] < words, head < heads && word[1] < words};
-  float x[2][8];
+  float x[2][8], c[8], sn[8];                                      // (all loads of the row first: one trip to memory)
+  const bool turns = p.angles != nullptr && live[0] && head < p.nh + p.nkv;
+  const float* cs = p.angles + size_t(row) * p.rotary_dim;
+  const int slot = p.slot_mapping[row], half = p.rotary_dim / 2;
+  if (turns && i < away) {
+    load8(cs + i * 8, c);
+    load8(cs + half + i * 8, sn);
+  }
   const T* from = static_cast<const T*>(p.qkv) + size_t(row) * p.row_stride + size_t(head) * p.hd;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -78,9 +91,7 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(StoreQ4Params p) {
     if (live[k]) load8(from + word[k] * 8, x[k]);
   }
   // ---- rotation of q and k heads
-  if (p.angles != nullptr && live[0] && head < p.nh + p.nkv) {
-    const int half = p.rotary_dim / 2;
-    const float* cs = p.angles + size_t(row) * p.rotary_dim;
+  if (turns) {
     if (p.interleaved) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -90,11 +101,8 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(StoreQ4Params p) {
           if (pair < half) rotate_pair(x[k][2 * e], x[k][2 * e + 1], cs[pair], cs[half + pair], x[k][2 * e], x[k][2 * e + 1]);
         }
     } else if (i < away) {
-      float c[8], s[8];
-      load8(cs + i * 8, c);
-      load8(cs + half + i * 8, s);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) rotate_pair(x[0][e], x[1][e], c[e], s[e], x[0][e], x[1][e]);
+      for (int e = 0; e < 8; ++e) rotate_pair(x[0][e], x[1][e], c[e], sn[e], x[0][e], x[1][e]);
     }
   }
   if (head < p.nh) {
@@ -105,8 +113,7 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(StoreQ4Params p) {
   }
   if (__all_sync(0xffffffffu, !live[0] || head < p.nh)) return;    // q heads alone
   // ---- the row's range (lanes of q heads and dead lanes go along)
-  float low = INFINITY, high = -INFINITY;
-  int bad = 0;
+  float low = INFINITY, high = -INFINITY, sick = 0.f;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     if (live[k]) {
@@ -114,16 +121,16 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(StoreQ4Params p) {
       for (int e = 0; e < 8; ++e) {
         low = fminf(low, x[k][e]);
         high = fmaxf(high, x[k][e]);
-        bad |= !(fabsf(x[k][e]) <= 3.402823466e38f);
+        sick = fmaf(x[k][e], 0.f, sick);                           // not a number from the first element on that is not finite
       }
     }
   for (int o = lanes >> 1; o > 0; o >>= 1) {
     low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
     high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-    bad |= __shfl_xor_sync(0xffffffffu, bad, o);
   }
+  const uint32_t all_sick = __ballot_sync(0xffffffffu, sick != 0.f);
+  bool bad = ((all_sick >> (threadIdx.x & 31 & -lanes)) & ((1u << lanes) - 1u)) != 0u;
   if (!live[0] || head < p.nh) return;
-  const int slot = p.slot_mapping[row];
   if (slot < 0) return;
   const int page = slot / p.block_size, off = slot - page * p.block_size;
   if (page >= p.num_pages) return;
@@ -131,42 +138,67 @@ __global__ void __launch_bounds__(kQ4Threads) store_q4_kernel(StoreQ4Params p) {
   const int kvh = head - p.nh - (is_k ? 0 : p.nkv);
   bf16 scale = __float2bfloat16_rn(__fdiv_rn(__fsub_rn(high, low), 15.f)), zero = __float2bfloat16_rn(low);
   const float s = __bfloat162float(scale), z = __bfloat162float(zero);
-  bad |= !(s <= 3.402823466e38f);
+  bad |= !(s <= kQ4Finite);
   const size_t bytes = q4::page_bytes(p.block_size, p.hd);
   uint8_t* base = (is_k ? p.k_out : p.v_out) + (size_t(page) * p.nkv + kvh) * bytes;
+  // A product with 1 / scale is at most 2^-18 off the quotient (of 16 and less; three roundings), so it rounds to the same code
+  // where it is not that near to a half.  Where one of the lane's is near (one lane in 2,000), or the scale is so small that its
+  // reciprocal is none, the divisions are done.
+  const float per = s > 1e-30f ? __frcp_rn(s) : 0.f;
+  float farthest = s > 1e-30f || s == 0.f ? 0.f : 1.f;                         // from a whole number
+  uint32_t codes[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    if (!live[k]) continue;
-    uint32_t code[8];
+    codes[k] = 0u - kQ4MagicWord;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float t = s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[k][e], z), s)) : 0.f;
-      code[e] = bad ? 0u : uint32_t(fminf(fmaxf(t, 0.f), 15.f));
+      const float t = fminf(fmaxf(__fsub_rn(x[k][e], z) * per, 0.f), 15.f), n = __fadd_rn(t, kQ4Magic);
+      farthest = fmaxf(farthest, fabsf(__fsub_rn(t, __fsub_rn(n, kQ4Magic))));
+      codes[k] += __float_as_uint(n) << (4 * (e >> 1) + 16 * (e & 1));
     }
-    *reinterpret_cast<uint32_t*>(base + size_t(off) * (p.hd / 2) + word[k] * 4) = q4::pack_codes(code);
   }
+  if (farthest > 0.5f - 1.f / 65536.f) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t code[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float t = s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[k][e], z), s)) : 0.f;
+        code[e] = uint32_t(fminf(fmaxf(t, 0.f), 15.f));
+      }
+      codes[k] = q4::pack_codes(code);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (live[k]) *reinterpret_cast<uint32_t*>(base + size_t(off) * (p.hd / 2) + word[k] * 4) = bad ? 0u : codes[k];
   if (bad) scale = zero = __ushort_as_bfloat16(0x7fc0);
   if (i == 0)
     *reinterpret_cast<uint32_t*>(base + size_t(p.block_size) * (p.hd / 2) + off * 4) =
         uint32_t(__bfloat16_as_ushort(scale)) | (uint32_t(__bfloat16_as_ushort(zero)) << 16);
 }
 
+// (code from 128 + code, which a shift and an and-or give two at a time as bfloat16; the product is exact: 8 + 4 bits)
 __device__ __forceinline__ void values8(uint32_t word, uint32_t pair, float (&x)[8]) {
   const float s = q4::scale_of(pair), z = q4::zero_of(pair);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = __fadd_rn(z, __fmul_rn(s, q4::code_of(word, e)));      // (the product is exact: 8 + 4 bits)
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t two = q4::two_codes_128(word, i);
+    x[2 * i] = __fadd_rn(z, __fmul_rn(s, __uint_as_float(two << 16) - 128.f));
+    x[2 * i + 1] = __fadd_rn(z, __fmul_rn(s, __uint_as_float(two & 0xffff0000u) - 128.f));
+  }
 }
 
-// Rows of slots back as values: k_rows and v_rows [rows, nkv * hd].  Rows without a slot stay as they are.
+// Rows of slots back as values: k_rows and v_rows [rows, nkv * hd].  Rows without a slot stay as they are.  A lane has two words.
 template <typename T>
 __global__ void __launch_bounds__(kQ4Threads)
 read_q4_kernel(const uint8_t* k_cache, const uint8_t* v_cache, const int* __restrict__ slot_mapping, T* __restrict__ k_rows,
-               T* __restrict__ v_rows, long long k_stride, long long v_stride, int nkv, int hd, int block_size, int num_pages) {
+               T* __restrict__ v_rows, long long k_stride, long long v_stride, int nkv, int hd, int block_size, int num_pages, int log2_lanes) {
   pdl_launch_dependents();
   pdl_wait();
-  const int words = hd / 8, item = blockIdx.y * kQ4Threads + threadIdx.x;
-  const int row = blockIdx.x, head = item / words, word = item - head * words;
-  if (head >= 2 * nkv) return;
+  const int item = blockIdx.y * blockDim.x + threadIdx.x;
+  const int row = blockIdx.x, head = item >> log2_lanes, word = 2 * (item & ((1 << log2_lanes) - 1));
+  if (head >= 2 * nkv || word >= hd / 8) return;
   const int slot = slot_mapping[row];
   if (slot < 0) return;
   const int page = slot / block_size, off = slot - page * block_size;
@@ -174,10 +206,18 @@ read_q4_kernel(const uint8_t* k_cache, const uint8_t* v_cache, const int* __rest
   const bool is_k = head < nkv;
   const int kvh = is_k ? head : head - nkv;
   const uint8_t* base = (is_k ? k_cache : v_cache) + (size_t(page) * nkv + kvh) * q4::page_bytes(block_size, hd);
+  const uint32_t pair = *reinterpret_cast<const uint32_t*>(base + size_t(block_size) * (hd / 2) + off * 4);
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>(base + size_t(off) * (hd / 2)) + word;
+  T* to = (is_k ? k_rows + size_t(row) * k_stride : v_rows + size_t(row) * v_stride) + size_t(kvh) * hd + word * 8;
+  const bool second = word + 1 < hd / 8;
+  const uint32_t w[2] = {codes[0], second ? codes[1] : 0u};
   float x[8];
-  values8(*reinterpret_cast<const uint32_t*>(base + size_t(off) * (hd / 2) + word * 4),
-          *reinterpret_cast<const uint32_t*>(base + size_t(block_size) * (hd / 2) + off * 4), x);
-  store8((is_k ? k_rows + size_t(row) * k_stride : v_rows + size_t(row) * v_stride) + size_t(kvh) * hd + word * 8, x);
+  values8(w[0], pair, x);
+  store8(to, x);
+  if (second) {
+    values8(w[1], pair, x);
+    store8(to + 8, x);
+  }
 }
 
 // The pages of requests `first_seq` .. `first_seq + grid.y` as bfloat16 pages [request, block][nkv, block_size, hd]: those that hold
@@ -213,19 +253,35 @@ unpack_pages_q4_kernel(const uint8_t* k_cache, const uint8_t* v_cache, const int
   }
 }
 
+// Lanes of a head, as a power of two: hd / 16, rounded up.
+int q4_log2_lanes(int hd) {
+  int n = 0;
+  while ((16 << n) < hd) ++n;
+  return n;
+}
+// A row's items in blocks of like size: (rows, blocks), threads.
+void q4_grid(int rows, int items, dim3& grid, dim3& block) {
+  const int pieces = (items + kQ4Threads - 1) / kQ4Threads;
+  grid = dim3(rows, pieces);
+  block = dim3(((items + pieces - 1) / pieces + 31) / 32 * 32);
+}
+
 template <typename T>
 int launch_store_q4(const StoreQ4Params& p, cudaStream_t s) {
-  const int items = (p.nh + 2 * p.nkv) << p.log2_lanes;
-  return pdl_launch(store_q4_kernel<T>, dim3(p.rows, (items + kQ4Threads - 1) / kQ4Threads), dim3(kQ4Threads), 0, s, p);
+  dim3 grid, block;
+  q4_grid(p.rows, (p.nh + 2 * p.nkv) << p.log2_lanes, grid, block);
+  return pdl_launch(store_q4_kernel<T>, grid, block, 0, s, p);
 }
 
 template <typename T>
 int launch_read_q4(const void* k_cache, const void* v_cache, const int* slots, void* k_rows, void* v_rows, long long k_stride,
                    long long v_stride, int rows, int nkv, int hd, int block_size, int num_pages, cudaStream_t s) {
-  const int items = 2 * nkv * (hd / 8);
-  return pdl_launch(read_q4_kernel<T>, dim3(rows, (items + kQ4Threads - 1) / kQ4Threads), dim3(kQ4Threads), 0, s,
+  const int log2_lanes = q4_log2_lanes(hd);
+  dim3 grid, block;
+  q4_grid(rows, 2 * nkv << log2_lanes, grid, block);
+  return pdl_launch(read_q4_kernel<T>, grid, block, 0, s,
                     (const uint8_t*)k_cache, (const uint8_t*)v_cache, slots, (T*)k_rows, (T*)v_rows, k_stride, v_stride, nkv, hd,
-                    block_size, num_pages);
+                    block_size, num_pages, log2_lanes);
 }
 
 bool q4_sizes_ok(int nkv, int hd, int block_size, int num_pages) {
@@ -260,8 +316,7 @@ KVCM_API long long kvcm_q4_page_bytes(int block_size, int hd) { return (long lon
     p.slot_mapping = slot_mapping; p.k_out = (uint8_t*)k_cache; p.v_out = (uint8_t*)v_cache; p.q_out = q_out;                  \
     p.q_stride = q_stride; p.rows = rows; p.nh = nh; p.nkv = nkv; p.hd = hd; p.block_size = block_size;                        \
     p.num_pages = num_pages;                                                                                                   \
-    p.log2_lanes = 0;                                                                                                          \
-    while ((16 << p.log2_lanes) < hd) ++p.log2_lanes;                                                                           \
+    p.log2_lanes = q4_log2_lanes(hd);                                                                                          \
     return launch_store_q4<T>(p, (cudaStream_t)stream);                                                                        \
   }                                                                                                                           \
   KVCM_API int kvcm_read_cache_q4_##SUFFIX(const void* k_cache, const void* v_cache, const int* slot_mapping, void* k_rows,    \
