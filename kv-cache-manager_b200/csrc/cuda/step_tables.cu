@@ -14,6 +14,7 @@
 // barrier stands between the last read of start and count and the first write, so that ctx_len may be start and free_left may
 // be free_count (a step that is replayed from a graph advances itself).  Integer sums only: the results do not depend on order.
 // What bounds it: three dependent trips to memory (lengths, table or stack, the store) and the launch; the bytes are a few KB to 1 MB.
+// B200: 250 requests of one row 4.5 us, 64 portions of some 120 rows 6.5 us.
 //
 // The kernels of a step read these arrays before their dependency wait, so this kernel is launched the ordinary way and never
 // lets its dependents start early (see pdl.cuh): whoever comes after it finds the arrays complete.
