@@ -119,7 +119,11 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(TabParams p) {
   }
   Triple total = warp_sum_of[31];
   int code = 0, detail = 0;
-  if (first_bad != 0x7fffffff) { code = first_bad & 3; detail = first_bad >> 2; }
+  if (first_bad != 0x7fffffff) {
+    code = first_bad & 3;
+    detail = first_bad >> 2;
+    if (code == kTabRows) detail = p.n[detail];    // (the text speaks of rows)
+  }
   else if (total.rows > p.rows) { code = kTabRows; detail = total.rows; }
   else if (total.tiles > p.tiles && p.tile_seq != nullptr) { code = kTabTiles; detail = total.tiles; }
   else if (count < 0 || count > p.stack) { code = kTabStack; detail = count; }

@@ -124,7 +124,7 @@ def test_a_replayed_graph_goes_on_from_step_to_step():
 
 @pytest.mark.parametrize("change,code,number", [
     (dict(n=[1, -1, 2]), 1, 1), (dict(start=[0, 5, -3]), 1, 2), (dict(start=[0, 63, 9], n=[1, 2, 1]), 2, 1), (dict(n=[3, 4, 4]), 3, 11),
-    (dict(n=[1, 11, 1]), 3, 1), (dict(n=[2, 2, 2], tiles=2), 4, 3), (dict(count=0, n=[1, 1, 1]), 5, 1), (dict(count=99), 6, 99), (dict(count=-1), 6, -1),
+    (dict(n=[1, 11, 1]), 3, 11), (dict(n=[2, 2, 2], tiles=2), 4, 3), (dict(count=0, n=[1, 1, 1]), 5, 1), (dict(count=99), 6, 99), (dict(count=-1), 6, -1),
     (dict(n=[1, 2 ** 31 - 1, 1]), 2, 1)])
 def test_a_step_that_cannot_be_changes_nothing(change, code, number):
     """10 rows of room, tables of 64 positions, requests of 16, 5 and 9 positions."""
