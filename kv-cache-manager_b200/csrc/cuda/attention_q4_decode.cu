@@ -10,8 +10,10 @@
 //        larger products would.   q.k = scale (q.code) + zero sum(q)  follows in float32.
 //   O^T  in float16, m16n8k16: an element of two neighbouring keys is one register (the words of the two keys, half by half), as
 //        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of the power of two
-//        above the largest scale that the warp has seen (a float16 below one), so a weight is rounded by 2^-12 of itself, and by
-//        2^-25 of the largest where it is smaller than 2^-14.
+//        above the largest that the warp has seen (a float16 below one), so a weight is rounded by 2^-12 of itself, and by
+//        2^-25 of the largest weight where it is smaller than 2^-14 of it.
+//        (Units of the largest scale alone, whatever its key's probability, cost 2 % less and let one large value without weight take
+//        the others' bits.)
 //   P goes from accumulators to operands by a transposing register move (movmatrix): no shared memory in between.
 // The scores of the next step are formed under the softmax of this one.  Pages come by 16-byte asynchronous copies into a ring of
 // steps per warp: no barriers between warps, pages of any size.
@@ -20,11 +22,11 @@
 // distributed shared memory, or equal shares of all requests' tiles of 128 keys, for batches of ragged or many requests: a share
 // begins and ends inside a request, the two pieces go through scratch memory, and a second kernel joins them.
 //
-// What bounds it, B200: instructions.  A step of 32 keys x 128 elements x 4 heads costs a warp some 550, of which products are 24; an
-// SM's four schedulers are 63 % busy (waits for the products' own results in between) and memory 5.1 TB/s: 64 requests of 8,192
-// keys, 32 heads on 8 of 128 elements, 571 MB: 112 us (88 at the rate of a copy).  64 requests of 100 to 8,192 keys (106 MB): 42 us,
-// of which the shares' starts and the second kernel are about 12.  27 requests of up to 1,024 keys behind a window, capped: 11 us;
-// 8 of 1,500 keys 7.9 us; one of 148 keys 4.8 us: launch, lengths, table, q and keys behind one another.
+// What bounds it, B200: instructions.  A step of 32 keys x 128 elements x 4 heads costs a warp some 560, of which products are 24; an
+// SM's four schedulers are 63 % busy (waits for the products' own results in between) and memory 5.0 TB/s: 64 requests of 8,192
+// keys, 32 heads on 8 of 128 elements, 571 MB: 115 us (88 at the rate of a copy).  64 requests of 100 to 8,192 keys (106 MB): 43 us,
+// of which the shares' starts and the second kernel are about 12.  27 requests of up to 1,024 keys behind a window, capped: 11.5 us;
+// 8 of 1,500 keys 8.1 us; one of 148 keys 5.0 us: launch, lengths, table, q and keys behind one another.
 #include <cooperative_groups.h>
 
 #include "attention_mma.cuh"
@@ -523,7 +525,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
               }
           }
           scores(next, ahead);                                     // (behind the last step: of what lies there, and nobody reads it)
-          // ---- running maximum; and the unit of the weights: the power of two above the largest scale so far
+          // ---- running maximum
           float top[HG];
           bool moved = false;
 #pragma unroll
@@ -534,14 +536,15 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
             top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 16));
             moved |= top[h] > m[h];
           }
-          const uint32_t largest = __reduce_max_sync(0xffffffffu, vpair[lane] << 16);
-          if (__any_sync(0xffffffffu, moved || largest >= unit)) {
-            float grown[HG], f = 1.f;
-            if (largest >= unit) {
-              const uint32_t unit_new = min((largest & 0x7f800000u) + 0x00800000u, 0x7f000000u);
-              f = __uint_as_float(unit) / __uint_as_float(unit_new);
-              unit = unit_new;
+          auto rescale = [&](const float (&f)[HG]) {
+#pragma unroll
+            for (int k = 0; k < S::kTiles; ++k) {
+              o[k][0] *= f[0]; o[k][2] *= f[0];
+              if constexpr (HG == 2) { o[k][1] *= f[1]; o[k][3] *= f[1]; }
             }
+          };
+          if (__any_sync(0xffffffffu, moved)) {
+            float grown[HG], most = 0.f;
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
               const float m_new = fmaxf(m[h], top[h]);
@@ -549,29 +552,55 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
               m[h] = m_new;
               l[h] *= grown[h];
               zacc[h] *= grown[h];
-              grown[h] *= f;
+              if (t4 + 4 * h < w.heads_here) most = fmaxf(most, grown[h]);
             }
+            // the weights so far have become at most `most` of what they were, and so may their unit
+            most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+            const uint32_t unit_new = min((__float_as_uint(__uint_as_float(unit) * most) & 0x7f800000u) + 0x00800000u, unit);
+            const float f = most > 0.f ? __uint_as_float(unit) / __uint_as_float(unit_new) : 1.f;
+            unit = unit_new;
 #pragma unroll
-            for (int k = 0; k < S::kTiles; ++k) {
-              o[k][0] *= grown[0]; o[k][2] *= grown[0];
-              if constexpr (HG == 2) { o[k][1] *= grown[1]; o[k][3] *= grown[1]; }
-            }
+            for (int h = 0; h < HG; ++h) grown[h] *= f;
+            rescale(grown);
           }
-          const float per_unit = __uint_as_float(0x7f000000u - unit);         // 1 / unit
+          // ---- weights p scale, and their unit: a power of two above the largest so far
+          float most_of[HG];
+#pragma unroll
+          for (int h = 0; h < HG; ++h) most_of[h] = 0.f;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
             const uint32_t pa = vpair[mt * 16 + row_g], pb = vpair[mt * 16 + row_g + 8];
             const float sa = q4::scale_of(pa), za = fmaf(8.f, sa, q4::zero_of(pa));
             const float sb = q4::scale_of(pb), zb = fmaf(8.f, sb, q4::zero_of(pb));
-            const float ua = sa * per_unit, ub = sb * per_unit;
-            float wa[2] = {0.f, 0.f}, wb[2] = {0.f, 0.f};
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
               const float ea = fast_exp2(x[mt][0][h] - m[h]), eb = fast_exp2(x[mt][1][h] - m[h]);
               l[h] += ea + eb;
               zacc[h] = fmaf(ea, za, fmaf(eb, zb, zacc[h]));
-              wa[h] = ea * ua;
-              wb[h] = eb * ub;
+              x[mt][0][h] = ea * sa;
+              x[mt][1][h] = eb * sb;
+              most_of[h] = fmaxf(most_of[h], fmaxf(x[mt][0][h], x[mt][1][h]));
+            }
+          }
+          float largest = t4 < w.heads_here ? most_of[0] : 0.f;    // (heads that are not there have q zero and all keys alike)
+          if (HG == 2 && t4 + 4 < w.heads_here) largest = fmaxf(largest, most_of[HG - 1]);
+          const uint32_t reached = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
+          if (reached >= unit) {
+            const uint32_t unit_new = min((reached & 0x7f800000u) + 0x00800000u, 0x7f000000u);
+            float f[HG];
+#pragma unroll
+            for (int h = 0; h < HG; ++h) f[h] = __uint_as_float(unit) / __uint_as_float(unit_new);
+            unit = unit_new;
+            rescale(f);
+          }
+          const float per_unit = __uint_as_float(0x7f000000u - unit);         // 1 / unit
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            float wa[2] = {0.f, 0.f}, wb[2] = {0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+              wa[h] = x[mt][0][h] * per_unit;
+              wb[h] = x[mt][1][h] * per_unit;
             }
             // columns of O: 2 t4 is head t4, 2 t4 + 1 head t4 + 4 (of one group: nobody)
             const uint32_t b0 = transposed(pack_half(wa[0], wa[1])), b1 = transposed(pack_half(wb[0], wb[1]));

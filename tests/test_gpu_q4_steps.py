@@ -284,3 +284,34 @@ def test_portions_do_not_see_masked_rows_that_are_no_numbers(hd, how):
                 sees = (pos >= key) & ((pos < key + window) if window else True)
                 assert got[sees].isnan().all() and torch.equal(got[~sees], clean[~sees]), (window, key, which)
     K().check_errors()
+
+
+# ------------------------------------------------------------------------------------------- values of very different size
+
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 1, 128), (1, 1, 64), (8, 1, 96), (6, 2, 128)])
+@pytest.mark.parametrize("force", [1, 3, -1])
+def test_a_large_value_without_weight_does_not_cost_the_others_their_bits(nh, nkv, hd, force):
+    """Values 2^24 times the others, whose keys have scores far below the rest (p < 2^-200): one in the midst of a request, and the first
+    32 of another, which are all there is until the rest comes.  The result is the others', to a rounding of it and of their
+    weights (2^-12 each, below the 2^-8 of max |v|)."""
+    B, n, at = 16, 400, [[37], range(32)]
+    tables, pages, ctx = make_step([(n - 1, 1), (n - 1, 1)], B, 21)
+    g = torch.Generator().manual_seed(22)
+    x = torch.randn((2, pages, B, nkv, hd), generator=g)
+    q = torch.randn((2, nh * hd), generator=g).abs().add(0.5).to(torch.bfloat16)
+    for i, t in ((i, t) for i in range(2) for t in at[i]):
+        page = int(tables[i, t // B])
+        x[0, page, t % B] = -6.0 + 0.1 * x[0, page, t % B]                 # q > 0: its scores are low in every head
+        x[1, page, t % B] *= 2.0 ** 24
+    kc, vc = (torch.zeros((pages, nkv, P.page_bytes(B, hd)), dtype=torch.uint8) for _ in range(2))
+    for p in range(pages):
+        for o in range(B):
+            P.write(kc, B, p, o, x[0, p, o])
+            P.write(vc, B, p, o, x[1, p, o])
+    out = torch.empty((2, nh * hd), dtype=torch.bfloat16, device=DEV)
+    ctx.options = {"attn_parts": force}
+    scale = 4.0 * hd ** -0.5
+    K().attention_decode_q4(q.to(DEV), out, kc.to(DEV), vc.to(DEV), tables.to(DEV), ctx, nh, nkv, hd, B, scale)
+    k, v = P.read(kc, hd, B), P.read(vc, hd, B)
+    want = P.attention(q.double().view(2, nh, hd), k, v, tables, [(n - 1, 1), (n - 1, 1)], nh, nkv, B, scale)
+    check_attention(out.view(2, nh, hd), want, 6.0, "bfloat16", n + hd)
