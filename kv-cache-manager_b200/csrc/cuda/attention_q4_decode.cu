@@ -30,6 +30,7 @@
 #include <cooperative_groups.h>
 
 #include "attention_mma.cuh"
+#include "packed.cuh"
 #include "pdl.cuh"
 #include "q4.cuh"
 
@@ -956,3 +957,5 @@ KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, vo
   return pdl_launch(attn_decode_q4_merge_kernel, dim3(seqs, nh), dim3(hd < 64 ? 32 : 64), 0, (cudaStream_t)stream, (const float*)p.part_o,
                     (const float*)p.part_ml, p.out, out_stride, nh, hd, num_parts, p.sink);
 }
+
+KVCM_PACKED(kvcm_attention_decode_q4_bf16)

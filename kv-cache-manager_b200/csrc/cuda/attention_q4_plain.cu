@@ -6,6 +6,7 @@
 // A chunk of 512 keys at a time: a thread forms the scores of whole keys (a key's codes are hd/2 bytes), then the products with
 // V are dealt out as words of eight elements, groups of threads taking every n-th key each, joined at the end in the groups'
 // order.  What bounds it is instructions: a code costs a shift, a mask, a conversion and a fused multiply-add.
+#include "packed.cuh"
 #include "pdl.cuh"
 #include "q4.cuh"
 
@@ -147,3 +148,6 @@ using namespace kvcm;
 
 KVCM_PLAIN_Q4(bf16, bf16)
 KVCM_PLAIN_Q4(f32, float)
+
+KVCM_PACKED(kvcm_attention_plain_q4_bf16)
+KVCM_PACKED(kvcm_attention_plain_q4_f32)

@@ -27,6 +27,7 @@
 // A thread of warps 8-14 copies what it unpacks itself (cp.async into shared memory, a tile ahead) and so waits for nobody else's.
 // Masks: key <= position, optional window.  Every wait is bounded; one that runs out sets the error word of the tcgen05 attention
 // family (codes 17 and up) and ends the block.
+#include "packed.cuh"
 #include "pdl.cuh"
 #include "q4.cuh"
 #include "tcgen05_common.cuh"
@@ -609,3 +610,5 @@ KVCM_API int kvcm_attention_prefill_q4_bf16(const void* q, long long q_stride, i
   if (hd == 64) return softcap > 0.f ? launch_prefill_q4<64, true>(mq, p, grid, s) : launch_prefill_q4<64, false>(mq, p, grid, s);
   return softcap > 0.f ? launch_prefill_q4<128, true>(mq, p, grid, s) : launch_prefill_q4<128, false>(mq, p, grid, s);
 }
+
+KVCM_PACKED(kvcm_attention_prefill_q4_bf16)

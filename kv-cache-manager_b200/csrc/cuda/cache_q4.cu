@@ -16,6 +16,7 @@
 // places counted through and taken apart by 64-bit divisions.  What is left is waiting: a block is one load, a few hundred
 // instructions and a store; packed pairs of float32 (50 us), other block sizes and cache hints (no change) do not help.  Reading the
 // 8 + 8 KV heads back: 11.5 us (43 MB), 16.7 with a word a lane and codes converted from whole numbers.
+#include "packed.cuh"
 #include "pdl.cuh"
 #include "q4.cuh"
 
@@ -344,3 +345,9 @@ KVCM_API int kvcm_unpack_pages_q4_bf16(const void* k_cache, const void* v_cache,
                     (const uint8_t*)v_cache, block_tables, max_blocks, seq_q_len, seq_ctx_len, (bf16*)k_pages, (bf16*)v_pages, first_seq,
                     blocks, nkv, hd, block_size, num_pages, window);
 }
+
+KVCM_PACKED(kvcm_rope_cache_q4_bf16)
+KVCM_PACKED(kvcm_rope_cache_q4_f32)
+KVCM_PACKED(kvcm_read_cache_q4_bf16)
+KVCM_PACKED(kvcm_read_cache_q4_f32)
+KVCM_PACKED(kvcm_unpack_pages_q4_bf16)

@@ -21,6 +21,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace kvcm {
 
@@ -217,3 +218,5 @@ KVCM_API int kvcm_step_tables(const int* start, const int* n, int* block_tables,
   cfg.numAttrs = blocks > 1 ? 1 : 0;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, step_tables_kernel, p));
 }
+
+KVCM_PACKED(kvcm_step_tables)

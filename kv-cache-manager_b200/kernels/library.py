@@ -9,6 +9,7 @@ kernels (used by the benchmark's ``gpu_launches``).
 from __future__ import annotations
 
 import ctypes
+import struct
 import types
 from typing import Optional
 
@@ -569,23 +570,25 @@ def prefill_tcgen05_supported(hd: int, block_size: int, shared_kv: bool = False)
 
 
 class _Entry:
-    """One C entry point: argument types set once (p address, l 64-bit, i 32-bit, f float), called with plain numbers on a given
-    device's current stream.  A launch of a small kernel costs more on the host than on the GPU, and most of that was wrapping."""
-    _TYPES = {"p": ctypes.c_void_p, "l": ctypes.c_longlong, "i": ctypes.c_int, "f": ctypes.c_float}
+    """One C entry point (p address, l 64-bit, i 32-bit, f float; the stream behind them), called with plain numbers on a given device's
+    current stream.  Its packed face takes all of them as 8-byte slots: a launch of a small kernel costs more on the host than on
+    the GPU, and most of that was turning arguments into C ones."""
 
     def __init__(self, symbol: str, types: str) -> None:
-        self.symbol, self.types, self.fn = symbol, types, None
+        self.symbol, self.fn = symbol, None
+        self.pack = struct.Struct("".join("d" if c == "f" else "q" for c in types + "p")).pack
+
+    def _load(self):
+        self.fn = getattr(_lib(), self.symbol + "_packed")
+        self.fn.argtypes, self.fn.restype = [ctypes.c_char_p], ctypes.c_int
+        return self.fn
 
     def __call__(self, device: int, *args) -> int:
-        if self.fn is None:
-            fn = getattr(_lib(), self.symbol)
-            fn.argtypes = [self._TYPES[c] for c in self.types] + [ctypes.c_void_p]
-            fn.restype = ctypes.c_int
-            self.fn = fn
+        fn = self.fn or self._load()
         if device == torch._C._cuda_getDevice():
-            return self.fn(*args, torch._C._cuda_getCurrentRawStream(device))
+            return fn(self.pack(*args, torch._C._cuda_getCurrentRawStream(device)))
         with torch.cuda.device(device):
-            return self.fn(*args, torch._C._cuda_getCurrentRawStream(device))
+            return fn(self.pack(*args, torch._C._cuda_getCurrentRawStream(device)))
 
 
 def _one_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
@@ -609,8 +612,8 @@ def _launched(rc: int, name: str, detail: str, *numbers) -> None:
         profile_mark(name)
 
 
-def _at(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 # ------------------------------------------------------------------ a cache in 4 bits (csrc/cuda/q4.cuh)
@@ -626,12 +629,12 @@ def _q4_cache(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, nkv: int,
         raise KernelError(f"{name}: head sizes are multiples of 8 up to 256")
     if not 0 < block_size <= 65536:
         raise KernelError(f"{name}: block_size of 1 to 65536 rows")
-    pages = k_cache.shape[0]
-    want = (pages, nkv, q4_page_bytes(block_size, hd))
-    for t in (k_cache, v_cache):
-        if t.dtype != torch.uint8 or t.dim() != 3 or t.shape[1:] != want[1:] or not t.is_contiguous() or t.data_ptr() % 16:
-            raise KernelError(f"{name}: caches must be contiguous uint8 [pages, {want[1]}, {want[2]}] on 16 bytes")
-    if pages == 0 or v_cache.shape[0] != pages:
+    shape, row = k_cache.shape, q4_page_bytes(block_size, hd)
+    if len(shape) != 3 or shape[1] != nkv or shape[2] != row or v_cache.shape[1:] != shape[1:] or k_cache.dtype != torch.uint8 \
+            or v_cache.dtype != torch.uint8 or not k_cache.is_contiguous() or not v_cache.is_contiguous() \
+            or (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise KernelError(f"{name}: caches must be contiguous uint8 [pages, {nkv}, {row}] on 16 bytes")
+    if shape[0] == 0 or v_cache.shape[0] != shape[0]:
         raise KernelError(f"{name}: k and v pools differ in their number of pages")
 
 
