@@ -20,8 +20,10 @@
 // Roles (16 warps, 128 registers a thread): 0-3 and 4-7 softmax and output of the two groups; 8-11 turn keys into operands and
 // their pairs into scales, 12-14 values; one thread of warp 15 brings Q and issues the products, the groups in turn, so that the
 // products of one run under the softmax of the other.
-// What bounds it: at head_dim 128 a tile's exponentials (256 x 128 at 16 a cycle) and its products each take 2,048 cycles; a
-// handshake between roles takes some 250 cycles, and four of them lie between two softmaxes of a group.  B200, 32 heads on 8 of
+// What bounds it: at head_dim 128 a tile of 256 x 128 takes some 5,500 cycles.  Its exponentials (16 a cycle) and its products each
+// take 2,048; shared memory is busy 3,300 by count (the products' operands 1,540, the keys' scales, read by every row's warp,
+// 1,020, unpacking 770); a handshake between roles takes some 250, and four of them lie between two softmaxes of a group.  Two
+// threads a row, each half of a tile's keys (16 softmax warps at 80 registers), take longer, 1,438 us for the 1,100 below.  B200, 32 heads on 8 of
 // 128: 2,048 rows 73 us (470 TFLOP/s causal), four portions of 1,500 rows behind 6,000
 // keys 1,100 us (670 TFLOP/s); 148 rows of heads of 64 10 us.
 // A thread of warps 8-14 copies what it unpacks itself (cp.async into shared memory, a tile ahead) and so waits for nobody else's.
