@@ -712,12 +712,13 @@ def _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, blo
     _q4_cache(name, k_cache, v_cache, nkv, hd, block_size)
     if q.dtype != out.dtype or q.dtype not in _SUFFIX:
         raise KernelError(f"{name}: q and out must be bfloat16 or float32 rows of one type")
-    width = nh * hd
-    if q.dim() != 2 or out.dim() != 2 or out.shape[0] != q.shape[0] or q.shape[1] < width or out.shape[1] < width:
+    width, rows, to = nh * hd, q.shape, out.shape
+    if len(rows) != 2 or len(to) != 2 or to[0] != rows[0] or rows[1] < width or to[1] < width:
         raise KernelError(f"{name}: q and out must be rows of {nh} heads of {hd}")
     if q.stride(1) != 1 or out.stride(1) != 1:
         raise KernelError(f"{name}: rows must be dense")
-    if block_tables.dtype != _I32 or block_tables.dim() != 2 or not block_tables.is_contiguous() or block_tables.shape[1] == 0:
+    tables = block_tables.shape
+    if block_tables.dtype != _I32 or len(tables) != 2 or tables[1] == 0 or not block_tables.is_contiguous():
         raise KernelError(f"{name}: block_tables must be contiguous int32 [S, max_blocks]")
     if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nh or not sink.is_contiguous()):
         raise KernelError(f"{name}: sink must be float32 [heads]")
@@ -794,9 +795,11 @@ def attention_decode_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tenso
     _ints(name, "seq_ctx_len", lengths, S)
     if not attention_q4_supported(hd, q.dtype):
         raise KernelError(f"{name}: bfloat16 rows, heads of 32 to 256 elements in steps of 32")
-    if q.data_ptr() % 16 or q.stride(0) % 8 or out.data_ptr() % 8 or out.stride(0) % 4:
+    at, to, step, out_step = q.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0)
+    if at % 16 or step % 8 or to % 8 or out_step % 4:
         raise KernelError(f"{name}: q rows must be 16-byte aligned, out rows 8-byte aligned")
-    if block_tables.shape[0] < S:
+    requests, max_blocks = block_tables.shape
+    if requests < S:
         raise KernelError(f"{name}: a page table for each of {S} rows")
     device = _one_device(name, q, out, k_cache, v_cache, block_tables, lengths, sink)
     if S == 0:
@@ -810,9 +813,8 @@ def attention_decode_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tenso
         scratch = torch.empty(shares * 16 * (hd + 2) + S * nh * 2, dtype=torch.float32, device=q.device)
     elif parts > 1 and not in_cluster:
         scratch = torch.empty(S * nh * parts * (hd + 2), dtype=torch.float32, device=q.device)
-    rc = _DECODE_Q4(device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
-                    block_tables.data_ptr(), block_tables.shape[1], lengths.data_ptr(), S, nh, nkv, hd, block_size, scale, window,
-                    size, parts, shares, _at(scratch), int(in_cluster), softcap, _at(sink))
+    rc = _DECODE_Q4(device, at, step, to, out_step, k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], block_tables.data_ptr(), max_blocks,
+                    lengths.data_ptr(), S, nh, nkv, hd, block_size, scale, window, size, parts, shares, _at(scratch), int(in_cluster), softcap, _at(sink))
     _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
     if scratch is not None:
         add_launches(1)                     # the merge kernel
@@ -924,7 +926,7 @@ def step_tables(seq_start: torch.Tensor, seq_q_len: torch.Tensor, block_tables: 
         raise KernelError(f"{name}: block_size and tile_rows must be positive")
     for t in (seq_start, seq_q_len, block_tables, free_pages, free_count, seq_q_start, seq_ctx_len, positions, row_seq, slot_mapping, free_left,
               status, tile_seq, tile_q0):
-        if t is not None and (t.dtype != _I32 or not t.is_contiguous()):
+        if t is not None and (t.dtype is not _I32 or not t.is_contiguous()):
             raise KernelError(f"{name}: contiguous int32 arrays")
     if seq_start.numel() != S or seq_q_start.numel() != S or seq_ctx_len.numel() != S:
         raise KernelError(f"{name}: per-request arrays of {S}")
