@@ -824,8 +824,9 @@ def paged_attention_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor
                        ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
                        sink: Optional[torch.Tensor] = None) -> None:
     """``paged_attention`` over a cache in 4 bits: attention of all rows of a step, rows [0, ctx.decode_seqs) single-row entries, the
-    rest the rows of longer portions; a row without keys gives zeros.  float32 rows, other head sizes and
-    ``ctx.options['attention'] == 'plain'``: ``attention_plain_q4`` for every row."""
+    rest the rows of longer portions; a row without keys gives zeros.  Single row i is request i's: requests that bring nothing stand
+    behind the others.  ``ctx.max_decode_ctx`` and ``ctx.max_ctx`` are at least the longest contexts (of a recorded step: the longest it
+    will see).  float32 rows, other head sizes and ``ctx.options['attention'] == 'plain'``: ``attention_plain_q4`` for every row."""
     if ctx.options.get("attention", "auto") == "plain" or not attention_q4_supported(hd, q.dtype):
         attention_plain_q4(q, out, k_cache, v_cache, block_tables, ctx.row_seq, ctx.positions, nh, nkv, hd, block_size, scale, window,
                            softcap, sink)
@@ -917,7 +918,7 @@ def step_tables(seq_start: torch.Tensor, seq_q_len: torch.Tensor, block_tables: 
     and ``free_left`` may be ``free_count``: a step replayed from a CUDA graph then goes on from the one before.
     ``status`` [4]: (0, 0, rows, tiles), or (code, number, 0, 0) where the step cannot be (``raise_on_step_tables``): pages, counts
     and lengths are then as before and every row is one behind the last.  The host reads it when it likes; nothing waits here.
-    The requests stay in the caller's order: entries of one row come first where attention takes them as such."""
+    The requests stay in the caller's order: entries of one row come first where attention takes them as such, those of none last."""
     name = "step_tables"
     S, T = seq_q_len.numel(), positions.numel()
     if not 0 < S <= 8192:
