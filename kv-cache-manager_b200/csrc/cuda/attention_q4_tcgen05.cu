@@ -170,7 +170,8 @@ __device__ __forceinline__ float qf_largest(const uint32_t (&s)[32], const QfSca
   return mx;
 }
 
-// What a row has in tensor memory times alpha: O, and the first `chunks` pieces of 32 probabilities.  (The whole warp takes part.)
+// What a row has in tensor memory times alpha: O, and the first `chunks` pieces of 32 probabilities, which are rounded to bfloat16
+// once more by that (a tile's pieces at most three times, and only where scores climb inside the tile).  The whole warp takes part.
 template <int HD>
 __device__ __noinline__ void qf_rescale(uint32_t o_addr, bool has_o, uint32_t p_addr, int chunks, float alpha) {
   uint32_t v[16];
@@ -182,6 +183,7 @@ __device__ __noinline__ void qf_rescale(uint32_t o_addr, bool has_o, uint32_t p_
     for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
     qf_st16(o_addr + uint32_t(c * 16), v);
   }
+  if (chunks > 0) tc5::st_wait();                                  // loads of tensor memory pass stores that nobody waited for
 #pragma unroll 1
   for (int c = 0; c < chunks; ++c) {
     qf_ld16(p_addr + uint32_t(c * 16), v);

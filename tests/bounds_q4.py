@@ -1,0 +1,81 @@
+"""How far attention over the cache in 4 bits may be off, row by row and element by element, from the roundings that its kernels do.
+
+With x_j = zero_j + scale_j code_j and probabilities p_j (sum 1), in units in the last place of the types, half a step each:
+ * bfloat16 results: 2^-8 |o|; float32 results 2^-24 |o|.
+ * weights: the kernels on tensor cores round p_j scale_j once where it enters a product with code_j - 8 (float16 2^-11 in single rows,
+   bfloat16 2^-8 in portions, there up to three times more where a maximum is renewed inside a tile): ``weight`` * sum p scale |code - 8|.
+   float16 weights below 2^-14 of the unit, which is at most twice the largest, are off by up to 2^-25 of it:
+   2^-24 max(p scale) * sum |code - 8|, ``small`` times.
+ * float32 sums: ``terms`` * 2^-24 of the sum of the terms' sizes, sum p (15 scale + |zero|).
+ * a score that is off by e changes the result by at most e * sum p |x - o|.  A score's terms are q_d code_d scale and zero q_d: e is
+   (hd + 8) * 2^-24 of their sizes (portions: codes enter with 128 added, which is taken out again: 2 * 143 scale |q_d|), single rows' q
+   in addition max|q| / 65024 * scale * sum code (q in 16 bits); exponentials and products around them 8 * 2^-24 (1 + |score|).
+"""
+import torch
+
+import plain_q4 as P
+
+
+def parts(cache, hd, B):
+    """Codes, scale, zero (float64) of all rows of a cache: [pages, nkv, B, hd], [pages, nkv, B, 1] twice."""
+    pages, nkv, _ = cache.shape
+    n = B * hd // 2
+    pair = cache[..., n:n + 4 * B].contiguous().view(torch.bfloat16).double().view(pages, nkv, B, 2)
+    scale, zero = pair[..., :1], pair[..., 1:]
+    x = P.read(cache, hd, B)
+    code = torch.where(scale > 0, (x - zero) / torch.where(scale > 0, scale, torch.ones_like(scale)), torch.zeros_like(x)).round()
+    return code, scale, zero
+
+
+KINDS = {"single": dict(weight=2.0 ** -11, small=1, result=2.0 ** -8, q16=True, offset=0.0),
+         "portion": dict(weight=2.0 ** -8, small=0, result=2.0 ** -8, q16=False, offset=2 * 143.0),
+         "climbing portion": dict(weight=4 * 2.0 ** -8, small=0, result=2.0 ** -8, q16=False, offset=2 * 143.0),
+         "plain bfloat16": dict(weight=0.0, small=0, result=2.0 ** -8, q16=False, offset=0.0),
+         "plain float32": dict(weight=0.0, small=0, result=2.0 ** -24, q16=False, offset=0.0)}
+
+
+def attention(kind, q, kc, vc, tables, spans, nh, nkv, hd, B, scale, window=0, lost=None):
+    """float64 rows [rows, nh, hd] and the room around each; ``lost``: (first, last) keys left out of the sums (a planted mistake)."""
+    c = KINDS[kind]
+    eps = 2.0 ** -24
+    k_of, v_of = parts(kc, hd, B), parts(vc, hd, B)
+    want, room = torch.zeros_like(q), torch.zeros_like(q)
+    row = 0
+    for i, (start, n) in enumerate(spans):
+        end = start + n
+        ids = tables[i, :(end + B - 1) // B].long()
+        kcode, ks, kz, vcode, vs, vz = (x[ids].transpose(0, 1).flatten(1, 2)[:, :end] for x in (*k_of, *v_of))
+        at = torch.arange(start, end)[:, None]
+        key = torch.arange(end)
+        seen = (key <= at) & (key > at - window if window else torch.ones_like(key, dtype=torch.bool))
+        if lost is not None:
+            seen = seen & ~((key >= lost[0]) & (key < lost[1]))
+        for h in range(nh):
+            g = h // (nh // nkv)
+            x, s1, z1 = vz[g] + vs[g] * vcode[g], vs[g], vz[g]
+            rows = q[row:row + n, h]
+            s = (rows @ (kz[g] + ks[g] * kcode[g]).T) * scale
+            s = s.masked_fill(~seen, -torch.inf)
+            p = torch.nan_to_num(torch.softmax(s, -1))
+            o = p @ x
+            coded = torch.full_like(kcode[g], c["offset"]) if c["offset"] else kcode[g]
+            size = (rows.abs() @ (ks[g] * coded + kz[g].abs()).T) * scale     # of a score's terms
+            e = (hd + 8) * eps * size + 8 * eps * (1 + s.abs())
+            if c["q16"]:
+                e = e + rows.abs().amax(-1, keepdim=True) / 65024 * (ks[g] * kcode[g]).sum(-1) * scale
+            e = torch.where(seen, e, torch.zeros_like(e)).amax(-1, keepdim=True)
+            apart = torch.stack([(p[r][:, None] * (x - o[r]).abs()).sum(0) for r in range(n)])
+            centred = (vcode[g] - 8).abs()
+            top = (p * s1[:, 0]).amax(-1, keepdim=True)
+            want[row:row + n, h] = o
+            room[row:row + n, h] = (c["result"] * o.abs() + c["weight"] * ((p * s1[:, 0]) @ centred) + c["small"] * eps * top * (seen.double() @ centred)
+                                    + (end + hd) * eps * (p @ (15 * s1 + z1.abs())) + e * apart)
+        row += n
+    return want, room * 1.05                                         # products of the roundings with one another
+
+
+def check(got, want, room):
+    got = got.double().cpu()
+    assert torch.isfinite(got).all()
+    over = ((got - want).abs() / room.clamp(min=1e-300)).nan_to_num(0.0)
+    assert over.max() <= 1, (over.max().item(), int(over.argmax()))
