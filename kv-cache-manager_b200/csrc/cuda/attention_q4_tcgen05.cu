@@ -255,8 +255,14 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
   const int tile = int(gridDim.y) - 1 - int(blockIdx.y), head = blockIdx.x;
   int* const error = p.error;
   const int seq = p.tile_seq[tile], q0 = p.tile_q0[tile];
-  if (seq < 0 || (q0 & (kQfRows - 1))) return;                     // no tile, or one that belongs to a block before
+  // (Whoever leaves waits too: a launch of nothing but empty tiles would else be over before the kernel in front of it, and
+  // the one behind it waits for this launch alone.)
+  if (seq < 0 || (q0 & (kQfRows - 1))) {                           // no tile, or one that belongs to a block before
+    pdl_wait();
+    return;
+  }
   if (tc5::s32(smem_raw) & 1023) {
+    pdl_wait();
     if (threadIdx.x == 0) atomicExch(error, (17 << 16) | int(blockIdx.y & 0xffff));
     return;
   }
