@@ -206,9 +206,10 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
   float* bl = bm + kQ4Heads;                                       // [8]
   const bool shares = p.num_parts == 0;
 
+  // Everything is read behind the wait: a caller may have written a whole prompt by the kernel before this one, and the lengths by
+  // one of the same step (step_tables, or a sum of its own), which nothing else makes visible here.
   pdl_launch_dependents();
-  // The step's integers are there before the step's kernels; keys, also old ones, only behind the wait: a caller may have
-  // written a whole prompt by the kernel before this one.
+  pdl_wait();
   auto length = [&](int s) { return min(p.seq_ctx_len[s], p.max_keys); };     // (a context ends with its table)
   auto first_key = [&](int ctx) { return ctx > 0 ? first_visible(ctx - 1, p.window, 0) : 0; };
   // a request's cost for each head: its tiles of keys behind the start
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
     }
     U = (long long)total * H;
     takers = min((long long)gridDim.x, U);                         // (a block between two that share a request then has a piece of it)
-    if (blockIdx.x >= takers) { pdl_wait(); return; }
+    if (blockIdx.x >= takers) return;
     const long long u0 = U * blockIdx.x / takers, u1 = U * (blockIdx.x + 1) / takers;
     left = u1 - u0;
     if ((long long)in_front * H <= u0 && u0 < (long long)(in_front + mine) * H) {
@@ -260,7 +261,6 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
     unit_h = int(at / n);
     at_cost = int(at - (long long)unit_h * n);
   }
-  pdl_wait();
 
   const size_t head_bytes = q4::page_bytes(p.block_size, HD);
   const unsigned head_units = unsigned(head_bytes / 16);

@@ -254,15 +254,13 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
   // heads fastest and the last tiles, which see most keys, first
   const int tile = int(gridDim.y) - 1 - int(blockIdx.y), head = blockIdx.x;
   int* const error = p.error;
+  // The tiles and lengths too may come from a kernel of the same step, so they are read behind the wait.  (Whoever leaves waits as
+  // well: a launch of nothing but empty tiles would else be over before the kernel in front of it, and the one behind it waits
+  // for this launch alone.)
+  pdl_wait();
   const int seq = p.tile_seq[tile], q0 = p.tile_q0[tile];
-  // (Whoever leaves waits too: a launch of nothing but empty tiles would else be over before the kernel in front of it, and
-  // the one behind it waits for this launch alone.)
-  if (seq < 0 || (q0 & (kQfRows - 1))) {                           // no tile, or one that belongs to a block before
-    pdl_wait();
-    return;
-  }
+  if (seq < 0 || (q0 & (kQfRows - 1))) return;                     // no tile, or one that belongs to a block before
   if (tc5::s32(smem_raw) & 1023) {
-    pdl_wait();
     if (threadIdx.x == 0) atomicExch(error, (17 << 16) | int(blockIdx.y & 0xffff));
     return;
   }
@@ -304,7 +302,6 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
   tc5::fence_after();
   const uint32_t tmem = tmem_base;
   pdl_launch_dependents();                                         // (only with the tensor memory in hand, see attention_tcgen05.cu)
-  pdl_wait();
 
   auto fail = [&](int code) {
     atomicExch(error, (code << 16) | int(blockIdx.y & 0xffff));

@@ -79,3 +79,90 @@ def test_tiles_of_no_request_between_single_rows_and_their_reader(hd, parts):
         g.replay()
         assert torch.equal(first, want[:, :2 * hd]) and torch.equal(k2, caches[0]) and torch.equal(v2, caches[1])
     K().check_errors()
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("parts", [0, 3, -1])
+def test_lengths_from_the_kernel_right_before(hd, parts):
+    """The contexts' ends are formed on the device by the launch in front of the call, others every time."""
+    S = 12
+    s = Step(S, [3000] * S, 4, 1, hd, 0)
+    s.ctx.options, s.ctx.rows, s.q = {"attn_parts": parts}, S, s.q[:S].contiguous()
+    source, lengths = torch.zeros(S + 1, **I32), s.ctx.seq_ctx_len
+    out = torch.empty_like(s.q)
+
+    def step():
+        torch.add(source, 1, out=lengths)
+        s.attend(out)
+    g = captured(step)
+    for i in range(40):
+        ends = torch.tensor([(97 * i + 211 * j) % 2990 for j in range(S)] + [0], dtype=torch.int32)
+        source.copy_(ends)
+        g.replay()
+        got = out.clone()
+        lengths.copy_(ends + 1)
+        torch.cuda.synchronize()
+        s.attend(out)
+        torch.cuda.synchronize()
+        assert torch.equal(got, out), i
+    K().check_errors()
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_tiles_from_the_kernel_right_before(hd):
+    """Portions whose tiles, starts and lengths are formed by the launches in front of the call: another division of 300 rows every time."""
+    nh, nkv, B, T, tiles = 4, 1, 16, 300, 9
+    k, v = random_cache(60, nkv, B, hd, 1), random_cache(60, nkv, B, hd, 2)
+    tables = torch.randperm(60, generator=torch.Generator().manual_seed(3)).int().view(2, 30).to(DEV)
+    q = torch.randn((T, nh * hd), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(DEV)
+    i = lambda n: torch.full((n,), -1, **I32)
+    ctx = types.SimpleNamespace(rows=T, seqs=2, decode_seqs=0, prefill_tiles=tiles, tile_rows=64, max_ctx=480, max_decode_ctx=0, max_q_len=T, options={},
+                                positions=i(T), row_seq=i(T), seq_q_start=i(2).zero_(), seq_q_len=i(2).zero_(), seq_ctx_len=i(2).zero_(), tile_seq=i(tiles),
+                                tile_q0=i(tiles))
+    names = ("seq_q_start", "seq_q_len", "seq_ctx_len", "tile_seq", "tile_q0")
+    source = {n: getattr(ctx, n) - 1 for n in names}
+    out = torch.empty_like(q)
+
+    def attend():
+        K().paged_attention_q4(q, out, k, v, tables, ctx, nh, nkv, hd, B, hd ** -0.5)
+
+    def step():
+        for n in names:
+            torch.add(source[n], 1, out=getattr(ctx, n))
+        attend()
+    g = captured(step)
+    for r in range(30):
+        a = 2 + (37 * r) % (T - 4)
+        of = [(s, q0) for s, n in enumerate((a, T - a)) for q0 in range(0, n, 64)]
+        of += [(-1, -1)] * (tiles - len(of))
+        values = dict(seq_q_start=[0, a], seq_q_len=[a, T - a], seq_ctx_len=[a + r, T - a + 3 * r], tile_seq=[t for t, _ in of], tile_q0=[t for _, t in of])
+        for n in names:
+            source[n].copy_(torch.tensor(values[n], dtype=torch.int32) - 1)
+        g.replay()
+        got = out.clone()
+        for n in names:
+            getattr(ctx, n).copy_(torch.tensor(values[n], dtype=torch.int32))
+        torch.cuda.synchronize()
+        attend()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out), r
+    K().check_errors()
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_steps_of_many_rows_made_in_place_and_attended(hd):
+    """Steps of more rows than one block of ``step_tables`` takes (a cluster makes them), lengths and the free pages' count advanced in
+    place, from a graph: rows written, attention over them."""
+    from test_gpu_q4_steps import Loop
+    loop = Loop([0, 37, 64], 2, 1, hd, 16, 170, 400, 2750, 50, seed=hd)
+    portions = [[1100, 900, 702], [2, 1400, 1040], [0, 30, 600]]
+    loop.fill(portions[0])
+    loop.launch()
+    loop.check(portions[0])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        loop.launch()
+    for ns in portions[1:]:
+        loop.fill(ns)
+        g.replay()
+        loop.check(ns)
