@@ -14,10 +14,12 @@
 // barrier stands between the last read of start and count and the first write, so that ctx_len may be start and free_left may
 // be free_count (a step that is replayed from a graph advances itself).  Integer sums only: the results do not depend on order.
 // What bounds it: three dependent trips to memory (lengths, table or stack, the store) and the launch; the bytes are a few KB to 1 MB.
-// B200: 250 requests of one row 4.5 us, 64 portions of some 120 rows 6.5 us.
+// B200: 250 requests of one row 5.1 us, 64 portions of some 120 rows 7.1 us, of which the second launch is 0.6.
 //
-// The kernels of a step read these arrays before their dependency wait, so this kernel is launched the ordinary way and never
-// lets its dependents start early (see pdl.cuh): whoever comes after it finds the arrays complete.
+// Many kernels of a step read its integers before their dependency wait, as what a completed launch has written (pdl.cuh).  A kernel
+// that is launched early behind this one would start when its blocks have ended, which completes nothing, so both this kernel
+// and an empty one behind it are launched the ordinary way: the empty one starts when this one is complete, and whoever starts
+// behind that, however early, finds the arrays.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -169,8 +171,9 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(TabParams p) {
     *p.free_left = count - total.pages;
     p.status[0] = code; p.status[1] = detail; p.status[2] = total.rows; p.status[3] = total.tiles;
   }
-  __threadfence();                                 // (whoever starts at this kernel's end may read before its dependency wait)
 }
+
+__global__ void step_tables_done_kernel() {}
 
 }  // namespace kvcm
 
@@ -216,7 +219,10 @@ KVCM_API int kvcm_step_tables(const int* start, const int* n, int* block_tables,
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = blocks > 1 ? 1 : 0;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, step_tables_kernel, p));
+  const int rc = static_cast<int>(cudaLaunchKernelEx(&cfg, step_tables_kernel, p));
+  if (rc != 0) return rc;
+  step_tables_done_kernel<<<1, 32, 0, (cudaStream_t)stream>>>();
+  return static_cast<int>(cudaGetLastError());
 }
 
 KVCM_PACKED(kvcm_step_tables)

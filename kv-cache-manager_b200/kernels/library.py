@@ -914,7 +914,8 @@ def step_tables(seq_start: torch.Tensor, seq_q_len: torch.Tensor, block_tables: 
     more) rows behind them; ``free_pages[:free_count]`` are the free pages, taken from the top.
     Out: ``block_tables`` with the new pages, ``free_left``, ``seq_q_start``, ``seq_ctx_len`` (start + rows), per row ``positions``,
     ``row_seq`` and ``slot_mapping`` (rows behind the last one: -1, 0, -1), per tile of ``tile_rows`` rows of a request with more
-    than one row ``tile_seq`` and ``tile_q0`` (behind the last one -1); both may be left out.  ``seq_ctx_len`` may be ``seq_start``
+    than one row ``tile_seq`` and ``tile_q0`` (behind the last one -1, which ``attention_prefill_q4`` passes over; the bfloat16 kernels
+    want real tiles only); both may be left out.  ``seq_ctx_len`` may be ``seq_start``
     and ``free_left`` may be ``free_count``: a step replayed from a CUDA graph then goes on from the one before.
     ``status`` [4]: (0, 0, rows, tiles), or (code, number, 0, 0) where the step cannot be (``raise_on_step_tables``): pages, counts
     and lengths are then as before and every row is one behind the last.  The host reads it when it likes; nothing waits here.
@@ -947,6 +948,7 @@ def step_tables(seq_start: torch.Tensor, seq_q_len: torch.Tensor, block_tables: 
                       row_seq.data_ptr(), slot_mapping.data_ptr(), _at(tile_seq), _at(tile_q0), free_left.data_ptr(), status.data_ptr(),
                       S, T, tiles, block_size, tile_rows)
     _launched(rc, name, "({} requests, {} rows, {} tiles)", S, T, tiles)
+    add_launches(1)                         # the empty kernel behind it
 
 
 def raise_on_step_tables(status) -> None:

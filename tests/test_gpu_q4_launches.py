@@ -166,3 +166,33 @@ def test_steps_of_many_rows_made_in_place_and_attended(hd):
         loop.fill(ns)
         g.replay()
         loop.check(ns)
+
+
+def test_single_rows_in_bfloat16_behind_the_tables_of_their_step():
+    """Kernels that read a step's integers ahead of their wait, right behind the launch that makes them: the bfloat16 attention, lengths
+    advanced in place, from a graph."""
+    S, nh, nkv, hd, B, width = 300, 4, 1, 64, 16, 24
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn((S * width, nkv, B, hd), generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    q = torch.randn((S, nh * hd), generator=g).to(torch.bfloat16).to(DEV)
+    i = lambda n, x=0: torch.full((n,), x, **I32)
+    tables, free, count, status = i(S * width, -1).view(S, width), torch.randperm(S * width, generator=g).int().to(DEV), i(1, S * width), i(4)
+    ctx = types.SimpleNamespace(rows=S, seqs=S, decode_seqs=S, prefill_tiles=0, tile_rows=64, max_ctx=width * B, max_decode_ctx=width * B, max_q_len=1,
+                                positions=i(S), row_seq=i(S), slot_mapping=i(S), seq_q_start=i(S), seq_q_len=i(S, 1), seq_ctx_len=i(S), options={})
+    out = torch.empty_like(q)
+
+    def attend(o):
+        K().paged_attention(q, o, k, v, tables, ctx, nh, nkv, hd, hd ** -0.5)
+
+    def step():
+        K().step_tables(ctx.seq_ctx_len, ctx.seq_q_len, tables, free, count, B, seq_q_start=ctx.seq_q_start, seq_ctx_len=ctx.seq_ctx_len,
+                        positions=ctx.positions, row_seq=ctx.row_seq, slot_mapping=ctx.slot_mapping, free_left=count, status=status)
+        attend(out)
+    graph = captured(step)
+    for n in range(2, 60):
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert ctx.seq_ctx_len.tolist() == [n] * S and status.tolist() == [0, 0, S, 0]
+        attend(out)
+        assert torch.equal(got, out), n
