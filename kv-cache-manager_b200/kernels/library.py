@@ -847,10 +847,10 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
     the step's arrays with tiles of 64 rows (tiles of request -1 are none; ``ctx.max_ctx`` is at least the longest context; a context
     ends with its page table).  Heads of 64 and 128 elements: one kernel that unpacks pages beside the products.  Other heads, or
     ``ctx.options['attn_prefill'] == 'unpack'``: the pages that the portions see are laid out in bfloat16, in scratch of the call,
-    and read by ``attention_prefill`` (keys and values rounded once more, and a value that is not a number also reaches rows of its
-    tile that do not see it).  B200, heads of 128, one kernel | laid out: 148 rows 10 | 12 us, 2,048 rows 73 | 109, 100 rows behind
-    2,000 keys, three requests, 57 | 93; heads of 64, four portions of 500 rows behind 3,000 keys, 255 | 219, which the second
-    rounding does not buy."""
+    and read by ``attention_prefill``'s 'mma' kernel (keys and values rounded once more, and a value that is not a number also reaches
+    rows of its tile that do not see it).  B200, one kernel | laid out: heads of 128, 148 rows 13 | 32 us, 2,048 rows 77 | 305, 100 rows
+    behind up to 2,000 keys, three requests, 50 | 134; heads of 64, four portions of 500 rows behind up to 3,000 keys, 135 | 287.
+    Laid out, 2,048 rows: 32 heads on 8 of 32 elements 114 us, 10 on 5 of 96 172, 4 on 2 of 256 171."""
     name = "attention_prefill_q4"
     _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, block_size, window, softcap, sink)
     S = ctx.seq_ctx_len.numel()
@@ -891,7 +891,9 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
         step = types.SimpleNamespace(
             seq_q_start=pad(ctx.seq_q_start, 0), seq_q_len=pad(ctx.seq_q_len, 0), seq_ctx_len=pad(ctx.seq_ctx_len, 1).clamp_(max=blocks * block_size),
             tile_seq=torch.where(ctx.tile_seq < 0, S, ctx.tile_seq), tile_q0=ctx.tile_q0.clamp(min=0), prefill_tiles=ctx.prefill_tiles,
-            tile_rows=ctx.tile_rows, options=ctx.options)
+            tile_rows=ctx.tile_rows, options={"attn_prefill": "mma"})
+        # ('mma' reads these arrays behind its dependency wait and no key below the window; the other kernel takes the arrays for
+        # old ones and multiplies what lies below the window, where no page was laid out, by zero)
         attention_prefill(q, out, pages[0], pages[1], tables, step, nh, nkv, hd, scale, window, softcap, sink)
 
 
