@@ -533,7 +533,8 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
       tc5::fence_after();
       if (alive) {
         if (p.sink && m != -INFINITY) l += qf_exp2(p.sink[head] * 1.4426950408889634f - m);
-        const float inv = l == 0.f ? 0.f : 1.f / l, z = z2.x + z2.y;
+        const bool none = l == 0.f;                                // no key: zeros (a group without a tile has nothing in tensor memory)
+        const float inv = none ? 0.f : 1.f / l, z = z2.x + z2.y;
         bf16* dst = p.out + size_t(q_start + q0 + row) * p.out_stride + size_t(head) * HD;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
@@ -541,6 +542,8 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
           tc5::ld32(o_addr + uint32_t(c * 32), ov);                // (all lanes of the warp take part in the load)
           tc5::ld_wait();
           if (row < rows_here) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ov[i] = none ? 0u : ov[i];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               __nv_bfloat162 h[4];

@@ -10,6 +10,7 @@ With x_j = zero_j + scale_j code_j and probabilities p_j (sum 1), in units in th
  * a score that is off by e changes the result by at most e * sum p |x - o|.  A score's terms are q_d code_d scale and zero q_d: e is
    (hd + 8) * 2^-24 of their sizes (portions: codes enter with 128 added, which is taken out again: 2 * 143 scale |q_d|), single rows' q
    in addition max|q| / 65024 * scale * sum code (q in 16 bits); exponentials and products around them 8 * 2^-24 (1 + |score|).
+ * pages laid out in bfloat16: keys, values and probabilities are rounded there, 2^-8 of each.
 """
 import torch
 
@@ -30,6 +31,7 @@ def parts(cache, hd, B):
 KINDS = {"single": dict(weight=2.0 ** -11, small=1, result=2.0 ** -8, q16=True, offset=0.0),
          "portion": dict(weight=2.0 ** -8, small=0, result=2.0 ** -8, q16=False, offset=2 * 143.0),
          "climbing portion": dict(weight=4 * 2.0 ** -8, small=0, result=2.0 ** -8, q16=False, offset=2 * 143.0),
+         "laid out": dict(weight=0.0, small=0, result=2.0 ** -8, q16=False, offset=0.0, again=2.0 ** -8),
          "plain bfloat16": dict(weight=0.0, small=0, result=2.0 ** -8, q16=False, offset=0.0),
          "plain float32": dict(weight=0.0, small=0, result=2.0 ** -24, q16=False, offset=0.0)}
 
@@ -63,13 +65,16 @@ def attention(kind, q, kc, vc, tables, spans, nh, nkv, hd, B, scale, window=0, l
             e = (hd + 8) * eps * size + 8 * eps * (1 + s.abs())
             if c["q16"]:
                 e = e + rows.abs().amax(-1, keepdim=True) / 65024 * (ks[g] * kcode[g]).sum(-1) * scale
+            again = c.get("again", 0.0)
+            e = e + again * (rows.abs() @ (kz[g] + ks[g] * kcode[g]).abs().T) * scale
             e = torch.where(seen, e, torch.zeros_like(e)).amax(-1, keepdim=True)
             apart = torch.stack([(p[r][:, None] * (x - o[r]).abs()).sum(0) for r in range(n)])
             centred = (vcode[g] - 8).abs()
             top = (p * s1[:, 0]).amax(-1, keepdim=True)
             want[row:row + n, h] = o
             room[row:row + n, h] = (c["result"] * o.abs() + c["weight"] * ((p * s1[:, 0]) @ centred) + c["small"] * eps * top * (seen.double() @ centred)
-                                    + (end + hd) * eps * (p @ (15 * s1 + z1.abs())) + e * apart)
+                                    + (end + hd) * eps * (p @ (15 * s1 + z1.abs())) + e * apart
+                                    + 2 * again * (p @ x.abs()))
         row += n
     return want, room * 1.05                                         # products of the roundings with one another
 

@@ -41,3 +41,33 @@ def test_maxima_renewed_inside_a_tile(hd, step):
     K().check_errors()
     want, room = bounds.attention("climbing portion", q.double().view(-1, nh, hd), kc, vc, tables, spans, nh, nkv, hd, B, hd ** -0.5)
     bounds.check(out.view(-1, nh, hd), want, room)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 96])
+@pytest.mark.parametrize("n,keys", [(300, 32), (300, 160), (140, 16), (600, 16), (129, 64)])
+def test_rows_before_the_first_key_of_a_short_table(hd, n, keys):
+    """A portion longer than its page table: the context ends with the table, and the rows in front of its keys see nothing and are zero."""
+    from test_gpu_q4 import make_cache
+    nh, nkv, B = 2, 1, 16
+    tables, pages, ctx = make_step([(0, keys), (5, 200)], B, 2)
+    kc, vc = make_cache(pages, nkv, B, hd, 3), make_cache(pages, nkv, B, hd, 4)
+    tables = tables[:, :keys // B].contiguous()                     # the second request too is longer than its table
+    rows = n + 200
+    q = torch.randn((rows, nh * hd), generator=torch.Generator().manual_seed(5)).to(torch.bfloat16)
+    tiles = [(0, t) for t in range(0, n, 64)] + [(1, t) for t in range(0, 200, 64)]
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    ctx.rows, ctx.prefill_tiles, ctx.max_ctx = rows, len(tiles), max(n, 205)
+    ctx.seq_q_start, ctx.seq_q_len, ctx.seq_ctx_len = i([0, n]), i([n, 200]), i([n, 205])
+    ctx.tile_seq, ctx.tile_q0 = i([t for t, _ in tiles]), i([t for _, t in tiles])
+    for _ in range(3):
+        out = torch.full_like(q, 9.0, device=DEV)
+        K().attention_prefill_q4(q.to(DEV), out, kc.to(DEV), vc.to(DEV), tables.to(DEV), ctx, nh, nkv, hd, B, hd ** -0.5)
+        torch.cuda.synchronize()
+        K().check_errors()
+        for request, first, count in ((0, 0, n), (1, n, 200)):
+            blind = max(0, count - keys)
+            assert not out[first:first + blind].any()
+            got = out[first + blind:first + count].cpu()
+            want, room = bounds.attention("portion" if hd != 96 else "laid out", q.double()[first + blind:first + count].view(-1, nh, hd), kc, vc, tables[request:request + 1],
+                                          [(keys - (count - blind), count - blind)], nh, nkv, hd, B, hd ** -0.5)
+            bounds.check(got.view(-1, nh, hd), want, room)
