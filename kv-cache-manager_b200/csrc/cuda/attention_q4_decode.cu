@@ -10,10 +10,10 @@
 //        larger products would.   q.k = scale (q.code) + zero sum(q)  follows in float32.
 //   O^T  in float16, m16n8k16: an element of two neighbouring keys is one register (the words of the two keys, half by half), as
 //        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of the power of two
-//        above the largest that the warp has seen (a float16 below one), so a weight is rounded by 2^-12 of itself, and by
-//        2^-25 of the largest weight where it is smaller than 2^-14 of it.
-//        (Units of the largest scale alone, whatever its key's probability, cost 2 % less and let one large value without weight take
-//        the others' bits.)
+//        above the head's largest that the warp has seen (a float16 below one), so a weight is rounded by 2^-11 of itself at most, and by
+//        2^-25 of that unit where it is smaller than 2^-14 of it.
+//        (Units of the largest scale alone, whatever its key's probability, let one large value without weight take the others' bits,
+//        a unit for all heads of a warp one that has weight in one head only.)
 //   P goes from accumulators to operands by a transposing register move (movmatrix): no shared memory in between.
 // The scores of the next step are formed under the softmax of this one.  Pages come by 16-byte asynchronous copies into a ring of
 // steps per warp: no barriers between warps, pages of any size.
@@ -321,7 +321,9 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
     float o[S::kTiles][4];
 #pragma unroll
     for (int i = 0; i < S::kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    uint32_t unit = 0x00800000u;                                   // the power of two that weights are divided by, as a float's bits
+    // the powers of two that the heads' weights are divided by, as floats' bits: a head's own, so that a large value which has weight
+    // in one head takes no bits from the others
+    uint32_t unit[2] = {0x00800000u, 0x00800000u};
     if (w.begin < w.end) {
       // ---- q as the second operand: column g of group h is half g % 2 of head 4 h + g / 2, elements in the order in which a lane's
       // codes lie (of a word's eight, bytes 0, 4, 1, 5 and 2, 6, 3, 7)
@@ -545,7 +547,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
             }
           };
           if (__any_sync(0xffffffffu, moved)) {
-            float grown[HG], most = 0.f;
+            float grown[HG];
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
               const float m_new = fmaxf(m[h], top[h]);
@@ -553,15 +555,11 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
               m[h] = m_new;
               l[h] *= grown[h];
               zacc[h] *= grown[h];
-              if (t4 + 4 * h < w.heads_here) most = fmaxf(most, grown[h]);
+              // the weights so far have become `grown` of what they were, and so may their unit
+              const uint32_t unit_new = min((__float_as_uint(__uint_as_float(unit[h]) * grown[h]) & 0x7f800000u) + 0x00800000u, unit[h]);
+              if (grown[h] > 0.f) grown[h] *= __uint_as_float(unit[h]) / __uint_as_float(unit_new);
+              unit[h] = unit_new;
             }
-            // the weights so far have become at most `most` of what they were, and so may their unit
-            most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-            const uint32_t unit_new = min((__float_as_uint(__uint_as_float(unit) * most) & 0x7f800000u) + 0x00800000u, unit);
-            const float f = most > 0.f ? __uint_as_float(unit) / __uint_as_float(unit_new) : 1.f;
-            unit = unit_new;
-#pragma unroll
-            for (int h = 0; h < HG; ++h) grown[h] *= f;
             rescale(grown);
           }
           // ---- weights p scale, and their unit: a power of two above the largest so far
@@ -583,25 +581,32 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
               most_of[h] = fmaxf(most_of[h], fmaxf(x[mt][0][h], x[mt][1][h]));
             }
           }
-          float largest = t4 < w.heads_here ? most_of[0] : 0.f;    // (heads that are not there have q zero and all keys alike)
-          if (HG == 2 && t4 + 4 < w.heads_here) largest = fmaxf(largest, most_of[HG - 1]);
-          const uint32_t reached = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
-          if (reached >= unit) {
-            const uint32_t unit_new = min((reached & 0x7f800000u) + 0x00800000u, 0x7f000000u);
+          bool beyond = false;
+#pragma unroll
+          for (int h = 0; h < HG; ++h) beyond |= __float_as_uint(most_of[h]) >= unit[h];
+          if (__any_sync(0xffffffffu, beyond)) {
             float f[HG];
 #pragma unroll
-            for (int h = 0; h < HG; ++h) f[h] = __uint_as_float(unit) / __uint_as_float(unit_new);
-            unit = unit_new;
+            for (int h = 0; h < HG; ++h) {
+#pragma unroll
+              for (int off = 4; off <= 16; off *= 2) most_of[h] = fmaxf(most_of[h], __shfl_xor_sync(0xffffffffu, most_of[h], off));
+              // (up to 2^126: its reciprocal is a normal number)
+              const uint32_t unit_new = max(unit[h], min((__float_as_uint(most_of[h]) & 0x7f800000u) + 0x00800000u, 0x7e800000u));
+              f[h] = __uint_as_float(unit[h]) / __uint_as_float(unit_new);
+              unit[h] = unit_new;
+            }
             rescale(f);
           }
-          const float per_unit = __uint_as_float(0x7f000000u - unit);         // 1 / unit
+          float per_unit[HG];                                      // 1 / unit
+#pragma unroll
+          for (int h = 0; h < HG; ++h) per_unit[h] = __uint_as_float(0x7f000000u - unit[h]);
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
             float wa[2] = {0.f, 0.f}, wb[2] = {0.f, 0.f};
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
-              wa[h] = x[mt][0][h] * per_unit;
-              wb[h] = x[mt][1][h] * per_unit;
+              wa[h] = x[mt][0][h] * per_unit[h];
+              wb[h] = x[mt][1][h] * per_unit[h];
             }
             // columns of O: 2 t4 is head t4, 2 t4 + 1 head t4 + 4 (of one group: nobody)
             const uint32_t b0 = transposed(pack_half(wa[0], wa[1])), b1 = transposed(pack_half(wb[0], wb[1]));
@@ -670,7 +675,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
         zacc[h] += __shfl_xor_sync(0xffffffffu, zacc[h], off);
       }
-    const float f_low = __uint_as_float(unit), f_high = f_low * 0.0625f;
+    const float f_low[2] = {__uint_as_float(unit[0]), __uint_as_float(unit[1])}, f_high[2] = {f_low[0] * 0.0625f, f_low[1] * 0.0625f};
     float* row0 = mo + (warp * kQ4Heads + t4) * HD;
     float* row1 = row0 + 4 * HD;
 #pragma unroll
@@ -678,18 +683,18 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int d = 8 * (g * S::kFull + j) + 2 * k;
-        const float f = (k & 1) ? f_high : f_low;
+        const float (&f)[2] = (k & 1) ? f_high : f_low;
         const float (&c)[4] = o[4 * j + k];
-        *reinterpret_cast<float2*>(row0 + d) = make_float2(fmaf(c[0], f, zacc[0]), fmaf(c[2], f, zacc[0]));
-        if constexpr (HG == 2) *reinterpret_cast<float2*>(row1 + d) = make_float2(fmaf(c[1], f, zacc[1]), fmaf(c[3], f, zacc[1]));
+        *reinterpret_cast<float2*>(row0 + d) = make_float2(fmaf(c[0], f[0], zacc[0]), fmaf(c[2], f[0], zacc[0]));
+        if constexpr (HG == 2) *reinterpret_cast<float2*>(row1 + d) = make_float2(fmaf(c[1], f[1], zacc[1]), fmaf(c[3], f[1], zacc[1]));
       }
     if constexpr (S::kHalf) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int d = 8 * (8 * S::kFull + (g >> 1)) + 4 * k + (g & 1);
         const float (&c)[4] = o[4 * S::kFull + k];
-        row0[d] = fmaf(c[0], f_low, zacc[0]); row0[d + 2] = fmaf(c[2], f_high, zacc[0]);
-        if constexpr (HG == 2) { row1[d] = fmaf(c[1], f_low, zacc[1]); row1[d + 2] = fmaf(c[3], f_high, zacc[1]); }
+        row0[d] = fmaf(c[0], f_low[0], zacc[0]); row0[d + 2] = fmaf(c[2], f_high[0], zacc[0]);
+        if constexpr (HG == 2) { row1[d] = fmaf(c[1], f_low[1], zacc[1]); row1[d + 2] = fmaf(c[3], f_high[1], zacc[1]); }
       }
     }
     if (g == 0) {
