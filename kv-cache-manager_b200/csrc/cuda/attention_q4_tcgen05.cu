@@ -3,10 +3,12 @@
 //
 // One block per (256 query rows of a request, query head), as two groups of 128 rows that share every tile of keys and values.  Per
 // tile of 128 keys and group:
-//     S = Q C^T   C = 128 + the key's codes (bfloat16, exact), accumulator in tensor memory
-//     softmax     one thread a row:  x = scale_k S + (zero_k - 128 scale_k) sum(q),  p = 2^(x - m),  P = bfloat16(p scale_v)
+//     S = Q C^T   C = the key's codes - 8 (bfloat16, exact), accumulator in tensor memory
+//     softmax     one thread a row:  x = scale_k S + (zero_k + 8 scale_k) sum(q),  p = 2^(x - m),  P = bfloat16(p scale_v)
 //     O += P W    W = the value's codes - 8 (exact), MN-major operand, O in tensor memory for the whole block
 // and at the end  o = (O + sum p (zero_v + 8 scale_v)) / sum p.
+// (Codes enter around zero: 128 + code would spare the subtraction, but the float32 sums would then carry terms ten times as large
+// as the score's, which are taken out again behind them.)
 // Keys and values are never rounded; P is, to bfloat16.  (With V = bfloat16(zero + scale code) as the operand three instructions for two
 // scores fall away, 1,045 us instead of 1,098 for four portions behind long prefixes; but the result is then 1.7 times as far off as its own rounding, with P's alone 1.4 times.)
 // A row takes its products 32 at a time, relative to the maximum that it knows, without looking for theirs: where 32 probabilities
@@ -198,9 +200,7 @@ __device__ __noinline__ void qf_rescale(uint32_t o_addr, bool has_o, uint32_t p_
   tc5::st_wait();
 }
 
-// 16 bytes of codes (elements 32 ch .. 32 ch + 31 of row r) as bfloat16 into a 128-byte swizzled tile [HD/64][128 rows][64]:
-// 128 + code, or code - 8.
-template <bool CENTRE>
+// 16 bytes of codes (elements 32 ch .. 32 ch + 31 of row r) as bfloat16 into a 128-byte swizzled tile [HD/64][128 rows][64]: code - 8.
 __device__ __forceinline__ void qf_spread(unsigned char* tile, const unsigned char* from, int r, int ch) {
   const uint4 u = *reinterpret_cast<const uint4*>(from);
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -211,7 +211,7 @@ __device__ __forceinline__ void qf_spread(unsigned char* tile, const unsigned ch
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       e[i] = q4::two_codes_128(w[j], i);
-      if (CENTRE) asm("sub.rn.bf16x2 %0, %0, %1;\n" : "+r"(e[i]) : "r"(0x43084308u));
+      asm("sub.rn.bf16x2 %0, %0, %1;\n" : "+r"(e[i]) : "r"(0x43084308u));
     }
     *reinterpret_cast<uint4*>(row + ((((ch & 1) * 4 + j) ^ (r & 7)) * 16)) = make_uint4(e[0], e[1], e[2], e[3]);
   }
@@ -402,13 +402,13 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
       float* f = reinterpret_cast<float*>(scales + (n % kQfScaleRing) * (kQfKeys / 2) + (t >> 1)) + (t & 1);
       const float unit = CAP ? 1.f : p.scale_log2, ks = q4::scale_of(kp), vs = q4::scale_of(vp);
       f[0] = ks * unit;
-      f[2] = fmaf(-128.f, ks, q4::zero_of(kp)) * unit;
+      f[2] = fmaf(8.f, ks, q4::zero_of(kp)) * unit;
       f[4] = vs;
       f[6] = fmaf(8.f, vs, q4::zero_of(vp));
 #pragma unroll
       for (int i = 0; i < unpack.kPerThread; ++i) {
         int r, ch;
-        if (unpack.piece(i, r, ch)) qf_spread<false>(k_s + (n % kQfStages) * KB * kQfTile, raw + r * (HD / 2) + ch * 16, r, ch);
+        if (unpack.piece(i, r, ch)) qf_spread(k_s + (n % kQfStages) * KB * kQfTile, raw + r * (HD / 2) + ch * 16, r, ch);
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kQfThreads, 1) attn_prefill_q4_kernel(const __
 #pragma unroll
       for (int i = 0; i < unpack.kPerThread; ++i) {
         int r, ch;
-        if (unpack.piece(i, r, ch)) qf_spread<true>(v_s + (n % kQfStages) * KB * kQfTile, codes + r * (HD / 2) + ch * 16, r, ch);
+        if (unpack.piece(i, r, ch)) qf_spread(v_s + (n % kQfStages) * KB * kQfTile, codes + r * (HD / 2) + ch * 16, r, ch);
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();

@@ -9,8 +9,8 @@ With x_j = zero_j + scale_j code_j and probabilities p_j (sum 1), in units in th
  * float32 sums: 2^-24 of the sum of the terms' sizes, sum p (15 scale + |zero|), for each addition that a term goes through: at most
    one a key and hd; in single rows a fourth of the keys (four warps), one a piece of 128 where pieces are joined, and 16.
  * scores that are off by e_j change the result by at most sum p_j e_j |x_j - o|, whatever all of them are off by together.  A
-   score's terms are q_d code_d scale and zero q_d: e is (hd + 8) * 2^-24 of their sizes (portions: codes enter with 128 added, which is taken
-   out again: 2 * 143 scale |q_d|), single rows' q in addition max|q| / 65024 * sum |scale code - mean over the keys| (q in 16 bits);
+   score's terms are q_d code_d scale and zero q_d: e is (hd + 8) * 2^-24 of their sizes (portions: of q_d (code_d - 8) scale
+   and (zero + 8 scale) q_d), single rows' q in addition max|q| / 65024 * sum |scale code - mean over the keys| (q in 16 bits);
    exponentials and products around them 8 * 2^-24 (1 + |score|).
  * pages laid out in bfloat16: keys, values and probabilities are rounded there, 2^-8 of each.
 """
@@ -30,12 +30,12 @@ def parts(cache, hd, B):
     return code, scale, zero
 
 
-KINDS = {"single": dict(weight=2.0 ** -11, small=1, result=2.0 ** -8, q16=True, offset=0.0),
-         "portion": dict(weight=2.0 ** -8, small=0, result=2.0 ** -8, q16=False, offset=2 * 143.0),
-         "climbing portion": dict(weight=4 * 2.0 ** -8, small=0, result=2.0 ** -8, q16=False, offset=2 * 143.0),
-         "laid out": dict(weight=0.0, small=0, result=2.0 ** -8, q16=False, offset=0.0, again=2.0 ** -8),
-         "plain bfloat16": dict(weight=0.0, small=0, result=2.0 ** -8, q16=False, offset=0.0),
-         "plain float32": dict(weight=0.0, small=0, result=2.0 ** -24, q16=False, offset=0.0)}
+KINDS = {"single": dict(weight=2.0 ** -11, small=1, result=2.0 ** -8, q16=True, centred=False),
+         "portion": dict(weight=2.0 ** -8, small=0, result=2.0 ** -8, q16=False, centred=True),
+         "climbing portion": dict(weight=4 * 2.0 ** -8, small=0, result=2.0 ** -8, q16=False, centred=True),
+         "laid out": dict(weight=0.0, small=0, result=2.0 ** -8, q16=False, centred=False, again=2.0 ** -8),
+         "plain bfloat16": dict(weight=0.0, small=0, result=2.0 ** -8, q16=False, centred=False),
+         "plain float32": dict(weight=0.0, small=0, result=2.0 ** -24, q16=False, centred=False)}
 
 
 def attention(kind, q, kc, vc, tables, spans, nh, nkv, hd, B, scale, window=0, lost=None):
@@ -63,8 +63,8 @@ def attention(kind, q, kc, vc, tables, spans, nh, nkv, hd, B, scale, window=0, l
             s = s.masked_fill(~seen, -torch.inf)
             p = torch.nan_to_num(torch.softmax(s, -1))
             o = p @ x
-            coded = torch.full_like(kcode[g], c["offset"]) if c["offset"] else kcode[g]
-            size = (rows.abs() @ (ks[g] * coded + kz[g].abs()).T) * scale     # of a score's terms
+            middle = 8 if c["centred"] else 0
+            size = (rows.abs() @ (ks[g] * (kcode[g] - middle).abs() + (kz[g] + middle * ks[g]).abs()).T) * scale     # of a score's terms
             e = (hd + 8) * eps * size + 8 * eps * (1 + s.abs())
             if c["q16"]:
                 coded = ks[g] * kcode[g]
@@ -92,8 +92,12 @@ def check(got, want, room):
 
 def cache_of(x):
     """The pages of rows x [pages, nkv, B, hd]."""
-    pages, nkv, B, hd = x.shape
-    code, scale, zero = P.quantised(x)
+    return pages_of(*P.quantised(x))
+
+
+def pages_of(code, scale, zero):
+    """The pages of rows of codes [pages, nkv, B, hd] (whole numbers), scales and zeros [pages, nkv, B, 1] (bfloat16)."""
+    pages, nkv, B, hd = code.shape
     w = sum(code[..., e::8] << P.SHIFTS[e] for e in range(8))
     cache = torch.zeros((pages, nkv, P.page_bytes(B, hd)), dtype=torch.uint8)
     n = B * hd // 2

@@ -71,3 +71,27 @@ def test_rows_before_the_first_key_of_a_short_table(hd, n, keys):
             want, room = bounds.attention("portion" if hd != 96 else "laid out", q.double()[first + blind:first + count].view(-1, nh, hd), kc, vc, tables[request:request + 1],
                                           [(keys - (count - blind), count - blind)], nh, nkv, hd, B, hd ** -0.5)
             bounds.check(got.view(-1, nh, hd), want, room)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 100.0])
+def test_large_queries_and_keys_that_all_score_the_same(hd, size):
+    """Queries of very different elements, up to ``size``; keys of two scales, every one of which scores zero because its codes lie around 8 in
+    pairs that cancel.  Values are 1 under one scale and -1 under the other: a score's error that grows with its scale shows at once."""
+    nh, nkv, B, n = 2, 1, 16, 320
+    tables, pages, ctx = make_step([(40, n - 40)], B, 1)
+    g = torch.Generator().manual_seed(hd)
+    half = torch.randint(1, 8, (pages, nkv, B, hd // 2), generator=g)
+    code = torch.stack((8 + half, 8 - half), -1).flatten(-2)
+    large = torch.rand((pages, nkv, B, 1), generator=g) < 0.5
+    scale = torch.where(large, 1.0, 1.0 / 64).to(torch.bfloat16)
+    kc = bounds.pages_of(code, scale, (-8 * scale.float()).to(torch.bfloat16))
+    vc = bounds.pages_of(torch.zeros_like(code), torch.zeros_like(scale), torch.where(large, 1.0, -1.0).to(torch.bfloat16))
+    q = size * torch.exp2(-14 * torch.rand((ctx.rows, nh * hd // 2), generator=g))
+    q = q.repeat_interleave(2, dim=-1).to(torch.bfloat16)
+    out = torch.full_like(q, 9.0, device=DEV)
+    K().attention_prefill_q4(q.to(DEV), out, kc.to(DEV), vc.to(DEV), tables.to(DEV), ctx, nh, nkv, hd, B, hd ** -0.5)
+    torch.cuda.synchronize()
+    K().check_errors()
+    want, room = bounds.attention("portion", q.double().view(-1, nh, hd), kc, vc, tables, [(40, n - 40)], nh, nkv, hd, B, hd ** -0.5)
+    bounds.check(out.view(-1, nh, hd), want, room)
