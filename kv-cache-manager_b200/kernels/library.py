@@ -709,6 +709,8 @@ def _q4_attention(name, q, out, k_cache, v_cache, block_tables, nh, nkv, hd, blo
         raise KernelError(f"{name}: {nh} query heads are not a multiple of {nkv} KV heads")
     if window < 0 or softcap < 0.0:
         raise KernelError(f"{name}: window and softcap must not be negative")
+    if window > 0x7fffffff:
+        raise KernelError(f"{name}: a window of {window} keys does not fit 32 bits")
     _q4_cache(name, k_cache, v_cache, nkv, hd, block_size)
     if q.dtype != out.dtype or q.dtype not in _SUFFIX:
         raise KernelError(f"{name}: q and out must be bfloat16 or float32 rows of one type")
@@ -804,7 +806,9 @@ def attention_decode_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tenso
     device = _one_device(name, q, out, k_cache, v_cache, block_tables, lengths, sink)
     if S == 0:
         return
-    span = ctx.max_decode_ctx if window <= 0 else min(ctx.max_decode_ctx, window + 31)
+    span = min(ctx.max_decode_ctx, max_blocks * block_size, 1 << 30)       # (a context ends with its table)
+    if window > 0:
+        span = min(span, window + 31)
     size, parts = decode_partitions_q4(S, nh, nkv, hd, span, device, ctx.options.get("attn_parts", 0))
     in_cluster = 1 < parts <= CLUSTER_PARTS and ctx.options.get("attn_merge", "cluster") == "cluster"
     scratch, shares = None, 0
