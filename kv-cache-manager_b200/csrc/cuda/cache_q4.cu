@@ -293,9 +293,6 @@ bool q4_sizes_ok(int nkv, int hd, int block_size, int num_pages) {
 
 using namespace kvcm;
 
-// Bytes of a page of one KV head.
-KVCM_API long long kvcm_q4_page_bytes(int block_size, int hd) { return (long long)q4::page_bytes(block_size, hd); }
-
 // q|k|v rows (nh + 2 nkv heads of hd) -> rotated q rows in q_out, k and v in the pages of their slots (slot < 0: nowhere).
 // `angles` [rows, rotary_dim] float32, cosines then sines (null: no rotation).  All rows and addresses on 16 bytes.
 #define KVCM_STORE_Q4(SUFFIX, T)                                                                                              \
