@@ -9,9 +9,9 @@
 //        product.  Exact but for q's rounding, 2^-17 of its largest element, which moves a score by less than float32 sums of
 //        larger products would.   q.k = scale (q.code) + zero sum(q)  follows in float32.
 //   O^T  in float16, m16n8k16: an element of two neighbouring keys is one register (the words of the two keys, half by half), as
-//        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of the power of two
-//        above the head's largest that the warp has seen (a float16 below one), so a weight is rounded by 2^-11 of itself at most, and by
-//        2^-25 of that unit where it is smaller than 2^-14 of it.
+//        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of a power of two,
+//        at most twice the head's largest that the warp has seen, so a weight is rounded by 2^-11 of itself at most, and by 2^-25 of
+//        that unit where it is smaller than 2^-14 of it.
 //        (Units of the largest scale alone, whatever its key's probability, let one large value without weight take the others' bits,
 //        a unit for all heads of a warp one that has weight in one head only.)
 //   P goes from accumulators to operands by a transposing register move (movmatrix): no shared memory in between.
@@ -47,6 +47,9 @@ constexpr float kQ4Lowest = 3.402823466e38f;
 // What it costs to start on a request and head, in tiles of 128 keys, for the shares: its table, its q, an empty ring.  (64 ragged
 // requests: 54 us without it, 47, 44 and 41 with 2, 4 and 6.)
 constexpr int kQ4Start = 6;
+// Exponents (of float32) by which a weight may be above its unit before the unit is formed anew: 2^12 is far from float16's end, and
+// a unit that is too small costs no bits.  Without it eight heads' units were formed anew every other step.
+constexpr uint32_t kQ4UnitRoom = 12u << 23;
 
 struct DecodeQ4Params {
   const bf16* q; long long q_stride;
@@ -557,12 +560,12 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
               zacc[h] *= grown[h];
               // the weights so far have become `grown` of what they were, and so may their unit
               const uint32_t unit_new = min((__float_as_uint(__uint_as_float(unit[h]) * grown[h]) & 0x7f800000u) + 0x00800000u, unit[h]);
-              if (grown[h] > 0.f) grown[h] *= __uint_as_float(unit[h]) / __uint_as_float(unit_new);
+              if (grown[h] > 0.f) grown[h] *= __uint_as_float(0x3f800000u + (unit[h] - unit_new));      // (unit / unit_new)
               unit[h] = unit_new;
             }
             rescale(grown);
           }
-          // ---- weights p scale, and their unit: a power of two above the largest so far
+          // ---- weights p scale, and their unit
           float most_of[HG];
 #pragma unroll
           for (int h = 0; h < HG; ++h) most_of[h] = 0.f;
@@ -583,7 +586,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
           }
           bool beyond = false;
 #pragma unroll
-          for (int h = 0; h < HG; ++h) beyond |= __float_as_uint(most_of[h]) >= unit[h];
+          for (int h = 0; h < HG; ++h) beyond |= __float_as_uint(most_of[h]) >= unit[h] + kQ4UnitRoom;
           if (__any_sync(0xffffffffu, beyond)) {
             float f[HG];
 #pragma unroll
@@ -592,7 +595,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
               for (int off = 4; off <= 16; off *= 2) most_of[h] = fmaxf(most_of[h], __shfl_xor_sync(0xffffffffu, most_of[h], off));
               // (up to 2^126: its reciprocal is a normal number)
               const uint32_t unit_new = max(unit[h], min((__float_as_uint(most_of[h]) & 0x7f800000u) + 0x00800000u, 0x7e800000u));
-              f[h] = __uint_as_float(unit[h]) / __uint_as_float(unit_new);
+              f[h] = __uint_as_float(0x3f800000u - min(unit_new - unit[h], 0x3f800000u));     // unit / unit_new; zero below 2^-126
               unit[h] = unit_new;
             }
             rescale(f);
