@@ -490,8 +490,8 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
             for (int h = 0; h < HG; ++h) {
               const float na = fmaf(256.f, __int_as_float(c[h][0]) - 12582912.f, __int_as_float(c[h][1]) - 12582912.f);
               const float nb = fmaf(256.f, __int_as_float(c[h][2]) - 12582912.f, __int_as_float(c[h][3]) - 12582912.f);
-              x[mt][0][h] = fmaf(sa * na, step[h], za * qs[h]);
-              x[mt][1][h] = fmaf(sb * nb, step[h], zb * qs[h]);
+              x[mt][0][h] = fmaf(sa * step[h], na, za * qs[h]);      // (large keys and small queries, or the reverse, meet first)
+              x[mt][1][h] = fmaf(sb * step[h], nb, zb * qs[h]);
               if constexpr (CAP) {
                 x[mt][0][h] = fast_tanh(x[mt][0][h] * p.cap_pre) * p.scale_log2;
                 x[mt][1][h] = fast_tanh(x[mt][1][h] * p.cap_pre) * p.scale_log2;
