@@ -22,11 +22,13 @@
 // distributed shared memory, or equal shares of all requests' tiles of 128 keys, for batches of ragged or many requests: a share
 // begins and ends inside a request, the two pieces go through scratch memory, and a second kernel joins them.
 //
-// What bounds it, B200: instructions.  A step of 32 keys x 128 elements x 4 heads costs a warp some 560, of which products are 24; an
+// What bounds it, B200: instructions.  A step of 32 keys x 128 elements x 4 heads costs a warp some 550, of which products are 24; an
 // SM's four schedulers are 63 % busy (waits for the products' own results in between) and memory 5.0 TB/s: 64 requests of 8,192
-// keys, 32 heads on 8 of 128 elements, 571 MB: 114 us (88 at the rate of a copy).  64 requests of 100 to 8,192 keys (106 MB): 41.6 us,
-// of which the shares' starts and the second kernel are about 11.  27 requests of up to 1,024 keys behind a window, capped: 11.5 us;
-// 8 of 1,500 keys 8.1 us; one of 148 keys 5.0 us: launch, lengths, table, q and keys behind one another.
+// keys, 32 heads on 8 of 128 elements, 571 MB: 113 us (88 at the rate of a copy; up to 127 on a GPU that has been at it for seconds).  64
+// requests of 100 to 8,192 keys (106 MB): 41.3 us, of which the shares' starts and the second kernel are about 11.  27 requests of up
+// to 1,024 keys behind a window, capped: 11.4 us; 8 of 1,500 keys 7.9 us; one of 148 keys 4.8 us: launch, lengths, table, q and keys
+// behind one another.  One of 32,768 keys 38 us (5.5 at the rate of a copy): equal shares cut it into some 70 pieces a head, which eight
+// blocks join one after another.
 #include <cooperative_groups.h>
 
 #include "attention_mma.cuh"
@@ -44,8 +46,9 @@ constexpr int kQ4Heads = 8;                        // most query heads of a bloc
 constexpr int kQ4TabMax = 512;                     // page-table entries of a partition kept in shared memory
 constexpr int kQ4ClusterParts = 8;
 constexpr float kQ4Lowest = 3.402823466e38f;
-// What it costs to start on a request and head, in tiles of 128 keys, for the shares: its table, its q, an empty ring.  (64 ragged
-// requests: 54 us without it, 47, 44 and 41 with 2, 4 and 6.)
+// What it costs to start on a request and head, in tiles of 128 keys, for the shares: its table, its q, an empty ring.  (0, 2, 4, 6 and
+// 8, ragged requests up to 8,192 keys, heads of 128: 64 of them 54, 45, 43, 41 and 42 us; 100 shorter ones 64, 48, 46, 44 and 45;
+// 16 of them 32, 30, 30, 29 and 27.)
 constexpr int kQ4Start = 6;
 // Exponents (of float32) by which a weight may be above its unit before the unit is formed anew: 2^12 is far from float16's end, and
 // a unit that is too small costs no bits.  Without it eight heads' units were formed anew every other step.
@@ -772,7 +775,7 @@ __global__ void attn_decode_q4_merge_kernel(const float* part_o, const float* pa
 
 // The pieces of a request and its four or eight heads that blocks part_first[0] .. part_first[1] have left, in their order: the first
 // block's lies in its second place, the others' in their first.  Up to six are asked for at once, maxima, sums and outputs in one trip
-// to memory (64 ragged requests in all 42.9 -> 41.6 us).  A long request has many: the weights of 128 of them at a time are formed
+// to memory (64 ragged requests in all 1.3 us less).  A long request has many: the weights of 128 of them at a time are formed
 // side by side, so that what follows one another is additions.
 constexpr int kQ4JoinAtOnce = 128;
 constexpr int kQ4JoinFew = 6;
@@ -895,8 +898,8 @@ __global__ void __launch_bounds__(128) attn_decode_q4_shares_kernel(const float*
 }
 
 // Steps in flight.  Four blocks of three an SM for one group of heads at 128 registers a thread; two groups want 168, and then
-// three blocks of four steps.  (64 requests of 8,192 keys, 8 KV heads of 128: 112 us with four blocks, 121 with three; 8 requests of
-// 1,536, 4 KV heads of 64 with eight query heads each: 8.6 and 7.9.)
+// three blocks of four steps.  (The other way round: 64 requests of 8,192 keys, 8 KV heads of 128, 113 us both; eight query heads on
+// each of 4 KV heads of 64, 8 requests of 1,536 keys 8.6 us and not 7.9, but 64 of some 2,048 30 and not 33.)
 template <int HD, int HG> constexpr int q4_decode_stages() { return HD > 128 || HG == 1 ? 3 : 4; }
 
 // Query heads of a block: four where a KV head has no more, else eight.

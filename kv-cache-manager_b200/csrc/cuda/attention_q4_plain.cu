@@ -5,7 +5,10 @@
 //
 // A chunk of 512 keys at a time: a thread forms the scores of whole keys (a key's codes are hd/2 bytes), then the products with
 // V are dealt out as words of eight elements, groups of threads taking every n-th key each, joined at the end in the groups'
-// order.  What bounds it is instructions: a code costs a shift, a mask, a conversion and a fused multiply-add.
+// order.  What bounds it is instructions: a code costs a shift, a mask, a conversion and a fused multiply-add, and it costs them once for
+// every query head and row that reads it.  B200, float32 rows: 8 requests of some 1,536 keys, 32 heads on 4 of 64, 49 us, 64 of 100 to
+// 8,192 keys, 32 on 8 of 128, 722 us (0.5 and 16 at the rate of a copy); a portion of 2,048 rows 4.9 ms (7.0 TFLOP/s), of heads of 40,
+// 8 on 2, 0.47 ms.
 #include "packed.cuh"
 #include "pdl.cuh"
 #include "q4.cuh"

@@ -7,10 +7,11 @@
 //     softmax     one thread a row:  x = scale_k S + (zero_k + 8 scale_k) sum(q),  p = 2^(x - m),  P = bfloat16(p scale_v)
 //     O += P W    W = the value's codes - 8 (exact), MN-major operand, O in tensor memory for the whole block
 // and at the end  o = (O + sum p (zero_v + 8 scale_v)) / sum p.
-// (Codes enter around zero: 128 + code would spare the subtraction, but the float32 sums would then carry terms ten times as large
-// as the score's, which are taken out again behind them.)
-// Keys and values are never rounded; P is, to bfloat16.  (With V = bfloat16(zero + scale code) as the operand three instructions for two
-// scores fall away, 1,045 us instead of 1,098 for four portions behind long prefixes; but the result is then 1.7 times as far off as its own rounding, with P's alone 1.4 times.)
+// (Codes enter around zero: 128 + code would spare the subtraction, 1,097 us instead of 1,119 for four portions behind long prefixes,
+// but the float32 sums would then carry terms ten times as large as the score's, which are taken out again behind them.)
+// Keys and values are never rounded; P is, to bfloat16, and once more where a maximum is renewed inside its tile.  (With V =
+// bfloat16(zero + scale code) as the operand three instructions for two scores fall away, 5 % less time; but the result is then 1.7
+// times as far off as its own rounding, with P's alone 1.4 times.)
 // A row takes its products 32 at a time, relative to the maximum that it knows, without looking for theirs: where 32 probabilities
 // add up to more than 2^12 (or the row has seen nothing yet) their maximum is found, sums, O and the tile's earlier probabilities
 // are rescaled, and the 32 are taken again, which after the first tiles hardly ever happens.  The largest probability then lies
@@ -25,9 +26,9 @@
 // What bounds it: at head_dim 128 a tile of 256 x 128 takes some 5,500 cycles.  Its exponentials (16 a cycle) and its products each
 // take 2,048; shared memory is busy 3,300 by count (the products' operands 1,540, the keys' scales, read by every row's warp,
 // 1,020, unpacking 770); a handshake between roles takes some 250, and four of them lie between two softmaxes of a group.  Two
-// threads a row, each half of a tile's keys (16 softmax warps at 80 registers), take longer, 1,438 us for the 1,100 below.  B200, 32 heads on 8 of
-// 128: 2,048 rows 73 us (470 TFLOP/s causal), four portions of 1,500 rows behind 6,000
-// keys 1,100 us (670 TFLOP/s); 148 rows of heads of 64 10 us.
+// threads a row, each half of a tile's keys (16 softmax warps at 80 registers), took 1,438 us where one took 1,100.  B200, 32 heads
+// on 8 of 128: 2,048 rows 77 us (445 TFLOP/s causal), four portions of 1,500 rows behind 6,000 keys 1,119 us (660 TFLOP/s); 148 rows of
+// heads of 64 11.3 us.  Reading tiles and lengths behind the dependency wait is some 2 us of the 77.
 // A thread of warps 8-14 copies what it unpacks itself (cp.async into shared memory, a tile ahead) and so waits for nobody else's.
 // Masks: key <= position, optional window.  Every wait is bounded; one that runs out sets the error word of the tcgen05 attention
 // family (codes 17 and up) and ends the block.

@@ -11,11 +11,12 @@
 // and a 4-byte store of codes), in rotate-half pairs the two that turn with one another, so that angles are read once for both and
 // nothing is exchanged; the lanes of a head (hd / 16, rounded up to a power of two) sit in one warp and find minimum and
 // maximum by shuffles.  A block has up to 256 such pairs of one row (grid: rows x equal pieces of a row), so nothing is divided to
-// find one's place, and codes are found without divisions too (see there).  8,192 rows of 48 heads of 128 (180 MB): 44 us, 4.1 TB/s
+// find one's place, and codes are found without divisions too (see there).  8,192 rows of 48 heads of 128 (180 MB): 43 us, 4.2 TB/s
 // (28 us at the rate of a copy); 55 with 16 divisions a lane, 71 with one word a lane and partners exchanged by shuffles, 96 with
 // places counted through and taken apart by 64-bit divisions.  What is left is waiting: a block is one load, a few hundred
 // instructions and a store; packed pairs of float32 (50 us), other block sizes and cache hints (no change) do not help.  Reading the
-// 8 + 8 KV heads back: 11.5 us (43 MB), 16.7 with a word a lane and codes converted from whole numbers.
+// 8 + 8 KV heads back: 11.7 us (43 MB, 6.5 at that rate), 16.7 with a word a lane and codes converted from whole numbers.  float32 rows:
+// written in 56 us (53 at that rate), read back in 20 (12).
 #include "packed.cuh"
 #include "pdl.cuh"
 #include "q4.cuh"

@@ -751,8 +751,9 @@ def decode_partitions_q4(seqs: int, nh: int, nkv: int, hd: int, max_ctx: int, de
 
     As many partitions as a cluster merges and the GPU holds at once (an eighth more: not all are full), none for up to 256 keys;
     where they would be longer than 1,024 keys, equal shares of all requests' keys.  B200, microseconds, heads of 128, 8 KV heads,
-    partitions | shares: 4 requests up to 2,048 keys 8.7 | 14, 32 of 1,024 15 | 23, 16 ragged ones up to 8,192 34 | 30, 64 of them
-    62 | 41, 64 of 8,192 117 | 112; 148 keys of one request: one partition 4.8, two 5.5."""
+    partitions (their best number) | shares: 4 requests up to 2,048 keys 9.0 | 14.5, 32 of 1,024 16 | 21, 16 ragged ones up to 8,192
+    35 | 29, 64 of them 62 | 41, 64 of 8,192 113 | 117, one of 32,768 24 | 38 and of 131,072 61 | 63 (sixteen partitions, which no cluster
+    merges); 148 keys of one request: one partition 4.8, two 5.7."""
     max_ctx = max(max_ctx, 1)
     heads = 4 if nh <= 4 * nkv else 8
     blocks = max(1, seqs * nkv * ((nh // nkv + heads - 1) // heads))
@@ -925,7 +926,8 @@ def step_tables(seq_start: torch.Tensor, seq_q_len: torch.Tensor, block_tables: 
     and ``free_left`` may be ``free_count``: a step replayed from a CUDA graph then goes on from the one before.
     ``status`` [4]: (0, 0, rows, tiles), or (code, number, 0, 0) where the step cannot be (``raise_on_step_tables``): pages, counts
     and lengths are then as before and every row is one behind the last.  The host reads it when it likes; nothing waits here.
-    The requests stay in the caller's order: entries of one row come first where attention takes them as such, those of none last."""
+    The requests stay in the caller's order.  ``paged_attention_q4`` takes row i < ``ctx.decode_seqs`` as request i's, so entries of one row
+    come first there and those of none last; a request of one row behind them has no tile, and nothing attends its row."""
     name = "step_tables"
     S, T = seq_q_len.numel(), positions.numel()
     if not 0 < S <= 8192:
