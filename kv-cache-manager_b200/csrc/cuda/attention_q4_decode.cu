@@ -9,11 +9,12 @@
 //        product.  Exact but for q's rounding, 2^-17 of its largest element, which moves a score by less than float32 sums of
 //        larger products would.   q.k = scale (q.code) + zero sum(q)  follows in float32.
 //   O^T  in float16, m16n8k16: an element of two neighbouring keys is one register (the words of the two keys, half by half), as
-//        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of a power of two,
-//        at most twice the head's largest that the warp has seen, so a weight is rounded by 2^-11 of itself at most, and by 2^-25 of
-//        that unit where it is smaller than 2^-14 of it.
+//        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of at most
+//        the head's largest that the warp has seen, so a weight is rounded by 2^-11 of itself at most, and by 2^-25 of that unit where
+//        it is smaller than 2^-14 of it.  What a new maximum makes of the weights so far it makes of their unit, and O stays as it is.
 //        (Units of the largest scale alone, whatever its key's probability, let one large value without weight take the others' bits,
-//        a unit for all heads of a warp one that has weight in one head only.)
+//        a unit for all heads of a warp one that has weight in one head only, one that is kept a power of two one that scores climb
+//        away from slowly.)
 //   P goes from accumulators to operands by a transposing register move (movmatrix): no shared memory in between.
 // The scores of the next step are formed under the softmax of this one.  Pages come by 16-byte asynchronous copies into a ring of
 // steps per warp: no barriers between warps, pages of any size.
@@ -46,13 +47,14 @@ constexpr int kQ4Heads = 8;                        // most query heads of a bloc
 constexpr int kQ4TabMax = 512;                     // page-table entries of a partition kept in shared memory
 constexpr int kQ4ClusterParts = 8;
 constexpr float kQ4Lowest = 3.402823466e38f;
+constexpr float kQ4Least = 1.17549435e-38f;        // 2^-126
 // What it costs to start on a request and head, in tiles of 128 keys, for the shares: its table, its q, an empty ring.  (0, 2, 4, 6 and
 // 8, ragged requests up to 8,192 keys, heads of 128: 64 of them 54, 45, 43, 41 and 42 us; 100 shorter ones 64, 48, 46, 44 and 45;
 // 16 of them 32, 30, 30, 29 and 27.)
 constexpr int kQ4Start = 6;
-// Exponents (of float32) by which a weight may be above its unit before the unit is formed anew: 2^12 is far from float16's end, and
-// a unit that is too small costs no bits.  Without it eight heads' units were formed anew every other step.
-constexpr uint32_t kQ4UnitRoom = 12u << 23;
+// How far a weight may be above its unit before the unit is formed anew: far from float16's end, and a unit that is too small costs
+// no bits.  Without it eight heads' units were formed anew every other step.
+constexpr float kQ4UnitRoom = 4096.f;
 
 struct DecodeQ4Params {
   const bf16* q; long long q_stride;
@@ -327,9 +329,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
     float o[S::kTiles][4];
 #pragma unroll
     for (int i = 0; i < S::kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    // the powers of two that the heads' weights are divided by, as floats' bits: a head's own, so that a large value which has weight
-    // in one head takes no bits from the others
-    uint32_t unit[2] = {0x00800000u, 0x00800000u};
+    float unit[2] = {kQ4Least, kQ4Least};                          // what the heads' weights are divided by
     if (w.begin < w.end) {
       // ---- q as the second operand: column g of group h is half g % 2 of head 4 h + g / 2, elements in the order in which a lane's
       // codes lie (of a word's eight, bytes 0, 4, 1, 5 and 2, 6, 3, 7)
@@ -553,20 +553,15 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
             }
           };
           if (__any_sync(0xffffffffu, moved)) {
-            float grown[HG];
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
               const float m_new = fmaxf(m[h], top[h]);
-              grown[h] = fast_exp2(m[h] - m_new);                  // (zero where nothing was seen yet)
+              const float grown = fast_exp2(m[h] - m_new);         // (zero where nothing was seen yet)
               m[h] = m_new;
-              l[h] *= grown[h];
-              zacc[h] *= grown[h];
-              // the weights so far have become `grown` of what they were, and so may their unit
-              const uint32_t unit_new = min((__float_as_uint(__uint_as_float(unit[h]) * grown[h]) & 0x7f800000u) + 0x00800000u, unit[h]);
-              if (grown[h] > 0.f) grown[h] *= __uint_as_float(0x3f800000u + (unit[h] - unit_new));      // (unit / unit_new)
-              unit[h] = unit_new;
+              l[h] *= grown;
+              zacc[h] *= grown;
+              unit[h] *= grown;                                    // the weights so far have become `grown` of what they were
             }
-            rescale(grown);
           }
           // ---- weights p scale, and their unit
           float most_of[HG];
@@ -589,23 +584,23 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
           }
           bool beyond = false;
 #pragma unroll
-          for (int h = 0; h < HG; ++h) beyond |= __float_as_uint(most_of[h]) >= unit[h] + kQ4UnitRoom;
+          for (int h = 0; h < HG; ++h) beyond |= most_of[h] >= unit[h] * kQ4UnitRoom || !(unit[h] >= kQ4Least);
           if (__any_sync(0xffffffffu, beyond)) {
             float f[HG];
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
 #pragma unroll
               for (int off = 4; off <= 16; off *= 2) most_of[h] = fmaxf(most_of[h], __shfl_xor_sync(0xffffffffu, most_of[h], off));
-              // (up to 2^126: its reciprocal is a normal number)
-              const uint32_t unit_new = max(unit[h], min((__float_as_uint(most_of[h]) & 0x7f800000u) + 0x00800000u, 0x7e800000u));
-              f[h] = __uint_as_float(0x3f800000u - min(unit_new - unit[h], 0x3f800000u));     // unit / unit_new; zero below 2^-126
+              // (2^-126 to 2^126: it and its reciprocal are normal numbers)
+              const float unit_new = fmaxf(fmaxf(unit[h], kQ4Least), fminf(most_of[h], 1.f / kQ4Least));
+              f[h] = unit[h] / unit_new;
               unit[h] = unit_new;
             }
             rescale(f);
           }
-          float per_unit[HG];                                      // 1 / unit
+          float per_unit[HG];
 #pragma unroll
-          for (int h = 0; h < HG; ++h) per_unit[h] = __uint_as_float(0x7f000000u - unit[h]);
+          for (int h = 0; h < HG; ++h) asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(per_unit[h]) : "f"(unit[h]));
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
             float wa[2] = {0.f, 0.f}, wb[2] = {0.f, 0.f};
@@ -681,7 +676,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
         zacc[h] += __shfl_xor_sync(0xffffffffu, zacc[h], off);
       }
-    const float f_low[2] = {__uint_as_float(unit[0]), __uint_as_float(unit[1])}, f_high[2] = {f_low[0] * 0.0625f, f_low[1] * 0.0625f};
+    const float f_low[2] = {unit[0], unit[1]}, f_high[2] = {f_low[0] * 0.0625f, f_low[1] * 0.0625f};
     float* row0 = mo + (warp * kQ4Heads + t4) * HD;
     float* row1 = row0 + 4 * HD;
 #pragma unroll

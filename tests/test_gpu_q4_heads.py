@@ -1,4 +1,6 @@
 """Single rows over the cache in 4 bits: what a head gives does not depend on the heads beside it (bounds: bounds_q4.py)."""
+import types
+
 import pytest
 import torch
 
@@ -36,3 +38,27 @@ def test_a_large_value_with_weight_in_one_head_only(nh, nkv, hd, bits, force):
     K().attention_decode_q4(q.to(DEV), out, kc.to(DEV), vc.to(DEV), tables.to(DEV), ctx, nh, nkv, hd, B, scale)
     want, room = bounds.attention("single", q.double().view(2, nh, hd), kc, vc, tables, [(n - 1, 1), (n - 1, 1)], nh, nkv, hd, B, scale)
     bounds.check(out.view(2, nh, hd), want, room)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 1, 128), (8, 1, 64), (2, 2, 96), (6, 1, 256)])
+@pytest.mark.parametrize("climb", [0.3, 0.9, 1.1, 3.0])
+@pytest.mark.parametrize("force", [1, 3, -1])
+def test_a_large_value_that_scores_climb_away_from(nh, nkv, hd, climb, force):
+    """Scores that climb by ``climb`` (in log2) from 128 keys to the next, and a value 2^20 times the others among the first 32: at the end
+    it has little or no weight, however slowly it was left behind."""
+    B, n = 16, 4000
+    tables, pages, _ = make_step([(n - 1, 1)], B, 5)
+    g = torch.Generator().manual_seed(6)
+    k, v = 0.02 * torch.randn((pages, nkv, B, hd), generator=g), torch.randn((pages, nkv, B, hd), generator=g)
+    per_key = climb / (hd ** 0.5 * 1.4426950408889634)                     # q is about one: q.k hd^-0.5 log2(e) = climb
+    blocks = -(-n // B)
+    steps = torch.arange(blocks * B).view(blocks, 1, B, 1) // 128
+    k[tables[0, :blocks].long()] += steps * per_key
+    v[int(tables[0, 0]), :, 7] *= 2.0 ** 20
+    kc, vc = bounds.cache_of(k), bounds.cache_of(v)
+    q = (1 + 0.1 * torch.randn((1, nh * hd), generator=g)).to(torch.bfloat16)
+    out = torch.empty_like(q, device=DEV)
+    ctx = types.SimpleNamespace(seq_ctx_len=torch.tensor([n], dtype=torch.int32, device=DEV), max_decode_ctx=n, options={"attn_parts": force})
+    K().attention_decode_q4(q.to(DEV), out, kc.to(DEV), vc.to(DEV), tables.to(DEV), ctx, nh, nkv, hd, B, hd ** -0.5)
+    want, room = bounds.attention("single", q.double().view(1, nh, hd), kc, vc, tables, [(n - 1, 1)], nh, nkv, hd, B, hd ** -0.5)
+    bounds.check(out.view(1, nh, hd), want, room)
