@@ -24,6 +24,7 @@
 
 #include "common.cuh"
 #include "packed.cuh"
+#include "pdl.cuh"
 
 namespace kvcm {
 
@@ -221,8 +222,7 @@ KVCM_API int kvcm_step_tables(const int* start, const int* n, int* block_tables,
   cfg.numAttrs = blocks > 1 ? 1 : 0;
   const int rc = static_cast<int>(cudaLaunchKernelEx(&cfg, step_tables_kernel, p));
   if (rc != 0) return rc;
-  step_tables_done_kernel<<<1, 32, 0, (cudaStream_t)stream>>>();
-  return static_cast<int>(cudaGetLastError());
+  return pdl_launch_if(false, step_tables_done_kernel, dim3(1), dim3(32), 0, (cudaStream_t)stream);
 }
 
 KVCM_PACKED(kvcm_step_tables)
