@@ -6,8 +6,8 @@
 //   S^T  in whole numbers, m16n8k32: a lane's codes of a key are hd/4 elements in a row (any order of the contraction is as good as
 //        another if q is read in the same one) and enter as they are, four to a register for one shift and two ands a word; q enters
 //        as 16-bit fixed point relative to its head's largest element, in two 8-bit halves that are two columns: four heads to a
-//        product.  Exact but for q's rounding, 2^-17 of its largest element, which moves a score by less than float32 sums of
-//        larger products would.   q.k = scale (q.code) + zero sum(q)  follows in float32.
+//        product.  Exact but for q's rounding, 2^-16 of its largest element: half a bfloat16 step of elements 2^-8 as large, less
+//        of the larger ones.  (zero sum(q) takes q as it is.)   q.k = scale (q.code) + zero sum(q)  follows in float32.
 //   O^T  in float16, m16n8k16: an element of two neighbouring keys is one register (the words of the two keys, half by half), as
 //        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of at most
 //        the head's largest that the warp has seen, so a weight is rounded by 2^-11 of itself at most, and by 2^-25 of that unit where
@@ -26,8 +26,8 @@
 // What bounds it, B200: instructions.  A step of 32 keys x 128 elements x 4 heads costs a warp some 550, of which products are 24; an
 // SM's four schedulers are 63 % busy (waits for the products' own results in between) and memory 5.0 TB/s: 64 requests of 8,192
 // keys, 32 heads on 8 of 128 elements, 571 MB: 113 us (88 at the rate of a copy; up to 127 on a GPU that has been at it for seconds).  64
-// requests of 100 to 8,192 keys (106 MB): 41.3 us, of which the shares' starts and the second kernel are about 11.  27 requests of up
-// to 1,024 keys behind a window, capped: 11.4 us; 8 of 1,500 keys 7.9 us; one of 148 keys 4.8 us: launch, lengths, table, q and keys
+// requests of 100 to 8,192 keys (106 MB): 41.0 us, of which the shares' starts and the second kernel are about 11.  27 requests of up
+// to 1,024 keys behind a window, capped: 10.8 us; 8 of 1,500 keys 8.4 us; one of 148 keys 4.8 us: launch, lengths, table, q and keys
 // behind one another.  One of 32,768 keys 38 us (5.5 at the rate of a copy): equal shares cut it into some 70 pieces a head, which eight
 // blocks join one after another.
 #include <cooperative_groups.h>
@@ -893,8 +893,9 @@ __global__ void __launch_bounds__(128) attn_decode_q4_shares_kernel(const float*
 }
 
 // Steps in flight.  Four blocks of three an SM for one group of heads at 128 registers a thread; two groups want 168, and then
-// three blocks of four steps.  (The other way round: 64 requests of 8,192 keys, 8 KV heads of 128, 113 us both; eight query heads on
-// each of 4 KV heads of 64, 8 requests of 1,536 keys 8.6 us and not 7.9, but 64 of some 2,048 30 and not 33.)
+// three blocks of four steps.  (The other way round: 64 requests of 8,192 keys, 8 KV heads of 128, 114 us and not 112, ragged 42.5 and
+// not 41; eight query heads on each of 4 KV heads of 64, 8 requests of 1,536 keys 8.8 us and not 8.3, but 64 of some 2,048 30 and
+// not 34.)
 template <int HD, int HG> constexpr int q4_decode_stages() { return HD > 128 || HG == 1 ? 3 : 4; }
 
 // Query heads of a block: four where a KV head has no more, else eight.
