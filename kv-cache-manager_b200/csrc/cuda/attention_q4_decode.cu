@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
       of_h = blockIdx.y;
       const int from = base + int(blockIdx.x) * p.part_size;
       w.begin = max(lo, from);
-      w.end = min(ctx, from + p.part_size);
+      w.end = int(blockIdx.x) + 1 == p.num_parts ? ctx : min(ctx, from + p.part_size);     // (the last one takes what is left)
       if (p.num_parts > 1 && !p.cluster_merge) w.slot = blockIdx.x;
     } else {
       of_h = unit_h;

@@ -790,7 +790,8 @@ def attention_decode_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tenso
                         ctx, nh: int, nkv: int, hd: int, block_size: int, scale: float, window: int = 0, softcap: float = 0.0,
                         sink: Optional[torch.Tensor] = None) -> None:
     """Single-row entries over a cache in 4 bits: q and out hold one bfloat16 row a request, in the order of the batch's entries;
-    ``ctx.seq_ctx_len`` says how many keys each sees (0: the row is zero), ``ctx.max_decode_ctx`` is at least the longest.
+    ``ctx.seq_ctx_len`` says how many keys each sees (0: the row is zero), ``ctx.max_decode_ctx`` is about the longest: the keys are
+    divided by it, and beyond it one block takes what is left.
     ``window``: the last ``window`` keys only; ``softcap``, ``sink`` as in ``attention_plain``."""
     name = "attention_decode_q4"
     S, lengths = q.shape[0], ctx.seq_ctx_len
@@ -830,8 +831,8 @@ def paged_attention_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor
                        sink: Optional[torch.Tensor] = None) -> None:
     """``paged_attention`` over a cache in 4 bits: attention of all rows of a step, rows [0, ctx.decode_seqs) single-row entries, the
     rest the rows of longer portions; a row without keys gives zeros.  Single row i is request i's: requests that bring nothing stand
-    behind the others.  ``ctx.max_decode_ctx`` and ``ctx.max_ctx`` are at least the longest contexts (of a recorded step: the longest it
-    will see).  float32 rows, other head sizes and ``ctx.options['attention'] == 'plain'``: ``attention_plain_q4`` for every row."""
+    behind the others.  ``ctx.max_ctx`` is at least the longest context of the portions (of a recorded step: the longest it will see), ``ctx.max_decode_ctx``
+    about that of the single rows.  float32 rows, other head sizes and ``ctx.options['attention'] == 'plain'``: ``attention_plain_q4`` for every row."""
     if ctx.options.get("attention", "auto") == "plain" or not attention_q4_supported(hd, q.dtype):
         attention_plain_q4(q, out, k_cache, v_cache, block_tables, ctx.row_seq, ctx.positions, nh, nkv, hd, block_size, scale, window,
                            softcap, sink)

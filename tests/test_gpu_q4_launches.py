@@ -196,3 +196,23 @@ def test_single_rows_in_bfloat16_behind_the_tables_of_their_step():
         assert ctx.seq_ctx_len.tolist() == [n] * S and status.tolist() == [0, 0, S, 0]
         attend(out)
         assert torch.equal(got, out), n
+
+
+@pytest.mark.parametrize("parts", [0, 1, 3, 8, 12])
+@pytest.mark.parametrize("window", [0, 900])
+def test_contexts_longer_than_was_said(parts, window):
+    """The longest context only says how the keys are divided: one that grew beyond it is attended whole."""
+    S, ends = 5, [10, 300, 700, 1500, 64]
+    s = Step(S, ends, 4, 1, 64, 0)
+    s.ctx.rows, s.q = S, s.q[:S].contiguous()
+    want, got = torch.empty_like(s.q), torch.empty_like(s.q)
+    s.ctx.options = {"attention": "plain"}
+    s.attend(want, window=window)
+    s.ctx.options = {"attn_parts": parts}
+    for longest in (1500, 1000, 300, 1):
+        s.ctx.max_decode_ctx = longest
+        s.attend(got, window=window)
+        # two roundings to bfloat16 and the weights' (2^-11 of at most the largest value)
+        room = 2.0 ** -7 * want.float().abs() + 2.0 ** -10 * 4.0
+        assert ((got.float() - want.float()).abs() <= room).all(), longest
+    K().check_errors()
