@@ -9,12 +9,13 @@
 //        product.  Exact but for q's rounding, 2^-16 of its largest element: half a bfloat16 step of elements 2^-8 as large, less
 //        of the larger ones.  (zero sum(q) takes q as it is.)   q.k = scale (q.code) + zero sum(q)  follows in float32.
 //   O^T  in float16, m16n8k16: an element of two neighbouring keys is one register (the words of the two keys, half by half), as
-//        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of at most
-//        the head's largest that the warp has seen, so a weight is rounded by 2^-11 of itself at most, and by 2^-25 of that unit where
-//        it is smaller than 2^-14 of it.  What a new maximum makes of the weights so far it makes of their unit, and O stays as it is.
+//        code - 8 (exact), and  sum p x = sum (p scale)(code - 8) + sum p (zero + 8 scale).  p scale enters in units of the power of
+//        two in the head's largest weight that the warp has seen, so a weight is rounded by 2^-11 of itself at most (the largest key's not
+//        at all: it is its scale), and by 2^-25 of that unit where it is smaller than 2^-14 of it.
 //        (Units of the largest scale alone, whatever its key's probability, let one large value without weight take the others' bits,
-//        a unit for all heads of a warp one that has weight in one head only, one that is kept a power of two one that scores climb
-//        away from slowly.)
+//        a unit for all heads of a warp one that has weight in one head only, one that forgets how large the largest weight was by now
+//        one that scores climb away from slowly.  A unit of the largest weight itself, which O would not have to follow, rounds the
+//        largest key's weight too: a fifth more results off by a bfloat16 step.)
 //   P goes from accumulators to operands by a transposing register move (movmatrix): no shared memory in between.
 // The scores of the next step are formed under the softmax of this one.  Pages come by 16-byte asynchronous copies into a ring of
 // steps per warp: no barriers between warps, pages of any size.
@@ -26,8 +27,8 @@
 // What bounds it, B200: instructions.  A step of 32 keys x 128 elements x 4 heads costs a warp some 550, of which products are 24; an
 // SM's four schedulers are 63 % busy (waits for the products' own results in between) and memory 5.0 TB/s: 64 requests of 8,192
 // keys, 32 heads on 8 of 128 elements, 571 MB: 113 us (88 at the rate of a copy; up to 127 on a GPU that has been at it for seconds).  64
-// requests of 100 to 8,192 keys (106 MB): 41.0 us, of which the shares' starts and the second kernel are about 11.  27 requests of up
-// to 1,024 keys behind a window, capped: 10.8 us; 8 of 1,500 keys 8.4 us; one of 148 keys 4.8 us: launch, lengths, table, q and keys
+// requests of 100 to 8,192 keys (106 MB): 41.4 us, of which the shares' starts and the second kernel are about 11.  27 requests of up
+// to 1,024 keys behind a window, capped: 11.4 us; 8 of 1,500 keys 8.0 us; one of 148 keys 4.8 us: launch, lengths, table, q and keys
 // behind one another.  One of 32,768 keys 38 us (5.5 at the rate of a copy): equal shares cut it into some 70 pieces a head, which eight
 // blocks join one after another.
 #include <cooperative_groups.h>
@@ -52,9 +53,9 @@ constexpr float kQ4Least = 1.17549435e-38f;        // 2^-126
 // 8, ragged requests up to 8,192 keys, heads of 128: 64 of them 54, 45, 43, 41 and 42 us; 100 shorter ones 64, 48, 46, 44 and 45;
 // 16 of them 32, 30, 30, 29 and 27.)
 constexpr int kQ4Start = 6;
-// How far a weight may be above its unit before the unit is formed anew: far from float16's end, and a unit that is too small costs
-// no bits.  Without it eight heads' units were formed anew every other step.
-constexpr float kQ4UnitRoom = 4096.f;
+// Exponents (of float32) by which a weight may be above its unit before the unit is formed anew: 2^12 is far from float16's end, and
+// a unit that is too small costs no bits.  Without it eight heads' units were formed anew every other step.
+constexpr uint32_t kQ4UnitRoom = 12u << 23;
 
 struct DecodeQ4Params {
   const bf16* q; long long q_stride;
@@ -120,6 +121,8 @@ __device__ __forceinline__ uint32_t high_codes(uint32_t v) {
   asm("sub.f16x2 %0, %0, %1;\n" : "+r"(r) : "r"(0x64806480u));
   return r;
 }
+// The largest power of two in a positive number, as a float's bits.
+__device__ __forceinline__ uint32_t power_of_two(float x) { return __float_as_uint(x) & 0x7f800000u; }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
     float o[S::kTiles][4];
 #pragma unroll
     for (int i = 0; i < S::kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float unit[2] = {kQ4Least, kQ4Least};                          // what the heads' weights are divided by
+    float heaviest[2] = {kQ4Least, kQ4Least};                      // weight of a head so far; the power of two in it is their unit
     if (w.begin < w.end) {
       // ---- q as the second operand: column g of group h is half g % 2 of head 4 h + g / 2, elements in the order in which a lane's
       // codes lie (of a word's eight, bytes 0, 4, 1, 5 and 2, 6, 3, 7)
@@ -553,15 +556,20 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
             }
           };
           if (__any_sync(0xffffffffu, moved)) {
+            float grown[HG];
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
               const float m_new = fmaxf(m[h], top[h]);
-              const float grown = fast_exp2(m[h] - m_new);         // (zero where nothing was seen yet)
+              grown[h] = fast_exp2(m[h] - m_new);                  // (zero where nothing was seen yet)
               m[h] = m_new;
-              l[h] *= grown;
-              zacc[h] *= grown;
-              unit[h] *= grown;                                    // the weights so far have become `grown` of what they were
+              l[h] *= grown[h];
+              zacc[h] *= grown[h];
+              // the weights so far have become `grown` of what they were, and so has the largest of them
+              const uint32_t unit = power_of_two(heaviest[h]);
+              heaviest[h] = fmaxf(heaviest[h] * grown[h], kQ4Least);
+              if (grown[h] > 0.f) grown[h] *= __uint_as_float(0x3f800000u + (unit - power_of_two(heaviest[h])));     // (old unit / new unit)
             }
+            rescale(grown);
           }
           // ---- weights p scale, and their unit
           float most_of[HG];
@@ -584,23 +592,24 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
           }
           bool beyond = false;
 #pragma unroll
-          for (int h = 0; h < HG; ++h) beyond |= most_of[h] >= unit[h] * kQ4UnitRoom || !(unit[h] >= kQ4Least);
+          for (int h = 0; h < HG; ++h) beyond |= __float_as_uint(most_of[h]) >= power_of_two(heaviest[h]) + kQ4UnitRoom;
           if (__any_sync(0xffffffffu, beyond)) {
             float f[HG];
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
 #pragma unroll
               for (int off = 4; off <= 16; off *= 2) most_of[h] = fmaxf(most_of[h], __shfl_xor_sync(0xffffffffu, most_of[h], off));
-              // (2^-126 to 2^126: it and its reciprocal are normal numbers)
-              const float unit_new = fmaxf(fmaxf(unit[h], kQ4Least), fminf(most_of[h], 1.f / kQ4Least));
-              f[h] = unit[h] / unit_new;
-              unit[h] = unit_new;
+              // (up to 2^126: its reciprocal is a normal number)
+              const float now = fmaxf(heaviest[h], fminf(most_of[h], 1.f / kQ4Least));
+              const uint32_t apart = power_of_two(now) - power_of_two(heaviest[h]);
+              f[h] = __uint_as_float(0x3f800000u - min(apart, 0x3f800000u));                   // old unit / new unit; zero below 2^-126
+              heaviest[h] = now;
             }
             rescale(f);
           }
           float per_unit[HG];
 #pragma unroll
-          for (int h = 0; h < HG; ++h) asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(per_unit[h]) : "f"(unit[h]));
+          for (int h = 0; h < HG; ++h) per_unit[h] = __uint_as_float(0x7f000000u - power_of_two(heaviest[h]));
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
             float wa[2] = {0.f, 0.f}, wb[2] = {0.f, 0.f};
@@ -676,7 +685,7 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
         zacc[h] += __shfl_xor_sync(0xffffffffu, zacc[h], off);
       }
-    const float f_low[2] = {unit[0], unit[1]}, f_high[2] = {f_low[0] * 0.0625f, f_low[1] * 0.0625f};
+    const float f_low[2] = {__uint_as_float(power_of_two(heaviest[0])), __uint_as_float(power_of_two(heaviest[1]))}, f_high[2] = {f_low[0] * 0.0625f, f_low[1] * 0.0625f};
     float* row0 = mo + (warp * kQ4Heads + t4) * HD;
     float* row1 = row0 + 4 * HD;
 #pragma unroll
@@ -893,9 +902,9 @@ __global__ void __launch_bounds__(128) attn_decode_q4_shares_kernel(const float*
 }
 
 // Steps in flight.  Four blocks of three an SM for one group of heads at 128 registers a thread; two groups want 168, and then
-// three blocks of four steps.  (The other way round: 64 requests of 8,192 keys, 8 KV heads of 128, 114 us and not 112, ragged 42.5 and
-// not 41; eight query heads on each of 4 KV heads of 64, 8 requests of 1,536 keys 8.8 us and not 8.3, but 64 of some 2,048 30 and
-// not 34.)
+// three blocks of four steps.  (The other way round: 64 requests of 8,192 keys, 8 KV heads of 128, 113.6 us and not 113.2, ragged 42.4
+// and not 41.4, behind a window 10.5 and not 11.4; eight query heads on each of 4 KV heads of 64, 8 requests of 1,536 keys 8.6 us and not
+// 8.0, but 64 of some 2,048 30 and not 33.)
 template <int HD, int HG> constexpr int q4_decode_stages() { return HD > 128 || HG == 1 ? 3 : 4; }
 
 // Query heads of a block: four where a KV head has no more, else eight.
