@@ -12,7 +12,7 @@
              tables, holders, the stack of free pages, where every page went, the pools.
 
 The cache: codes in 8 bits (e4m3: a sign, four bits of exponent, three of fraction) [pages, KV heads, page, dim], a float32 scale
-[pages, KV heads] which is a power of two, the least 2^e (e >= -100) with 448 * 2^e not below the page's largest element; a row
+[pages, KV heads] which is a power of two, the least 2^e (e >= -60) with 448 * 2^e not below the page's largest element; a row
 stands for scale * code.  A page whose first row is written begins anew; else its scale never shrinks, and where it grows the rows
 that are there are rounded to the new one.
 
@@ -29,7 +29,7 @@ own = False
 
 DEVICE = "cuda:0"
 FP8 = torch.float8_e4m3fn
-LEAST = -100                       # exponent of the smallest scale
+LEAST = -60                        # exponent of the smallest scale
 
 
 # ------------------------------------------------------------------------------------------------ cases
