@@ -8,6 +8,7 @@ kernels (used by the benchmark's ``gpu_launches``).
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import struct
 import types
@@ -889,6 +890,12 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                     ctx.seq_ctx_len.data_ptr(), pages[0].data_ptr(), pages[1].data_ptr(), first, seqs, blocks, nkv, hd, block_size,
                     k_cache.shape[0], window)
     _launched(rc, name, "(hd={}, nkv={})", hd, nkv)
+    _attend_laid_out(q, out, pages, ctx, S, first, blocks, block_size, device, nh, nkv, hd, scale, window, softcap, sink)
+
+
+def _attend_laid_out(q, out, pages, ctx, S, first, blocks, block_size, device, nh, nkv, hd, scale, window, softcap, sink) -> None:
+    """A step's portions over the pages that were laid out for them: ``pages`` bfloat16 [2, requests * blocks, nkv, block_size, hd], of the
+    requests from ``first`` on."""
     with torch.cuda.device(device):
         # tiles of no request become those of one more, which has no row and sees one key
         pad = lambda t, v: torch.nn.functional.pad(t[:S], (0, 1), value=v)
@@ -901,6 +908,173 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
         # ('mma' reads these arrays behind its dependency wait and no key below the window; the other kernel takes the arrays for
         # old ones and multiplies what lies below the window, where no page was laid out, by zero)
         attention_prefill(q, out, pages[0], pages[1], tables, step, nh, nkv, hd, scale, window, softcap, sink)
+
+
+# ------------------------------------------------------------------ a cache in 8 bits (csrc/cuda/q8.cuh)
+
+Q8 = torch.float8_e4m3fn
+
+
+def _q8_cache(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, nkv: int, hd: int) -> int:
+    """Checks a cache in 8 bits; its block_size."""
+    if hd % 8 or not 8 <= hd <= 256:
+        raise KernelError(f"{name}: head sizes are multiples of 8 up to 256")
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[1] != nkv or shape[3] != hd or nkv <= 0 or v_cache.shape != shape or k_cache.dtype != Q8 or v_cache.dtype != Q8 \
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous() or (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise KernelError(f"{name}: caches must be contiguous float8_e4m3fn [pages, {nkv}, block_size, {hd}] on 16 bytes, k and v alike")
+    if not 0 < shape[2] <= 65536 or shape[0] == 0:
+        raise KernelError(f"{name}: block_size of 1 to 65536 rows, and at least one page")
+    for t in (k_scale, v_scale):
+        if t.dtype != torch.float32 or t.shape != shape[:2] or not t.is_contiguous():
+            raise KernelError(f"{name}: scales must be contiguous float32 [pages, {nkv}]")
+    return shape[2]
+
+
+_STORE_Q8 = {s: _Entry("kvcm_rope_cache_q8_" + s, "plpiipppppp" + "liiiiii") for s in ("f32", "bf16")}
+_READ_Q8 = {s: _Entry("kvcm_read_cache_q8_" + s, "ppppp" + "pp" + "lliiiii") for s in ("f32", "bf16")}
+_PLAIN_Q8 = {s: _Entry("kvcm_attention_plain_q8_" + s, "plplpppp" + "ipipp" + "iiiii" + "fifp") for s in ("f32", "bf16")}
+_PLAIN_PROMPT = {s: _Entry("kvcm_prompt_attention_plain_" + s, "plplplpl" + "pppp" + "iii" + "iii" + "fifp") for s in ("f32", "bf16")}
+
+
+def rope_cache_q8(qkv: torch.Tensor, table: Optional[torch.Tensor], interleaved: bool, slot_mapping: torch.Tensor, k_cache: torch.Tensor,
+                  v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, q_out: torch.Tensor, nh: int, nkv: int, hd: int) -> None:
+    """Rotates the q and k heads of fused rows [T, (nh + 2 nkv) hd] with the step's angles and writes k (rotated, not rounded in
+    between) and v in 8 bits into the rows' page slots; the rotated q rows go to ``q_out`` [T, nh hd] (which may be those columns of
+    ``qkv`` itself).  The k and v columns of ``qkv`` stay as they are.  ``k_cache``, ``v_cache``: float8_e4m3fn [pages, nkv, block_size, hd];
+    ``k_scale``, ``v_scale``: float32 [pages, nkv]; an element stands for scale * code.  The scale of a page and head is a power of two, the least
+    2^e (e >= -60) with 448 * 2^e not below its largest element.  A call that writes a page's first row begins the page anew; else
+    the scale never shrinks, and where it grows the page's rows are rounded to the new one.
+    ``table``: float32 [T, rotary_dim], cosines then sines of every row (``rope_table`` makes it; a table narrower than hd rotates the
+    first elements of a head); None: no rotation.  rotary_dim is a multiple of 16 in rotate-half pairs, of 2 in interleaved ones.
+    Rows with a slot below zero (or beyond the pool) are written nowhere.  Rows of one page stand next to each other (in any order), and
+    no two rows share a slot.  Elements that are not finite read back as not-a-number and leave the scale alone."""
+    name = "rope_cache_q8"
+    T, suffix = qkv.shape[0], _suffix(qkv)
+    block_size = _q8_cache(name, k_cache, v_cache, k_scale, v_scale, nkv, hd)
+    _q4_rows(name, "qkv", qkv, T, (nh + 2 * nkv) * hd, qkv.dtype)
+    _q4_rows(name, "q_out", q_out, T, nh * hd, qkv.dtype)
+    _ints(name, "slot_mapping", slot_mapping, T)
+    rotary = 0
+    if table is not None:
+        rotary = table.shape[-1]
+        if table.dtype != torch.float32 or table.dim() != 2 or table.shape[0] < T or not table.is_contiguous() or table.data_ptr() % 16:
+            raise KernelError(f"{name}: table float32 [T, rotary_dim]")
+        if not 0 < rotary <= hd or rotary % (2 if interleaved else 16):
+            raise KernelError(f"{name}: rotary_dim {rotary} (a multiple of 16 in rotate-half pairs, of 2 in interleaved ones, at most {hd})")
+    device = _one_device(name, qkv, table, slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out)
+    rc = _STORE_Q8[suffix](device, qkv.data_ptr(), qkv.stride(0), _at(table), rotary, int(interleaved), slot_mapping.data_ptr(),
+                           k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), q_out.data_ptr(),
+                           q_out.stride(0), T, nh, nkv, hd, block_size, k_cache.shape[0])
+    _launched(rc, name, "(hd={}, rotary_dim={})", hd, rotary)
+
+
+def read_cache_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor,
+                  k_rows: torch.Tensor, v_rows: torch.Tensor) -> None:
+    """The values that the given slots of a cache in 8 bits stand for, as rows [T, nkv hd] of bfloat16 or float32 (for rows that move
+    to another cache, or to look at them).  Rows with a slot below zero (or beyond the pool) are left as they were."""
+    name = "read_cache_q8"
+    T, suffix = k_rows.shape[0], _suffix(k_rows)
+    nkv, hd = (k_cache.shape[1], k_cache.shape[3]) if k_cache.dim() == 4 else (0, 8)
+    block_size = _q8_cache(name, k_cache, v_cache, k_scale, v_scale, nkv, hd)
+    _q4_rows(name, "k_rows", k_rows, T, nkv * hd, k_rows.dtype)
+    _q4_rows(name, "v_rows", v_rows, T, nkv * hd, k_rows.dtype)
+    _ints(name, "slot_mapping", slot_mapping, T)
+    device = _one_device(name, k_cache, v_cache, k_scale, v_scale, slot_mapping, k_rows, v_rows)
+    rc = _READ_Q8[suffix](device, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(),
+                          k_rows.data_ptr(), v_rows.data_ptr(), k_rows.stride(0), v_rows.stride(0), T, nkv, hd, block_size, k_cache.shape[0])
+    _launched(rc, name, "(hd={})", hd)
+
+
+def _attention_rows(name, q, out, nh, nkv, hd, window, softcap, sink) -> None:
+    """What calls of attention over a cache in 8 bits or over a prompt's own rows have to keep to alike."""
+    if nkv <= 0 or nh <= 0 or nh % nkv:
+        raise KernelError(f"{name}: {nh} query heads are not a multiple of {nkv} KV heads")
+    if window < 0 or softcap < 0.0:
+        raise KernelError(f"{name}: window and softcap must not be negative")
+    if window > 0x7fffffff:
+        raise KernelError(f"{name}: a window of {window} keys does not fit 32 bits")
+    if hd % 8 or not 8 <= hd <= 256:
+        raise KernelError(f"{name}: head sizes are multiples of 8 up to 256")
+    if q.dtype != out.dtype or q.dtype not in _SUFFIX:
+        raise KernelError(f"{name}: q and out must be bfloat16 or float32 rows of one type")
+    width, rows, to = nh * hd, q.shape, out.shape
+    if len(rows) != 2 or len(to) != 2 or to[0] != rows[0] or rows[1] < width or to[1] < width:
+        raise KernelError(f"{name}: q and out must be rows of {nh} heads of {hd}")
+    if q.stride(1) != 1 or out.stride(1) != 1:
+        raise KernelError(f"{name}: rows must be dense")
+    if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nh or not sink.is_contiguous()):
+        raise KernelError(f"{name}: sink must be float32 [heads]")
+
+
+def _page_tables(name, block_tables) -> None:
+    if block_tables.dtype != _I32 or block_tables.dim() != 2 or block_tables.shape[1] == 0 or not block_tables.is_contiguous():
+        raise KernelError(f"{name}: block_tables must be contiguous int32 [S, max_blocks]")
+
+
+def attention_plain_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                       v_scale: torch.Tensor, block_tables: torch.Tensor, row_seq: torch.Tensor, positions: torch.Tensor, nh: int, nkv: int,
+                       hd: int, scale: float, window: int = 0, softcap: float = 0.0, sink: Optional[torch.Tensor] = None) -> None:
+    """``attention_plain`` over a cache in 8 bits: one row a block, float32 arithmetic, q and out in bfloat16 or float32."""
+    name = "attention_plain_q8"
+    T = out.shape[0]
+    _attention_rows(name, q, out, nh, nkv, hd, window, softcap, sink)
+    block_size = _q8_cache(name, k_cache, v_cache, k_scale, v_scale, nkv, hd)
+    _page_tables(name, block_tables)
+    _ints(name, "row_seq", row_seq, T)
+    _ints(name, "positions", positions, T)
+    device = _one_device(name, q, out, k_cache, v_cache, k_scale, v_scale, block_tables, row_seq, positions, sink)
+    rc = _PLAIN_Q8[_SUFFIX[q.dtype]](
+        device, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), k_cache.shape[0], block_tables.data_ptr(), block_tables.shape[1], row_seq.data_ptr(), positions.data_ptr(), T, nh,
+        nkv, hd, block_size, scale, window, softcap, _at(sink))
+    _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
+
+
+def paged_attention_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                       v_scale: torch.Tensor, block_tables: torch.Tensor, ctx, nh: int, nkv: int, hd: int, scale: float, window: int = 0,
+                       softcap: float = 0.0, sink: Optional[torch.Tensor] = None) -> None:
+    """``paged_attention`` over a cache in 8 bits: attention of all rows of a step, rows [0, ctx.decode_seqs) single-row entries, the
+    rest the rows of longer portions; a row without keys gives zeros.  Single row i is request i's: requests that bring nothing stand
+    behind the others."""
+    attention_plain_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_tables, ctx.row_seq, ctx.positions, nh, nkv, hd, scale, window,
+                       softcap, sink)
+
+
+# ------------------------------------------------------------------ prompts over their own rows
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, ctx, nh: int, nkv: int, hd: int, scale: float,
+                     window: int = 0, softcap: float = 0.0, sink: Optional[torch.Tensor] = None) -> None:
+    """Causal attention of whole prompts over their own rows: no cache, no pages.  q [T, nh hd], k and v [T, nkv hd] are rows of a step (row
+    strides free: columns of a fused q|k|v are taken as they lie), out [T, nh hd].  The prompts lie one behind another: request i
+    has rows seq_q_start[i] .. + seq_q_len[i] of ``ctx``, whose row j sees the rows 0 .. j of its own request, whatever ``seq_ctx_len``
+    says.  ``ctx`` has the step's arrays with tiles of 64 rows, as for ``paged_attention``: entries [0, ctx.decode_seqs) are prompts of one row,
+    the others' rows are named by tiles (of request -1: none).  Rows of no prompt are left as they were.
+    ``window``: the last ``window`` rows only; ``softcap``, ``sink`` as in ``attention_plain``.
+    A prompt that goes into a quantised cache attends keys and values that are not rounded yet, which no read of that cache can give it back."""
+    name = "prompt_attention"
+    _attention_rows(name, q, out, nh, nkv, hd, window, softcap, sink)
+    T = q.shape[0]
+    for what, t in (("k", k), ("v", v)):
+        if t.dtype != q.dtype or t.dim() != 2 or t.shape[0] != T or t.shape[1] < nkv * hd or t.stride(1) != 1:
+            raise KernelError(f"{name}: {what} must be {q.dtype} rows [{T}, {nkv * hd}] with dense elements")
+    S = ctx.seq_q_start.numel()
+    _ints(name, "seq_q_start", ctx.seq_q_start, S)
+    _ints(name, "seq_q_len", ctx.seq_q_len, S)
+    _ints(name, "tile_seq", ctx.tile_seq, ctx.prefill_tiles)
+    _ints(name, "tile_q0", ctx.tile_q0, ctx.prefill_tiles)
+    if ctx.tile_rows != 64:
+        raise KernelError(f"{name}: the batch must be tiled in 64 query rows")
+    if ctx.decode_seqs > S:
+        raise KernelError(f"{name}: {ctx.decode_seqs} prompts of one row in a step of {S} requests")
+    device = _one_device(name, q, k, v, out, ctx.seq_q_start, ctx.seq_q_len, ctx.tile_seq, ctx.tile_q0, sink)
+    if ctx.prefill_tiles + ctx.decode_seqs == 0:
+        return
+    rc = _PLAIN_PROMPT[_SUFFIX[q.dtype]](
+        device, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
+        ctx.tile_seq.data_ptr(), ctx.tile_q0.data_ptr(), ctx.seq_q_start.data_ptr(), ctx.seq_q_len.data_ptr(), ctx.prefill_tiles, 64,
+        ctx.decode_seqs, nh, nkv, hd, scale, window, softcap, _at(sink))
+    _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
 
 
 # ------------------------------------------------------------------ a step's arrays from lengths
@@ -965,6 +1139,147 @@ def raise_on_step_tables(status) -> None:
     code, number = int(status[0]), int(status[1])
     if code:
         raise KernelError("step_tables: " + STEP_TABLE_ERRORS.get(code, f"code {code}").format(number))
+
+
+# ------------------------------------------------------------------ pages that requests share (csrc/cuda/pages.cu)
+
+PAGE_ERRORS = {1: "entry {0} names a request that there is not", 2: "{0} is named twice", 3: "request {0} holds pages, or begins in this call",
+               4: "the length of request {0} exceeds its page table", 5: "page {0} is not in the pool, or free",
+               6: "{0} pages are missing from the stack of free ones", 7: "a count of {0} lies outside the stack of free pages",
+               8: "page {0} is given back by more requests than hold it"}
+_FORK = _Entry("kvcm_fork_requests", "ppi" + "pipipipip" + "i" + "ppppp" + "pi")
+_RELEASE = _Entry("kvcm_release_requests", "pi" + "pipipipip" + "i" + "pppp")
+_COMPACT = _Entry("kvcm_compact_pages", "pipipipip" + "i" + "pppppp" + "pi")
+_COPY_PAGES = _Entry("kvcm_copy_pages", "ppii" + "pi")
+
+
+def _pools(name: str, pools, pages: int):
+    """Pools as the library reads them: address, layers, bytes between layers, bytes of a page."""
+    if len(pools) > 64:
+        raise KernelError(f"{name}: at most 64 pools")
+    table = array.array("q")
+    for t in pools:
+        if t.dim() < 3 or t.shape[1] != pages or t.numel() == 0 or not t[0].is_contiguous():
+            raise KernelError(f"{name}: pools must be [layers, {pages}, ...], the pages of a layer dense")
+        size = t.element_size()
+        table.extend((t.data_ptr(), t.shape[0], t.stride(0) * size, t.stride(1) * size))
+    return table
+
+
+def _page_state(name: str, seq_len, block_tables, shared, free_pages, free_count, block_size, status, *others) -> int:
+    S = seq_len.numel()
+    for t in (seq_len, block_tables, shared, free_pages, free_count, status, *others):
+        if t.dtype is not _I32 or not t.is_contiguous():
+            raise KernelError(f"{name}: contiguous int32 arrays")
+    if not 0 < S <= 65536 or block_tables.dim() != 2 or block_tables.shape[0] != S or block_tables.shape[1] == 0:
+        raise KernelError(f"{name}: 1 to 65536 requests, block_tables [{S}, max_blocks]")
+    if block_size <= 0 or block_tables.shape[1] * block_size > 0x7fffffff - block_size:
+        raise KernelError(f"{name}: block_size must be positive, positions of a table fit 32 bits")
+    if shared.numel() == 0 or free_count.numel() != 1 or status.numel() < 4:
+        raise KernelError(f"{name}: shared [pages], free_count [1], status [4]")
+    return S
+
+
+def copy_pages(pools, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Pages ``src[i]`` -> ``dst[i]`` (int32, on the device) of every pool, a tensor [layers, pages, ...] of any type whose layers are dense (a
+    single layer: ``cache[None]``).  Pairs with a page below zero or beyond the pool are none.  No page is a target twice, or source and target."""
+    name = "copy_pages"
+    if len(pools) == 0:
+        raise KernelError(f"{name}: at least one pool")
+    pages = pools[0].shape[1] if pools[0].dim() >= 3 else 0
+    table = _pools(name, pools, pages)
+    n = src.numel()
+    _ints(name, "src", src, n)
+    _ints(name, "dst", dst, n)
+    if dst.numel() != n:
+        raise KernelError(f"{name}: as many targets as sources")
+    device = _one_device(name, src, dst, *pools)
+    if n == 0:
+        return
+    rc = _COPY_PAGES(device, src.data_ptr(), dst.data_ptr(), n, pages, table.buffer_info()[0], len(pools))
+    _launched(rc, name, "({} pages, {} pools)", n, len(pools))
+    add_launches(1)                         # the empty kernel behind it
+
+
+def fork_requests(parents: torch.Tensor, children: torch.Tensor, seq_len: torch.Tensor, block_tables: torch.Tensor, shared: torch.Tensor,
+                  free_pages: torch.Tensor, free_count: torch.Tensor, block_size: int, pools=(), *, seq_len_out: torch.Tensor,
+                  shared_out: torch.Tensor, free_left: torch.Tensor, status: torch.Tensor) -> None:
+    """Requests that begin as copies of others (samples of one prompt, branches of a search), on the device.  All arrays int32.
+
+    Entry k: request ``children[k]``, which holds nothing so far, becomes a copy of ``parents[k]`` (below zero: no entry).  The whole pages
+    of the parent's ``seq_len`` positions are shared, the one behind them, which both will write to, is copied in every pool (``copy_pages``)
+    into a page from the top of the stack ``free_pages[:free_count]``, in the entries' order.
+    ``shared`` [pages]: requests that hold a page beyond the first.  Pages that ``step_tables`` takes have 0, as it is where a page is free.
+    Out: the children's rows of ``block_tables``, ``seq_len_out``, ``shared_out``, ``free_left`` (each may be its input; the others start as
+    copies).  A child is named once and is nobody's parent in the call; one parent may have many.
+    ``status`` [4]: (0, 0, pages taken, 0), or (code, number, 0, 0) where the call cannot be (``raise_on_pages``): everything is then as
+    before.  The host reads it when it likes; nothing waits here."""
+    name = "fork_requests"
+    S = _page_state(name, seq_len, block_tables, shared, free_pages, free_count, block_size, status, parents, children, seq_len_out, shared_out, free_left)
+    K, pages = parents.numel(), shared.numel()
+    if K > 8192 or children.numel() != K:
+        raise KernelError(f"{name}: up to 8192 parents and as many children")
+    if seq_len_out.numel() != S or shared_out.numel() != pages or free_left.numel() != 1:
+        raise KernelError(f"{name}: seq_len_out [{S}], shared_out [{pages}], free_left [1]")
+    table = _pools(name, pools, pages)
+    device = _one_device(name, seq_len, block_tables, shared, free_pages, free_count, status, parents, children, seq_len_out, shared_out, free_left, *pools)
+    moves = torch.empty(1 + 2 * K, dtype=_I32, device=seq_len.device)
+    rc = _FORK(device, parents.data_ptr(), children.data_ptr(), K, seq_len.data_ptr(), S, block_tables.data_ptr(), block_tables.shape[1],
+               shared.data_ptr(), pages, free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), block_size, seq_len_out.data_ptr(),
+               shared_out.data_ptr(), free_left.data_ptr(), moves.data_ptr(), status.data_ptr(), table.buffer_info()[0], len(pools))
+    _launched(rc, name, "({} entries, {} requests)", K, S)
+    add_launches(2 if len(pools) else 1)    # the pages, and the empty kernel behind them
+
+
+def release_requests(requests: torch.Tensor, seq_len: torch.Tensor, block_tables: torch.Tensor, shared: torch.Tensor, free_pages: torch.Tensor,
+                     free_count: torch.Tensor, block_size: int, *, seq_len_out: torch.Tensor, shared_out: torch.Tensor, free_left: torch.Tensor,
+                     status: torch.Tensor) -> None:
+    """Requests that end, on the device: each page of ``requests`` (int32; below zero: no entry; none twice) loses a holder, and those
+    without one go onto the stack behind ``free_pages[:free_count]``, the lowest number on top.  Their lengths become zero; their rows of
+    ``block_tables`` stay as they are, and nothing reads them.  Arrays and ``status`` as for ``fork_requests``: (0, 0, pages given back, 0)."""
+    name = "release_requests"
+    S = _page_state(name, seq_len, block_tables, shared, free_pages, free_count, block_size, status, requests, seq_len_out, shared_out, free_left)
+    K, pages = requests.numel(), shared.numel()
+    if K > 8192:
+        raise KernelError(f"{name}: up to 8192 requests a call")
+    if seq_len_out.numel() != S or shared_out.numel() != pages or free_left.numel() != 1:
+        raise KernelError(f"{name}: seq_len_out [{S}], shared_out [{pages}], free_left [1]")
+    device = _one_device(name, seq_len, block_tables, shared, free_pages, free_count, status, requests, seq_len_out, shared_out, free_left)
+    rc = _RELEASE(device, requests.data_ptr(), K, seq_len.data_ptr(), S, block_tables.data_ptr(), block_tables.shape[1], shared.data_ptr(), pages,
+                  free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), block_size, seq_len_out.data_ptr(), shared_out.data_ptr(),
+                  free_left.data_ptr(), status.data_ptr())
+    _launched(rc, name, "({} entries, {} requests)", K, S)
+    add_launches(1)                         # the empty kernel behind it
+
+
+def compact_pages(seq_len: torch.Tensor, block_tables: torch.Tensor, shared: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                  block_size: int, pools=(), *, tables_out: torch.Tensor, shared_out: torch.Tensor, free_out: torch.Tensor,
+                  page_map: torch.Tensor, status: torch.Tensor) -> None:
+    """Moves the pages in use (those not on the stack, ``used`` of them) into the pages 0 .. used - 1 of every pool, so that what lies behind can
+    be given back or saved in one piece.  The r-th used page from ``used`` on goes into the r-th free page below; the others stay.
+    Out: ``tables_out``, ``shared_out``, ``free_out`` (each may be its input; entries of the stack behind the count are left as they were), with
+    ``used`` on top of the stack, and ``page_map`` [pages]: where every page went, -1 for free ones, for whoever else knows pages by number.
+    Arrays and ``status`` as for ``fork_requests``: (0, 0, pages moved, 0)."""
+    name = "compact_pages"
+    S = _page_state(name, seq_len, block_tables, shared, free_pages, free_count, block_size, status, tables_out, shared_out, free_out, page_map)
+    pages = shared.numel()
+    if tables_out.shape != block_tables.shape or shared_out.numel() != pages or free_out.numel() != free_pages.numel() or page_map.numel() != pages:
+        raise KernelError(f"{name}: tables_out, shared_out and free_out like their inputs, page_map [{pages}]")
+    table = _pools(name, pools, pages)
+    device = _one_device(name, seq_len, block_tables, shared, free_pages, free_count, status, tables_out, shared_out, free_out, page_map, *pools)
+    moves = torch.empty(1 + 2 * pages, dtype=_I32, device=seq_len.device)
+    rc = _COMPACT(device, seq_len.data_ptr(), S, block_tables.data_ptr(), block_tables.shape[1], shared.data_ptr(), pages, free_pages.data_ptr(),
+                  free_pages.numel(), free_count.data_ptr(), block_size, tables_out.data_ptr(), shared_out.data_ptr(), free_out.data_ptr(),
+                  page_map.data_ptr(), moves.data_ptr(), status.data_ptr(), table.buffer_info()[0], len(pools))
+    _launched(rc, name, "({} requests, {} pages)", S, pages)
+    add_launches(2 if len(pools) else 1)    # the pages, and the empty kernel behind them
+
+
+def raise_on_pages(status) -> None:
+    """Raises ``KernelError`` where the status of a ``fork_requests``, ``release_requests`` or ``compact_pages`` call (read to the host) names a refusal."""
+    code, number = int(status[0]), int(status[1])
+    if code:
+        raise KernelError("pages: " + PAGE_ERRORS.get(code, f"code {code}").format(number))
 
 
 def attention_tcgen05_error() -> int:
