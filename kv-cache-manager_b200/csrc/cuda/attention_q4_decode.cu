@@ -31,9 +31,7 @@
 // to 1,024 keys behind a window, capped: 11.4 us; 8 of 1,500 keys 8.0 us; one of 148 keys 4.8 us: launch, lengths, table, q and keys
 // behind one another.  One of 32,768 keys 38 us (5.5 at the rate of a copy): equal shares cut it into some 70 pieces a head, which eight
 // blocks join one after another.
-#include <cooperative_groups.h>
-
-#include "attention_mma.cuh"
+#include "decode_join.cuh"
 #include "packed.cuh"
 #include "pdl.cuh"
 #include "q4.cuh"
@@ -41,12 +39,13 @@
 namespace kvcm {
 
 constexpr int kQ4Warps = 4;
-constexpr int kQ4DecodeThreads = 32 * kQ4Warps;
+constexpr int kQ4DecodeThreads = kDecodeThreads;
+static_assert(kQ4DecodeThreads == 32 * kQ4Warps, "four warps");
 constexpr int kQ4Step = 32;                        // keys of a warp's step
 constexpr int kQ4Tile = kQ4Step * kQ4Warps;        // keys of a round of the block
-constexpr int kQ4Heads = 8;                        // most query heads of a block
+constexpr int kQ4Heads = kDecodeHeads;
 constexpr int kQ4TabMax = 512;                     // page-table entries of a partition kept in shared memory
-constexpr int kQ4ClusterParts = 8;
+constexpr int kQ4ClusterParts = kDecodeClusterParts;
 constexpr float kQ4Lowest = 3.402823466e38f;
 constexpr float kQ4Least = 1.17549435e-38f;        // 2^-126
 // What it costs to start on a request and head, in tiles of 128 keys, for the shares: its table, its q, an empty ring.  (0, 2, 4, 6 and
@@ -151,48 +150,6 @@ template <int HD, int STAGES> constexpr size_t q4_decode_core_smem() {
   return ring > merge ? ring : merge;
 }
 template <int HD, int STAGES> constexpr size_t q4_decode_smem() { return q4_decode_core_smem<HD, STAGES>() + kQ4TabMax * sizeof(int); }
-
-// The partitions of a cluster: every block has its partial result in its own shared memory (bo [8][HD], bm maximum, bl sum; an
-// empty partition has bm = -inf and no bo).  The outputs are dealt out over the blocks, four adjacent elements an item; each adds
-// the partitions up in their order.
-template <int HD>
-__device__ __forceinline__ void q4_cluster_tail(const DecodeQ4Params& p, int seq, int head0, int heads_here, float* bo, float* bm, float* bl) {
-  namespace cg = cooperative_groups;
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();
-  const int P = p.num_parts;
-  constexpr int Q = HD / 4;
-  for (int it = int(cluster.block_rank()) * kQ4DecodeThreads + threadIdx.x; it < heads_here * Q; it += P * kQ4DecodeThreads) {
-    const int r = it / Q, d = (it - r * Q) * 4;
-    float m[kQ4ClusterParts], l[kQ4ClusterParts], top = -INFINITY;
-    float4 o[kQ4ClusterParts];
-#pragma unroll
-    for (int i = 0; i < kQ4ClusterParts; ++i) {
-      m[i] = -INFINITY; l[i] = 0.f; o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i < P) {
-        m[i] = *cluster.map_shared_rank(bm + r, i);
-        l[i] = *cluster.map_shared_rank(bl + r, i);
-        o[i] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(bo + r * HD + d, i));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kQ4ClusterParts; ++i) top = fmaxf(top, m[i]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < kQ4ClusterParts; ++i) {
-      if (l[i] == 0.f) continue;                                   // nothing there, and its bo is not written
-      const float f = fast_exp2(m[i] - top);
-      acc.x = fmaf(f, o[i].x, acc.x); acc.y = fmaf(f, o[i].y, acc.y); acc.z = fmaf(f, o[i].z, acc.z); acc.w = fmaf(f, o[i].w, acc.w);
-      sum = fmaf(f, l[i], sum);
-    }
-    if (p.sink && sum != 0.f) sum += fast_exp2(p.sink[head0 + r] * 1.4426950408889634f - top);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    bf16* dst = p.out + size_t(seq) * p.out_stride + size_t(head0 + r) * HD + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-  }
-  cluster.sync();                                                  // nobody leaves while its memory is read
-}
 
 // A block's piece of work: keys [begin, end) of one request for eight query heads of a KV head.
 struct Q4Segment {
@@ -746,158 +703,11 @@ __global__ void __launch_bounds__(kQ4DecodeThreads, HD > 128 ? 2 : HG == 1 ? 4 :
       }
     }
     if (!shares) {
-      if (p.cluster_merge) q4_cluster_tail<HD>(p, w.seq, w.head0, w.heads_here, bo, bm, bl);
+      if (p.cluster_merge) decode_cluster_tail<HD>(p, w.seq, w.head0, w.heads_here, bo, bm, bl);
       return;
     }
     if (left <= 0) return;
     __syncthreads();                                               // the merge gives way to the rings
-  }
-}
-
-// More partitions than a cluster merges, out of scratch memory, in their order.
-__global__ void attn_decode_q4_merge_kernel(const float* part_o, const float* part_ml, bf16* __restrict__ out, long long out_stride, int nh,
-                                            int hd, int num_parts, const float* __restrict__ sink) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int seq = blockIdx.x, head = blockIdx.y;
-  const size_t base = (size_t(seq) * nh + head) * num_parts;
-  float top = -INFINITY;
-  for (int i = 0; i < num_parts; ++i) top = fmaxf(top, part_ml[(base + i) * 2]);
-  for (int d = threadIdx.x; d < hd; d += blockDim.x) {
-    float acc = 0.f, sum = 0.f;
-    for (int i = 0; i < num_parts; ++i) {
-      const float li = part_ml[(base + i) * 2 + 1];
-      if (li == 0.f) continue;
-      const float f = exp2f(part_ml[(base + i) * 2] - top);
-      acc = fmaf(f, part_o[(base + i) * hd + d], acc);
-      sum = fmaf(f, li, sum);
-    }
-    if (sink && sum != 0.f) sum += exp2f(sink[head] * 1.4426950408889634f - top);
-    out[size_t(seq) * out_stride + size_t(head) * hd + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : acc / sum);
-  }
-}
-
-// The pieces of a request and its four or eight heads that blocks part_first[0] .. part_first[1] have left, in their order: the first
-// block's lies in its second place, the others' in their first.  Up to six are asked for at once, maxima, sums and outputs in one trip
-// to memory (64 ragged requests in all 1.3 us less).  A long request has many: the weights of 128 of them at a time are formed
-// side by side, so that what follows one another is additions.
-constexpr int kQ4JoinAtOnce = 128;
-constexpr int kQ4JoinFew = 6;
-__global__ void __launch_bounds__(128) attn_decode_q4_shares_kernel(const float* part_o, const float* part_ml, const int* part_first,
-                                                                    const int* __restrict__ seq_ctx_len, bf16* __restrict__ out,
-                                                                    long long out_stride, int nh, int nkv, int hd, int tile_heads,
-                                                                    const float* __restrict__ sink) {
-  __shared__ float weight[kQ4JoinAtOnce][kQ4Heads];
-  __shared__ float tops[4][kQ4Heads], all_top[kQ4Heads], all_sum[kQ4Heads];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int G = nh / nkv, head_tiles = (G + tile_heads - 1) / tile_heads, H = nkv * head_tiles;
-  const int seq = blockIdx.x, h = blockIdx.y, kvh = h / head_tiles, ht = h - kvh * head_tiles;
-  const int head0 = kvh * G + ht * tile_heads, heads_here = min(tile_heads, G - ht * tile_heads);
-  const int tid = threadIdx.x, quads = hd / 4, items = heads_here * quads;
-  if (seq_ctx_len[seq] <= 0) {
-    for (int it = tid; it < items; it += 128) {
-      const int r = it / quads, d = (it - r * quads) * 4;
-      *reinterpret_cast<uint2*>(out + size_t(seq) * out_stride + size_t(head0 + r) * hd + d) = make_uint2(0u, 0u);
-    }
-    return;
-  }
-  const int first = part_first[(seq * H + h) * 2], pieces = part_first[(seq * H + h) * 2 + 1] - first + 1;
-  if (pieces == 1) return;                                         // one block had it all
-  auto at = [&](int i, int r) { return size_t(2 * (first + i) + (i == 0)) * kQ4Heads + r; };
-  if (pieces <= kQ4JoinFew) {                                      // the usual request: all of them asked for at once
-    for (int it = tid; it < items; it += 128) {
-      const int r = it / quads, d = (it - r * quads) * 4;
-      float2 ml[kQ4JoinFew];
-      float4 v[kQ4JoinFew];
-#pragma unroll
-      for (int i = 0; i < kQ4JoinFew; ++i) {
-        ml[i] = make_float2(-INFINITY, 0.f);
-        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < pieces) {
-          ml[i] = *reinterpret_cast<const float2*>(part_ml + at(i, r) * 2);
-          v[i] = *reinterpret_cast<const float4*>(part_o + at(i, r) * hd + d);
-        }
-      }
-      float top = -INFINITY, sum = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < kQ4JoinFew; ++i) top = fmaxf(top, ml[i].x);
-#pragma unroll
-      for (int i = 0; i < kQ4JoinFew; ++i) {
-        if (ml[i].y == 0.f) continue;
-        const float f = fast_exp2(ml[i].x - top);
-        sum = fmaf(f, ml[i].y, sum);
-        o.x = fmaf(f, v[i].x, o.x); o.y = fmaf(f, v[i].y, o.y); o.z = fmaf(f, v[i].z, o.z); o.w = fmaf(f, v[i].w, o.w);
-      }
-      if (sink && sum != 0.f) sum += fast_exp2(sink[head0 + r] * 1.4426950408889634f - top);
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<uint2*>(out + size_t(seq) * out_stride + size_t(head0 + r) * hd + d) =
-          make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-    }
-    return;
-  }
-  // the largest maximum of every head
-  {
-    const int r = tid & 7;
-    float top = -INFINITY;
-    if (r < heads_here)
-      for (int i = tid >> 3; i < pieces; i += 16) top = fmaxf(top, part_ml[at(i, r) * 2]);
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    if ((tid & 31) < 8) tops[tid >> 5][r] = top;
-    __syncthreads();
-    if (tid < 8) {
-      all_top[tid] = fmaxf(fmaxf(tops[0][tid], tops[1][tid]), fmaxf(tops[2][tid], tops[3][tid]));
-      all_sum[tid] = 0.f;
-    }
-    __syncthreads();
-  }
-  constexpr int kMost = kQ4Heads * 256 / 4 / 128;                  // items of a thread
-  float4 acc[kMost];
-#pragma unroll
-  for (int k = 0; k < kMost; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < pieces; i0 += kQ4JoinAtOnce) {
-    const int n = min(kQ4JoinAtOnce, pieces - i0);
-    for (int j = tid; j < n * kQ4Heads; j += 128) {
-      const int i = j >> 3, r = j & 7;
-      float w = 0.f;
-      if (r < heads_here) {
-        const float l = part_ml[at(i0 + i, r) * 2 + 1];
-        w = l == 0.f ? 0.f : fast_exp2(part_ml[at(i0 + i, r) * 2] - all_top[r]);
-      }
-      weight[i][r] = w;
-    }
-    __syncthreads();
-    if (tid < heads_here) {                                        // (one thread a head: the sums keep their order)
-      float sum = all_sum[tid];
-      for (int i = 0; i < n; ++i) sum = fmaf(weight[i][tid], part_ml[at(i0 + i, tid) * 2 + 1], sum);
-      all_sum[tid] = sum;
-    }
-#pragma unroll
-    for (int k = 0; k < kMost; ++k) {
-      const int it = tid + k * 128;
-      if (it >= items) break;
-      const int r = it / quads, d = (it - r * quads) * 4;
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float f = weight[i][r];
-        const float4 v = *reinterpret_cast<const float4*>(part_o + at(i0 + i, r) * hd + d);
-        acc[k].x = fmaf(f, v.x, acc[k].x); acc[k].y = fmaf(f, v.y, acc[k].y); acc[k].z = fmaf(f, v.z, acc[k].z); acc[k].w = fmaf(f, v.w, acc[k].w);
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int k = 0; k < kMost; ++k) {
-    const int it = tid + k * 128;
-    if (it >= items) break;
-    const int r = it / quads, d = (it - r * quads) * 4;
-    float sum = all_sum[r];
-    if (sink && sum != 0.f) sum += fast_exp2(sink[head0 + r] * 1.4426950408889634f - all_top[r]);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint2*>(out + size_t(seq) * out_stride + size_t(head0 + r) * hd + d) =
-        make_uint2(pack_bf16(acc[k].x * inv, acc[k].y * inv), pack_bf16(acc[k].z * inv, acc[k].w * inv));
   }
 }
 
@@ -1002,9 +812,9 @@ KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, vo
 #undef X
   if (rc != 0 || num_parts == 1 || cluster_merge) return rc;
   if (num_parts == 0)
-    return pdl_launch(attn_decode_q4_shares_kernel, dim3(seqs, nkv * head_tiles), dim3(128), 0, (cudaStream_t)stream, (const float*)p.part_o,
+    return pdl_launch(attn_decode_shares_kernel, dim3(seqs, nkv * head_tiles), dim3(128), 0, (cudaStream_t)stream, (const float*)p.part_o,
                       (const float*)p.part_ml, (const int*)p.part_first, seq_ctx_len, p.out, out_stride, nh, nkv, hd, tile_heads, sink);
-  return pdl_launch(attn_decode_q4_merge_kernel, dim3(seqs, nh), dim3(hd < 64 ? 32 : 64), 0, (cudaStream_t)stream, (const float*)p.part_o,
+  return pdl_launch(attn_decode_merge_kernel, dim3(seqs, nh), dim3(hd < 64 ? 32 : 64), 0, (cudaStream_t)stream, (const float*)p.part_o,
                     (const float*)p.part_ml, p.out, out_stride, nh, hd, num_parts, p.sink);
 }
 

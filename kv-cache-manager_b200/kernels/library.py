@@ -899,7 +899,7 @@ def _attend_laid_out(q, out, pages, ctx, S, first, blocks, block_size, device, n
     with torch.cuda.device(device):
         # tiles of no request become those of one more, which has no row and sees one key
         pad = lambda t, v: torch.nn.functional.pad(t[:S], (0, 1), value=v)
-        tables = torch.arange(-first * blocks, (seqs + 1) * blocks, dtype=torch.int32, device=q.device).view(S + 1, blocks)
+        tables = torch.arange(-first * blocks, (S - first + 1) * blocks, dtype=torch.int32, device=q.device).view(S + 1, blocks)
         tables[S].zero_()
         step = types.SimpleNamespace(
             seq_q_start=pad(ctx.seq_q_start, 0), seq_q_len=pad(ctx.seq_q_len, 0), seq_ctx_len=pad(ctx.seq_ctx_len, 1).clamp_(max=blocks * block_size),
@@ -935,6 +935,10 @@ _STORE_Q8 = {s: _Entry("kvcm_rope_cache_q8_" + s, "plpiipppppp" + "liiiiii") for
 _READ_Q8 = {s: _Entry("kvcm_read_cache_q8_" + s, "ppppp" + "pp" + "lliiiii") for s in ("f32", "bf16")}
 _PLAIN_Q8 = {s: _Entry("kvcm_attention_plain_q8_" + s, "plplpppp" + "ipipp" + "iiiii" + "fifp") for s in ("f32", "bf16")}
 _PLAIN_PROMPT = {s: _Entry("kvcm_prompt_attention_plain_" + s, "plplplpl" + "pppp" + "iii" + "iii" + "fifp") for s in ("f32", "bf16")}
+_PREFILL_Q8 = _Entry("kvcm_attention_prefill_q8_bf16", "plipl" + "ppppipi" + "ppppp" + "iiiii" + "fifp")
+_PROMPT = _Entry("kvcm_prompt_attention_bf16", "plplpl" + "ipl" + "pppp" + "iiiii" + "fifp")
+_DECODE_Q8 = _Entry("kvcm_attention_decode_q8_bf16", "plplpppp" + "ipip" + "iiiii" + "fiiiipifp")
+_UNPACK_Q8 = _Entry("kvcm_unpack_pages_q8_bf16", "pppp" + "pi" + "pppp" + "iiiiiiii")
 
 
 def rope_cache_q8(qkv: torch.Tensor, table: Optional[torch.Tensor], interleaved: bool, slot_mapping: torch.Tensor, k_cache: torch.Tensor,
@@ -1031,17 +1035,154 @@ def attention_plain_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor
     _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
 
 
+def decode_partitions_q8(seqs: int, nh: int, nkv: int, hd: int, max_ctx: int, device: int, force_parts: int = 0):
+    """How ``attention_decode_q8`` splits the context: (keys per partition, number of partitions), no partitions for equal shares.
+
+    As many partitions as a cluster merges and the GPU holds at once (an eighth more: not all are full), none for up to 256 keys;
+    where they would be longer than 1,024 keys, equal shares of all requests' keys."""
+    max_ctx = max(max_ctx, 1)
+    blocks = max(1, seqs * nkv * ((nh // nkv + 7) // 8))
+    most = (max_ctx + Q4_PART_KEYS - 1) // Q4_PART_KEYS
+    if force_parts < 0:
+        return Q4_PART_KEYS, 0
+    if force_parts > 0:
+        parts = min(force_parts, most)
+    else:
+        room = _q8_resident_blocks(hd, device) * 9 // 8 // blocks
+        parts = max(1, min(CLUSTER_PARTS, room, most if max_ctx > 2 * Q4_PART_KEYS else 1))
+    size = ((max_ctx + parts - 1) // parts + Q4_PART_KEYS - 1) // Q4_PART_KEYS * Q4_PART_KEYS
+    if force_parts == 0 and size > 1024:
+        return Q4_PART_KEYS, 0
+    return size, (max_ctx + size - 1) // size
+
+
+def _q8_resident_blocks(hd: int, device: int) -> int:
+    key = ("q8", hd, device)
+    n = _RESIDENT.get(key)
+    if n is None:
+        with torch.cuda.device(device):
+            n = max(int(_lib().kvcm_attention_decode_q8_blocks_per_sm(int(hd))), 1) * sm_count(torch.device("cuda", device))
+        _RESIDENT[key] = n
+    return n
+
+
+def attention_decode_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, block_tables: torch.Tensor, ctx, nh: int, nkv: int, hd: int, scale: float, window: int = 0,
+                        softcap: float = 0.0, sink: Optional[torch.Tensor] = None) -> None:
+    """Single-row entries over a cache in 8 bits: q and out hold one bfloat16 row a request, in the order of the batch's entries;
+    ``ctx.seq_ctx_len`` says how many keys each sees (0: the row is zero), ``ctx.max_decode_ctx`` is about the longest: the keys are
+    divided by it, and beyond it one block takes what is left.
+    ``window``: the last ``window`` keys only; ``softcap``, ``sink`` as in ``attention_plain``."""
+    name = "attention_decode_q8"
+    S, lengths = q.shape[0], ctx.seq_ctx_len
+    _attention_rows(name, q, out, nh, nkv, hd, window, softcap, sink)
+    block_size = _q8_cache(name, k_cache, v_cache, k_scale, v_scale, nkv, hd)
+    _page_tables(name, block_tables)
+    _ints(name, "seq_ctx_len", lengths, S)
+    if not attention_q4_supported(hd, q.dtype):
+        raise KernelError(f"{name}: bfloat16 rows, heads of 32 to 256 elements in steps of 32")
+    at, to, step, out_step = q.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0)
+    if at % 16 or step % 8 or to % 8 or out_step % 4:
+        raise KernelError(f"{name}: q rows must be 16-byte aligned, out rows 8-byte aligned")
+    requests, max_blocks = block_tables.shape
+    if requests < S:
+        raise KernelError(f"{name}: a page table for each of {S} rows")
+    device = _one_device(name, q, out, k_cache, v_cache, k_scale, v_scale, block_tables, lengths, sink)
+    if S == 0:
+        return
+    span = min(ctx.max_decode_ctx, max_blocks * block_size, 1 << 30)       # (a context ends with its table)
+    if window > 0:
+        span = min(span, window + 31)
+    size, parts = decode_partitions_q8(S, nh, nkv, hd, span, device, ctx.options.get("attn_parts", 0))
+    in_cluster = 1 < parts <= CLUSTER_PARTS and ctx.options.get("attn_merge", "cluster") == "cluster"
+    scratch, shares = None, 0
+    if parts == 0:
+        shares = _q8_resident_blocks(hd, device)
+        scratch = torch.empty(shares * 16 * (hd + 2) + S * nh * 2, dtype=torch.float32, device=q.device)
+    elif parts > 1 and not in_cluster:
+        scratch = torch.empty(S * nh * parts * (hd + 2), dtype=torch.float32, device=q.device)
+    rc = _DECODE_Q8(device, at, step, to, out_step, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_cache.shape[0],
+                    block_tables.data_ptr(), max_blocks, lengths.data_ptr(), S, nh, nkv, hd, block_size, scale, window, size, parts, shares,
+                    _at(scratch), int(in_cluster), softcap, _at(sink))
+    _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
+    if scratch is not None:
+        add_launches(1)                     # the merge kernel
+
+
 def paged_attention_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                        v_scale: torch.Tensor, block_tables: torch.Tensor, ctx, nh: int, nkv: int, hd: int, scale: float, window: int = 0,
                        softcap: float = 0.0, sink: Optional[torch.Tensor] = None) -> None:
     """``paged_attention`` over a cache in 8 bits: attention of all rows of a step, rows [0, ctx.decode_seqs) single-row entries, the
     rest the rows of longer portions; a row without keys gives zeros.  Single row i is request i's: requests that bring nothing stand
-    behind the others."""
-    attention_plain_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_tables, ctx.row_seq, ctx.positions, nh, nkv, hd, scale, window,
-                       softcap, sink)
+    behind the others.  ``ctx.max_ctx`` is at least the longest context of the portions (of a recorded step: the longest it will see),
+    ``ctx.max_decode_ctx`` about that of the single rows.  float32 rows, other head sizes than multiples of 32 and
+    ``ctx.options['attention'] == 'plain'``: ``attention_plain_q8`` for every row."""
+    if ctx.options.get("attention", "auto") == "plain" or not attention_q4_supported(hd, q.dtype):
+        attention_plain_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_tables, ctx.row_seq, ctx.positions, nh, nkv, hd, scale, window,
+                           softcap, sink)
+        return
+    nd = ctx.decode_seqs
+    if nd > 0:
+        all_single = nd == q.shape[0]
+        attention_decode_q8(q if all_single else q[:nd], out if all_single else out[:nd], k_cache, v_cache, k_scale, v_scale, block_tables, ctx,
+                            nh, nkv, hd, scale, window, softcap, sink)
+    if ctx.rows > nd:
+        attention_prefill_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_tables, ctx, nh, nkv, hd, scale, window, softcap, sink)
+
+
+def attention_prefill_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                         v_scale: torch.Tensor, block_tables: torch.Tensor, ctx, nh: int, nkv: int, hd: int, scale: float, window: int = 0,
+                         softcap: float = 0.0, sink: Optional[torch.Tensor] = None) -> None:
+    """Rows of portions longer than one token over a cache in 8 bits; q and out are the step's full bfloat16 row arrays, ``ctx`` has
+    the step's arrays with tiles of 64 rows (tiles of request -1 are none; ``ctx.max_ctx`` is at least the longest context; a context
+    ends with its page table).  Heads of 64 and 128 elements and pages of a multiple of 8 rows: one kernel that turns codes into operands beside
+    the products.  Others, or ``ctx.options['attn_prefill'] == 'unpack'``: the pages that the portions see are laid out in bfloat16
+    (exactly), in scratch of the call, and read by ``attention_prefill``'s 'mma' kernel (where a value that is not a number also reaches
+    rows of its tile that do not see it)."""
+    name = "attention_prefill_q8"
+    _attention_rows(name, q, out, nh, nkv, hd, window, softcap, sink)
+    block_size = _q8_cache(name, k_cache, v_cache, k_scale, v_scale, nkv, hd)
+    _page_tables(name, block_tables)
+    S = ctx.seq_ctx_len.numel()
+    for what in ("seq_q_start", "seq_q_len", "seq_ctx_len"):
+        _ints(name, what, getattr(ctx, what), S)
+    _ints(name, "tile_seq", ctx.tile_seq, ctx.prefill_tiles)
+    _ints(name, "tile_q0", ctx.tile_q0, ctx.prefill_tiles)
+    if not attention_q4_supported(hd, q.dtype):
+        raise KernelError(f"{name}: bfloat16 rows, heads of 32 to 256 elements in steps of 32")
+    if q.data_ptr() % 16 or q.stride(0) % 8 or out.data_ptr() % 16 or out.stride(0) % 8:
+        raise KernelError(f"{name}: q and out rows must be 16-byte aligned")
+    if ctx.tile_rows != 64:
+        raise KernelError(f"{name}: the batch must be tiled in 64 query rows")
+    if block_tables.shape[0] < S:
+        raise KernelError(f"{name}: a page table for each of {S} entries")
+    device = _one_device(name, q, out, k_cache, v_cache, k_scale, v_scale, block_tables, sink, ctx.seq_q_start, ctx.seq_q_len, ctx.seq_ctx_len,
+                         ctx.tile_seq, ctx.tile_q0)
+    first, seqs = ctx.decode_seqs, S - ctx.decode_seqs
+    if seqs <= 0 or ctx.prefill_tiles == 0:
+        return
+    if hd in (64, 128) and block_size % 8 == 0 and ctx.options.get("attn_prefill", "auto") != "unpack":
+        rc = _PREFILL_Q8(device, q.data_ptr(), q.stride(0), q.shape[0], out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+                         k_scale.data_ptr(), v_scale.data_ptr(), k_cache.shape[0], block_tables.data_ptr(), block_tables.shape[1],
+                         ctx.tile_seq.data_ptr(), ctx.tile_q0.data_ptr(), ctx.seq_q_start.data_ptr(), ctx.seq_q_len.data_ptr(),
+                         ctx.seq_ctx_len.data_ptr(), ctx.prefill_tiles, nh, nkv, hd, block_size, scale, window, softcap, _at(sink))
+        _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
+        return
+    blocks = min(block_tables.shape[1], (ctx.max_ctx + block_size - 1) // block_size)
+    pages = torch.empty((2, seqs * blocks, nkv, block_size, hd), dtype=torch.bfloat16, device=q.device)
+    rc = _UNPACK_Q8(device, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+                    block_tables.shape[1], ctx.seq_q_len.data_ptr(), ctx.seq_ctx_len.data_ptr(), pages[0].data_ptr(), pages[1].data_ptr(),
+                    first, seqs, blocks, nkv, hd, block_size, k_cache.shape[0], window)
+    _launched(rc, name, "(hd={}, nkv={})", hd, nkv)
+    _attend_laid_out(q, out, pages, ctx, S, first, blocks, block_size, device, nh, nkv, hd, scale, window, softcap, sink)
 
 
 # ------------------------------------------------------------------ prompts over their own rows
+
+def prompt_attention_supported(hd: int, dtype: torch.dtype) -> bool:
+    """True where ``prompt_attention`` has its kernel on tensor cores (and rows that start on 16 bytes): bfloat16, heads of up to 128 elements."""
+    return dtype == torch.bfloat16 and hd % 8 == 0 and 8 <= hd <= 128
+
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, ctx, nh: int, nkv: int, hd: int, scale: float,
                      window: int = 0, softcap: float = 0.0, sink: Optional[torch.Tensor] = None) -> None:
@@ -1050,7 +1191,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
     has rows seq_q_start[i] .. + seq_q_len[i] of ``ctx``, whose row j sees the rows 0 .. j of its own request, whatever ``seq_ctx_len``
     says.  ``ctx`` has the step's arrays with tiles of 64 rows, as for ``paged_attention``: entries [0, ctx.decode_seqs) are prompts of one row,
     the others' rows are named by tiles (of request -1: none).  Rows of no prompt are left as they were.
-    ``window``: the last ``window`` rows only; ``softcap``, ``sink`` as in ``attention_plain``.
+    ``window``: the last ``window`` rows only; ``softcap``, ``sink`` as in ``attention_plain``.  bfloat16 rows that start on 16 bytes, heads of
+    up to 128 elements: one kernel on tensor cores; float32 rows, larger heads, other alignments and
+    ``ctx.options['attention'] == 'plain'``: one row a block, in float32.
     A prompt that goes into a quantised cache attends keys and values that are not rounded yet, which no read of that cache can give it back."""
     name = "prompt_attention"
     _attention_rows(name, q, out, nh, nkv, hd, window, softcap, sink)
@@ -1069,6 +1212,14 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
         raise KernelError(f"{name}: {ctx.decode_seqs} prompts of one row in a step of {S} requests")
     device = _one_device(name, q, k, v, out, ctx.seq_q_start, ctx.seq_q_len, ctx.tile_seq, ctx.tile_q0, sink)
     if ctx.prefill_tiles + ctx.decode_seqs == 0:
+        return
+    if prompt_attention_supported(hd, q.dtype) and ctx.options.get("attention", "auto") != "plain" \
+            and (q.data_ptr() | k.data_ptr() | v.data_ptr() | out.data_ptr()) % 16 == 0 \
+            and (q.stride(0) | k.stride(0) | v.stride(0) | out.stride(0)) % 8 == 0:
+        rc = _PROMPT(device, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), T, out.data_ptr(), out.stride(0),
+                     ctx.tile_seq.data_ptr(), ctx.tile_q0.data_ptr(), ctx.seq_q_start.data_ptr(), ctx.seq_q_len.data_ptr(), ctx.prefill_tiles,
+                     ctx.decode_seqs, nh, nkv, hd, scale, window, softcap, _at(sink))
+        _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
         return
     rc = _PLAIN_PROMPT[_SUFFIX[q.dtype]](
         device, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0),
