@@ -6,9 +6,9 @@
 //     S = Q K^T   accumulator in tensor memory
 //     softmax     one thread a row:  p = 2^(x - m), x the scaled scores; P lies in tensor memory over the scores that it was made of
 //     O += P V    V as the MN-major operand, O in tensor memory for the whole block
-// A row takes its scores 32 at a time, relative to the maximum that it knows, without looking for theirs: where 32 probabilities
-// add up to more than 2^12 (or the row has seen nothing yet) their maximum is found, sums, O and the tile's earlier probabilities
-// are rescaled, and the 32 are taken again, which after the first tiles hardly ever happens.
+// A row takes a tile's scores relative to the maximum that it knows, without looking for theirs: where their probabilities add up
+// to more than 2^12 (prompts: leave 2^-40 .. 2^20; or the row has seen nothing yet) their maximum is found, sum and O are rescaled, and the tile is taken
+// again, which after the first tiles hardly ever happens.
 // The products of a group run in order: S of the next tile behind O += P V of this one, so one barrier says that S is there, that
 // O holds the tile before, and that P has been read.
 //
@@ -18,8 +18,7 @@
 // out of the products: the key's enters the score's factor, the value's, a power of two, the probability's exponent
 // (2^(x - m) scale = 2^(x - m + log2 scale): weights in place of probabilities), one factor for eight keys, which lie in one page.
 // m is the reference of the weights, and sums take the weights' scales out again.  q enters as float16 times a power of two for
-// each row, exact but for elements 2^-29 as large as the row's largest.  P is rounded to float16 (prompts: bfloat16), and once more where a
-// maximum is renewed inside its tile.
+// each row, exact but for elements 2^-29 as large as the row's largest.  P is rounded to float16 (prompts: bfloat16).
 //
 // Values that are not finite and that some row of a tile does not see would come to it as zero times them.  Rows past the
 // last are zeros in shared memory; a row whose result is not finite looks whether an unseen value was the reason, and is then
@@ -43,10 +42,11 @@ constexpr int kArTile = 128 * 128;                 // [128 rows][64 elements of 
 constexpr int kArStages = 2;                       // tiles of keys, and of values
 constexpr int kArRing = 4;                         // tiles' scales
 constexpr int kArKeyWarps = 4, kArValueWarps = 3;  // pages: who turns codes into operands
-constexpr float kArMost = 4096.f;                  // a row's sum of 32 weights from which its maximum is renewed
+constexpr float kArMost = 4096.f;                  // pages: a row's sum of a tile's weights from which its maximum is renewed
+constexpr float kArMostPrompt = 1048576.f, kArLeast = 9.094947e-13f;      // prompts: 2^20, and 2^-40
 // tensor memory: S of group g at column g * 128 (and P in its first 64 columns); O of group g at 256 + g * HD
 
-struct ArScales { float key, value, out; };        // of eight keys: scale, log2 of the value's less the block's, 2^-(that)
+struct alignas(16) ArScales { float key, value, out; };        // of eight keys: scale, log2 of the value's less the block's, 2^-(that)
 
 struct RowsParams {
   bf16* out; long long out_stride;
@@ -54,7 +54,7 @@ struct RowsParams {
   const bf16* k; long long k_stride; const bf16* v; long long v_stride;                      // prompts
   const uint8_t* k_codes; const uint8_t* v_codes; const float* k_scale; const float* v_scale;      // pages
   const int* block_tables; int max_blocks, max_keys;      // keys that a request's table has pages for
-  const int* tile_seq; const int* tile_q0; int tiles;     // tiles of 64 rows; a block takes every fourth and its three successors
+  const int* tile_seq; const int* tile_q0; int tiles, blocks;      // tiles of 64 rows; a block takes one and its three successors
   const int* seq_q_start; const int* seq_q_len; const int* seq_ctx_len;
   int nh, nkv, hd, block_size, log2_block, num_pages, window;
   float scale_log2, cap_pre;
@@ -63,6 +63,20 @@ struct RowsParams {
 };
 
 namespace {
+
+// tc5::mbar_wait for waits of a microsecond: the thread sleeps in the instruction and does not take its scheduler's turns.
+__device__ __forceinline__ bool ar_wait(uint64_t* bar, uint32_t parity) {
+  unsigned long long start = 0;
+  for (;;) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(tc5::s32(bar)), "r"(parity), "r"(100000u) : "memory");
+    if (done) return true;
+    const unsigned long long now = tc5::now_ns();
+    if (start == 0) start = now;
+    else if (now - start > tc5::kWaitLimitNs) return false;
+  }
+}
 
 __device__ __forceinline__ float ar_exp2(float x) {
   float y;
@@ -73,6 +87,17 @@ __device__ __forceinline__ float ar_tanh(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(ar_exp2(x * 2.8853900817779268f) + 1.f));
   return fmaf(-2.f, r, 1.f);
+}
+__device__ __forceinline__ float2 ar_mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 w, x, y;\nmov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float ar_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 // a * b + c of two floats at once
 __device__ __forceinline__ float2 ar_fma2(float2 a, float2 b, float2 c) {
@@ -109,12 +134,29 @@ __device__ __forceinline__ void ar_wait32(uint32_t (&v)[32]) {
   asm volatile("" : "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]),
                     "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
-// The product with its first operand in tensor memory: 16-bit elements, two neighbours of a row to a column.
-__device__ __forceinline__ void ar_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t db, uint32_t instr, uint32_t accumulate) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-               ::"r"(d_tmem), "r"(a_tmem), "l"(db), "r"(instr), "r"(accumulate) : "memory");
+// The products and their commit, as one thread of a warp that stays together issues them (`one`: it is this thread): addresses and
+// descriptors are then the same in all lanes, which the compiler may keep where the instruction wants them.
+__device__ __forceinline__ void ar_mma_ss(uint32_t one, uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t instr, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+               ::"r"(d_tmem), "l"(da), "l"(db), "r"(instr), "r"(accumulate), "r"(one) : "memory");
 }
+// With the first operand in tensor memory: 16-bit elements, two neighbours of a row to a column.
+__device__ __forceinline__ void ar_mma_ts(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint64_t db, uint32_t instr, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(d_tmem), "r"(a_tmem), "l"(db), "r"(instr), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void ar_commit(uint32_t one, uint64_t* bar) {
+  asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n"
+               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(tc5::s32(bar)), "r"(one) : "memory");
+}
+__device__ __forceinline__ uint32_t ar_elect() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(one));
+  return one;
+}
+__device__ __forceinline__ int ar_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 // A box of [rows][64 elements] of one head: x element, y head, z row.
 __device__ __forceinline__ void ar_tma_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n"
@@ -134,36 +176,45 @@ template <bool HALF> __device__ __forceinline__ float2 ar_unpack(uint32_t v) {
 // What turns a row's products into scores: x = s * factor (capped: tanh(s * factor) * scale_log2).
 struct ArRow { float factor, scale_log2; };
 
-// The scores of two keys behind their tanh or factor, plus `add`.
-template <bool CAP>
+// The scores of two keys behind their tanh or factor, plus `add`.  SMALL: behind a factor that brought them into [-1, 1], where tanh is
+// an odd polynomial of degree 11 (least largest error, 5.8e-7, from an exchange algorithm), which costs no exponentials.
+template <bool CAP, bool SMALL = false>
 __device__ __forceinline__ float2 ar_scores(uint32_t s0, uint32_t s1, float factor, float scale_log2, float add) {
   const float2 s = make_float2(__uint_as_float(s0), __uint_as_float(s1));
-  if constexpr (CAP) return make_float2(fmaf(ar_tanh(s.x * factor), scale_log2, add), fmaf(ar_tanh(s.y * factor), scale_log2, add));
+  if constexpr (CAP && SMALL) {
+    constexpr float c[6] = {0.999999463558197f, -0.33329397439956665f, 0.13284258544445038f, -0.05168433114886284f, 0.016832629218697548f, -0.0031027502845972776f};
+    const float2 y = ar_mul2(s, make_float2(factor, factor)), z = ar_mul2(y, y);
+    float2 t = ar_fma2(z, make_float2(c[5], c[5]), make_float2(c[4], c[4]));
+#pragma unroll
+    for (int i = 3; i >= 0; --i) t = ar_fma2(z, t, make_float2(c[i], c[i]));
+    return ar_fma2(ar_mul2(t, y), make_float2(scale_log2, scale_log2), make_float2(add, add));
+  } else if constexpr (CAP) return make_float2(fmaf(ar_tanh(s.x * factor), scale_log2, add), fmaf(ar_tanh(s.y * factor), scale_log2, add));
   else return ar_fma2(s, make_float2(factor, factor), make_float2(add, add));
 }
 
-// 32 products of a row into weights; `weights` their sum, `sum` that of the probabilities.  MASK: only keys [a, b) of the 32 count.
+// 32 products of a row into weights, added to `w2`, and probabilities, added to `l2` (pages).  MASK: only the `seen` of the 32 count.
 // AGAIN: the maximum is known, so nothing is above 2^12 but what scores of 2^24 and more are rounded by.
-template <bool CAP, bool PAGES, bool MASK, bool AGAIN>
-__device__ __forceinline__ void ar_exponentials(const uint32_t (&s)[32], const ArScales* sc, uint32_t (&packed)[16], const ArRow& row, float m,
-                                                int a, int b, float& weights, float& sum) {
-  float2 w2 = make_float2(0.f, 0.f), l2 = make_float2(0.f, 0.f);
+template <bool CAP, bool PAGES, bool MASK, bool AGAIN, bool SMALL>
+__device__ __forceinline__ void ar_exponentials(const uint32_t (&s)[32], const ArScales* sc, uint32_t* packed, const ArRow& row, float m,
+                                                uint32_t seen, float2& w2, float2& l2) {
+  if constexpr (MASK) asm volatile("" : "+r"(seen));               // (its bits are looked at here, not ahead of the branches before)
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float factor = row.factor, add = -m, out = 1.f;
     if constexpr (PAGES) {
-      factor *= sc[j].key;
-      add += sc[j].value;
-      out = sc[j].out;
+      const float4 f = *reinterpret_cast<const float4*>(sc + j);
+      factor *= f.x;
+      add += f.y;
+      out = f.z;
     }
     float2 g0, g1;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = 8 * j + 2 * k;
-      float2 t = ar_scores<CAP>(s[i], s[i + 1], factor, row.scale_log2, add);
+      float2 t = ar_scores<CAP, SMALL>(s[i], s[i + 1], factor, row.scale_log2, add);
       if constexpr (MASK) {
-        t.x = i >= a && i < b ? t.x : -INFINITY;
-        t.y = i + 1 >= a && i + 1 < b ? t.y : -INFINITY;
+        t.x = seen & (1u << i) ? t.x : -INFINITY;
+        t.y = seen & (2u << i) ? t.y : -INFINITY;
       }
       if constexpr (AGAIN) t = make_float2(t.x > 12.f ? 12.f : t.x, t.y > 12.f ? 12.f : t.y);      // (not-a-number stays)
       const float2 e = make_float2(ar_exp2(t.x), ar_exp2(t.y));
@@ -174,13 +225,58 @@ __device__ __forceinline__ void ar_exponentials(const uint32_t (&s)[32], const A
     w2 = ar_add2(w2, g0);
     if constexpr (PAGES) l2 = ar_fma2(g0, make_float2(out, out), l2);
   }
+}
+
+// Bits [a, b) of a word.
+__device__ __forceinline__ uint32_t ar_bits(int a, int b) {
+  const uint32_t below_b = b >= 32 ? 0xffffffffu : b <= 0 ? 0u : (1u << b) - 1u, below_a = a >= 32 ? 0xffffffffu : a <= 0 ? 0u : (1u << a) - 1u;
+  return below_b & ~below_a;
+}
+
+// Whether the factor brings all of the warp's products into [-1, 1].
+template <bool PAGES>
+__device__ __forceinline__ bool ar_small(const uint32_t (&s)[32], const ArScales* sc, float row_factor) {
+  float largest = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float factor = PAGES ? row_factor * sc[j].key : row_factor;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 y = ar_mul2(make_float2(__uint_as_float(s[8 * j + 2 * k]), __uint_as_float(s[8 * j + 2 * k + 1])), make_float2(factor, factor));
+      const float2 z = ar_mul2(y, y);
+      largest = ar_max3(largest, z.x, z.y);
+    }
+  }
+  return !__any_sync(0xffffffffu, largest > 1.f);
+}
+
+// A thread's products of a tile into weights, two to a register.  Of `chunks` 32.
+template <int CHUNKS, bool CAP, bool PAGES, bool MASK, bool AGAIN>
+__device__ __forceinline__ void ar_tile(uint32_t s_addr, const ArScales* sc, uint32_t (&packed)[16 * CHUNKS], const ArRow& row, float m, int a, int b,
+                                        int chunks, float& weights, float& sum) {
+  uint32_t s[32];
+  float2 w2 = make_float2(0.f, 0.f), l2 = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    if (!MASK || c < chunks) {
+      tc5::ld32(s_addr + uint32_t(c * 32), s);
+      ar_wait32(s);
+      if (CAP && ar_small<PAGES>(s, sc + c * 4, row.factor))
+        ar_exponentials<CAP, PAGES, MASK, AGAIN, true>(s, sc + c * 4, packed + c * 16, row, m, MASK ? ar_bits(a - c * 32, b - c * 32) : 0u, w2, l2);
+      else
+        ar_exponentials<CAP, PAGES, MASK, AGAIN, false>(s, sc + c * 4, packed + c * 16, row, m, MASK ? ar_bits(a - c * 32, b - c * 32) : 0u, w2, l2);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) packed[c * 16 + i] = 0u;
+    }
+  }
   weights = w2.x + w2.y;
   sum = PAGES ? l2.x + l2.y : weights;
 }
 
 // The largest of the 32 weights' exponents, less m.
 template <bool CAP, bool PAGES>
-__device__ __forceinline__ float ar_largest(const uint32_t (&s)[32], const ArScales* sc, const ArRow& row, float m, int a, int b) {
+__device__ __forceinline__ float ar_largest(const uint32_t (&s)[32], const ArScales* sc, const ArRow& row, float m, uint32_t seen) {
   float mx = -INFINITY;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -189,39 +285,34 @@ __device__ __forceinline__ float ar_largest(const uint32_t (&s)[32], const ArSca
     for (int k = 0; k < 4; ++k) {
       const int i = 8 * j + 2 * k;
       const float2 t = ar_scores<CAP>(s[i], s[i + 1], factor, row.scale_log2, add);
-      mx = (i >= a && i < b) ? fmaxf(mx, t.x) : mx;
-      mx = (i + 1 >= a && i + 1 < b) ? fmaxf(mx, t.y) : mx;
+      mx = seen & (1u << i) ? fmaxf(mx, t.x) : mx;
+      mx = seen & (2u << i) ? fmaxf(mx, t.y) : mx;
     }
   }
   return mx;
 }
 
-// What a row has in tensor memory times alpha: O, and the first `chunks` pieces of 32 weights, which are rounded once more by
-// that (a tile's pieces at most three times, and only where scores climb inside the tile).  The whole warp takes part.
-template <int HD, bool HALF>
-__device__ __noinline__ void ar_rescale(uint32_t o_addr, bool has_o, uint32_t p_addr, int chunks, float alpha) {
+// `columns` of what a row has in O times alpha.  The whole warp takes part.
+__device__ __noinline__ void ar_rescale(uint32_t o_addr, int columns, float alpha) {
   uint32_t v[16];
 #pragma unroll 1
-  for (int c = 0; has_o && c < HD / 16; ++c) {
-    ar_ld16(o_addr + uint32_t(c * 16), v);
+  for (int c = 0; c < columns; c += 16) {
+    ar_ld16(o_addr + uint32_t(c), v);
     tc5::ld_wait();
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-    ar_st16(o_addr + uint32_t(c * 16), v);
-  }
-  if (chunks > 0) tc5::st_wait();                                  // loads of tensor memory pass stores that nobody waited for
-#pragma unroll 1
-  for (int c = 0; c < chunks; ++c) {
-    ar_ld16(p_addr + uint32_t(c * 16), v);
-    tc5::ld_wait();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 f = ar_unpack<HALF>(v[i]);
-      v[i] = ar_pack<HALF>(f.x * alpha, f.y * alpha);
-    }
-    ar_st16(p_addr + uint32_t(c * 16), v);
+    ar_st16(o_addr + uint32_t(c), v);
   }
   tc5::st_wait();
+}
+
+// A barrier of the warps that share rows, and whether any of their threads said so.
+template <int SPLIT> __device__ __forceinline__ bool ar_either(int id, bool mine) {
+  if (SPLIT == 1) return __any_sync(0xffffffffu, mine);
+  uint32_t any;
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.or.pred.aligned q, %2, 64, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+               : "=r"(any) : "r"(uint32_t(mine)), "r"(id) : "memory");
+  return any != 0u;
 }
 
 // Keys and values of one request and KV head, element by element.
@@ -310,7 +401,9 @@ __device__ __forceinline__ void ar_spread(unsigned char* tile, uint4 u, int r, i
 template <int HD, bool PAGES> constexpr size_t ar_smem() {
   return size_t(2 + 2 * kArStages) * (HD / 64) * kArTile + (PAGES ? kArRing * (kArKeys / 8) * sizeof(ArScales) : 0);
 }
-template <bool PAGES> constexpr int ar_threads() { return PAGES ? 512 : 320; }
+template <bool PAGES> constexpr int ar_split() { return PAGES ? 1 : 2; }         // threads of a row
+template <bool PAGES> constexpr int ar_threads() { return 256 * ar_split<PAGES>() + (PAGES ? 256 : 64); }
+
 
 template <int HD, bool CAP, bool PAGES>
 __global__ void __launch_bounds__(ar_threads<PAGES>(), 1)
@@ -318,7 +411,8 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ RowsParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   constexpr int KB = HD / 64;                                      // 64-wide blocks of a head
-  constexpr int kMmaWarp = PAGES ? 15 : 9;
+  constexpr int SPLIT = ar_split<PAGES>(), kSoftmaxWarps = 8 * SPLIT, CHUNKS = 4 / SPLIT, kSpan = kArKeys / SPLIT;
+  constexpr int kMmaWarp = ar_threads<PAGES>() / 32 - 1;
   constexpr int kPieces = HD / 16;                                 // pages: 16-byte pieces of a row of codes
   unsigned char* q_s = smem_raw;                                   // [2][KB][128 rows][64]
   unsigned char* k_s = q_s + 2 * KB * kArTile;                     // [stages][KB][128 keys][64]
@@ -327,6 +421,8 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   __shared__ __align__(8) uint64_t q_full, q_ready, k_full[kArStages], v_full[kArStages], k_free[kArStages], v_free[kArStages], v_tail,
       sc_full[kArRing], s_full[2], p_full[2], o_full;
   __shared__ uint32_t tmem_base;
+  __shared__ float told[SPLIT][kArRows];                           // what the threads of a row tell each other
+  __shared__ int left[8][2];                                       // that a warp gave up
   __shared__ float value_base;                                     // log2 of the value scale that weights are relative to
   __shared__ volatile int abort_flag;
 
@@ -336,16 +432,34 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   // Tiles and lengths may come from a kernel of the same step, so they are read behind the wait.  (Whoever leaves waits as
   // well: a launch of nothing but empty tiles would else be over before the kernel in front of it.)
   pdl_wait();
-  int seq, q0, most = kArRows;
-  if (!PAGES && tile >= p.tiles) {                                 // a prompt of one row
-    seq = tile - p.tiles;
-    q0 = 0;
+  int seq = -1, q0 = 0, most = kArRows;
+  if (!PAGES && tile >= p.blocks) {                                // a prompt of one row
+    seq = tile - p.blocks;
     most = 1;
-  } else {
-    seq = p.tile_seq[tile];
-    q0 = p.tile_q0[tile];
+  } else {                                                         // the tile-th of those that begin a block
+    for (int t0 = 0, before = 0; t0 < p.tiles; t0 += 128) {
+      int s[4], q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i * 32 + int(threadIdx.x & 31);
+        s[i] = t < p.tiles ? p.tile_seq[t] : -1;
+        q[i] = t < p.tiles ? p.tile_q0[t] : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t leads = __ballot_sync(0xffffffffu, s[i] >= 0 && (q[i] & (kArRows - 1)) == 0);
+        const int at = tile - before;
+        before += __popc(leads);
+        if (seq < 0 && at >= 0 && tile < before) {
+          const int from = __fns(leads, 0, at + 1);
+          seq = __shfl_sync(0xffffffffu, s[i], from);
+          q0 = __shfl_sync(0xffffffffu, q[i], from);
+        }
+      }
+      if (seq >= 0) break;
+    }
   }
-  if (seq < 0 || (q0 & (kArRows - 1))) return;                     // no tile, or one that belongs to a block before
+  if (seq < 0) return;                                             // fewer than the host had to reckon with
   const int q_start = p.seq_q_start[seq], q_len = p.seq_q_len[seq];
   const int rows_here = min(most, q_len - q0);
   if (rows_here <= 0) return;
@@ -353,7 +467,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     if (threadIdx.x == 0) atomicExch(error, (33 << 16) | int(blockIdx.y & 0xffff));
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int ctx = PAGES ? min(p.seq_ctx_len[seq], p.max_keys) : q_len;       // (a context ends with its table)
   const int pos0 = ctx - q_len + q0;                               // position of the block's first row
   const int hi = pos0 + rows_here;                                 // keys [lo, hi) matter to the block
@@ -365,10 +479,11 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   const int n_tiles = (hi - 1) / kArKeys - j0 + 1, n_first = (hi_first - 1) / kArKeys - j0 + 1;
   const int kvh = head / (p.nh / p.nkv);
 
+  if (threadIdx.x < 16) left[threadIdx.x >> 1][threadIdx.x & 1] = 0;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     tc5::mbar_init(&q_full, 1);
-    tc5::mbar_init(&q_ready, 4 * groups);
+    tc5::mbar_init(&q_ready, 4 * SPLIT * groups);
     for (int i = 0; i < kArStages; ++i) {
       tc5::mbar_init(&k_full[i], PAGES ? kArKeyWarps : 1);
       tc5::mbar_init(&v_full[i], PAGES ? kArValueWarps : 1);
@@ -379,7 +494,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     for (int i = 0; i < kArRing; ++i) tc5::mbar_init(&sc_full[i], 1);
     for (int g = 0; g < 2; ++g) {
       tc5::mbar_init(&s_full[g], 1);
-      tc5::mbar_init(&p_full[g], 4);                               // a group's four warps
+      tc5::mbar_init(&p_full[g], 4 * SPLIT);                       // a group's warps
     }
     tc5::mbar_init(&o_full, 1);
     tc5::mbar_init_fence();
@@ -399,65 +514,73 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     abort_flag = 1;
   };
   auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {  // the warp stays together whatever a lane saw
-    if (__all_sync(0xffffffffu, tc5::mbar_wait(bar, parity))) return true;
+    if (__all_sync(0xffffffffu, ar_wait(bar, parity))) return true;
     if (!abort_flag && lane == 0) fail(code);                      // (the first to give up says so; the others' waits run out too)
     return false;
   };
 
   if (warp == kMmaWarp) {
-    // ---- one thread: the products
-    if (lane == 0) {
-      if (PAGES) {
-        tc5::mbar_expect_tx(&q_full, groups * KB * kArTile);
-        for (int g = 0; g < groups; ++g)
-          for (int kb = 0; kb < KB; ++kb)
-            ar_tma_3d(q_s + (g * KB + kb) * kArTile, &map_q, &q_full, kb * 64, head, q_start + q0 + g * kArGroupRows);
-      }
-      constexpr uint32_t kTypes = PAGES ? ~((7u << 7) | (7u << 10)) : ~0u;       // float16 or bfloat16
-      constexpr uint32_t idesc_s = tc5::idesc(kArGroupRows, kArKeys, false) & kTypes;
-      constexpr uint32_t idesc_o = tc5::idesc(kArGroupRows, HD, true) & kTypes;
-      constexpr uint64_t kStageStep = (KB * kArTile) >> 4;          // (descriptor addresses count units of 16 bytes)
-      const uint64_t dk = tc5::smem_desc(tc5::s32(k_s));
-      // values, MN-major: 64-wide blocks a leading offset apart
-      const uint64_t dv = (tc5::smem_desc(tc5::s32(v_s)) & ~(uint64_t(0x3fff) << 16)) | (uint64_t(kArTile >> 4) << 16);
-      bool ok = tc5::mbar_wait(PAGES ? &q_ready : &q_full, 0);
-      if (!ok) fail(34);
-      tc5::fence_after();
-      for (int n = 0; ok && n <= n_tiles; ++n) {
-        for (int g = 0; g < groups; ++g) {
-          const int mine = g == 0 ? n_first : n_tiles;
-          if (n >= 1 && n <= mine) {                               // O += P_(n-1) V_(n-1)
-            const int m = n - 1, st = m % kArStages;
-            if (!tc5::mbar_wait(&v_full[st], (m / kArStages) & 1)) { fail(35); ok = false; break; }
-            if (!tc5::mbar_wait(&p_full[g], m & 1)) { fail(36); ok = false; break; }
-            tc5::fence_after();
-            // (of the last tile only the steps of 16 keys that some row of the group sees)
-            const int steps = min(kArKeys, (g == 0 ? hi_first : hi) - (j0 + m) * kArKeys + 15) / 16;
-            for (int j = 0; j < steps; ++j)                        // 16 keys: 8 columns of P, 16 rows down V
-              ar_mma_ts(tmem + 256 + g * HD, tmem + g * kArKeys + j * 8, dv + st * kStageStep + uint64_t(j * (16 * 128 >> 4)), idesc_o,
-                        (m > 0 || j > 0) ? 1u : 0u);
-          }
-          if (n < mine) {                                          // S_n, over P_(n-1)
-            const int st = n % kArStages;
-            if (!tc5::mbar_wait(&k_full[st], (n / kArStages) & 1)) { fail(37); ok = false; break; }
-            tc5::fence_after();
-            const uint64_t dq = tc5::smem_desc(tc5::s32(q_s + g * KB * kArTile));
+    // ---- the products: the warp stays together, one thread of it issues
+    const uint32_t one = ar_elect();
+    if (PAGES && one) {
+      tc5::mbar_expect_tx(&q_full, groups * KB * kArTile);
+      for (int g = 0; g < groups; ++g)
+        for (int kb = 0; kb < KB; ++kb)
+          ar_tma_3d(q_s + (g * KB + kb) * kArTile, &map_q, &q_full, kb * 64, head, q_start + q0 + g * kArGroupRows);
+    }
+    __syncwarp();
+    constexpr uint32_t kTypes = PAGES ? ~((7u << 7) | (7u << 10)) : ~0u;         // float16 or bfloat16
+    constexpr uint32_t idesc_s = tc5::idesc(kArGroupRows, kArKeys, false) & kTypes;
+    constexpr uint32_t idesc_o = tc5::idesc(kArGroupRows, HD, true) & kTypes;
+    constexpr uint64_t kStageStep = (KB * kArTile) >> 4;            // (descriptor addresses count units of 16 bytes)
+    const uint64_t dq = tc5::smem_desc(tc5::s32(q_s)), dk = tc5::smem_desc(tc5::s32(k_s));
+    // values, MN-major: 64-wide blocks a leading offset apart
+    const uint64_t dv = (tc5::smem_desc(tc5::s32(v_s)) & ~(uint64_t(0x3fff) << 16)) | (uint64_t(kArTile >> 4) << 16);
+    const uint32_t base = uint32_t(ar_uniform(int(tmem)));
+    const int tiles = ar_uniform(n_tiles), tiles_first = ar_uniform(n_first), both = ar_uniform(groups);
+    // (of a group's last tile only the steps of 16 keys that some row of it sees)
+    const int last_steps = ar_uniform((hi - (j0 + n_tiles - 1) * kArKeys + 15) / 16), last_first = ar_uniform((hi_first - (j0 + n_first - 1) * kArKeys + 15) / 16);
+    bool ok = wait_all(PAGES ? &q_ready : &q_full, 0, 34);
+    tc5::fence_after();
+    for (int n = 0; ok && n <= tiles; ++n) {
+      const int st = n & 1;                                         // stage of tile n; tile n - 1 has the other
+      static_assert(kArStages == 2, "stages by parity");
+      for (int g = 0; g < both; ++g) {
+        const int mine = g == 0 ? tiles_first : tiles;
+        if (n >= 1 && n <= mine) {                                 // O += P_(n-1) V_(n-1)
+          if (!wait_all(&v_full[st ^ 1], ((n - 1) >> 1) & 1, 35) || !wait_all(&p_full[g], (n - 1) & 1, 36)) { ok = false; break; }
+          tc5::fence_after();
+          const uint64_t v = dv + (st ^ 1) * kStageStep;
+          const uint32_t d = base + 256 + g * HD, a = base + g * kArKeys;
+          const int steps = n < mine ? 8 : g == 0 ? last_first : last_steps;
+          // 16 keys: 8 columns of P (every thread's over its own products), 16 rows down V
+          if (steps == 8) {
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                tc5::mma(tmem + uint32_t(g * kArKeys), dq + uint64_t(kb * (kArTile >> 4) + 2 * j),
-                         dk + st * kStageStep + uint64_t(kb * (kArTile >> 4) + 2 * j), idesc_s, (kb > 0 || j > 0) ? 1u : 0u);
-            tc5::commit(&s_full[g]);                               // and O += P_(n-1) V_(n-1) before it
+            for (int j = 0; j < 8; ++j) ar_mma_ts(one, d, a + (SPLIT == 2 ? (j & 3) * 8 + (j >> 2) * 64 : j * 8), v + uint64_t(j * (16 * 128 >> 4)), idesc_o, (n > 1 || j > 0) ? 1u : 0u);
+          } else {
+#pragma unroll 1
+            for (int j = 0; j < steps; ++j) ar_mma_ts(one, d, a + (SPLIT == 2 ? (j & 3) * 8 + (j >> 2) * 64 : j * 8), v + uint64_t(j * (16 * 128 >> 4)), idesc_o, (n > 1 || j > 0) ? 1u : 0u);
           }
         }
-        if (!ok) break;
-        if (n < n_tiles) tc5::commit(&k_free[n % kArStages]);      // tile n of the keys is read,
-        if (n >= 1) tc5::commit(&v_free[(n - 1) % kArStages]);     // and n - 1 of the values
+        if (n < mine) {                                            // S_n, over P_(n-1)
+          if (!wait_all(&k_full[st], (n >> 1) & 1, 37)) { ok = false; break; }
+          tc5::fence_after();
+          const uint64_t q = dq + g * kStageStep, k = dk + st * kStageStep;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              ar_mma_ss(one, base + g * kArKeys, q + uint64_t(kb * (kArTile >> 4) + 2 * j), k + uint64_t(kb * (kArTile >> 4) + 2 * j), idesc_s,
+                        (kb > 0 || j > 0) ? 1u : 0u);
+          ar_commit(one, &s_full[g]);                              // and O += P_(n-1) V_(n-1) before it
+        }
       }
-      tc5::commit(&o_full);
+      if (!ok) break;
+      if (n < tiles) ar_commit(one, &k_free[st]);                  // tile n of the keys is read,
+      if (n >= 1) ar_commit(one, &v_free[st ^ 1]);                 // and n - 1 of the values
     }
-  } else if (!PAGES && warp == 8) {
+    ar_commit(one, &o_full);
+  } else if (!PAGES && warp == kSoftmaxWarps) {
     // ---- prompts: one thread asks for Q, K and V
     const int tail = hi - (j0 + n_tiles - 1) * kArKeys;            // keys of the last tile
     bool ok = true;
@@ -498,11 +621,11 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         if (ok && lane == 0) tc5::mbar_arrive(&v_full[st]);
       }
     }
-  } else if (PAGES && warp >= 8 && warp < 8 + kArKeyWarps + kArValueWarps) {
+  } else if (PAGES && warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kArKeyWarps + kArValueWarps) {
     // ---- pages: codes into operands; four warps the keys, three the values.  A thread asks for its pieces of the next tile behind
     // those of this one.
-    const bool is_k = warp < 8 + kArKeyWarps;
-    const int threads = 32 * (is_k ? kArKeyWarps : kArValueWarps), t = threadIdx.x - (is_k ? 256 : 256 + 32 * kArKeyWarps);
+    const bool is_k = warp < kSoftmaxWarps + kArKeyWarps;
+    const int threads = 32 * (is_k ? kArKeyWarps : kArValueWarps), t = int(threadIdx.x) - 32 * (kSoftmaxWarps + (is_k ? 0 : kArKeyWarps));
     constexpr int kMost = (kArKeys * kPieces + 32 * kArValueWarps - 1) / (32 * kArValueWarps);
     const uint8_t* const codes = is_k ? p.k_codes : p.v_codes;
     unsigned char* const to = is_k ? k_s : v_s;
@@ -519,7 +642,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           held[i] = *reinterpret_cast<const uint4*>(codes + keys.place(key0 + r) * HD + ch * 16);
       }
       of_group = make_float2(0.f, 1.f);
-      if (warp == 8 && lane < kArKeys / 8) {
+      if (warp == kSoftmaxWarps && lane < kArKeys / 8) {
         const int key = max(key0 + lane * 8, lo);
         if (key < min(hi, key0 + lane * 8 + 8)) {
           const size_t at = keys.place(key) / p.block_size;
@@ -532,7 +655,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     for (int n = 0; n < n_tiles; ++n) {
       const int st = n % kArStages;
       if (n >= kArStages && !wait_all(is_k ? &k_free[st] : &v_free[st], ((n / kArStages) & 1) ^ 1, is_k ? 40 : 41)) break;
-      if (warp == 8) {
+      if (warp == kSoftmaxWarps) {
         // (S_(n-2) is complete, so the weights of tile n - 3 are made, and the place of tile n - 4 is free)
         const float log_v = log2f(fmaxf(of_group.y, 1.17549435e-38f));
         if (n == 0) {
@@ -560,111 +683,122 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (lane == 0) tc5::mbar_arrive(is_k ? &k_full[st] : &v_full[st]);
       if (n + 1 < n_tiles) ask(n + 1);
     }
-  } else if (warp < 8 && (warp >> 2) < groups) {
-    // ---- softmax and output: this thread owns row r of its group (lane r of tensor memory)
-    const int g = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+  } else if (warp < kSoftmaxWarps && ((warp >> 2) & 1) < groups) {
+    // ---- softmax and output: one or two threads own row r of their group (lane r of tensor memory).  Two, each with half of a tile's
+    // keys, give a scheduler two warps of a group, whose exponentials, products and conversions run under each other's.
+    const int half = warp >> 3, g = (warp >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane, pair = 1 + (warp & 7);
     const int mine = g == 0 ? n_first : n_tiles, hi_mine = g == 0 ? hi_first : hi;
     const int row = g * kArGroupRows + r, pos = pos0 + row;        // rows beyond rows_here compute and store nothing
     const uint32_t lane_addr = tmem + (uint32_t(quarter * 32) << 16);
-    const uint32_t s_addr = lane_addr + g * kArKeys, o_addr = lane_addr + 256 + g * HD;
+    const uint32_t s_addr = lane_addr + g * kArKeys + half * kSpan, o_addr = lane_addr + 256 + g * HD + half * (HD / SPLIT);
     const int first = first_visible(pos, p.window, 0);
     const int group_pos = pos0 + g * kArGroupRows;                 // of the group's first row
     const int last_first = first_visible(group_pos + kArGroupRows - 1, p.window, 0);
+    float* const mine_told = &told[half][row];
+    const float* const other_told = &told[half ^ (SPLIT - 1)][row];
     bool alive = true;
     ArRow rf{CAP ? p.cap_pre : p.scale_log2, p.scale_log2};
     if constexpr (PAGES) {                                         // q as float16, its largest element between 2^14 and 2^15
       alive = wait_all(&q_full, 0, 42);
-      if (alive) {
-        unsigned char* const at = q_s + g * KB * kArTile + r * 128;
-        float largest = 0.f, bad = 0.f;
+      unsigned char* const at = q_s + g * KB * kArTile + r * 128;
+      float largest = 0.f, bad = 0.f;
 #pragma unroll 4
-        for (int c = 0; c < HD / 8; ++c) {
-          const uint4 u = *reinterpret_cast<const uint4*>(at + (c >> 3) * kArTile + (((c & 7) ^ (r & 7)) * 16));
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 u = *reinterpret_cast<const uint4*>(at + (c >> 3) * kArTile + (((c & 7) ^ (r & 7)) * 16));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = ar_unpack<false>(w[i]);
-            largest = fmaxf(largest, fmaxf(fabsf(f.x), fabsf(f.y)));
-            bad = fmaf(f.x, 0.f, fmaf(f.y, 0.f, bad));             // not-a-number where an element is not finite
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = ar_unpack<false>(w[i]);
+          largest = fmaxf(largest, fmaxf(fabsf(f.x), fabsf(f.y)));
+          bad = fmaf(f.x, 0.f, fmaf(f.y, 0.f, bad));               // not-a-number where an element is not finite
         }
-        // 2^(14 - exponent of the largest), and its reciprocal
-        const int e = min(max(int(__float_as_uint(largest) >> 23), 15), 254);
-        const float up = __uint_as_float(uint32_t(min(127 + 14 + 127 - e, 254)) << 23);
-        rf.factor *= __uint_as_float(uint32_t(254 - min(127 + 14 + 127 - e, 253)) << 23) + bad;
-#pragma unroll 4
-        for (int c = 0; c < HD / 8; ++c) {
-          uint4* const u = reinterpret_cast<uint4*>(at + (c >> 3) * kArTile + (((c & 7) ^ (r & 7)) * 16));
-          uint32_t w[4] = {u->x, u->y, u->z, u->w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = ar_unpack<false>(w[i]);
-            w[i] = ar_pack<true>(f.x * up, f.y * up);
-          }
-          *u = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-        __syncwarp();
-        if (lane == 0) tc5::mbar_arrive(&q_ready);
       }
+      ar_either<SPLIT>(pair, false);                                      // (both have read the row)
+      // 2^(14 - exponent of the largest), and its reciprocal
+      const int e = min(max(int(__float_as_uint(largest) >> 23), 15), 254);
+      const float up = __uint_as_float(uint32_t(268 - e) << 23);
+      rf.factor *= __uint_as_float(uint32_t(e - 14) << 23) + bad;
+#pragma unroll 4
+      for (int c = half * (HD / 8 / SPLIT); c < (half + 1) * (HD / 8 / SPLIT); ++c) {
+        uint4* const u = reinterpret_cast<uint4*>(at + (c >> 3) * kArTile + (((c & 7) ^ (r & 7)) * 16));
+        uint32_t w[4] = {u->x, u->y, u->z, u->w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = ar_unpack<false>(w[i]);
+          w[i] = ar_pack<true>(f.x * up, f.y * up);
+        }
+        *u = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) tc5::mbar_arrive(&q_ready);
     }
-    float m = -INFINITY;                                           // the maximum the row currently scales by
-    bool fresh = true;                                             // some row of the warp has none
-    float l = 0.f;
+    // What the row currently scales by, alike in its two threads: a maximum of its scores.  Prompts begin at zero, which is near enough to
+    // most rows' (weights of bfloat16 are as exact anywhere): their maximum is looked for where weights leave 2^-40 .. 2^20.
+    float m = PAGES ? -INFINITY : 0.f;
+    bool fresh = PAGES;                                            // some row of the warp has none
+    bool settled = PAGES;                                          // the row's was looked for
+    float l = 0.f;                                                 // of this thread's keys
     for (int n = 0; n < mine; ++n) {
       alive = alive && wait_all(&s_full[g], n & 1, 43) && (!PAGES || wait_all(&sc_full[n % kArRing], (n / kArRing) & 1, 44));
-      if (!alive) break;
       tc5::fence_after();
-      const ArScales* sc = scales + (n % kArRing) * (kArKeys / 8);
-      const int key0 = (j0 + n) * kArKeys;
-      // the keys of this tile that the row may see: [a, b) relative to it; masks only where some row of the group needs one
+      const ArScales* sc = scales + (n % kArRing) * (kArKeys / 8) + half * (kSpan / 8);
+      const int key0 = (j0 + n) * kArKeys + half * kSpan;
+      // the keys of this half of the tile that the row may see: [a, b) relative to it; masks only where some row of the group needs one
       const int a = max(first, lo) - key0, b = min(pos + 1, hi) - key0;
-      const bool full = key0 + kArKeys - 1 <= group_pos && key0 >= last_first;
-      const int chunks = (min(kArKeys, hi_mine - key0) + 31) / 32;
-      float sum = 0.f;
+      const bool full = key0 + kSpan - 1 <= group_pos && key0 >= last_first;
+      const int chunks = min(max(hi_mine - key0 + 31, 0) / 32, CHUNKS);
+      uint32_t packed[16 * CHUNKS];
+      float weights = 0.f, sum = 0.f;
+      if (alive && !fresh && chunks > 0) {
+        const float m_use = (m == -INFINITY) ? 0.f : m;
+        if (full) ar_tile<CHUNKS, CAP, PAGES, false, false>(s_addr, sc, packed, rf, m_use, a, b, chunks, weights, sum);
+        else ar_tile<CHUNKS, CAP, PAGES, true, false>(s_addr, sc, packed, rf, m_use, a, b, chunks, weights, sum);
+      }
+      // (a warp that gave up says so here, and both leave)
+      const bool small = !settled && max(a, 0) < min(b, kSpan) && l + weights < kArLeast;
+      if (ar_either<SPLIT>(pair, fresh || small || weights > (PAGES ? kArMost : kArMostPrompt) || !alive)) {      // hardly ever
+        const float m_use = (m == -INFINITY) ? 0.f : m;
+        float mx = -INFINITY;
 #pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
-        uint32_t s[32], packed[16];
-        tc5::ld32(s_addr + uint32_t(c * 32), s);
-        ar_wait32(s);
-        const ArScales* scc = sc + c * 4;
-        const int ac = a - c * 32, bc = b - c * 32;
-        float part, weights;
-        for (int pass = 0;; ++pass) {
-          const float m_use = (m == -INFINITY) ? 0.f : m;
-          bool renew = fresh;                                      // some row of the warp has seen nothing yet
-          if (!fresh) {
-            if (pass > 0) ar_exponentials<CAP, PAGES, true, true>(s, scc, packed, rf, m_use, ac, bc, weights, part);
-            else if (full) ar_exponentials<CAP, PAGES, false, false>(s, scc, packed, rf, m_use, ac, bc, weights, part);
-            else ar_exponentials<CAP, PAGES, true, false>(s, scc, packed, rf, m_use, ac, bc, weights, part);
-            renew = pass == 0 && weights > kArMost;                // (behind a renewal a part is at most 32)
-          }
-          if (!__any_sync(0xffffffffu, renew)) break;
-          const float mx = ar_largest<CAP, PAGES>(s, scc, rf, m_use, ac, bc);
-          const bool grows = renew && mx != -INFINITY && (m == -INFINITY || mx > 0.f);
-          const float alpha = grows && m != -INFINITY ? ar_exp2(-mx) : 1.f;
-          if (grows) m = m_use + mx;
-          sum *= alpha;
-          l *= alpha;
-          if (__any_sync(0xffffffffu, alpha != 1.f)) ar_rescale<HD, PAGES>(o_addr, n > 0, s_addr, c, alpha);
-          if (fresh) {
-            ar_exponentials<CAP, PAGES, true, true>(s, scc, packed, rf, (m == -INFINITY) ? 0.f : m, ac, bc, weights, part);
-            fresh = __any_sync(0xffffffffu, m == -INFINITY);
-            break;
-          }
+        for (int c = 0; alive && c < chunks; ++c) {
+          uint32_t s[32];
+          tc5::ld32(s_addr + uint32_t(c * 32), s);
+          ar_wait32(s);
+          mx = fmaxf(mx, ar_largest<CAP, PAGES>(s, sc + c * 4, rf, m_use, ar_bits(a - c * 32, b - c * 32)));
         }
-        sum += part;
-        ar_st16(s_addr + uint32_t(c * 16), packed);                // over products that are read
+        if (!settled && l >= kArLeast) mx = fmaxf(mx, 0.f);        // (what has weight already is not scaled up)
+        *mine_told = mx;
+        if (lane == 0) left[warp & 7][half] = !alive;
+        ar_either<SPLIT>(pair, false);
+        if (left[warp & 7][0] | left[warp & 7][1]) { alive = false; break; }
+        mx = fmaxf(mx, *other_told);
+        // (a reference that was not looked for may also come down, where nothing of weight has been added)
+        const bool grows = mx != -INFINITY && (m == -INFINITY || mx > 0.f || !settled);
+        const float alpha = grows && m != -INFINITY ? ar_exp2(fminf(-mx, 100.f)) : 1.f;
+        settled = settled || mx != -INFINITY;
+        if (grows) m = m_use + mx;
+        l *= alpha;
+        if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) ar_rescale(o_addr, HD / SPLIT, alpha);
+        if (chunks > 0) ar_tile<CHUNKS, CAP, PAGES, true, true>(s_addr, sc, packed, rf, (m == -INFINITY) ? 0.f : m, a, b, chunks, weights, sum);
+        fresh = __any_sync(0xffffffffu, m == -INFINITY);           // some row of the warp has seen nothing yet
       }
       l += sum;
+      if (chunks > 0) {                                            // over products that are read
+        tc5::st32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(packed));
+        if constexpr (SPLIT == 1) tc5::st32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(packed + 32));
+      }
       tc5::st_wait();
       tc5::fence_before();
       __syncwarp();
       if (lane == 0) tc5::mbar_arrive(&p_full[g]);
     }
     if (alive) alive = wait_all(&o_full, 0, 45);
+    *mine_told = l;
+    const bool both_alive = !ar_either<SPLIT>(pair, !alive);
     tc5::fence_after();
-    if (alive) {
+    if (both_alive) {
+      if constexpr (SPLIT == 2) l = half == 0 ? l + *other_told : *other_told + l;
       if (p.sink && m != -INFINITY) l += ar_exp2(p.sink[head] * 1.4426950408889634f - m);
       const bool none = l == 0.f;                                  // no key: zeros
       float inv = none ? 0.f : 1.f / l;
@@ -673,11 +807,12 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       bf16* dst = p.out + size_t(q_start + q0 + row) * p.out_stride + size_t(head) * p.hd;
       float sick = 0.f;
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
+      for (int c = 0; c < HD / 32 / SPLIT; ++c) {
         uint32_t ov[32];
         tc5::ld32(o_addr + uint32_t(c * 32), ov);                  // (all lanes of the warp take part in the load)
         ar_wait32(ov);
         if (row < rows_here) {
+          const int d0 = half * (HD / SPLIT) + c * 32;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint4 h;
@@ -688,19 +823,23 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
               sick = fmaf(x, 0.f, fmaf(y, 0.f, sick));
               hw[i] = ar_pack<false>(x, y);
             }
-            if (c * 32 + e * 8 < p.hd) *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = h;
+            if (d0 + e * 8 < p.hd) *reinterpret_cast<uint4*>(dst + d0 + e * 8) = h;
           }
         }
       }
-      // (the keys that the products of this row's group had: whole tiles, up to the last one's steps of 16 and the block's own)
-      uint32_t odd = __ballot_sync(0xffffffffu, sick != 0.f);
-      const int from = PAGES ? lo : j0 * kArKeys, to = min(hi, (hi_mine + 15) / 16 * 16);
-      while (odd) {
-        const int who = __ffs(odd) - 1;
-        odd &= odd - 1;
-        const int its = __shfl_sync(0xffffffffu, row, who);
-        ar_again<HD, CAP, PAGES>(p, seq, q_start, head, q_start + q0 + its, pos0 + its, first_visible(pos0 + its, p.window, 0), from, to);
-        __syncwarp();
+      if (ar_either<SPLIT>(pair, sick != 0.f)) {                          // (and every element of the rows is written)
+        *mine_told = sick;
+        ar_either<SPLIT>(pair, false);
+        // (the keys that the products of this row's group had: whole tiles, up to the last one's steps of 16 and the block's own)
+        uint32_t odd = half == 0 ? __ballot_sync(0xffffffffu, sick != 0.f || *other_told != 0.f) : 0u;
+        const int from = PAGES ? lo : j0 * kArKeys, to = min(hi, (hi_mine + 15) / 16 * 16);
+        while (odd) {
+          const int who = __ffs(odd) - 1;
+          odd &= odd - 1;
+          const int its = __shfl_sync(0xffffffffu, row, who);
+          ar_again<HD, CAP, PAGES>(p, seq, q_start, head, q_start + q0 + its, pos0 + its, first_visible(pos0 + its, p.window, 0), from, to);
+          __syncwarp();
+        }
       }
     }
     tc5::fence_before();
@@ -745,6 +884,12 @@ int rows_map(CUtensorMap* map, const void* base, long long rows, int heads, int 
   return r == CUDA_SUCCESS ? 0 : 20000 + int(r);
 }
 
+// Blocks of 256 rows that `tiles` tiles of `portions` requests are at most: of each the last block may be of one tile.
+int rows_blocks(int tiles, int portions) {
+  const long long n = ((long long)tiles + 3ll * portions) / 4;
+  return n < tiles ? int(n) : tiles;
+}
+
 bool aligned16(const void* at, long long stride) { return (reinterpret_cast<uintptr_t>(at) & 15) == 0 && stride % 8 == 0; }
 
 }  // namespace
@@ -752,15 +897,15 @@ bool aligned16(const void* at, long long stride) { return (reinterpret_cast<uint
 
 using namespace kvcm;
 
-// q: [total_rows, >= nh * hd]; tiles of 64 query rows as the batch builder makes them (tile_seq < 0: no tile); hd 64 or 128, block_size a
-// multiple of 8.
+// q: [total_rows, >= nh * hd]; tiles of 64 query rows as the batch builder makes them (tile_seq < 0: no tile), of at most `portions` requests;
+// hd 64 or 128, block_size a multiple of 8.
 KVCM_API int kvcm_attention_prefill_q8_bf16(const void* q, long long q_stride, int total_rows, void* out, long long out_stride,
                                             const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale,
                                             int num_pages, const int* block_tables, int max_blocks, const int* tile_seq, const int* tile_q0,
-                                            const int* seq_q_start, const int* seq_q_len, const int* seq_ctx_len, int tiles, int nh, int nkv,
-                                            int hd, int block_size, float scale, int window, float softcap, const float* sink,
-                                            void* stream) {
-  if (tiles <= 0) return 0;
+                                            const int* seq_q_start, const int* seq_q_len, const int* seq_ctx_len, int tiles, int portions,
+                                            int nh, int nkv, int hd, int block_size, float scale, int window, float softcap,
+                                            const float* sink, void* stream) {
+  if (tiles <= 0 || portions <= 0) return 0;
   if ((hd != 64 && hd != 128) || nkv <= 0 || nh <= 0 || nh % nkv || block_size <= 0 || block_size % 8 || block_size > q8::kMaxBlock ||
       max_blocks <= 0 || num_pages <= 0 || total_rows <= 0 || tiles > 65535)
     return KVCM_ERR_UNSUPPORTED;
@@ -782,15 +927,17 @@ KVCM_API int kvcm_attention_prefill_q8_bf16(const void* q, long long q_stride, i
   if (p.error == nullptr) return KVCM_ERR_UNSUPPORTED;
   p.log2_block = -1;
   for (int b = 0; b < 31; ++b) if ((1 << b) == block_size) p.log2_block = b;
-  return launch_rows<true>(mq, mq, mq, p, dim3(nh, tiles), (cudaStream_t)stream);
+  p.blocks = rows_blocks(tiles, portions);
+  return launch_rows<true>(mq, mq, mq, p, dim3(nh, p.blocks), (cudaStream_t)stream);
 }
 
-// q, k and v: rows of the prompts, one behind another; entries [0, singles) are prompts of one row, tiles name the others'.
+// q, k and v: rows of the prompts, one behind another; entries [0, singles) are prompts of one row, tiles name those of at most `portions`
+// others.
 KVCM_API int kvcm_prompt_attention_bf16(const void* q, long long q_stride, const void* k, long long k_stride, const void* v, long long v_stride,
                                         int total_rows, void* out, long long out_stride, const int* tile_seq, const int* tile_q0,
-                                        const int* seq_q_start, const int* seq_q_len, int tiles, int singles, int nh, int nkv, int hd,
+                                        const int* seq_q_start, const int* seq_q_len, int tiles, int portions, int singles, int nh, int nkv, int hd,
                                         float scale, int window, float softcap, const float* sink, void* stream) {
-  if (tiles < 0 || singles < 0 || (long long)tiles + singles > 65535) return KVCM_ERR_UNSUPPORTED;
+  if (tiles < 0 || portions < 0 || singles < 0 || (long long)tiles + singles > 65535) return KVCM_ERR_UNSUPPORTED;
   if (tiles + singles == 0) return 0;
   if (hd <= 0 || hd % 8 || hd > 128 || nkv <= 0 || nh <= 0 || nh % nkv || total_rows <= 0) return KVCM_ERR_UNSUPPORTED;
   if (!aligned16(q, q_stride) || !aligned16(k, k_stride) || !aligned16(v, v_stride) || !aligned16(out, out_stride)) return KVCM_ERR_UNSUPPORTED;
@@ -809,7 +956,8 @@ KVCM_API int kvcm_prompt_attention_bf16(const void* q, long long q_stride, const
   p.sink = sink;
   p.error = const_cast<int*>(kvcm_attention_tcgen05_error_address());
   if (p.error == nullptr) return KVCM_ERR_UNSUPPORTED;
-  return launch_rows<false>(mq, mk, mv, p, dim3(nh, tiles + singles), (cudaStream_t)stream);
+  p.blocks = rows_blocks(tiles, portions);
+  return p.blocks + singles == 0 ? 0 : launch_rows<false>(mq, mk, mv, p, dim3(nh, p.blocks + singles), (cudaStream_t)stream);
 }
 
 KVCM_PACKED(kvcm_attention_prefill_q8_bf16)

@@ -935,8 +935,8 @@ _STORE_Q8 = {s: _Entry("kvcm_rope_cache_q8_" + s, "plpiipppppp" + "liiiiii") for
 _READ_Q8 = {s: _Entry("kvcm_read_cache_q8_" + s, "ppppp" + "pp" + "lliiiii") for s in ("f32", "bf16")}
 _PLAIN_Q8 = {s: _Entry("kvcm_attention_plain_q8_" + s, "plplpppp" + "ipipp" + "iiiii" + "fifp") for s in ("f32", "bf16")}
 _PLAIN_PROMPT = {s: _Entry("kvcm_prompt_attention_plain_" + s, "plplplpl" + "pppp" + "iii" + "iii" + "fifp") for s in ("f32", "bf16")}
-_PREFILL_Q8 = _Entry("kvcm_attention_prefill_q8_bf16", "plipl" + "ppppipi" + "ppppp" + "iiiii" + "fifp")
-_PROMPT = _Entry("kvcm_prompt_attention_bf16", "plplpl" + "ipl" + "pppp" + "iiiii" + "fifp")
+_PREFILL_Q8 = _Entry("kvcm_attention_prefill_q8_bf16", "plipl" + "ppppipi" + "ppppp" + "iiiiii" + "fifp")
+_PROMPT = _Entry("kvcm_prompt_attention_bf16", "plplpl" + "ipl" + "pppp" + "iiiiii" + "fifp")
 _DECODE_Q8 = _Entry("kvcm_attention_decode_q8_bf16", "plplpppp" + "ipip" + "iiiii" + "fiiiipifp")
 _UNPACK_Q8 = _Entry("kvcm_unpack_pages_q8_bf16", "pppp" + "pi" + "pppp" + "iiiiiiii")
 
@@ -1165,7 +1165,7 @@ def attention_prefill_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
         rc = _PREFILL_Q8(device, q.data_ptr(), q.stride(0), q.shape[0], out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
                          k_scale.data_ptr(), v_scale.data_ptr(), k_cache.shape[0], block_tables.data_ptr(), block_tables.shape[1],
                          ctx.tile_seq.data_ptr(), ctx.tile_q0.data_ptr(), ctx.seq_q_start.data_ptr(), ctx.seq_q_len.data_ptr(),
-                         ctx.seq_ctx_len.data_ptr(), ctx.prefill_tiles, nh, nkv, hd, block_size, scale, window, softcap, _at(sink))
+                         ctx.seq_ctx_len.data_ptr(), ctx.prefill_tiles, seqs, nh, nkv, hd, block_size, scale, window, softcap, _at(sink))
         _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
         return
     blocks = min(block_tables.shape[1], (ctx.max_ctx + block_size - 1) // block_size)
@@ -1218,7 +1218,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
             and (q.stride(0) | k.stride(0) | v.stride(0) | out.stride(0)) % 8 == 0:
         rc = _PROMPT(device, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), T, out.data_ptr(), out.stride(0),
                      ctx.tile_seq.data_ptr(), ctx.tile_q0.data_ptr(), ctx.seq_q_start.data_ptr(), ctx.seq_q_len.data_ptr(), ctx.prefill_tiles,
-                     ctx.decode_seqs, nh, nkv, hd, scale, window, softcap, _at(sink))
+                     S - ctx.decode_seqs, ctx.decode_seqs, nh, nkv, hd, scale, window, softcap, _at(sink))
         _launched(rc, name, "(hd={}, nh={}, nkv={})", hd, nh, nkv)
         return
     rc = _PLAIN_PROMPT[_SUFFIX[q.dtype]](

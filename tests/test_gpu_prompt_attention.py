@@ -124,6 +124,24 @@ def test_what_a_row_does_not_see_may_be_anything(hd, window):
         assert bool(((got - want).abs() <= room)[clear].all())
 
 
+@pytest.mark.parametrize("levels", [(0.0, -90.0), (-90.0, 0.0), (-60.0, -200.0), (30.0, 5.0), (0.0, 250.0), (-200.0, -200.0)])
+@pytest.mark.parametrize("at", [1, 70, 150, 300])
+def test_scores_far_from_zero(levels, at):
+    """Scores of about one level up to row ``at`` and another behind it: references that have to be looked for, and such that must not come down."""
+    nh, nkv, hd = 2, 1, 64
+    wide = 8.0                                                      # q is (8, noise), k (level, noise): a score is about the level
+
+    def shape(qkv, starts):
+        a = starts[0]
+        qkv[:, :nh * hd:hd] = wide
+        n = qkv.shape[0]
+        level = torch.where(torch.arange(n) < a + at, torch.tensor(levels[0]), torch.tensor(levels[1]))
+        qkv[:, nh * hd] = (level * hd ** 0.5 / wide).to(qkv.dtype)
+    for a, n, got, want, room in check([420], nh, nkv, hd, q_size=0.3, poison=shape, behind=0):
+        far = (got - want).abs()
+        assert bool((far <= room).all()), float((far / room).max())
+
+
 def test_agrees_with_pages():
     """The same rows through bfloat16 pages: as far apart as both may be from the definition."""
     nh, nkv, hd, B, n = 4, 2, 128, 16, 333
