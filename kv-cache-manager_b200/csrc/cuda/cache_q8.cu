@@ -8,8 +8,8 @@
 // not-a-number and do not enter the maximum.
 //
 // Rows of one page stand next to each other in a step, so a page's rows are a run of rows.  One warp takes a run and one KV head:
-// it keeps the run's rows in registers (up to four rounds of as many rows as a warp has lanes for), finds their maximum by
-// shuffles, brings the page to its scale where that grows, and writes.  Runs longer than that are read a second time.  A lane has
+// it finds the rows' maximum by shuffles, brings the page to its scale where that grows, and reads the rows a second time to write
+// them (out of the nearest cache; the first as many rows as a warp has lanes for stay in registers).  A lane has
 // two words of eight elements that turn with one another, so that angles are read once for both and nothing is exchanged.
 #include "packed.cuh"
 #include "pdl.cuh"
@@ -19,7 +19,6 @@ namespace kvcm {
 
 constexpr int kQ8Threads = 256;
 constexpr int kQ8Warps = kQ8Threads / 32;
-constexpr int kQ8Keep = 4;                         // rounds of rows that stay in registers
 constexpr float kQ8Finite = 3.402823466e38f;
 
 namespace {
@@ -111,18 +110,25 @@ __device__ __forceinline__ void q8_load(const StoreQ8Params& p, const Q8Words& w
   }
 }
 
-// Eight elements as codes.  (x * 0 is zero, or not-a-number where x is not finite.)
-__device__ __forceinline__ uint2 q8_codes(const float (&x)[8], float per) {
+// Eight elements as codes; not-a-number of what is not finite (`finite`: everything is).
+__device__ __forceinline__ uint2 q8_codes(const float (&x)[8], float per, bool finite) {
   uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) c[i] = q8::codes2(fmaf(x[2 * i], 0.f, x[2 * i] * per), fmaf(x[2 * i + 1], 0.f, x[2 * i + 1] * per));
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i] * per, b = x[2 * i + 1] * per;
+    if (!finite) {                                                 // (x * 0 is zero, or not-a-number)
+      a = fmaf(x[2 * i], 0.f, a);
+      b = fmaf(x[2 * i + 1], 0.f, b);
+    }
+    c[i] = q8::codes2(a, b);
+  }
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
 
 // Blocks: windows of W rows x groups of eight warps.  A warp has one q head of the window's rows (W == 1: of as many heads as it has
 // lanes for), or one KV head of the runs that begin in the window.
 template <typename T, int W>
-__global__ void __launch_bounds__(kQ8Threads) store_q8_kernel(StoreQ8Params p) {
+__global__ void __launch_bounds__(kQ8Threads, 4) store_q8_kernel(StoreQ8Params p) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, unit = blockIdx.y * kQ8Warps + (threadIdx.x >> 5);
@@ -132,6 +138,7 @@ __global__ void __launch_bounds__(kQ8Threads) store_q8_kernel(StoreQ8Params p) {
   const int q_units = W == 1 ? (p.nh + R - 1) / R : p.nh;
   if (unit < q_units) {
     const int stop = min(w0 + W, p.rows);
+#pragma unroll 2
     for (int r = w0; r < stop; r += W == 1 ? 1 : R) {
       const int row = W == 1 ? r : r + group, head = W == 1 ? unit * R + group : unit;
       const bool there = row < stop && head < p.nh;
@@ -156,6 +163,8 @@ __global__ void __launch_bounds__(kQ8Threads) store_q8_kernel(StoreQ8Params p) {
     off = slot - page * p.block_size;
     return page < p.num_pages ? page : -1;
   };
+  float ahead[2][8];                                               // the first rows of a run; where a window is one row, asked for at once
+  if (W == 1) q8_load<T>(p, words, w0 + group, head, w0 + group < p.rows, ahead);
   int off;
   const int page = place(w0 - 1 + lane, off);
   const int before = __shfl_up_sync(0xffffffffu, page, 1);
@@ -179,21 +188,37 @@ __global__ void __launch_bounds__(kQ8Threads) store_q8_kernel(StoreQ8Params p) {
       more = k == 32;
     }
     // ---- its largest element
-    float x[kQ8Keep][2][8], most = 0.f;
+    // (the maximum passes over not-a-number; `sick` is that from the first element on that is not finite)
+    float most = 0.f, sick = 0.f;
     auto largest = [&](const float (&v)[2][8]) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) most = fabsf(v[k][e]) <= kQ8Finite ? fmaxf(most, fabsf(v[k][e])) : most;
+        for (int e = 0; e < 8; ++e) {
+          most = fmaxf(most, fabsf(v[k][e]));
+          sick = fmaf(v[k][e], 0.f, sick);
+        }
     };
-#pragma unroll
-    for (int it = 0; it < kQ8Keep; ++it) q8_load<T>(p, words, r0 + it * R + group, head, it * R + group < n, x[it]);
-#pragma unroll
-    for (int it = 0; it < kQ8Keep; ++it) largest(x[it]);
-    for (int r = kQ8Keep * R + group; r - group < n; r += R) {
+    if (W != 1) q8_load<T>(p, words, r0 + group, head, group < n, ahead);
+    if (group < n) largest(ahead);
+#pragma unroll 1
+    for (int r = R + group; r - group < n; r += R) {
       float v[2][8];
       q8_load<T>(p, words, r0 + r, head, r < n, v);
       largest(v);
+    }
+    const bool finite = !__any_sync(0xffffffffu, sick != 0.f);
+    if (!finite) {                                                 // of the finite elements alone
+      most = 0.f;
+#pragma unroll 1
+      for (int r = group; r - group < n; r += R) {
+        float v[2][8];
+        q8_load<T>(p, words, r0 + r, head, r < n, v);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) most = fabsf(v[k][e]) <= kQ8Finite ? fmaxf(most, fabsf(v[k][e])) : most;
+      }
     }
     most = warp_max(most);
     const float need = q8::scale_for(most), scale = !anew && old > need ? old : need, per = __frcp_rn(scale);
@@ -207,7 +232,7 @@ __global__ void __launch_bounds__(kQ8Threads) store_q8_kernel(StoreQ8Params p) {
         float v[8];
         q8::values4(u.x, ratio, v);
         q8::values4(u.y, ratio, v + 4);
-        *word = q8_codes(v, 1.f);
+        *word = q8_codes(v, 1.f, true);                            // (codes of not-a-number stay)
       }
       __syncwarp();
     }
@@ -219,11 +244,11 @@ __global__ void __launch_bounds__(kQ8Threads) store_q8_kernel(StoreQ8Params p) {
       uint8_t* to = base + size_t(slot - here * p.block_size) * p.hd;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        if (words.live[k]) *reinterpret_cast<uint2*>(to + words.at[k] * 8) = q8_codes(v[k], per);
+        if (words.live[k]) *reinterpret_cast<uint2*>(to + words.at[k] * 8) = q8_codes(v[k], per, finite);
     };
-#pragma unroll
-    for (int it = 0; it < kQ8Keep; ++it) write(it * R + group, x[it]);
-    for (int r = kQ8Keep * R + group; r < n; r += R) {
+    write(group, ahead);
+#pragma unroll 1
+    for (int r = R + group; r < n; r += R) {
       float v[2][8];
       q8_load<T>(p, words, r0 + r, head, true, v);
       write(r, v);
@@ -321,7 +346,8 @@ int launch_store_q8_as(const StoreQ8Params& p, cudaStream_t s) {
 }
 template <typename T>
 int launch_store_q8(const StoreQ8Params& p, cudaStream_t s) {
-  return p.rows <= 512 ? launch_store_q8_as<T, 1>(p, s) : launch_store_q8_as<T, 16>(p, s);
+  // Few rows: a window each, or a warp would take several requests' runs one behind another; many: windows as long as a usual page.
+  return p.rows <= 512 ? launch_store_q8_as<T, 1>(p, s) : p.rows <= 2048 ? launch_store_q8_as<T, 8>(p, s) : launch_store_q8_as<T, 16>(p, s);
 }
 
 }  // namespace
