@@ -86,12 +86,23 @@ struct Team {
   }
   // (between two barriers, so that nobody changes it or leaves)
   __device__ __forceinline__ unsigned long long first_wrong() {
-    unsigned long long w = *wrong;
-    for (int r = 0; r < blocks && blocks > 1; ++r) {
-      const unsigned long long o = *cg::this_cluster().map_shared_rank(wrong, r);
-      w = o < w ? o : w;
+    if (blocks == 1) return *wrong;
+    const int lane = threadIdx.x & 31;                             // (a lane a block: one trip)
+    unsigned long long w = lane < blocks ? *cg::this_cluster().map_shared_rank(wrong, lane) : ~0ull;
+#pragma unroll
+    for (int o = 1; o < kPgMaxBlocks; o *= 2) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, w, o);
+      w = other < w ? other : w;
     }
-    return w;
+    return __shfl_sync(0xffffffffu, w, 0);
+  }
+  // The sum of a number of every block, and of the blocks before this one.
+  __device__ __forceinline__ int sum(int* of_block, int& before) {
+    if (blocks == 1) { before = 0; return *of_block; }
+    const int lane = threadIdx.x & 31;
+    const int up = warp_scan(lane < blocks ? *cg::this_cluster().map_shared_rank(of_block, lane) : 0);
+    before = rank == 0 ? 0 : __shfl_sync(0xffffffffu, up, rank - 1);
+    return __shfl_sync(0xffffffffu, up, 31);
   }
 };
 
@@ -270,11 +281,9 @@ __global__ void __launch_bounds__(kPgThreads) release_requests_kernel(ReleasePar
     if (tid == 0) freed_here = total;
     team.sync();
     bad = team.first_wrong();
-    for (int r = 0; r < team.blocks; ++r) {
-      const int n = team.blocks > 1 ? *cg::this_cluster().map_shared_rank(&freed_here, r) : freed_here;
-      if (r < team.rank) at += n;
-      freed += n;
-    }
+    int before;
+    freed = team.sum(&freed_here, before);
+    at += before;
     if (bad == ~0ull && freed > s.stack - count) bad = (unsigned long long)kPgStack << 32 | unsigned(count + freed);
     team.sync();                                   // everybody knows, and has read who holds what
     if (bad == ~0ull) {
@@ -354,13 +363,11 @@ __global__ void __launch_bounds__(kPgThreads) compact_pages_kernel(CompactParams
   }
   team.sync();
   const unsigned long long bad = team.first_wrong();
-  int moved = 0;
-  for (int r = 0; r < team.blocks; ++r) {
-    const int h = team.blocks > 1 ? *cg::this_cluster().map_shared_rank(&holes_here, r) : holes_here;
-    const int m = team.blocks > 1 ? *cg::this_cluster().map_shared_rank(&movers_here, r) : movers_here;
-    if (r < team.rank) { hole_at += h; mover_at += m; }
-    moved += m;
-  }
+  int before;
+  team.sum(&holes_here, before);
+  hole_at += before;
+  const int moved = team.sum(&movers_here, before);
+  mover_at += before;
   if (bad == ~0ull)
     for (int i = i0; i < i1; ++i) {
       const bool is_free = __ldcg(&p.map[i]) < 0;
@@ -469,8 +476,8 @@ static_assert(kPgMaxEntries * 4 + kPgMaxSeqs / 8 <= 47 * 1024, "the entries' arr
 
 template <typename Params>
 int launch_cluster(void (*kernel)(Params), const Params& p, long long work, size_t smem, cudaStream_t s) {
-  // one block for little work (no cluster barrier), up to eight for much
-  long long blocks = (work + 2 * kPgThreads - 1) / (2 * kPgThreads);
+  // one block for little work (no cluster barrier), up to eight for much: a request's pages are a warp's, a round of them three trips to memory
+  long long blocks = (work + kPgThreads - 1) / kPgThreads;
   blocks = blocks < 1 ? 1 : blocks > kPgMaxBlocks ? kPgMaxBlocks : blocks;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(blocks));
