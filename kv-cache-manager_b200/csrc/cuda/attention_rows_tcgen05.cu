@@ -126,6 +126,12 @@ __device__ __forceinline__ void ar_st16(uint32_t taddr, const uint32_t (&v)[16])
                : "memory");
 }
 // Waits for the loads of tensor memory that the thread has asked for; `v` is one of them (nothing of it is used before).
+__device__ __forceinline__ void ar_wait16(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :: "memory");
+}
 __device__ __forceinline__ void ar_wait32(uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;\n"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
@@ -192,14 +198,14 @@ __device__ __forceinline__ float2 ar_scores(uint32_t s0, uint32_t s1, float fact
   else return ar_fma2(s, make_float2(factor, factor), make_float2(add, add));
 }
 
-// 32 products of a row into weights, added to `w2`, and probabilities, added to `l2` (pages).  MASK: only the `seen` of the 32 count.
+// N products of a row into weights, added to `w2`, and probabilities, added to `l2` (pages).  MASK: only the `seen` of them count.
 // AGAIN: the maximum is known, so nothing is above 2^12 but what scores of 2^24 and more are rounded by.
-template <bool CAP, bool PAGES, bool MASK, bool AGAIN, bool SMALL>
-__device__ __forceinline__ void ar_exponentials(const uint32_t (&s)[32], const ArScales* sc, uint32_t* packed, const ArRow& row, float m,
+template <bool CAP, bool PAGES, bool MASK, bool AGAIN, bool SMALL, int N>
+__device__ __forceinline__ void ar_exponentials(const uint32_t (&s)[N], const ArScales* sc, uint32_t* packed, const ArRow& row, float m,
                                                 uint32_t seen, float2& w2, float2& l2) {
   if constexpr (MASK) asm volatile("" : "+r"(seen));               // (its bits are looked at here, not ahead of the branches before)
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < N / 8; ++j) {
     float factor = row.factor, add = -m, out = 1.f;
     if constexpr (PAGES) {
       const float4 f = *reinterpret_cast<const float4*>(sc + j);
@@ -234,11 +240,11 @@ __device__ __forceinline__ uint32_t ar_bits(int a, int b) {
 }
 
 // Whether the factor brings all of the warp's products into [-1, 1].
-template <bool PAGES>
-__device__ __forceinline__ bool ar_small(const uint32_t (&s)[32], const ArScales* sc, float row_factor) {
+template <bool PAGES, int N>
+__device__ __forceinline__ bool ar_small(const uint32_t (&s)[N], const ArScales* sc, float row_factor) {
   float largest = 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < N / 8; ++j) {
     const float factor = PAGES ? row_factor * sc[j].key : row_factor;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -250,24 +256,47 @@ __device__ __forceinline__ bool ar_small(const uint32_t (&s)[32], const ArScales
   return !__any_sync(0xffffffffu, largest > 1.f);
 }
 
-// A thread's products of a tile into weights, two to a register.  Of `chunks` 32.
+// A thread's products of a tile into weights, two to a register.  Of `chunks` 32.  A thread with all of a row's products takes them by
+// 16, the next ones under way while 16 are worked on; of two, which run under each other, each has the registers for 32 at once.
 template <int CHUNKS, bool CAP, bool PAGES, bool MASK, bool AGAIN>
 __device__ __forceinline__ void ar_tile(uint32_t s_addr, const ArScales* sc, uint32_t (&packed)[16 * CHUNKS], const ArRow& row, float m, int a, int b,
                                         int chunks, float& weights, float& sum) {
-  uint32_t s[32];
   float2 w2 = make_float2(0.f, 0.f), l2 = make_float2(0.f, 0.f);
+  if constexpr (CHUNKS == 4) {
+    uint32_t s[2][16];
+    ar_ld16(s_addr, s[0]);
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    if (!MASK || c < chunks) {
-      tc5::ld32(s_addr + uint32_t(c * 32), s);
-      ar_wait32(s);
-      if (CAP && ar_small<PAGES>(s, sc + c * 4, row.factor))
-        ar_exponentials<CAP, PAGES, MASK, AGAIN, true>(s, sc + c * 4, packed + c * 16, row, m, MASK ? ar_bits(a - c * 32, b - c * 32) : 0u, w2, l2);
+    for (int c = 0; c < 8; ++c) {
+      if (MASK && c >= 2 * chunks) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) packed[c * 8 + i] = 0u;
+        continue;
+      }
+      ar_wait16(s[c & 1]);
+      if (c < 7) ar_ld16(s_addr + uint32_t(c * 16 + 16), s[(c + 1) & 1]);
+      const uint32_t seen = MASK ? ar_bits(a - c * 16, b - c * 16) : 0u;
+      if (CAP && ar_small<PAGES>(s[c & 1], sc + c * 2, row.factor))
+        ar_exponentials<CAP, PAGES, MASK, AGAIN, true>(s[c & 1], sc + c * 2, packed + c * 8, row, m, seen, w2, l2);
       else
-        ar_exponentials<CAP, PAGES, MASK, AGAIN, false>(s, sc + c * 4, packed + c * 16, row, m, MASK ? ar_bits(a - c * 32, b - c * 32) : 0u, w2, l2);
-    } else {
+        ar_exponentials<CAP, PAGES, MASK, AGAIN, false>(s[c & 1], sc + c * 2, packed + c * 8, row, m, seen, w2, l2);
+    }
+    if (MASK) tc5::ld_wait();
+  } else {
+    uint32_t s[32];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) packed[c * 16 + i] = 0u;
+    for (int c = 0; c < CHUNKS; ++c) {
+      if (!MASK || c < chunks) {
+        tc5::ld32(s_addr + uint32_t(c * 32), s);
+        ar_wait32(s);
+        const uint32_t seen = MASK ? ar_bits(a - c * 32, b - c * 32) : 0u;
+        if (CAP && ar_small<PAGES>(s, sc + c * 4, row.factor))
+          ar_exponentials<CAP, PAGES, MASK, AGAIN, true>(s, sc + c * 4, packed + c * 16, row, m, seen, w2, l2);
+        else
+          ar_exponentials<CAP, PAGES, MASK, AGAIN, false>(s, sc + c * 4, packed + c * 16, row, m, seen, w2, l2);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) packed[c * 16 + i] = 0u;
+      }
     }
   }
   weights = w2.x + w2.y;
@@ -423,6 +452,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   __shared__ uint32_t tmem_base;
   __shared__ float told[SPLIT][kArRows];                           // what the threads of a row tell each other
   __shared__ int left[8][2];                                       // that a warp gave up
+  __shared__ size_t group_at[2][2][PAGES ? kArKeys / 8 : 1];       // pages: where keys, and values, of a tile are, by eights
   __shared__ float value_base;                                     // log2 of the value scale that weights are relative to
   __shared__ volatile int abort_flag;
 
@@ -622,42 +652,56 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       }
     }
   } else if (PAGES && warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kArKeyWarps + kArValueWarps) {
-    // ---- pages: codes into operands; four warps the keys, three the values.  A thread asks for its pieces of the next tile behind
-    // those of this one.
+    // ---- pages: codes into operands; four warps the keys, three the values.  The first warp of each says where a tile's groups of eight
+    // keys lie; a thread asks for its pieces of the next tile behind those of this one.
     const bool is_k = warp < kSoftmaxWarps + kArKeyWarps;
-    const int threads = 32 * (is_k ? kArKeyWarps : kArValueWarps), t = int(threadIdx.x) - 32 * (kSoftmaxWarps + (is_k ? 0 : kArKeyWarps));
-    constexpr int kMost = (kArKeys * kPieces + 32 * kArValueWarps - 1) / (32 * kArValueWarps);
-    const uint8_t* const codes = is_k ? p.k_codes : p.v_codes;
+    const int warps = is_k ? kArKeyWarps : kArValueWarps, wq = warp - kSoftmaxWarps - (is_k ? 0 : kArKeyWarps);
+    constexpr int kRows = 32 / kPieces, kParts = 8 / kRows;        // rows of a warp's piece, pieces of eight keys
+    constexpr int kAll = kArKeys / kRows, kMost = (kAll + kArValueWarps - 1) / kArValueWarps;
+    const uint8_t* const codes = (is_k ? p.k_codes : p.v_codes) + (lane % kPieces) * 16 + (lane / kPieces) * HD;
     unsigned char* const to = is_k ? k_s : v_s;
     const ArKeys<true> keys{p, p.block_tables + size_t(seq) * p.max_blocks, 0, kvh};
     uint4 held[kMost];
-    float2 of_group;                                               // scales of the eight keys that a lane of the first warp has
+    float2 of_group = make_float2(0.f, 1.f);                       // scales of the eight keys that a lane of the first warp has
+    // where the eight keys of a lane of a first warp are in tile n, counted in rows of a head, and their scales
+    auto look = [&](int n) {
+      const int key0 = (j0 + n) * kArKeys + lane * 8, key = max(key0, lo);
+      if (wq != 0 || lane >= kArKeys / 8 || n >= n_tiles) return;
+      of_group = make_float2(0.f, 1.f);
+      size_t at = 0;
+      if (key < min(hi, key0 + 8)) {
+        at = keys.place(key);
+        if (is_k) of_group = make_float2(p.k_scale[at / p.block_size], p.v_scale[at / p.block_size]);
+        at -= key - key0;
+      }
+      group_at[is_k ? 0 : 1][n & 1][lane] = at;
+    };
     auto ask = [&](int n) {
       const int key0 = (j0 + n) * kArKeys;
+      const size_t* const at = group_at[is_k ? 0 : 1][n & 1];
+      const bool inside = key0 >= lo && key0 + kArKeys <= hi;
 #pragma unroll
       for (int i = 0; i < kMost; ++i) {
-        const int piece = i * threads + t, r = piece / kPieces, ch = piece % kPieces;
+        const int piece = i * warps + wq, r = piece * kRows + lane / kPieces;
         held[i] = make_uint4(0u, 0u, 0u, 0u);                      // (keys of nobody: zero times them stays zero)
-        if (piece < kArKeys * kPieces && key0 + r >= lo && key0 + r < hi)
-          held[i] = *reinterpret_cast<const uint4*>(codes + keys.place(key0 + r) * HD + ch * 16);
-      }
-      of_group = make_float2(0.f, 1.f);
-      if (warp == kSoftmaxWarps && lane < kArKeys / 8) {
-        const int key = max(key0 + lane * 8, lo);
-        if (key < min(hi, key0 + lane * 8 + 8)) {
-          const size_t at = keys.place(key) / p.block_size;
-          of_group = make_float2(p.k_scale[at], p.v_scale[at]);
-        }
+        if (piece < kAll && (inside || (key0 + r >= lo && key0 + r < hi)))
+          held[i] = *reinterpret_cast<const uint4*>(codes + (at[piece / kParts] + (piece % kParts) * kRows) * HD);
       }
     };
+    auto together = [&]() { asm volatile("barrier.cta.sync.aligned %0, %1;\n" ::"r"(is_k ? 9 : 10), "r"(32 * warps) : "memory"); };
+    look(0);
+    together();
     ask(0);
     float base = 0.f;
+    bool there_is = true;                                          // room for the tile
     for (int n = 0; n < n_tiles; ++n) {
       const int st = n % kArStages;
-      if (n >= kArStages && !wait_all(is_k ? &k_free[st] : &v_free[st], ((n / kArStages) & 1) ^ 1, is_k ? 40 : 41)) break;
+      const float2 scale = of_group;
+      look(n + 1);
+      there_is = there_is && (n < kArStages || wait_all(is_k ? &k_free[st] : &v_free[st], ((n / kArStages) & 1) ^ 1, is_k ? 40 : 41));
       if (warp == kSoftmaxWarps) {
         // (S_(n-2) is complete, so the weights of tile n - 3 are made, and the place of tile n - 4 is free)
-        const float log_v = log2f(fmaxf(of_group.y, 1.17549435e-38f));
+        const float log_v = log2f(fmaxf(scale.y, 1.17549435e-38f));
         if (n == 0) {
           base = __shfl_sync(0xffffffffu, log_v, (lo % kArKeys) / 8);
           if (lane == 0) value_base = base;
@@ -665,22 +709,25 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         if (lane < kArKeys / 8) {
           const bool there = (j0 + n) * kArKeys + lane * 8 < hi && (j0 + n) * kArKeys + lane * 8 + 8 > lo;
           ArScales s;
-          s.key = of_group.x;
+          s.key = scale.x;
           s.value = there ? log_v - base : 0.f;
           s.out = there ? exp2f(base - log_v) : 0.f;
           scales[(n % kArRing) * (kArKeys / 8) + lane] = s;
         }
         __syncwarp();
-        if (lane == 0) tc5::mbar_arrive(&sc_full[n % kArRing]);
+        if (there_is && lane == 0) tc5::mbar_arrive(&sc_full[n % kArRing]);
       }
+      if (there_is) {
 #pragma unroll
-      for (int i = 0; i < kMost; ++i) {
-        const int piece = i * threads + t;
-        if (piece < kArKeys * kPieces) ar_spread<HD>(to + st * KB * kArTile, held[i], piece / kPieces, piece % kPieces);
+        for (int i = 0; i < kMost; ++i) {
+          const int piece = i * warps + wq;
+          if (piece < kAll) ar_spread<HD>(to + st * KB * kArTile, held[i], piece * kRows + lane / kPieces, lane % kPieces);
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tc5::mbar_arrive(is_k ? &k_full[st] : &v_full[st]);
       }
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      __syncwarp();
-      if (lane == 0) tc5::mbar_arrive(is_k ? &k_full[st] : &v_full[st]);
+      together();                                                  // (whoever gave up comes along to the end, and the others' waits run out too)
       if (n + 1 < n_tiles) ask(n + 1);
     }
   } else if (warp < kSoftmaxWarps && ((warp >> 2) & 1) < groups) {
