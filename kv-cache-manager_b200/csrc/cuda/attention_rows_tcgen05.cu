@@ -257,30 +257,33 @@ __device__ __forceinline__ bool ar_small(const uint32_t (&s)[N], const ArScales*
 }
 
 // A thread's products of a tile into weights, two to a register.  Of `chunks` 32.  A thread with all of a row's products takes them by
-// 16, the next ones under way while 16 are worked on; of two, which run under each other, each has the registers for 32 at once.
+// 16, the next ones under way while 16 are worked on; of two, which run under each other, each has the registers for 32 at once, or for
+// 16 and the polynomial of capped scores (16 ragged prompts 130 us in place of 160).
 template <int CHUNKS, bool CAP, bool PAGES, bool MASK, bool AGAIN>
 __device__ __forceinline__ void ar_tile(uint32_t s_addr, const ArScales* sc, uint32_t (&packed)[16 * CHUNKS], const ArRow& row, float m, int a, int b,
                                         int chunks, float& weights, float& sum) {
   float2 w2 = make_float2(0.f, 0.f), l2 = make_float2(0.f, 0.f);
-  if constexpr (CHUNKS == 4) {
-    uint32_t s[2][16];
-    ar_ld16(s_addr, s[0]);
+  if constexpr (CHUNKS == 4 || CAP) {
+    constexpr int kAhead = CHUNKS == 4 ? 1 : 0;
+    uint32_t s[kAhead + 1][16];
+    if (kAhead) ar_ld16(s_addr, s[0]);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
+    for (int c = 0; c < 2 * CHUNKS; ++c) {
       if (MASK && c >= 2 * chunks) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) packed[c * 8 + i] = 0u;
         continue;
       }
-      ar_wait16(s[c & 1]);
-      if (c < 7) ar_ld16(s_addr + uint32_t(c * 16 + 16), s[(c + 1) & 1]);
+      if (!kAhead) ar_ld16(s_addr + uint32_t(c * 16), s[0]);
+      ar_wait16(s[c & kAhead]);
+      if (kAhead && c < 2 * CHUNKS - 1) ar_ld16(s_addr + uint32_t(c * 16 + 16), s[(c + 1) & kAhead]);
       const uint32_t seen = MASK ? ar_bits(a - c * 16, b - c * 16) : 0u;
-      if (CAP && ar_small<PAGES>(s[c & 1], sc + c * 2, row.factor))
-        ar_exponentials<CAP, PAGES, MASK, AGAIN, true>(s[c & 1], sc + c * 2, packed + c * 8, row, m, seen, w2, l2);
+      if (CAP && ar_small<PAGES>(s[c & kAhead], sc + c * 2, row.factor))
+        ar_exponentials<CAP, PAGES, MASK, AGAIN, true>(s[c & kAhead], sc + c * 2, packed + c * 8, row, m, seen, w2, l2);
       else
-        ar_exponentials<CAP, PAGES, MASK, AGAIN, false>(s[c & 1], sc + c * 2, packed + c * 8, row, m, seen, w2, l2);
+        ar_exponentials<CAP, PAGES, MASK, AGAIN, false>(s[c & kAhead], sc + c * 2, packed + c * 8, row, m, seen, w2, l2);
     }
-    if (MASK) tc5::ld_wait();
+    if (kAhead && MASK) tc5::ld_wait();
   } else {
     uint32_t s[32];
 #pragma unroll
