@@ -5,7 +5,8 @@
 //
 // A chunk of 512 keys at a time: a thread forms the scores of whole keys, then the products with V are dealt out as words of eight
 // elements, groups of threads taking every n-th key each, joined at the end in the groups' order.  What bounds it is instructions:
-// every row and query head converts a key's elements anew.
+// every row and query head converts a key's elements anew.  B200: single rows of 64 requests of 8,192 keys, 32 heads on 8 of 128, 1.88 ms; four
+// portions of about 1,500 rows behind 5,000 keys 80 ms; a prompt of 8,192 rows 550 ms.
 #include "packed.cuh"
 #include "pdl.cuh"
 #include "q8.cuh"
