@@ -24,11 +24,16 @@
 // last are zeros in shared memory; a row whose result is not finite looks whether an unseen value was the reason, and is then
 // attended once more without the tensor cores.
 //
-// What bounds it: a group's chain of softmax and products, of which two groups' overlap.  A tile of 256 x 128 takes some 3,300 cycles at
-// prompts of heads of 128, the products 2,048 of them; a product of 128 x 64 takes as long as one of 128 x 128, so smaller tiles that would
-// let S run ahead of the softmax lose (720 us for 8,192 rows against 640 at the time).  A block's beginning and end are 7 us.  B200, 32 heads on 8 of 128:
-// a prompt of 8,192 rows 477 us (1,150 TFLOP/s; 550 after seconds of it, under the power cap), four portions of about 1,500 rows behind
-// 5,000 keys 682 (740 TFLOP/s); 16 ragged prompts of some 600 rows, 16 heads, window, capped, sinks 130; five of 110 rows of heads of 64 17.
+// Prompts' blocks stay: three tiles before its end a block asks for another that has not begun and takes its work, so that Q, K and V come
+// while rows are written (16 ragged prompts 75 us in place of 104 without cap, asked for at a block's beginning 94).
+//
+// What bounds it: a group's chain of softmax and products, of which two groups' overlap.  A tile of 256 x 128 takes some 3,200 cycles at
+// prompts of heads of 128, the products 2,048 of them, and the exponential units as many; the issuing warp's instructions between
+// products, of which a barrier's wait or a commit is some hundred cycles, are the gap (four commits a tile in place of five, two barriers in place of
+// four: 468 -> 444 us).  A product of 128 x 64 takes as long as one of 128 x 128, so smaller tiles that would
+// let S run ahead of the softmax lose (720 us for 8,192 rows against 640 at the time).  B200, 32 heads on 8 of 128:
+// a prompt of 8,192 rows 445 us (1,235 TFLOP/s; 520 after seconds of it, under the power cap), four portions of about 1,500 rows behind
+// 5,000 keys 683 (740 TFLOP/s); 16 ragged prompts of some 600 rows, 16 heads, window, capped, sinks 104; five of 110 rows of heads of 64 17.
 //
 // Every wait is bounded; one that runs out sets the error word of the tcgen05 attention family (codes 33 and up) and ends the block.
 #include <cuda_fp16.h>
@@ -436,6 +441,86 @@ __device__ __forceinline__ void ar_spread(unsigned char* tile, uint4 u, int r, i
   *reinterpret_cast<uint4*>(row + (((c + 1 - swap) ^ (r & 7)) * 16)) = swap ? half[0] : half[1];
 }
 
+// A block's work: up to 256 rows of a request and a head.  rows 0: none.
+struct ArItem { int seq, head, q0, q_start, q_len, rows, ctx; };
+
+// The work of block (x, y), looked up by a whole warp: heads fastest; the last tiles, which see most keys, first, and prompts of one row last.
+template <bool PAGES>
+__device__ __forceinline__ ArItem ar_item(const RowsParams& p, int x, int y) {
+  const int tile = p.blocks - 1 - y;
+  ArItem it{-1, x, 0, 0, 0, 0, 0};
+  int most = kArRows;
+  if (!PAGES && tile < 0) {                                        // a prompt of one row
+    it.seq = -1 - tile;
+    most = 1;
+  } else {                                                         // the tile-th of those that begin a block
+    for (int t0 = 0, before = 0; t0 < p.tiles; t0 += 128) {
+      int s[4], q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i * 32 + int(threadIdx.x & 31);
+        s[i] = t < p.tiles ? p.tile_seq[t] : -1;
+        q[i] = t < p.tiles ? p.tile_q0[t] : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool begins = s[i] >= 0 && (q[i] & (kArRows - 1)) == 0;
+        const uint32_t leads = __ballot_sync(0xffffffffu, begins);
+        const int at = tile - before;
+        before += __popc(leads);
+        if (it.seq < 0 && at >= 0 && tile < before) {
+          const int from = __ffs(__ballot_sync(0xffffffffu, begins && __popc(leads & ((1u << (threadIdx.x & 31)) - 1u)) == at)) - 1;
+          it.seq = __shfl_sync(0xffffffffu, s[i], from);
+          it.q0 = __shfl_sync(0xffffffffu, q[i], from);
+        }
+      }
+      if (it.seq >= 0) break;
+    }
+  }
+  if (it.seq < 0) return it;                                       // fewer than the host had to reckon with
+  it.q_start = p.seq_q_start[it.seq];
+  it.q_len = p.seq_q_len[it.seq];
+  it.rows = max(min(most, it.q_len - it.q0), 0);
+  it.ctx = PAGES ? min(p.seq_ctx_len[it.seq], p.max_keys) : it.q_len;          // (a context ends with its table)
+  return it;
+}
+
+// What it has to do with keys.
+struct ArSpan {
+  int pos0, hi, lo, j0, groups, hi_first, n_tiles, n_first, kvh;
+  __device__ __forceinline__ ArSpan(const RowsParams& p, const ArItem& it) {
+    pos0 = it.ctx - it.q_len + it.q0;                              // position of the block's first row
+    hi = pos0 + it.rows;                                           // keys [lo, hi) matter to the block
+    lo = first_visible(pos0, p.window, 0);
+    j0 = lo / kArKeys;
+    groups = it.rows > kArGroupRows ? 2 : 1;
+    // a group's keys end with its last row's own, and so do its tiles
+    hi_first = groups == 1 ? hi : pos0 + kArGroupRows;
+    n_tiles = (hi - 1) / kArKeys - j0 + 1;
+    n_first = (hi_first - 1) / kArKeys - j0 + 1;
+    kvh = it.head / (p.nh / p.nkv);
+  }
+};
+
+// Asks for the work of a block of the grid that has not begun, in its place (the answer in 16 bytes of shared memory, counted on `bar`).
+__device__ __forceinline__ void ar_ask_block(uint4* answer, uint64_t* bar) {
+  tc5::mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n"
+               ::"r"(tc5::s32(answer)), "r"(tc5::s32(bar)) : "memory");
+}
+// Whether there was one, and which.
+__device__ __forceinline__ bool ar_block_answer(const uint4* answer, int& x, int& y) {
+  uint32_t is, bx = 0, by = 0;
+  asm volatile("{\n.reg .pred p;\n.reg .b128 r;\nld.shared.b128 r, [%3];\n"
+               "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\nselp.u32 %2, 1, 0, p;\n"
+               "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, %1, _, _}, r;\n}\n"
+               : "+r"(bx), "+r"(by), "=r"(is) : "r"(tc5::s32(answer)) : "memory");
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  x = int(bx);
+  y = int(by);
+  return is != 0u;
+}
+
 template <int HD, bool PAGES> constexpr size_t ar_smem() {
   return size_t(2 + 2 * kArStages) * (HD / 64) * kArTile + (PAGES ? kArRing * (kArKeys / 8) * sizeof(ArScales) : 0);
 }
@@ -456,8 +541,10 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   unsigned char* k_s = q_s + 2 * KB * kArTile;                     // [stages][KB][128 keys][64]
   unsigned char* v_s = k_s + kArStages * KB * kArTile;
   ArScales* scales = reinterpret_cast<ArScales*>(v_s + kArStages * KB * kArTile);          // [ring][16 groups of eight keys]
-  __shared__ __align__(8) uint64_t q_full, q_ready, k_full[kArStages], v_full[kArStages], k_free[kArStages], v_free[kArStages], v_tail,
-      sc_full[kArRing], s_full[2], p_full[2], o_full;
+  __shared__ __align__(8) uint64_t q_full, q_ready, k_full[kArStages], v_full[kArStages], kv_free[kArStages], v_tail,
+      sc_full[kArRing], s_full[2], p_full[2], o_full[2], next_told, item_full[2], item_free[2];
+  __shared__ __align__(16) uint4 next_block;
+  __shared__ ArItem items[2];                                      // the work in hand; prompts: and what comes behind it
   __shared__ uint32_t tmem_base;
   __shared__ float told[SPLIT][kArRows];                           // what the threads of a row tell each other
   __shared__ int left[8][2];                                       // that a warp gave up
@@ -465,77 +552,41 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   __shared__ float value_base;                                     // log2 of the value scale that weights are relative to
   __shared__ volatile int abort_flag;
 
-  // heads fastest and the last tiles, which see most keys, first
-  const int tile = int(gridDim.y) - 1 - int(blockIdx.y), head = blockIdx.x;
   int* const error = p.error;
   // Tiles and lengths may come from a kernel of the same step, so they are read behind the wait.  (Whoever leaves waits as
   // well: a launch of nothing but empty tiles would else be over before the kernel in front of it.)
   pdl_wait();
-  int seq = -1, q0 = 0, most = kArRows;
-  if (!PAGES && tile >= p.blocks) {                                // a prompt of one row
-    seq = tile - p.blocks;
-    most = 1;
-  } else {                                                         // the tile-th of those that begin a block
-    for (int t0 = 0, before = 0; t0 < p.tiles; t0 += 128) {
-      int s[4], q[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = t0 + i * 32 + int(threadIdx.x & 31);
-        s[i] = t < p.tiles ? p.tile_seq[t] : -1;
-        q[i] = t < p.tiles ? p.tile_q0[t] : -1;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t leads = __ballot_sync(0xffffffffu, s[i] >= 0 && (q[i] & (kArRows - 1)) == 0);
-        const int at = tile - before;
-        before += __popc(leads);
-        if (seq < 0 && at >= 0 && tile < before) {
-          const int from = __fns(leads, 0, at + 1);
-          seq = __shfl_sync(0xffffffffu, s[i], from);
-          q0 = __shfl_sync(0xffffffffu, q[i], from);
-        }
-      }
-      if (seq >= 0) break;
-    }
-  }
-  if (seq < 0) return;                                             // fewer than the host had to reckon with
-  const int q_start = p.seq_q_start[seq], q_len = p.seq_q_len[seq];
-  const int rows_here = min(most, q_len - q0);
-  if (rows_here <= 0) return;
+  const ArItem begin = ar_item<PAGES>(p, blockIdx.x, blockIdx.y);
+  if (begin.rows == 0) return;
   if (tc5::s32(smem_raw) & 1023) {
     if (threadIdx.x == 0) atomicExch(error, (33 << 16) | int(blockIdx.y & 0xffff));
     return;
   }
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int ctx = PAGES ? min(p.seq_ctx_len[seq], p.max_keys) : q_len;       // (a context ends with its table)
-  const int pos0 = ctx - q_len + q0;                               // position of the block's first row
-  const int hi = pos0 + rows_here;                                 // keys [lo, hi) matter to the block
-  const int lo = first_visible(pos0, p.window, 0);
-  const int j0 = lo / kArKeys;
-  const int groups = rows_here > kArGroupRows ? 2 : 1;
-  // a group's keys end with its last row's own, and so do its tiles
-  const int hi_first = groups == 1 ? hi : pos0 + kArGroupRows;
-  const int n_tiles = (hi - 1) / kArKeys - j0 + 1, n_first = (hi_first - 1) / kArKeys - j0 + 1;
-  const int kvh = head / (p.nh / p.nkv);
 
   if (threadIdx.x < 16) left[threadIdx.x >> 1][threadIdx.x & 1] = 0;
   if (threadIdx.x == 0) {
     abort_flag = 0;
+    items[0] = begin;
     tc5::mbar_init(&q_full, 1);
-    tc5::mbar_init(&q_ready, 4 * SPLIT * groups);
+    tc5::mbar_init(&q_ready, 4 * SPLIT * (begin.rows > kArGroupRows ? 2 : 1));
     for (int i = 0; i < kArStages; ++i) {
       tc5::mbar_init(&k_full[i], PAGES ? kArKeyWarps : 1);
       tc5::mbar_init(&v_full[i], PAGES ? kArValueWarps : 1);
-      tc5::mbar_init(&k_free[i], 1);
-      tc5::mbar_init(&v_free[i], 1);
+      tc5::mbar_init(&kv_free[i], 1);
     }
     tc5::mbar_init(&v_tail, 1);
     for (int i = 0; i < kArRing; ++i) tc5::mbar_init(&sc_full[i], 1);
     for (int g = 0; g < 2; ++g) {
       tc5::mbar_init(&s_full[g], 1);
+      tc5::mbar_init(&o_full[g], 1);
       tc5::mbar_init(&p_full[g], 4 * SPLIT);                       // a group's warps
     }
-    tc5::mbar_init(&o_full, 1);
+    tc5::mbar_init(&next_told, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc5::mbar_init(&item_full[i], 1);
+      tc5::mbar_init(&item_free[i], kSoftmaxWarps + 1);            // softmax and products
+    }
     tc5::mbar_init_fence();
   }
   if (warp == kMmaWarp) {
@@ -558,14 +609,26 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     return false;
   };
 
+  // Prompts' blocks stay and take the work of blocks that have not begun, so that its Q, K and V come while the rows before are attended and
+  // written.  Whether there is work with number `n` of the block, in items[n & 1] until all have left it.
+  auto there_is_item = [&](int n) {
+    if (n == 0) return true;
+    return !PAGES && wait_all(&item_full[n & 1], ((n - 1) >> 1) & 1, 47) && items[n & 1].rows > 0;
+  };
+  auto leave_item = [&](int n) {
+    __syncwarp();
+    if (!PAGES && lane == 0) tc5::mbar_arrive(&item_free[n & 1]);
+  };
+
   if (warp == kMmaWarp) {
-    // ---- the products: the warp stays together, one thread of it issues
+    // ---- the products: the warp stays together, one thread of it issues.  Step n is O += P_(n-1) V_(n-1) and S_n of either group.
     const uint32_t one = ar_elect();
     if (PAGES && one) {
-      tc5::mbar_expect_tx(&q_full, groups * KB * kArTile);
-      for (int g = 0; g < groups; ++g)
+      const ArSpan w(p, begin);
+      tc5::mbar_expect_tx(&q_full, w.groups * KB * kArTile);
+      for (int g = 0; g < w.groups; ++g)
         for (int kb = 0; kb < KB; ++kb)
-          ar_tma_3d(q_s + (g * KB + kb) * kArTile, &map_q, &q_full, kb * 64, head, q_start + q0 + g * kArGroupRows);
+          ar_tma_3d(q_s + (g * KB + kb) * kArTile, &map_q, &q_full, kb * 64, begin.head, begin.q_start + begin.q0 + g * kArGroupRows);
     }
     __syncwarp();
     constexpr uint32_t kTypes = PAGES ? ~((7u << 7) | (7u << 10)) : ~0u;         // float16 or bfloat16
@@ -576,100 +639,134 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     // values, MN-major: 64-wide blocks a leading offset apart
     const uint64_t dv = (tc5::smem_desc(tc5::s32(v_s)) & ~(uint64_t(0x3fff) << 16)) | (uint64_t(kArTile >> 4) << 16);
     const uint32_t base = uint32_t(ar_uniform(int(tmem)));
-    const int tiles = ar_uniform(n_tiles), tiles_first = ar_uniform(n_first), both = ar_uniform(groups);
-    // (of a group's last tile only the steps of 16 keys that some row of it sees)
-    const int last_steps = ar_uniform((hi - (j0 + n_tiles - 1) * kArKeys + 15) / 16), last_first = ar_uniform((hi_first - (j0 + n_first - 1) * kArKeys + 15) / 16);
-    bool ok = wait_all(PAGES ? &q_ready : &q_full, 0, 34);
-    tc5::fence_after();
-    for (int n = 0; ok && n <= tiles; ++n) {
-      const int st = n & 1;                                         // stage of tile n; tile n - 1 has the other
-      static_assert(kArStages == 2, "stages by parity");
-      for (int g = 0; g < both; ++g) {
-        const int mine = g == 0 ? tiles_first : tiles;
-        if (n >= 1 && n <= mine) {                                 // O += P_(n-1) V_(n-1)
-          if (!wait_all(&v_full[st ^ 1], ((n - 1) >> 1) & 1, 35) || !wait_all(&p_full[g], (n - 1) & 1, 36)) { ok = false; break; }
-          tc5::fence_after();
-          const uint64_t v = dv + (st ^ 1) * kStageStep;
-          const uint32_t d = base + 256 + g * HD, a = base + g * kArKeys;
-          const int steps = n < mine ? 8 : g == 0 ? last_first : last_steps;
-          // 16 keys: 8 columns of P (every thread's over its own products), 16 rows down V
-          if (steps == 8) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) ar_mma_ts(one, d, a + (SPLIT == 2 ? (j & 3) * 8 + (j >> 2) * 64 : j * 8), v + uint64_t(j * (16 * 128 >> 4)), idesc_o, (n > 1 || j > 0) ? 1u : 0u);
-          } else {
-#pragma unroll 1
-            for (int j = 0; j < steps; ++j) ar_mma_ts(one, d, a + (SPLIT == 2 ? (j & 3) * 8 + (j >> 2) * 64 : j * 8), v + uint64_t(j * (16 * 128 >> 4)), idesc_o, (n > 1 || j > 0) ? 1u : 0u);
-          }
-        }
-        if (n < mine) {                                            // S_n, over P_(n-1)
-          if (!wait_all(&k_full[st], (n >> 1) & 1, 37)) { ok = false; break; }
-          tc5::fence_after();
-          const uint64_t q = dq + g * kStageStep, k = dk + st * kStageStep;
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              ar_mma_ss(one, base + g * kArKeys, q + uint64_t(kb * (kArTile >> 4) + 2 * j), k + uint64_t(kb * (kArTile >> 4) + 2 * j), idesc_s,
-                        (kb > 0 || j > 0) ? 1u : 0u);
-          ar_commit(one, &s_full[g]);                              // and O += P_(n-1) V_(n-1) before it
-        }
-      }
-      if (!ok) break;
-      if (n < tiles) ar_commit(one, &k_free[st]);                  // tile n of the keys is read,
-      if (n >= 1) ar_commit(one, &v_free[st ^ 1]);                 // and n - 1 of the values
-    }
-    ar_commit(one, &o_full);
-  } else if (!PAGES && warp == kSoftmaxWarps) {
-    // ---- prompts: one thread asks for Q, K and V
-    const int tail = hi - (j0 + n_tiles - 1) * kArKeys;            // keys of the last tile
     bool ok = true;
-    for (int n = 0; ok && n < n_tiles; ++n) {
-      const int st = n % kArStages, key = q_start + (j0 + n) * kArKeys;
-      const uint32_t parity = ((n / kArStages) & 1) ^ 1;
-      // (the product of the last tile takes 16 keys at a time; behind the prompt's last come zeros)
-      const bool ends = n == n_tiles - 1 && tail % 16 != 0;
-      if (lane == 0) {
-        ok = tc5::mbar_wait(&k_free[st], parity);
-        if (ok) {
-          if (n == 0) {
-            tc5::mbar_expect_tx(&q_full, groups * KB * kArTile);
-            for (int g = 0; g < groups; ++g)
-              for (int kb = 0; kb < KB; ++kb)
-                ar_tma_3d(q_s + (g * KB + kb) * kArTile, &map_q, &q_full, kb * 64, head, q_start + q0 + g * kArGroupRows);
+    uint32_t step = 0, odd = 0;                                     // steps so far; bit g: whether the group's tiles of weights so far are odd
+    for (int number = 0; ok && there_is_item(number); ++number) {
+      const ArSpan w(p, items[number & 1]);
+      leave_item(number);
+      const int tiles = ar_uniform(w.n_tiles), tiles_first = ar_uniform(w.n_first), both = ar_uniform(w.groups);
+      // (of a group's last tile only the steps of 16 keys that some row of it sees)
+      const int last_steps = ar_uniform((w.hi - (w.j0 + w.n_tiles - 1) * kArKeys + 15) / 16);
+      const int last_first = ar_uniform((w.hi_first - (w.j0 + w.n_first - 1) * kArKeys + 15) / 16);
+      ok = wait_all(PAGES ? &q_ready : &q_full, number & 1, 34);
+      for (int n = 0; ok && n <= tiles; ++n, ++step) {
+        const int st = step & 1;                                    // of tile n of the keys and tile n - 1 of the values
+        static_assert(kArStages == 2, "stages by parity");
+        const uint32_t parity = (step >> 1) & 1;
+        ok = PAGES ? (n == 0 || wait_all(&v_full[st], ((n - 1) >> 1) & 1, 35)) : wait_all(&k_full[st], parity, 37);
+        for (int g = 0; ok && g < both; ++g) {
+          const int mine = g == 0 ? tiles_first : tiles;
+          if (n > mine) continue;
+          if (n >= 1) {                                             // O += P_(n-1) V_(n-1)
+            ok = wait_all(&p_full[g], (odd >> g) & 1, 36);
+            if (!ok) break;
+            odd ^= 1u << g;
+            tc5::fence_after();
+            const uint64_t v = dv + st * kStageStep;
+            const uint32_t d = base + 256 + g * HD, a = base + g * kArKeys;
+            const int steps = n < mine ? 8 : g == 0 ? last_first : last_steps;
+            // 16 keys: 8 columns of P (every thread's over its own products), 16 rows down V
+            if (steps == 8) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) ar_mma_ts(one, d, a + (SPLIT == 2 ? (j & 3) * 8 + (j >> 2) * 64 : j * 8), v + uint64_t(j * (16 * 128 >> 4)), idesc_o, (n > 1 || j > 0) ? 1u : 0u);
+            } else {
+#pragma unroll 1
+              for (int j = 0; j < steps; ++j) ar_mma_ts(one, d, a + (SPLIT == 2 ? (j & 3) * 8 + (j >> 2) * 64 : j * 8), v + uint64_t(j * (16 * 128 >> 4)), idesc_o, (n > 1 || j > 0) ? 1u : 0u);
+            }
           }
-          tc5::mbar_expect_tx(&k_full[st], KB * kArTile);
-          for (int kb = 0; kb < KB; ++kb) ar_tma_3d(k_s + (st * KB + kb) * kArTile, &map_k, &k_full[st], kb * 64, kvh, key);
-          ok = tc5::mbar_wait(&v_free[st], parity);
+          if (n < mine) {                                           // S_n, over P_(n-1)
+            if (PAGES && !wait_all(&k_full[st], parity, 37)) { ok = false; break; }
+            tc5::fence_after();
+            const uint64_t q = dq + g * kStageStep, k = dk + st * kStageStep;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                ar_mma_ss(one, base + g * kArKeys, q + uint64_t(kb * (kArTile >> 4) + 2 * j), k + uint64_t(kb * (kArTile >> 4) + 2 * j), idesc_s,
+                          (kb > 0 || j > 0) ? 1u : 0u);
+          }
+          ar_commit(one, n < mine ? &s_full[g] : &o_full[g]);       // (s_full: and O += P_(n-1) V_(n-1) before it)
         }
-        if (ok) {
-          uint64_t* const bar = ends ? &v_tail : &v_full[st];
-          tc5::mbar_expect_tx(bar, KB * kArTile);
-          for (int kb = 0; kb < KB; ++kb) ar_tma_3d(v_s + (st * KB + kb) * kArTile, &map_v, bar, kb * 64, kvh, key);
-        }
-        if (!ok && !abort_flag) fail(38);
+        if (ok) ar_commit(one, &kv_free[st]);
       }
-      ok = __shfl_sync(0xffffffffu, int(ok), 0);
-      if (ok && ends) {
-        ok = wait_all(&v_tail, 0, 39);
-        const int to = (tail + 15) / 16 * 16;
-        for (int kb = 0; ok && kb < KB; ++kb)
-          for (int i = tail * 8 + lane; i < to * 8; i += 32)
-            *reinterpret_cast<uint4*>(v_s + (st * KB + kb) * kArTile + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      if (PAGES) break;
+    }
+  } else if (!PAGES && warp == kSoftmaxWarps) {
+    // ---- prompts: one thread asks for Q, K, V and more work, which the warp looks up
+    bool ok = true;
+    int tails = 0, asked = 0;                                      // ends with zeros, questions
+    uint32_t step = 0;                                             // of the products
+    ArItem it = begin;
+    for (int number = 0; ok && it.rows > 0; ++number) {
+      const ArSpan w(p, it);
+      const int tail = w.hi - (w.j0 + w.n_tiles - 1) * kArKeys;    // keys of the last tile
+      // tile n of the keys and tile n - 1 of the values come, and are read, together
+      for (int n = 0; ok && n <= w.n_tiles; ++n, ++step) {
+        const int st = step & 1, key = it.q_start + (w.j0 + n) * kArKeys;
+        const bool has_k = n < w.n_tiles, has_v = n > 0;
+        // (the product of the last tile takes 16 keys at a time; behind the prompt's last come zeros)
+        const bool ends = n == w.n_tiles && tail % 16 != 0;
+        if (lane == 0) {
+          if (n == max(w.n_tiles - 3, 0)) ar_ask_block(&next_block, &next_told);        // (the later, the better blocks' ends fit)
+          ok = ar_wait(&kv_free[st], ((step >> 1) & 1) ^ 1);
+          if (ok && n == 0) {                                      // (the work before has had its last scores one step ago)
+            tc5::mbar_expect_tx(&q_full, w.groups * KB * kArTile);
+            for (int g = 0; g < w.groups; ++g)
+              for (int kb = 0; kb < KB; ++kb)
+                ar_tma_3d(q_s + (g * KB + kb) * kArTile, &map_q, &q_full, kb * 64, it.head, it.q_start + it.q0 + g * kArGroupRows);
+          }
+          if (ok) {
+            uint64_t* const bar = ends ? &v_tail : &k_full[st];
+            tc5::mbar_expect_tx(bar, (int(has_k) + int(has_v)) * KB * kArTile);
+            for (int kb = 0; has_k && kb < KB; ++kb) ar_tma_3d(k_s + (st * KB + kb) * kArTile, &map_k, bar, kb * 64, w.kvh, key);
+            for (int kb = 0; has_v && kb < KB; ++kb) ar_tma_3d(v_s + (st * KB + kb) * kArTile, &map_v, bar, kb * 64, w.kvh, key - kArKeys);
+          }
+          if (!ok && !abort_flag) fail(38);
+        }
+        ok = __shfl_sync(0xffffffffu, int(ok), 0);
+        if (ok && ends) {
+          ok = wait_all(&v_tail, tails & 1, 39);
+          ++tails;
+          const int to = (tail + 15) / 16 * 16;
+          for (int kb = 0; ok && kb < KB; ++kb)
+            for (int i = tail * 8 + lane; i < to * 8; i += 32)
+              *reinterpret_cast<uint4*>(v_s + (st * KB + kb) * kArTile + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+          __syncwarp();
+          if (ok && lane == 0) tc5::mbar_arrive(&k_full[st]);
+        }
+      }
+      // ---- the work behind it: of the next block that has some
+      for (;;) {
+        int x, y;
+        if (!wait_all(&next_told, asked & 1, 48)) { ok = false; it.rows = 0; break; }      // (also where a wait above ran out: an answer has to land)
+        ++asked;
+        if (!ar_block_answer(&next_block, x, y) || !ok) { it.rows = 0; break; }
+        it = ar_item<PAGES>(p, x, y);
+        if (it.rows > 0) break;
         __syncwarp();
-        if (ok && lane == 0) tc5::mbar_arrive(&v_full[st]);
+        if (lane == 0) ar_ask_block(&next_block, &next_told);
       }
+      const int to = (number + 1) & 1;
+      if (!wait_all(&item_free[to], (((number + 1) >> 1) & 1) ^ 1, 49)) break;
+      if (lane == 0) {
+        items[to] = it;
+        tc5::mbar_arrive(&item_full[to]);
+      }
+      __syncwarp();
     }
   } else if (PAGES && warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kArKeyWarps + kArValueWarps) {
     // ---- pages: codes into operands; four warps the keys, three the values.  The first warp of each says where a tile's groups of eight
     // keys lie; a thread asks for its pieces of the next tile behind those of this one.
+    const ArSpan w(p, begin);
+    const int lo = w.lo, hi = w.hi, j0 = w.j0, n_tiles = w.n_tiles;
     const bool is_k = warp < kSoftmaxWarps + kArKeyWarps;
     const int warps = is_k ? kArKeyWarps : kArValueWarps, wq = warp - kSoftmaxWarps - (is_k ? 0 : kArKeyWarps);
     constexpr int kRows = 32 / kPieces, kParts = 8 / kRows;        // rows of a warp's piece, pieces of eight keys
     constexpr int kAll = kArKeys / kRows, kMost = (kAll + kArValueWarps - 1) / kArValueWarps;
     const uint8_t* const codes = (is_k ? p.k_codes : p.v_codes) + (lane % kPieces) * 16 + (lane / kPieces) * HD;
     unsigned char* const to = is_k ? k_s : v_s;
-    const ArKeys<true> keys{p, p.block_tables + size_t(seq) * p.max_blocks, 0, kvh};
+    const ArKeys<true> keys{p, p.block_tables + size_t(begin.seq) * p.max_blocks, 0, w.kvh};
     uint4 held[kMost];
     float2 of_group = make_float2(0.f, 1.f);                       // scales of the eight keys that a lane of the first warp has
     // where the eight keys of a lane of a first warp are in tile n, counted in rows of a head, and their scales
@@ -704,10 +801,11 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     float base = 0.f;
     bool there_is = true;                                          // room for the tile
     for (int n = 0; n < n_tiles; ++n) {
-      const int st = n % kArStages;
+      // tile n of the keys is read in step n of the products, of the values in the one behind it
+      const int at_step = is_k ? n : n + 1, st = at_step & 1;
       const float2 scale = of_group;
       look(n + 1);
-      there_is = there_is && (n < kArStages || wait_all(is_k ? &k_free[st] : &v_free[st], ((n / kArStages) & 1) ^ 1, is_k ? 40 : 41));
+      there_is = there_is && wait_all(&kv_free[st], ((at_step >> 1) & 1) ^ 1, is_k ? 40 : 41);
       if (warp == kSoftmaxWarps) {
         // (S_(n-2) is complete, so the weights of tile n - 3 are made, and the place of tile n - 4 is free)
         const float log_v = log2f(fmaxf(scale.y, 1.17549435e-38f));
@@ -739,166 +837,192 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       together();                                                  // (whoever gave up comes along to the end, and the others' waits run out too)
       if (n + 1 < n_tiles) ask(n + 1);
     }
-  } else if (warp < kSoftmaxWarps && ((warp >> 2) & 1) < groups) {
+  } else if (warp < kSoftmaxWarps) {
     // ---- softmax and output: one or two threads own row r of their group (lane r of tensor memory).  Two, each with half of a tile's
     // keys, give a scheduler two warps of a group, whose exponentials, products and conversions run under each other's.
     const int half = warp >> 3, g = (warp >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane, pair = 1 + (warp & 7);
-    const int mine = g == 0 ? n_first : n_tiles, hi_mine = g == 0 ? hi_first : hi;
-    const int row = g * kArGroupRows + r, pos = pos0 + row;        // rows beyond rows_here compute and store nothing
+    int before = 0, works = 0;                                     // tiles of the group in the work before, and how much work it had
+    bool alive = true;
     const uint32_t lane_addr = tmem + (uint32_t(quarter * 32) << 16);
     const uint32_t s_addr = lane_addr + g * kArKeys + half * kSpan, o_addr = lane_addr + 256 + g * HD + half * (HD / SPLIT);
-    const int first = first_visible(pos, p.window, 0);
-    const int group_pos = pos0 + g * kArGroupRows;                 // of the group's first row
-    const int last_first = first_visible(group_pos + kArGroupRows - 1, p.window, 0);
+    const int row = g * kArGroupRows + r;                          // rows beyond the work's compute and store nothing
     float* const mine_told = &told[half][row];
     const float* const other_told = &told[half ^ (SPLIT - 1)][row];
-    bool alive = true;
-    ArRow rf{CAP ? p.cap_pre : p.scale_log2, p.scale_log2};
-    if constexpr (PAGES) {                                         // q as float16, its largest element between 2^14 and 2^15
-      alive = wait_all(&q_full, 0, 42);
-      unsigned char* const at = q_s + g * KB * kArTile + r * 128;
-      float largest = 0.f, bad = 0.f;
-#pragma unroll 4
-      for (int c = 0; c < HD / 8; ++c) {
-        const uint4 u = *reinterpret_cast<const uint4*>(at + (c >> 3) * kArTile + (((c & 7) ^ (r & 7)) * 16));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = ar_unpack<false>(w[i]);
-          largest = fmaxf(largest, fmaxf(fabsf(f.x), fabsf(f.y)));
-          bad = fmaf(f.x, 0.f, fmaf(f.y, 0.f, bad));               // not-a-number where an element is not finite
+    for (int number = 0; alive && there_is_item(number); ++number) {
+      const ArItem& it = items[number & 1];
+      int mine, hi_mine, key0, a, b, full_from, full_to;
+      {
+        const ArSpan w(p, it);
+        if (g >= w.groups) {
+          leave_item(number);
+          if (PAGES) break;
+          continue;
         }
+        mine = g == 0 ? w.n_first : w.n_tiles;
+        // the keys of this half of the tile that the row may see: [a, b) relative to it; masks only where some row of the group needs one
+        key0 = w.j0 * kArKeys + half * kSpan;
+        a = max(first_visible(w.pos0 + row, p.window, 0), w.lo) - key0;
+        b = min(w.pos0 + row + 1, w.hi) - key0;
+        hi_mine = (g == 0 ? w.hi_first : w.hi) - key0;
+        full_to = w.pos0 + g * kArGroupRows - kSpan + 1 - key0;      // of the group's first row
+        full_from = first_visible(w.pos0 + (g + 1) * kArGroupRows - 1, p.window, 0) - key0;
       }
-      ar_either<SPLIT>(pair, false);                                      // (both have read the row)
-      // 2^(14 - exponent of the largest), and its reciprocal
-      const int e = min(max(int(__float_as_uint(largest) >> 23), 15), 254);
-      const float up = __uint_as_float(uint32_t(268 - e) << 23);
-      rf.factor *= __uint_as_float(uint32_t(e - 14) << 23) + bad;
+      ArRow rf{CAP ? p.cap_pre : p.scale_log2, p.scale_log2};
+      if constexpr (PAGES) {                                         // q as float16, its largest element between 2^14 and 2^15
+        alive = wait_all(&q_full, 0, 42);
+        unsigned char* const at = q_s + g * KB * kArTile + r * 128;
+        float largest = 0.f, bad = 0.f;
 #pragma unroll 4
-      for (int c = half * (HD / 8 / SPLIT); c < (half + 1) * (HD / 8 / SPLIT); ++c) {
-        uint4* const u = reinterpret_cast<uint4*>(at + (c >> 3) * kArTile + (((c & 7) ^ (r & 7)) * 16));
-        uint32_t w[4] = {u->x, u->y, u->z, u->w};
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint4 u = *reinterpret_cast<const uint4*>(at + (c >> 3) * kArTile + (((c & 7) ^ (r & 7)) * 16));
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = ar_unpack<false>(w[i]);
-          w[i] = ar_pack<true>(f.x * up, f.y * up);
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = ar_unpack<false>(w[i]);
+            largest = fmaxf(largest, fmaxf(fabsf(f.x), fabsf(f.y)));
+            bad = fmaf(f.x, 0.f, fmaf(f.y, 0.f, bad));               // not-a-number where an element is not finite
+          }
         }
-        *u = make_uint4(w[0], w[1], w[2], w[3]);
+        ar_either<SPLIT>(pair, false);                                      // (both have read the row)
+        // 2^(14 - exponent of the largest), and its reciprocal
+        const int e = min(max(int(__float_as_uint(largest) >> 23), 15), 254);
+        const float up = __uint_as_float(uint32_t(268 - e) << 23);
+        rf.factor *= __uint_as_float(uint32_t(e - 14) << 23) + bad;
+#pragma unroll 4
+        for (int c = half * (HD / 8 / SPLIT); c < (half + 1) * (HD / 8 / SPLIT); ++c) {
+          uint4* const u = reinterpret_cast<uint4*>(at + (c >> 3) * kArTile + (((c & 7) ^ (r & 7)) * 16));
+          uint32_t w[4] = {u->x, u->y, u->z, u->w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = ar_unpack<false>(w[i]);
+            w[i] = ar_pack<true>(f.x * up, f.y * up);
+          }
+          *u = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tc5::mbar_arrive(&q_ready);
       }
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      __syncwarp();
-      if (lane == 0) tc5::mbar_arrive(&q_ready);
-    }
-    // What the row currently scales by, alike in its two threads: a maximum of its scores.  Prompts begin at zero, which is near enough to
-    // most rows' (weights of bfloat16 are as exact anywhere): their maximum is looked for where weights leave 2^-40 .. 2^20.
-    float m = PAGES ? -INFINITY : 0.f;
-    bool fresh = PAGES;                                            // some row of the warp has none
-    bool settled = PAGES;                                          // the row's was looked for
-    float l = 0.f;                                                 // of this thread's keys
-    for (int n = 0; n < mine; ++n) {
-      alive = alive && wait_all(&s_full[g], n & 1, 43) && (!PAGES || wait_all(&sc_full[n % kArRing], (n / kArRing) & 1, 44));
+      // What the row currently scales by, alike in its two threads: a maximum of its scores.  Prompts begin at zero, which is near enough to
+      // most rows' (weights of bfloat16 are as exact anywhere): their maximum is looked for where weights leave 2^-40 .. 2^20.
+      float m = PAGES ? -INFINITY : 0.f;
+      bool fresh = PAGES;                                            // some row of the warp has none
+      bool settled = PAGES;                                          // the row's was looked for
+      float l = 0.f;                                                 // of this thread's keys
+      for (int n = 0; n < mine; ++n) {
+        alive = alive && wait_all(&s_full[g], (before + n) & 1, 43) && (!PAGES || wait_all(&sc_full[n % kArRing], (n / kArRing) & 1, 44));
+        tc5::fence_after();
+        const ArScales* sc = scales + (n % kArRing) * (kArKeys / 8) + half * (kSpan / 8);
+        const bool full = full_to >= 0 && full_from <= 0;
+        const int chunks = min(max(hi_mine + 31, 0) / 32, CHUNKS);
+        uint32_t packed[16 * CHUNKS];
+        float weights = 0.f, sum = 0.f;
+        if (alive && !fresh && chunks > 0) {
+          const float m_use = (m == -INFINITY) ? 0.f : m;
+          if (full) ar_tile<CHUNKS, CAP, PAGES, false, false>(s_addr, sc, packed, rf, m_use, a, b, chunks, weights, sum);
+          else ar_tile<CHUNKS, CAP, PAGES, true, false>(s_addr, sc, packed, rf, m_use, a, b, chunks, weights, sum);
+        }
+        // (a warp that gave up says so here, and both leave)
+        const bool small = !settled && max(a, 0) < min(b, kSpan) && l + weights < kArLeast;
+        if (ar_either<SPLIT>(pair, fresh || small || weights > (PAGES ? kArMost : kArMostPrompt) || !alive)) {      // hardly ever
+          const float m_use = (m == -INFINITY) ? 0.f : m;
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; alive && c < chunks; ++c) {
+            uint32_t s[32];
+            tc5::ld32(s_addr + uint32_t(c * 32), s);
+            ar_wait32(s);
+            mx = fmaxf(mx, ar_largest<CAP, PAGES>(s, sc + c * 4, rf, m_use, ar_bits(a - c * 32, b - c * 32)));
+          }
+          if (!settled && l >= kArLeast) mx = fmaxf(mx, 0.f);        // (what has weight already is not scaled up)
+          *mine_told = mx;
+          if (lane == 0) left[warp & 7][half] = !alive;
+          ar_either<SPLIT>(pair, false);
+          if (left[warp & 7][0] | left[warp & 7][1]) { alive = false; break; }
+          mx = fmaxf(mx, *other_told);
+          // (a reference that was not looked for may also come down, where nothing of weight has been added)
+          const bool grows = mx != -INFINITY && (m == -INFINITY || mx > 0.f || !settled);
+          const float alpha = grows && m != -INFINITY ? ar_exp2(fminf(-mx, 100.f)) : 1.f;
+          settled = settled || mx != -INFINITY;
+          if (grows) m = m_use + mx;
+          l *= alpha;
+          if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) ar_rescale(o_addr, HD / SPLIT, alpha);
+          if (chunks > 0) ar_tile<CHUNKS, CAP, PAGES, true, true>(s_addr, sc, packed, rf, (m == -INFINITY) ? 0.f : m, a, b, chunks, weights, sum);
+          fresh = __any_sync(0xffffffffu, m == -INFINITY);           // some row of the warp has seen nothing yet
+        }
+        l += sum;
+        if (chunks > 0) {                                            // over products that are read
+          tc5::st32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(packed));
+          if constexpr (SPLIT == 1) tc5::st32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(packed + 32));
+        }
+        tc5::st_wait();
+        tc5::fence_before();
+        __syncwarp();
+        if (lane == 0) tc5::mbar_arrive(&p_full[g]);
+        a -= kArKeys;
+        b -= kArKeys;
+        hi_mine -= kArKeys;
+        full_from -= kArKeys;
+        full_to -= kArKeys;
+      }
+      if (alive) alive = wait_all(&o_full[g], works & 1, 45);
+      before += mine;
+      ++works;
+      *mine_told = l;
+      const bool both_alive = !ar_either<SPLIT>(pair, !alive);
       tc5::fence_after();
-      const ArScales* sc = scales + (n % kArRing) * (kArKeys / 8) + half * (kSpan / 8);
-      const int key0 = (j0 + n) * kArKeys + half * kSpan;
-      // the keys of this half of the tile that the row may see: [a, b) relative to it; masks only where some row of the group needs one
-      const int a = max(first, lo) - key0, b = min(pos + 1, hi) - key0;
-      const bool full = key0 + kSpan - 1 <= group_pos && key0 >= last_first;
-      const int chunks = min(max(hi_mine - key0 + 31, 0) / 32, CHUNKS);
-      uint32_t packed[16 * CHUNKS];
-      float weights = 0.f, sum = 0.f;
-      if (alive && !fresh && chunks > 0) {
-        const float m_use = (m == -INFINITY) ? 0.f : m;
-        if (full) ar_tile<CHUNKS, CAP, PAGES, false, false>(s_addr, sc, packed, rf, m_use, a, b, chunks, weights, sum);
-        else ar_tile<CHUNKS, CAP, PAGES, true, false>(s_addr, sc, packed, rf, m_use, a, b, chunks, weights, sum);
-      }
-      // (a warp that gave up says so here, and both leave)
-      const bool small = !settled && max(a, 0) < min(b, kSpan) && l + weights < kArLeast;
-      if (ar_either<SPLIT>(pair, fresh || small || weights > (PAGES ? kArMost : kArMostPrompt) || !alive)) {      // hardly ever
-        const float m_use = (m == -INFINITY) ? 0.f : m;
-        float mx = -INFINITY;
+      if (both_alive) {
+        const int first_row = it.q_start + it.q0, head = it.head, rows_here = it.rows;
+        if constexpr (SPLIT == 2) l = half == 0 ? l + *other_told : *other_told + l;
+        if (p.sink && m != -INFINITY) l += ar_exp2(p.sink[head] * 1.4426950408889634f - m);
+        const bool none = l == 0.f;                                  // no key: zeros
+        float inv = none ? 0.f : 1.f / l;
+        if constexpr (PAGES) inv *= exp2f(value_base);
+        inv = inv > 3.402823466e38f ? 3.402823466e38f : inv;         // (scores of 2^24 and more: sums may be next to nothing, and O too)
+        bf16* dst = p.out + size_t(first_row + row) * p.out_stride + size_t(head) * p.hd;
+        float sick = 0.f;
 #pragma unroll 1
-        for (int c = 0; alive && c < chunks; ++c) {
-          uint32_t s[32];
-          tc5::ld32(s_addr + uint32_t(c * 32), s);
-          ar_wait32(s);
-          mx = fmaxf(mx, ar_largest<CAP, PAGES>(s, sc + c * 4, rf, m_use, ar_bits(a - c * 32, b - c * 32)));
-        }
-        if (!settled && l >= kArLeast) mx = fmaxf(mx, 0.f);        // (what has weight already is not scaled up)
-        *mine_told = mx;
-        if (lane == 0) left[warp & 7][half] = !alive;
-        ar_either<SPLIT>(pair, false);
-        if (left[warp & 7][0] | left[warp & 7][1]) { alive = false; break; }
-        mx = fmaxf(mx, *other_told);
-        // (a reference that was not looked for may also come down, where nothing of weight has been added)
-        const bool grows = mx != -INFINITY && (m == -INFINITY || mx > 0.f || !settled);
-        const float alpha = grows && m != -INFINITY ? ar_exp2(fminf(-mx, 100.f)) : 1.f;
-        settled = settled || mx != -INFINITY;
-        if (grows) m = m_use + mx;
-        l *= alpha;
-        if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) ar_rescale(o_addr, HD / SPLIT, alpha);
-        if (chunks > 0) ar_tile<CHUNKS, CAP, PAGES, true, true>(s_addr, sc, packed, rf, (m == -INFINITY) ? 0.f : m, a, b, chunks, weights, sum);
-        fresh = __any_sync(0xffffffffu, m == -INFINITY);           // some row of the warp has seen nothing yet
-      }
-      l += sum;
-      if (chunks > 0) {                                            // over products that are read
-        tc5::st32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(packed));
-        if constexpr (SPLIT == 1) tc5::st32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(packed + 32));
-      }
-      tc5::st_wait();
-      tc5::fence_before();
-      __syncwarp();
-      if (lane == 0) tc5::mbar_arrive(&p_full[g]);
-    }
-    if (alive) alive = wait_all(&o_full, 0, 45);
-    *mine_told = l;
-    const bool both_alive = !ar_either<SPLIT>(pair, !alive);
-    tc5::fence_after();
-    if (both_alive) {
-      if constexpr (SPLIT == 2) l = half == 0 ? l + *other_told : *other_told + l;
-      if (p.sink && m != -INFINITY) l += ar_exp2(p.sink[head] * 1.4426950408889634f - m);
-      const bool none = l == 0.f;                                  // no key: zeros
-      float inv = none ? 0.f : 1.f / l;
-      if constexpr (PAGES) inv *= exp2f(value_base);
-      inv = inv > 3.402823466e38f ? 3.402823466e38f : inv;         // (scores of 2^24 and more: sums may be next to nothing, and O too)
-      bf16* dst = p.out + size_t(q_start + q0 + row) * p.out_stride + size_t(head) * p.hd;
-      float sick = 0.f;
-#pragma unroll 1
-      for (int c = 0; c < HD / 32 / SPLIT; ++c) {
-        uint32_t ov[32];
-        tc5::ld32(o_addr + uint32_t(c * 32), ov);                  // (all lanes of the warp take part in the load)
-        ar_wait32(ov);
-        if (row < rows_here) {
-          const int d0 = half * (HD / SPLIT) + c * 32;
+        for (int c = 0; c < HD / 32 / SPLIT; ++c) {
+          uint32_t ov[32];
+          tc5::ld32(o_addr + uint32_t(c * 32), ov);                  // (all lanes of the warp take part in the load)
+          ar_wait32(ov);
+          if (row < rows_here) {
+            const int d0 = half * (HD / SPLIT) + c * 32;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint4 h;
-            uint32_t* hw = reinterpret_cast<uint32_t*>(&h);
+            for (int e = 0; e < 4; ++e) {
+              uint4 h;
+              uint32_t* hw = reinterpret_cast<uint32_t*>(&h);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float x = none ? 0.f : __uint_as_float(ov[e * 8 + 2 * i]) * inv, y = none ? 0.f : __uint_as_float(ov[e * 8 + 2 * i + 1]) * inv;
-              sick = fmaf(x, 0.f, fmaf(y, 0.f, sick));
-              hw[i] = ar_pack<false>(x, y);
+              for (int i = 0; i < 4; ++i) {
+                const float x = none ? 0.f : __uint_as_float(ov[e * 8 + 2 * i]) * inv, y = none ? 0.f : __uint_as_float(ov[e * 8 + 2 * i + 1]) * inv;
+                sick = fmaf(x, 0.f, fmaf(y, 0.f, sick));
+                hw[i] = ar_pack<false>(x, y);
+              }
+              if (d0 + e * 8 < p.hd) *reinterpret_cast<uint4*>(dst + d0 + e * 8) = h;
             }
-            if (d0 + e * 8 < p.hd) *reinterpret_cast<uint4*>(dst + d0 + e * 8) = h;
+          }
+        }
+        if (ar_either<SPLIT>(pair, sick != 0.f)) {                          // (and every element of the rows is written)
+          *mine_told = sick;
+          ar_either<SPLIT>(pair, false);
+          // (the keys that the products of this row's group had: whole tiles, up to the last one's steps of 16 and the block's own)
+          uint32_t odd = half == 0 ? __ballot_sync(0xffffffffu, sick != 0.f || *other_told != 0.f) : 0u;
+          const ArSpan w(p, it);
+          const int from = PAGES ? w.lo : w.j0 * kArKeys, to = min(w.hi, ((g == 0 ? w.hi_first : w.hi) + 15) / 16 * 16);
+          while (odd) {
+            const int who = __ffs(odd) - 1;
+            odd &= odd - 1;
+            const int its = __shfl_sync(0xffffffffu, row, who);
+            ar_again<HD, CAP, PAGES>(p, it.seq, it.q_start, head, first_row + its, w.pos0 + its, first_visible(w.pos0 + its, p.window, 0), from, to);
+            __syncwarp();
           }
         }
       }
-      if (ar_either<SPLIT>(pair, sick != 0.f)) {                          // (and every element of the rows is written)
-        *mine_told = sick;
-        ar_either<SPLIT>(pair, false);
-        // (the keys that the products of this row's group had: whole tiles, up to the last one's steps of 16 and the block's own)
-        uint32_t odd = half == 0 ? __ballot_sync(0xffffffffu, sick != 0.f || *other_told != 0.f) : 0u;
-        const int from = PAGES ? lo : j0 * kArKeys, to = min(hi, (hi_mine + 15) / 16 * 16);
-        while (odd) {
-          const int who = __ffs(odd) - 1;
-          odd &= odd - 1;
-          const int its = __shfl_sync(0xffffffffu, row, who);
-          ar_again<HD, CAP, PAGES>(p, seq, q_start, head, q_start + q0 + its, pos0 + its, first_visible(pos0 + its, p.window, 0), from, to);
-          __syncwarp();
-        }
-      }
+      tc5::fence_before();
+      alive = both_alive;
+      leave_item(number);
+      if (PAGES) break;
     }
-    tc5::fence_before();
   }
   // every role ends here; after a wait that ran out, copies in flight get time to land before the shared memory is given up
   if (abort_flag) {

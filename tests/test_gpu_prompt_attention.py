@@ -87,6 +87,14 @@ def test_a_long_prompt():
     check([1, 1500], 2, 1, 64, window=700)
 
 
+@pytest.mark.parametrize("masks", [dict(), dict(window=90), dict(softcap=20.0, sink=True)])
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 4, 64), (40, 8, 128)])
+def test_more_blocks_than_the_gpu_holds(nh, nkv, hd, masks):
+    """Blocks of one and of two groups of rows, whole and with zeros behind the last row, in any order behind one another."""
+    check([1, 1, 300, 128, 17, 257, 2, 400, 129, 64, 500, 16, 200], nh, nkv, hd, pad=3, gap=2, **masks)
+    check([1] * 9, nh, nkv, hd, **masks)
+
+
 @pytest.mark.parametrize("q_size", [1e-3, 60.0])
 def test_prompts_of_other_sizes(q_size):
     check([400], 4, 2, 128, q_size=q_size)
