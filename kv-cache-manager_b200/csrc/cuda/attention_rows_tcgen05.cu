@@ -210,6 +210,8 @@ __device__ __forceinline__ float2 ar_scores(uint32_t s0, uint32_t s1, float fact
 }
 
 // N products of a row into weights, added to `w2`, and probabilities, added to `l2` (pages).  MASK: only the `seen` of them count.
+// Prompts' rows with few keys have them in masked tiles, whose sums take the weights as they were rounded: a row of one key is its value, and of
+// a few the roundings cancel in part (rows with many see no difference, and full tiles keep the two instructions a pair).
 // AGAIN: the maximum is known, so nothing is above 2^12 but what scores of 2^24 and more are rounded by.
 template <bool CAP, bool PAGES, bool MASK, bool AGAIN, bool SMALL, int N>
 __device__ __forceinline__ void ar_exponentials(const uint32_t (&s)[N], const ArScales* sc, uint32_t* packed, const ArRow& row, float m,
@@ -234,9 +236,10 @@ __device__ __forceinline__ void ar_exponentials(const uint32_t (&s)[N], const Ar
         t.y = seen & (2u << i) ? t.y : -INFINITY;
       }
       if constexpr (AGAIN) t = make_float2(t.x > 12.f ? 12.f : t.x, t.y > 12.f ? 12.f : t.y);      // (not-a-number stays)
-      const float2 e = make_float2(ar_exp2(t.x), ar_exp2(t.y));
-      if (k == 0) g0 = e; else if (k == 1) g1 = e; else if (k == 2) g0 = ar_add2(g0, e); else g1 = ar_add2(g1, e);
+      float2 e = make_float2(ar_exp2(t.x), ar_exp2(t.y));
       packed[i / 2] = ar_pack<PAGES>(e.x, e.y);
+      if constexpr (MASK && !PAGES) e = ar_unpack<false>(packed[i / 2]);
+      if (k == 0) g0 = e; else if (k == 1) g1 = e; else if (k == 2) g0 = ar_add2(g0, e); else g1 = ar_add2(g1, e);
     }
     g0 = ar_add2(g0, g1);
     w2 = ar_add2(w2, g0);

@@ -172,3 +172,13 @@ def test_agrees_with_pages():
                         ctx, nh, nkv, hd, hd ** -0.5)
     _, _, got, want, room = wants[0]
     assert bool(((out.cpu().double().view(n, nh, hd) - got).abs() <= 2 * room).all())
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_a_row_of_one_key_is_its_value(hd, softcap):
+    """Weights enter the sum as they were rounded: p v / p is off by two roundings of 2^-24, less than half a step of the result."""
+    for _, _, got, want, _ in check([1, 2, 130, 300], 4, 2, hd, window=1, softcap=softcap):
+        assert torch.equal(got, want)
+    for _, _, got, want, _ in check([5, 257], 4, 2, hd, softcap=softcap):
+        assert torch.equal(got[:1], want[:1])
