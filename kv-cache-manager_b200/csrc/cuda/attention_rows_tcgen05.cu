@@ -64,7 +64,7 @@ struct RowsParams {
   const bf16* q; long long q_stride;
   const bf16* k; long long k_stride; const bf16* v; long long v_stride;                      // prompts
   const uint8_t* k_codes; const uint8_t* v_codes; const float* k_scale; const float* v_scale;      // pages
-  const int* block_tables; int max_blocks, max_keys;      // keys that a request's table has pages for
+  const int* block_tables; int max_blocks, max_keys;      // keys that a request's table has pages for (prompts: no end)
   const int* tile_seq; const int* tile_q0; int tiles, blocks;      // tiles of 64 rows; a block takes one and its three successors
   const int* seq_q_start; const int* seq_q_len; const int* seq_ctx_len;
   int nh, nkv, hd, block_size, log2_block, num_pages, window;
@@ -384,15 +384,15 @@ template <bool PAGES> struct ArKeys {
   }
 };
 
-// A row whose result is not finite, by a whole warp: if a value that it does not see, of the keys [from, first) and (pos, to) that its
+// A row whose result is not finite, by a whole warp: if a value that it does not see, of the keys [from, first) and (last, to) that its
 // products had, is not finite, the row is attended again, key by key.
 template <int HD, bool CAP, bool PAGES>
-__device__ __noinline__ void ar_again(const RowsParams& p, int seq, int start, int head, int row, int pos, int first, int from, int to) {
+__device__ __noinline__ void ar_again(const RowsParams& p, int seq, int start, int head, int row, int first, int last, int from, int to) {
   const int lane = threadIdx.x & 31, kvh = head / (p.nh / p.nkv);
   const ArKeys<PAGES> keys{p, PAGES ? p.block_tables + size_t(seq) * p.max_blocks : nullptr, start, kvh};
   bool sick = false;
   for (int j = from + lane; j < to; j += 32) {
-    if (j >= first && j <= pos) continue;
+    if (j >= first && j <= last) continue;
     const size_t at = keys.place(j);
     for (int d = 0; d < p.hd; ++d) sick |= !(fabsf(keys.value(at, d)) <= 3.402823466e38f);
   }
@@ -404,7 +404,7 @@ __device__ __noinline__ void ar_again(const RowsParams& p, int seq, int start, i
     q[i] = d < p.hd ? ldf(p.q + size_t(row) * p.q_stride + size_t(head) * p.hd + d) : 0.f;
     o[i] = 0.f;
   }
-  for (int j = first; j <= pos; ++j) {
+  for (int j = first; j <= last; ++j) {
     const size_t at = keys.place(j);
     float s = 0.f;
 #pragma unroll
@@ -484,21 +484,23 @@ __device__ __forceinline__ ArItem ar_item(const RowsParams& p, int x, int y) {
   it.q_start = p.seq_q_start[it.seq];
   it.q_len = p.seq_q_len[it.seq];
   it.rows = max(min(most, it.q_len - it.q0), 0);
-  it.ctx = PAGES ? min(p.seq_ctx_len[it.seq], p.max_keys) : it.q_len;          // (a context ends with its table)
+  it.ctx = PAGES ? p.seq_ctx_len[it.seq] : it.q_len;
   return it;
 }
 
-// What it has to do with keys.
+// What it has to do with keys.  Pages: a context that is longer than its table leaves the rows where they are, and their keys end with the table
+// (rows, groups of rows and whole blocks may then see none; what is said of tiles holds for blocks that see some).
 struct ArSpan {
   int pos0, hi, lo, j0, groups, hi_first, n_tiles, n_first, kvh;
   __device__ __forceinline__ ArSpan(const RowsParams& p, const ArItem& it) {
+    const int keys = p.max_keys;
     pos0 = it.ctx - it.q_len + it.q0;                              // position of the block's first row
-    hi = pos0 + it.rows;                                           // keys [lo, hi) matter to the block
+    hi = min(pos0 + it.rows, keys);                                // keys [lo, hi) matter to the block
     lo = first_visible(pos0, p.window, 0);
     j0 = lo / kArKeys;
     groups = it.rows > kArGroupRows ? 2 : 1;
     // a group's keys end with its last row's own, and so do its tiles
-    hi_first = groups == 1 ? hi : pos0 + kArGroupRows;
+    hi_first = groups == 1 ? hi : min(pos0 + kArGroupRows, keys);
     n_tiles = (hi - 1) / kArKeys - j0 + 1;
     n_first = (hi_first - 1) / kArKeys - j0 + 1;
     kvh = it.head / (p.nh / p.nkv);
@@ -522,6 +524,15 @@ __device__ __forceinline__ bool ar_block_answer(const uint4* answer, int& x, int
   x = int(bx);
   y = int(by);
   return is != 0u;
+}
+
+// Rows that see no key: zeros.
+__device__ __noinline__ void ar_no_key(const RowsParams& p, int row0, int rows, int head) {
+  const int words = p.hd / 8;
+  for (int i = threadIdx.x; i < rows * words; i += blockDim.x) {
+    const int row = i / words, d = (i - row * words) * 8;
+    *reinterpret_cast<uint4*>(p.out + size_t(row0 + row) * p.out_stride + size_t(head) * p.hd + d) = make_uint4(0u, 0u, 0u, 0u);
+  }
 }
 
 template <int HD, bool PAGES> constexpr size_t ar_smem() {
@@ -561,6 +572,13 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   pdl_wait();
   const ArItem begin = ar_item<PAGES>(p, blockIdx.x, blockIdx.y);
   if (begin.rows == 0) return;
+  if constexpr (PAGES) {
+    const ArSpan w(p, begin);
+    if (w.hi <= w.lo) {
+      ar_no_key(p, begin.q_start + begin.q0, begin.rows, begin.head);
+      return;
+    }
+  }
   if (tc5::s32(smem_raw) & 1023) {
     if (threadIdx.x == 0) atomicExch(error, (33 << 16) | int(blockIdx.y & 0xffff));
     return;
@@ -867,7 +885,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         a = max(first_visible(w.pos0 + row, p.window, 0), w.lo) - key0;
         b = min(w.pos0 + row + 1, w.hi) - key0;
         hi_mine = (g == 0 ? w.hi_first : w.hi) - key0;
-        full_to = w.pos0 + g * kArGroupRows - kSpan + 1 - key0;      // of the group's first row
+        full_to = min(w.pos0 + g * kArGroupRows + 1, w.hi) - kSpan - key0;      // of the group's first row
         full_from = first_visible(w.pos0 + (g + 1) * kArGroupRows - 1, p.window, 0) - key0;
       }
       ArRow rf{CAP ? p.cap_pre : p.scale_log2, p.scale_log2};
@@ -1016,7 +1034,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const int who = __ffs(odd) - 1;
             odd &= odd - 1;
             const int its = __shfl_sync(0xffffffffu, row, who);
-            ar_again<HD, CAP, PAGES>(p, it.seq, it.q_start, head, first_row + its, w.pos0 + its, first_visible(w.pos0 + its, p.window, 0), from, to);
+            ar_again<HD, CAP, PAGES>(p, it.seq, it.q_start, head, first_row + its, first_visible(w.pos0 + its, p.window, 0), min(w.pos0 + its, w.hi - 1), from, to);
             __syncwarp();
           }
         }
@@ -1134,6 +1152,7 @@ KVCM_API int kvcm_prompt_attention_bf16(const void* q, long long q_stride, const
   p.k = (const bf16*)k; p.k_stride = k_stride; p.v = (const bf16*)v; p.v_stride = v_stride;
   p.tile_seq = tile_seq; p.tile_q0 = tile_q0; p.tiles = tiles; p.seq_q_start = seq_q_start; p.seq_q_len = seq_q_len;
   p.nh = nh; p.nkv = nkv; p.hd = hd; p.block_size = 1; p.window = window;
+  p.max_keys = 0x7fffffff;
   p.scale_log2 = (softcap > 0.f ? softcap : scale) * 1.4426950408889634f;
   p.cap_pre = softcap > 0.f ? scale / softcap : 0.f;
   p.sink = sink;
