@@ -17,7 +17,7 @@ struct PrefillParams {
   const bf16* q; int q_stride;
   bf16* out; int out_stride;
   const bf16* k_cache; const bf16* v_cache;
-  const int* block_tables; int max_blocks;
+  const int* block_tables; int max_blocks, max_keys;      // keys that a request's table has pages for
   const int* tile_seq; const int* tile_q0;
   const int* seq_q_start; const int* seq_q_len; const int* seq_ctx_len;
   int nh, nkv, block_size, window;
@@ -50,7 +50,7 @@ attn_prefill_kernel(PrefillParams p) {
   const int q_start = p.seq_q_start[seq], q_len = p.seq_q_len[seq], ctx = p.seq_ctx_len[seq];
   const int rows_here = min(BM, q_len - q0);
   const int pos0 = ctx - q_len + q0;                                // position of the tile's first row
-  const int hi = pos0 + rows_here;                                  // keys [lo, hi) matter to the tile
+  const int hi = min(pos0 + rows_here, p.max_keys);                 // keys [lo, hi) matter to the tile (a context ends with its table)
   const int lo = first_visible(pos0, p.window, p.chunk);
   const int* table = p.block_tables + size_t(seq) * p.max_blocks;
 
@@ -63,9 +63,9 @@ attn_prefill_kernel(PrefillParams p) {
   }
   // Tiles: those of the kept first keys that start below the window's first tile, then the window's.
   const int t_first = (lo / kKeyTile) * kKeyTile;
-  const int kend = p.keep_first > 0 ? min(p.keep_first, lo) : 0;    // kept keys below the tile's window: [0, kend)
+  const int kend = p.keep_first > 0 ? min(min(p.keep_first, lo), p.max_keys) : 0;      // kept keys below the tile's window: [0, kend)
   const int n_kept = min((kend + kKeyTile - 1) / kKeyTile, t_first / kKeyTile);
-  const int n_tiles = n_kept + (hi - t_first + kKeyTile - 1) / kKeyTile;
+  const int n_tiles = n_kept + max(hi - t_first + kKeyTile - 1, 0) / kKeyTile;
   const int load_lo = kend > 0 ? 0 : lo;
   auto tile_start = [&](int i) { return i < n_kept ? i * kKeyTile : t_first + (i - n_kept) * kKeyTile; };
   load_kv_tiles<HD>(kbuf, vbuf, p.k_cache, p.v_cache, table, tile_start(0), load_lo, n_kept > 0 ? kend : hi, kvh, p.nkv,
@@ -232,7 +232,9 @@ KVCM_API int kvcm_attention_prefill_keep_bf16(const void* q, int q_stride, void*
   PrefillParams p;
   p.q = (const bf16*)q; p.q_stride = q_stride; p.out = (bf16*)out; p.out_stride = out_stride;
   p.k_cache = (const bf16*)k_cache; p.v_cache = (const bf16*)v_cache;
-  p.block_tables = block_tables; p.max_blocks = max_blocks; p.tile_seq = tile_seq; p.tile_q0 = tile_q0;
+  p.block_tables = block_tables; p.max_blocks = max_blocks;
+  p.max_keys = (long long)max_blocks * block_size < 0x7fffffffll ? max_blocks * block_size : 0x7fffffff;
+  p.tile_seq = tile_seq; p.tile_q0 = tile_q0;
   p.seq_q_start = seq_q_start; p.seq_q_len = seq_q_len; p.seq_ctx_len = seq_ctx_len;
   p.nh = nh; p.nkv = nkv; p.block_size = block_size; p.window = window;
   p.keep_first = window > 0 && keep_first > 0 ? keep_first : 0;

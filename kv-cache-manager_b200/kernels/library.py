@@ -890,19 +890,21 @@ def attention_prefill_q4(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                     ctx.seq_ctx_len.data_ptr(), pages[0].data_ptr(), pages[1].data_ptr(), first, seqs, blocks, nkv, hd, block_size,
                     k_cache.shape[0], window)
     _launched(rc, name, "(hd={}, nkv={})", hd, nkv)
-    _attend_laid_out(q, out, pages, ctx, S, first, blocks, block_size, device, nh, nkv, hd, scale, window, softcap, sink)
+    # (rows are the last ones of a context that ends with its table)
+    _attend_laid_out(q, out, pages, ctx, ctx.seq_ctx_len.clamp(max=blocks * block_size), first, blocks, block_size, device, nh, nkv, hd, scale, window, softcap, sink)
 
 
-def _attend_laid_out(q, out, pages, ctx, S, first, blocks, block_size, device, nh, nkv, hd, scale, window, softcap, sink) -> None:
+def _attend_laid_out(q, out, pages, ctx, lengths, first, blocks, block_size, device, nh, nkv, hd, scale, window, softcap, sink) -> None:
     """A step's portions over the pages that were laid out for them: ``pages`` bfloat16 [2, requests * blocks, nkv, block_size, hd], of the
-    requests from ``first`` on."""
+    requests from ``first`` on.  ``lengths``: contexts, from which rows have their positions; keys end with the pages."""
+    S = lengths.numel()
     with torch.cuda.device(device):
         # tiles of no request become those of one more, which has no row and sees one key
         pad = lambda t, v: torch.nn.functional.pad(t[:S], (0, 1), value=v)
         tables = torch.arange(-first * blocks, (S - first + 1) * blocks, dtype=torch.int32, device=q.device).view(S + 1, blocks)
         tables[S].zero_()
         step = types.SimpleNamespace(
-            seq_q_start=pad(ctx.seq_q_start, 0), seq_q_len=pad(ctx.seq_q_len, 0), seq_ctx_len=pad(ctx.seq_ctx_len, 1).clamp_(max=blocks * block_size),
+            seq_q_start=pad(ctx.seq_q_start, 0), seq_q_len=pad(ctx.seq_q_len, 0), seq_ctx_len=pad(lengths, 1),
             tile_seq=torch.where(ctx.tile_seq < 0, S, ctx.tile_seq), tile_q0=ctx.tile_q0.clamp(min=0), prefill_tiles=ctx.prefill_tiles,
             tile_rows=ctx.tile_rows, options={"attn_prefill": "mma"})
         # ('mma' reads these arrays behind its dependency wait and no key below the window; the other kernel takes the arrays for
@@ -1137,9 +1139,9 @@ def attention_prefill_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                          v_scale: torch.Tensor, block_tables: torch.Tensor, ctx, nh: int, nkv: int, hd: int, scale: float, window: int = 0,
                          softcap: float = 0.0, sink: Optional[torch.Tensor] = None) -> None:
     """Rows of portions longer than one token over a cache in 8 bits; q and out are the step's full bfloat16 row arrays, ``ctx`` has
-    the step's arrays with tiles of 64 rows (tiles of request -1 are none; ``ctx.max_ctx`` is at least the longest context; a context
-    ends with its page table).  Heads of 64 and 128 elements and pages of a multiple of 8 rows: one kernel that turns codes into operands beside
-    the products.  Others, or ``ctx.options['attn_prefill'] == 'unpack'``: the pages that the portions see are laid out in bfloat16
+    the step's arrays with tiles of 64 rows (tiles of request -1 are none; ``ctx.max_ctx`` is at least the longest context; where a context
+    is longer than its page table its rows keep their positions and see the table's keys).  Heads of 64 and 128 elements and pages of a
+    multiple of 8 rows: one kernel that turns codes into operands beside the products.  Others, or ``ctx.options['attn_prefill'] == 'unpack'``: the pages that the portions see are laid out in bfloat16
     (exactly), in scratch of the call, and read by ``attention_prefill``'s 'mma' kernel (where a value that is not a number also reaches
     rows of its tile that do not see it)."""
     name = "attention_prefill_q8"
@@ -1177,7 +1179,7 @@ def attention_prefill_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                     block_tables.shape[1], ctx.seq_q_len.data_ptr(), ctx.seq_ctx_len.data_ptr(), pages[0].data_ptr(), pages[1].data_ptr(),
                     first, seqs, blocks, nkv, hd, block_size, k_cache.shape[0], window)
     _launched(rc, name, "(hd={}, nkv={})", hd, nkv)
-    _attend_laid_out(q, out, pages, ctx, S, first, blocks, block_size, device, nh, nkv, hd, scale, window, softcap, sink)
+    _attend_laid_out(q, out, pages, ctx, ctx.seq_ctx_len, first, blocks, block_size, device, nh, nkv, hd, scale, window, softcap, sink)
 
 
 # ------------------------------------------------------------------ prompts over their own rows

@@ -51,3 +51,12 @@ def test_portions_q8(spans, columns, nh, nkv, hd, masks):
 @pytest.mark.parametrize("masks", MASKS)
 def test_plain_rows_q8(masks):
     check_q8("plain bfloat16", [(5, 1), (900, 1), (40, 200)], 6, 4, 2, 64, 16, 42, options=dict(attention="plain"), **masks)
+
+
+@pytest.mark.parametrize("masks", MASKS)
+@pytest.mark.parametrize("spans,columns", PORTIONS + [([(400, 1), (100, 300)], 12)])
+@pytest.mark.parametrize("nh,nkv,hd,options", [(4, 2, 96, {}), (2, 1, 256, {}), (4, 2, 128, dict(attn_prefill="unpack"))])
+def test_portions_q8_through_laid_out_pages(spans, columns, nh, nkv, hd, options, masks):
+    if masks.get("window") and spans[0][1] == 1:
+        spans = spans[1:]                                           # (single rows behind a window: below)
+    check_q8("laid out", spans, columns, nh, nkv, hd, 16, 43, options=options, **masks)
