@@ -813,7 +813,8 @@ KVCM_API int kvcm_attention_decode_q4_bf16(const void* q, long long q_stride, vo
   if (rc != 0 || num_parts == 1 || cluster_merge) return rc;
   if (num_parts == 0)
     return pdl_launch(attn_decode_shares_kernel, dim3(seqs, nkv * head_tiles), dim3(128), 0, (cudaStream_t)stream, (const float*)p.part_o,
-                      (const float*)p.part_ml, (const int*)p.part_first, seq_ctx_len, p.out, out_stride, nh, nkv, hd, tile_heads, sink);
+                      (const float*)p.part_ml, (const int*)p.part_first, seq_ctx_len, 0x7fffffff, 0, p.out, out_stride, nh, nkv, hd, tile_heads,
+                      sink);
   return pdl_launch(attn_decode_merge_kernel, dim3(seqs, nh), dim3(hd < 64 ? 32 : 64), 0, (cudaStream_t)stream, (const float*)p.part_o,
                     (const float*)p.part_ml, p.out, out_stride, nh, hd, num_parts, p.sink);
 }

@@ -185,10 +185,15 @@ __global__ void __launch_bounds__(kDecodeThreads, HD > 128 ? 1 : 2) attn_decode_
   // one of the same step (step_tables, or a sum of its own), which nothing else makes visible here.
   pdl_launch_dependents();
   pdl_wait();
-  auto length = [&](int s) { return min(p.seq_ctx_len[s], p.max_keys); };     // (a context ends with its table)
+  auto length = [&](int s) { return p.seq_ctx_len[s]; };
   auto first_key = [&](int ctx) { return ctx > 0 ? first_visible(ctx - 1, p.window, 0) : 0; };
-  // a request's cost for each head: its tiles of keys behind the start
-  auto cost_of = [&](int ctx) { return ctx > 0 ? kQ8DStart + (ctx - first_key(ctx) / kQ8DStep * kQ8DStep + kQ8DTile - 1) / kQ8DTile : 0; };
+  // (keys end with the table, wherever the row is)
+  auto keys_of = [&](int ctx) { return min(ctx, p.max_keys); };
+  // a request's cost for each head: its tiles of keys behind the start (no key, no cost)
+  auto cost_of = [&](int ctx) {
+    const int keys = keys_of(ctx), lo = first_key(ctx);
+    return keys > lo ? kQ8DStart + (keys - lo / kQ8DStep * kQ8DStep + kQ8DTile - 1) / kQ8DTile : 0;
+  };
   const int H = p.nkv * head_tiles;
   // ---- where the block's work starts
   int seq, unit_h = 0, at_cost = 0;                                // shares: request, head tile of it, how far in
@@ -244,7 +249,7 @@ __global__ void __launch_bounds__(kDecodeThreads, HD > 128 ? 1 : 2) attn_decode_
   for (;;) {
     // ---- the next piece of work
     Q8Segment w;
-    const int ctx = length(seq), lo = first_key(ctx), base = lo / kQ8DStep * kQ8DStep;
+    const int ctx = length(seq), keys = keys_of(ctx), lo = first_key(ctx), base = lo / kQ8DStep * kQ8DStep;
     w.seq = seq;
     w.slot = -1;
     int of_h;
@@ -253,14 +258,14 @@ __global__ void __launch_bounds__(kDecodeThreads, HD > 128 ? 1 : 2) attn_decode_
       of_h = blockIdx.y;
       const int from = base + int(blockIdx.x) * p.part_size;
       w.begin = max(lo, from);
-      w.end = int(blockIdx.x) + 1 == p.num_parts ? ctx : min(ctx, from + p.part_size);     // (the last one takes what is left)
+      w.end = int(blockIdx.x) + 1 == p.num_parts ? keys : min(keys, from + p.part_size);     // (the last one takes what is left)
       if (p.num_parts > 1 && !p.cluster_merge) w.slot = blockIdx.x;
     } else {
       of_h = unit_h;
       const int n = cost_of(ctx), take = int(min((long long)(n - at_cost), left));
       const int tile0 = max(0, at_cost - kQ8DStart), tile1 = max(0, at_cost + take - kQ8DStart);
       w.begin = max(lo, base + tile0 * kQ8DTile);
-      w.end = min(ctx, base + tile1 * kQ8DTile);
+      w.end = min(keys, base + tile1 * kQ8DTile);
       empty = tile1 <= tile0;                                      // the start alone: the next block takes it
       if (tile0 > 0 || tile1 < n - kQ8DStart) w.slot = 2 * int(blockIdx.x) + (tile0 == 0 ? 1 : 0);
       if (!empty && tile0 == 0 && tid == 0) {                      // who reads the pieces of this request and head: blocks first .. last
@@ -276,7 +281,7 @@ __global__ void __launch_bounds__(kDecodeThreads, HD > 128 ? 1 : 2) attn_decode_
           unit_h = 0;
           before += n;
           if (left > 0)
-            do ++seq; while (length(seq) <= 0);             // (there is more, so there is such a request)
+            do ++seq; while (cost_of(length(seq)) == 0);    // (there is more, so there is such a request)
         }
       }
       if (empty) {
@@ -709,7 +714,7 @@ KVCM_API int kvcm_attention_decode_q8_bf16(const void* q, long long q_stride, vo
   if (rc != 0 || num_parts == 1 || cluster_merge) return rc;
   if (num_parts == 0)
     return pdl_launch(attn_decode_shares_kernel, dim3(seqs, nkv * head_tiles), dim3(128), 0, (cudaStream_t)stream, (const float*)p.part_o,
-                      (const float*)p.part_ml, (const int*)p.part_first, seq_ctx_len, p.out, out_stride, nh, nkv, hd, kDecodeHeads, sink);
+                      (const float*)p.part_ml, (const int*)p.part_first, seq_ctx_len, p.max_keys, window, p.out, out_stride, nh, nkv, hd, kDecodeHeads, sink);
   return pdl_launch(attn_decode_merge_kernel, dim3(seqs, nh), dim3(hd < 64 ? 32 : 64), 0, (cudaStream_t)stream, (const float*)p.part_o,
                     (const float*)p.part_ml, p.out, out_stride, nh, hd, num_parts, p.sink);
 }

@@ -14,7 +14,7 @@ constexpr int kDecodeHeads = 8;                    // most query heads of a bloc
 constexpr int kDecodeClusterParts = 8;
 
 // The partitions of a cluster: every block has its partial result in its own shared memory (bo [8][HD], bm maximum, bl sum; an
-// empty partition has bm = -inf and no bo).  The outputs are dealt out over the blocks, four adjacent elements an item; each adds
+// empty partition has bl = 0, a bm below every score, and no bo that is read).  The outputs are dealt out over the blocks, four adjacent elements an item; each adds
 // the partitions up in their order.
 template <int HD, typename Params>
 __device__ __forceinline__ void decode_cluster_tail(const Params& p, int seq, int head0, int heads_here, float* bo, float* bm, float* bl) {
@@ -42,7 +42,7 @@ __device__ __forceinline__ void decode_cluster_tail(const Params& p, int seq, in
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kDecodeClusterParts; ++i) {
-      if (l[i] == 0.f) continue;                                   // nothing there, and its bo is not written
+      if (l[i] == 0.f) continue;                                   // nothing there
       const float f = fast_exp2(m[i] - top);
       acc.x = fmaf(f, o[i].x, acc.x); acc.y = fmaf(f, o[i].y, acc.y); acc.z = fmaf(f, o[i].z, acc.z); acc.w = fmaf(f, o[i].w, acc.w);
       sum = fmaf(f, l[i], sum);
@@ -79,13 +79,14 @@ static __global__ void attn_decode_merge_kernel(const float* part_o, const float
 }
 
 // The pieces of a request and its four or eight heads that blocks part_first[0] .. part_first[1] have left, in their order: the first
-// block's lies in its second place, the others' in their first.  Up to six are asked for at once, maxima, sums and outputs in one trip
+// block's lies in its second place, the others' in their first.  A row whose window begins at `max_keys` or behind it has none.  Up to six are asked for at once, maxima, sums and outputs in one trip
 // to memory (64 ragged requests in all 1.3 us less).  A long request has many: the weights of 128 of them at a time are formed
 // side by side, so that what follows one another is additions.
 constexpr int kDecodeJoinAtOnce = 128;
 constexpr int kDecodeJoinFew = 6;
 static __global__ void __launch_bounds__(128) attn_decode_shares_kernel(const float* part_o, const float* part_ml, const int* part_first,
-                                                                    const int* __restrict__ seq_ctx_len, bf16* __restrict__ out,
+                                                                    const int* __restrict__ seq_ctx_len, int max_keys, int window,
+                                                                    bf16* __restrict__ out,
                                                                     long long out_stride, int nh, int nkv, int hd, int tile_heads,
                                                                     const float* __restrict__ sink) {
   __shared__ float weight[kDecodeJoinAtOnce][kDecodeHeads];
@@ -96,7 +97,8 @@ static __global__ void __launch_bounds__(128) attn_decode_shares_kernel(const fl
   const int seq = blockIdx.x, h = blockIdx.y, kvh = h / head_tiles, ht = h - kvh * head_tiles;
   const int head0 = kvh * G + ht * tile_heads, heads_here = min(tile_heads, G - ht * tile_heads);
   const int tid = threadIdx.x, quads = hd / 4, items = heads_here * quads;
-  if (seq_ctx_len[seq] <= 0) {
+  const int ctx = seq_ctx_len[seq];
+  if (ctx <= 0 || max_keys <= first_visible(ctx - 1, window, 0)) {        // no key
     for (int it = tid; it < items; it += 128) {
       const int r = it / quads, d = (it - r * quads) * 4;
       *reinterpret_cast<uint2*>(out + size_t(seq) * out_stride + size_t(head0 + r) * hd + d) = make_uint2(0u, 0u);

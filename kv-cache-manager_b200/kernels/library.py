@@ -1077,7 +1077,8 @@ def attention_decode_q8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tenso
     """Single-row entries over a cache in 8 bits: q and out hold one bfloat16 row a request, in the order of the batch's entries;
     ``ctx.seq_ctx_len`` says how many keys each sees (0: the row is zero), ``ctx.max_decode_ctx`` is about the longest: the keys are
     divided by it, and beyond it one block takes what is left.
-    ``window``: the last ``window`` keys only; ``softcap``, ``sink`` as in ``attention_plain``."""
+    ``window``: the last ``window`` keys only (where a context is longer than its page table: those of them that the table has; none: zeros);
+    ``softcap``, ``sink`` as in ``attention_plain``."""
     name = "attention_decode_q8"
     S, lengths = q.shape[0], ctx.seq_ctx_len
     _attention_rows(name, q, out, nh, nkv, hd, window, softcap, sink)

@@ -57,6 +57,12 @@ def test_plain_rows_q8(masks):
 @pytest.mark.parametrize("spans,columns", PORTIONS + [([(400, 1), (100, 300)], 12)])
 @pytest.mark.parametrize("nh,nkv,hd,options", [(4, 2, 96, {}), (2, 1, 256, {}), (4, 2, 128, dict(attn_prefill="unpack"))])
 def test_portions_q8_through_laid_out_pages(spans, columns, nh, nkv, hd, options, masks):
-    if masks.get("window") and spans[0][1] == 1:
-        spans = spans[1:]                                           # (single rows behind a window: below)
     check_q8("laid out", spans, columns, nh, nkv, hd, 16, 43, options=options, **masks)
+
+
+@pytest.mark.parametrize("masks", MASKS + [dict(window=900)])
+@pytest.mark.parametrize("options", [{}, dict(attn_parts=1), dict(attn_parts=4), dict(attn_parts=11), dict(attn_parts=4, attn_merge="kernel"), dict(attn_parts=-1)])
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 128), (12, 1, 64), (4, 4, 96)])
+def test_single_rows_q8(nh, nkv, hd, options, masks):
+    """Windows inside the table, across its end and behind it; contexts that fit between them."""
+    check_q8("single", [(2500, 1), (100, 1), (1000, 1), (959, 1), (960, 1), (1023, 1), (1300, 1), (0, 1), (1059, 1)], 60, nh, nkv, hd, 16, 44, options=options, **masks)
