@@ -231,7 +231,7 @@ unpack_pages_q4_kernel(const uint8_t* k_cache, const uint8_t* v_cache, const int
   pdl_launch_dependents();
   pdl_wait();
   const int seq = first_seq + blockIdx.y, block = blockIdx.x;
-  const int ctx = seq_ctx_len[seq];
+  const int ctx = int(min((long long)seq_ctx_len[seq], (long long)blocks * block_size));      // (a context ends with its table, and so do its rows)
   const int lo = first_visible(ctx - seq_q_len[seq], window, 0);
   if (block * block_size >= ctx || (block + 1) * block_size <= lo) return;
   const int words = hd / 8, per_head = block_size * words;
