@@ -36,7 +36,7 @@ struct DecodeParams {
   int keep_first;                      // with a window: the first keep_first keys of a request stay visible to every row
   int chunk;                           // > 0: only the keys of the position's own chunk of this many positions
   float scale_log2;                    // what a score is multiplied by on its way into exp2
-  float cap_pre;                       // > 0: capped scores, s <- tanh(s * cap_pre) first (cap_pre = scale / cap, scale_log2 = cap * log2 e)
+  float cap_pre;                       // not 0: capped scores, s <- tanh(s * cap_pre) first (cap_pre = scale / cap, scale_log2 = cap * log2 e)
   const float* sink;                   // per head, or null: exp(sink) joins the denominator where the result is normalised
   int log2_block;                      // log2(block_size) when it is a power of two, else -1
   int cluster_merge;                   // the partitions of a (request, head group) are one cluster
@@ -272,14 +272,14 @@ attn_decode_kernel(DecodeParams p) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[h][j] = (p.cap_pre > 0.f ? fast_tanh(s[h][j] * p.cap_pre) : s[h][j]) * p.scale_log2;
+          for (int j = 0; j < 4; ++j) s[h][j] = (p.cap_pre != 0.f ? fast_tanh(s[h][j] * p.cap_pre) : s[h][j]) * p.scale_log2;
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = kb + 8 * h + 2 * t4 + (j & 1);
-            const float capped = (p.cap_pre > 0.f ? fast_tanh(s[h][j] * p.cap_pre) : s[h][j]) * p.scale_log2;
+            const float capped = (p.cap_pre != 0.f ? fast_tanh(s[h][j] * p.cap_pre) : s[h][j]) * p.scale_log2;
             s[h][j] = ((key >= begin && key < end) || (has_kept && key < kend)) ? capped : -INFINITY;
           }
       }
@@ -509,8 +509,9 @@ KVCM_API int kvcm_attention_decode_keep_bf16(const void* q, int q_stride, void* 
   p.keep_first = window > 0 && keep_first > 0 ? keep_first : 0;
   p.chunk = chunk;
   p.part_size = part_size; p.num_parts = num_parts; p.cluster_merge = cluster_merge;
-  p.scale_log2 = (softcap > 0.f ? softcap : scale) * 1.4426950408889634f;
+  // (capped scores of a scale that is zero beside the cap are all zero, which no cap is needed for)
   p.cap_pre = softcap > 0.f ? scale / softcap : 0.f;
+  p.scale_log2 = (softcap <= 0.f ? scale : p.cap_pre != 0.f ? softcap : 0.f) * 1.4426950408889634f;
   p.sink = sink;
   p.order = nullptr;
   p.log2_block = -1;

@@ -24,7 +24,7 @@ struct PrefillParams {
   int keep_first;                   // with a window: the first keep_first keys of a request stay visible to every row
   int chunk;                        // > 0: only the keys of a row's own chunk of this many positions
   float scale_log2;                 // what a score is multiplied by on its way into exp2
-  float cap_pre;                    // > 0: capped scores, s <- tanh(s * cap_pre) first (cap_pre = scale / cap, scale_log2 = cap * log2 e)
+  float cap_pre;                    // not 0: capped scores, s <- tanh(s * cap_pre) first (cap_pre = scale / cap, scale_log2 = cap * log2 e)
   const float* sink;                // per head, or null: exp(sink) joins every row's denominator at the end
   int log2_block;
 };
@@ -134,7 +134,7 @@ attn_prefill_kernel(PrefillParams p) {
       for (int n = 0; n < kKeyTile / 8; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float v = (p.cap_pre > 0.f ? fast_tanh(s[n][j] * p.cap_pre) : s[n][j]) * p.scale_log2;
+          float v = (p.cap_pre != 0.f ? fast_tanh(s[n][j] * p.cap_pre) : s[n][j]) * p.scale_log2;
           if (needs_mask) {
             const int key = t0 + 8 * n + 2 * t4 + (j & 1);
             const int rp = row_pos[j >> 1];
@@ -239,8 +239,9 @@ KVCM_API int kvcm_attention_prefill_keep_bf16(const void* q, int q_stride, void*
   p.nh = nh; p.nkv = nkv; p.block_size = block_size; p.window = window;
   p.keep_first = window > 0 && keep_first > 0 ? keep_first : 0;
   p.chunk = chunk;
-  p.scale_log2 = (softcap > 0.f ? softcap : scale) * 1.4426950408889634f;
+  // (capped scores of a scale that is zero beside the cap are all zero, which no cap is needed for)
   p.cap_pre = softcap > 0.f ? scale / softcap : 0.f;
+  p.scale_log2 = (softcap <= 0.f ? scale : p.cap_pre != 0.f ? softcap : 0.f) * 1.4426950408889634f;
   p.sink = sink;
   p.log2_block = -1;
   for (int b = 0; b < 16; ++b) if ((1 << b) == block_size) p.log2_block = b;

@@ -1066,8 +1066,7 @@ int launch_rows_as(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
   return pdl_launch(attention_rows_kernel<HD, CAP, PAGES>, grid, dim3(ar_threads<PAGES>()), ar_smem<HD, PAGES>(), s, mq, mk, mv, p);
 }
 template <bool PAGES>
-int launch_rows(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const RowsParams& p, dim3 grid, cudaStream_t s) {
-  const bool cap = p.cap_pre > 0.f;
+int launch_rows(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const RowsParams& p, bool cap, dim3 grid, cudaStream_t s) {
   if (p.hd <= 64) return cap ? launch_rows_as<64, true, PAGES>(mq, mk, mv, p, grid, s) : launch_rows_as<64, false, PAGES>(mq, mk, mv, p, grid, s);
   return cap ? launch_rows_as<128, true, PAGES>(mq, mk, mv, p, grid, s) : launch_rows_as<128, false, PAGES>(mq, mk, mv, p, grid, s);
 }
@@ -1129,7 +1128,7 @@ KVCM_API int kvcm_attention_prefill_q8_bf16(const void* q, long long q_stride, i
   p.log2_block = -1;
   for (int b = 0; b < 31; ++b) if ((1 << b) == block_size) p.log2_block = b;
   p.blocks = rows_blocks(tiles, portions);
-  return launch_rows<true>(mq, mq, mq, p, dim3(nh, p.blocks), (cudaStream_t)stream);
+  return launch_rows<true>(mq, mq, mq, p, softcap > 0.f, dim3(nh, p.blocks), (cudaStream_t)stream);
 }
 
 // q, k and v: rows of the prompts, one behind another; entries [0, singles) are prompts of one row, tiles name those of at most `portions`
@@ -1159,7 +1158,7 @@ KVCM_API int kvcm_prompt_attention_bf16(const void* q, long long q_stride, const
   p.error = const_cast<int*>(kvcm_attention_tcgen05_error_address());
   if (p.error == nullptr) return KVCM_ERR_UNSUPPORTED;
   p.blocks = rows_blocks(tiles, portions);
-  return p.blocks + singles == 0 ? 0 : launch_rows<false>(mq, mk, mv, p, dim3(nh, p.blocks + singles), (cudaStream_t)stream);
+  return p.blocks + singles == 0 ? 0 : launch_rows<false>(mq, mk, mv, p, softcap > 0.f, dim3(nh, p.blocks + singles), (cudaStream_t)stream);
 }
 
 KVCM_PACKED(kvcm_attention_prefill_q8_bf16)

@@ -59,7 +59,7 @@ struct PrefillTcParams {
   int keep_first;                   // with a window: keys below this stay visible to every later row (0: none)
   int chunk;                        // > 0: only the keys of a row's own chunk of this many positions
   float scale_log2;                 // what a score is multiplied by on its way into exp2
-  float cap_pre;                    // > 0: scores are capped, s <- tanh(s * cap_pre) first (cap_pre = scale / cap and
+  float cap_pre;                    // not 0: scores are capped, s <- tanh(s * cap_pre) first (cap_pre = scale / cap and
                                     // scale_log2 = cap * log2(e))
   const float* sink;                // per head, or null: exp(sink) joins the row's denominator at the end
 };
@@ -267,7 +267,7 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
       __syncwarp();
       if (lane == 0) tc5::mbar_arrive(&s_free[n & 1]);                // S_(n+2) may be written
-      if (p.cap_pre > 0.f) {
+      if (p.cap_pre != 0.f) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -485,8 +485,9 @@ KVCM_API int kvcm_attention_prefill_tcgen05_bf16(const void* q, int q_stride, in
   p.nh = nh; p.nkv = nkv; p.block_size = block_size; p.window = window;
   p.keep_first = window > 0 ? keep_first : 0;
   p.chunk = chunk;
-  p.scale_log2 = (softcap > 0.f ? softcap : scale) * 1.4426950408889634f;
+  // (capped scores of a scale that is zero beside the cap are all zero, which no cap is needed for)
   p.cap_pre = softcap > 0.f ? scale / softcap : 0.f;
+  p.scale_log2 = (softcap <= 0.f ? scale : p.cap_pre != 0.f ? softcap : 0.f) * 1.4426950408889634f;
   p.sink = sink;
   const dim3 grid(nh, tiles);
   cudaStream_t s = (cudaStream_t)stream;
