@@ -466,6 +466,7 @@ KVCM_API int kvcm_attention_prefill_tcgen05_bf16(const void* q, int q_stride, in
   if (!kvcm_attention_tcgen05_supports_kv(hd, block_size, k_cache == v_cache) || nkv <= 0 || nh % nkv || keep_first < 0 ||
       chunk < 0 || (chunk > 0 && keep_first > 0))
     return KVCM_ERR_UNSUPPORTED;
+  if (scale < 0.f && softcap <= 0.f) return KVCM_ERR_UNSUPPORTED;        // (a row's largest score is the largest product)
   if ((q_stride % 8) || (out_stride % 8) || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) ||
       (reinterpret_cast<uintptr_t>(k_cache) & 15) || (reinterpret_cast<uintptr_t>(v_cache) & 15))
     return KVCM_ERR_UNSUPPORTED;

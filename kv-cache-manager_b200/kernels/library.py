@@ -534,7 +534,7 @@ def attention_prefill(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     """Rows of portions longer than one token; q/out are the step's full row arrays.
     ``ctx.options['attn_prefill']``: 'tcgen05' | 'mma' force a kernel; 'auto' takes the tcgen05
     kernel where it supports the sizes (head_dim 64 or 128, 256 when keys and values are the same pages; pages of
-    8 to 64 keys dividing 64, or multiples of 64)."""
+    8 to 64 keys dividing 64, or multiples of 64) and the scale is not negative."""
     _cuda(q, out, k_cache, v_cache, block_tables, sink)
     _need(sink is None or (sink.dtype == torch.float32 and sink.is_contiguous() and sink.numel() == nh),
           "attention_prefill: sink float32 [heads]")
@@ -548,7 +548,7 @@ def attention_prefill(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     B = k_cache.shape[2]
     kept = int(keep_first) if window > 0 else 0
     shared_kv = k_cache.data_ptr() == v_cache.data_ptr()
-    if mode != "mma" and (mode == "tcgen05" or prefill_tcgen05_supported(hd, B, shared_kv)):
+    if mode != "mma" and (mode == "tcgen05" or (prefill_tcgen05_supported(hd, B, shared_kv) and (scale >= 0.0 or softcap > 0.0))):
         _need(out.data_ptr() % 16 == 0 and out.stride(0) % 8 == 0, "attention_prefill: out rows must be 16-byte aligned")
         rc = _lib().kvcm_attention_prefill_tcgen05_bf16(
             _p(q), q.stride(0), q.shape[0], _p(out), out.stride(0), _p(k_cache), _p(v_cache), k_cache.shape[0],
