@@ -35,7 +35,8 @@
 // a prompt of 8,192 rows 445 us (1,235 TFLOP/s; 520 after seconds of it, under the power cap), four portions of about 1,500 rows behind
 // 5,000 keys 683 (740 TFLOP/s); 16 ragged prompts of some 600 rows, 16 heads, window, capped, sinks 104; five of 110 rows of heads of 64 17.
 //
-// Every wait is bounded; one that runs out sets the error word of the tcgen05 attention family (codes 33 and up) and ends the block.
+// Every wait for a barrier in memory is bounded; one that runs out sets the error word of the tcgen05 attention family (codes 33 and up) and ends the
+// block.  Warps that wait for one another at named barriers, which have no limit, take every such step together whatever they saw.
 #include <cuda_fp16.h>
 
 #include "packed.cuh"
@@ -869,7 +870,9 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const int row = g * kArGroupRows + r;                          // rows beyond the work's compute and store nothing
     float* const mine_told = &told[half][row];
     const float* const other_told = &told[half ^ (SPLIT - 1)][row];
-    for (int number = 0; alive && there_is_item(number); ++number) {
+    for (int number = 0; alive; ++number) {
+      // (the two warps of the same rows go on or leave together: each waits for the other at their barrier, and that wait has no limit)
+      if (ar_either<SPLIT>(pair, !there_is_item(number))) break;
       const ArItem& it = items[number & 1];
       int mine, hi_mine, key0, a, b, full_from, full_to;
       {
