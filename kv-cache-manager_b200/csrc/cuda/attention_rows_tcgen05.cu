@@ -35,8 +35,8 @@
 // a prompt of 8,192 rows 445 us (1,235 TFLOP/s; 520 after seconds of it, under the power cap), four portions of about 1,500 rows behind
 // 5,000 keys 683 (740 TFLOP/s); 16 ragged prompts of some 600 rows, 16 heads, window, capped, sinks 104; five of 110 rows of heads of 64 17.
 //
-// Every wait for a barrier in memory is bounded; one that runs out sets the error word of the tcgen05 attention family (codes 33 and up) and ends the
-// block.  Warps that wait for one another at named barriers, which have no limit, take every such step together whatever they saw.
+// Every wait for a barrier in memory is bounded (a second, in which no warp of the block has said that it is attending rows once more); one that
+// runs out sets the error word of the tcgen05 attention family (codes 33 and up) and ends the block.  Warps that wait for one another at named barriers, which have no limit, take every such step together whatever they saw.
 #include <cuda_fp16.h>
 
 #include "packed.cuh"
@@ -76,8 +76,10 @@ struct RowsParams {
 
 namespace {
 
+typedef volatile unsigned long long ArBeat;        // when a warp of the block was last seen at work that may take longer than a wait's limit
+
 // tc5::mbar_wait for waits of a microsecond: the thread sleeps in the instruction and does not take its scheduler's turns.
-__device__ __forceinline__ bool ar_wait(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool ar_wait(uint64_t* bar, uint32_t parity, const ArBeat* beat) {
   unsigned long long start = 0;
   for (;;) {
     uint32_t done;
@@ -86,7 +88,7 @@ __device__ __forceinline__ bool ar_wait(uint64_t* bar, uint32_t parity) {
     if (done) return true;
     const unsigned long long now = tc5::now_ns();
     if (start == 0) start = now;
-    else if (now - start > tc5::kWaitLimitNs) return false;
+    else if (now - start > tc5::kWaitLimitNs && (long long)(now - *beat) > (long long)tc5::kWaitLimitNs) return false;
   }
 }
 
@@ -375,57 +377,54 @@ template <bool PAGES> struct ArKeys {
       return size_t(start) + key;
     }
   }
-  __device__ __forceinline__ float key(size_t at, int d) const {
-    if constexpr (PAGES) return q8::floats2(p.k_codes[at * p.hd + d]).x * p.k_scale[at / p.block_size];
-    else return ldf(p.k + at * p.k_stride + size_t(kvh) * p.hd + d);
+  __device__ __forceinline__ static void floats8(uint4 u, float (&x)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = ar_unpack<false>(w[i]);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
   }
-  __device__ __forceinline__ float value(size_t at, int d) const {
-    if constexpr (PAGES) return q8::floats2(p.v_codes[at * p.hd + d]).x * p.v_scale[at / p.block_size];
-    else return ldf(p.v + at * p.v_stride + size_t(kvh) * p.hd + d);
+  // Elements 8 c .. 8 c + 7.
+  __device__ __forceinline__ void key8(size_t at, int c, float (&x)[8]) const { eight(true, at, c, x); }
+  __device__ __forceinline__ void value8(size_t at, int c, float (&x)[8]) const { eight(false, at, c, x); }
+  __device__ __forceinline__ void eight(bool is_k, size_t at, int c, float (&x)[8]) const {
+    if constexpr (PAGES) {
+      const uint2 u = *reinterpret_cast<const uint2*>((is_k ? p.k_codes : p.v_codes) + at * p.hd + c * 8);
+      const float scale = (is_k ? p.k_scale : p.v_scale)[at / p.block_size];
+      q8::values4(u.x, scale, x);
+      q8::values4(u.y, scale, x + 4);
+    } else {
+      floats8(*reinterpret_cast<const uint4*>((is_k ? p.k + at * p.k_stride : p.v + at * p.v_stride) + size_t(kvh) * p.hd + c * 8), x);
+    }
+  }
+  // Elements N lane .. N lane + N - 1 of a value, N = 2 or 4; zeros behind the head's.
+  template <int N> __device__ __forceinline__ void value(size_t at, float (&x)[N]) const {
+    const int d = N * int(threadIdx.x & 31);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 0.f;
+    if (d >= p.hd) return;
+    if constexpr (PAGES) {
+      const float scale = p.v_scale[at / p.block_size];
+      const uint8_t* const from = p.v_codes + at * p.hd + d;
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float2 f = q8::floats2(*reinterpret_cast<const uint16_t*>(from + i));
+        x[i] = f.x * scale;
+        x[i + 1] = f.y * scale;
+      }
+    } else {
+      const bf16* const from = p.v + at * p.v_stride + size_t(kvh) * p.hd + d;
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float2 f = ar_unpack<false>(*reinterpret_cast<const uint32_t*>(from + i));
+        x[i] = f.x;
+        x[i + 1] = f.y;
+      }
+    }
   }
 };
-
-// A row whose result is not finite, by a whole warp: if a value that it does not see, of the keys [from, first) and (last, to) that its
-// products had, is not finite, the row is attended again, key by key.
-template <int HD, bool CAP, bool PAGES>
-__device__ __noinline__ void ar_again(const RowsParams& p, int seq, int start, int head, int row, int first, int last, int from, int to) {
-  const int lane = threadIdx.x & 31, kvh = head / (p.nh / p.nkv);
-  const ArKeys<PAGES> keys{p, PAGES ? p.block_tables + size_t(seq) * p.max_blocks : nullptr, start, kvh};
-  bool sick = false;
-  for (int j = from + lane; j < to; j += 32) {
-    if (j >= first && j <= last) continue;
-    const size_t at = keys.place(j);
-    for (int d = 0; d < p.hd; ++d) sick |= !(fabsf(keys.value(at, d)) <= 3.402823466e38f);
-  }
-  if (!__any_sync(0xffffffffu, sick)) return;
-  float q[HD / 32], o[HD / 32], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < HD / 32; ++i) {
-    const int d = i * 32 + lane;
-    q[i] = d < p.hd ? ldf(p.q + size_t(row) * p.q_stride + size_t(head) * p.hd + d) : 0.f;
-    o[i] = 0.f;
-  }
-  for (int j = first; j <= last; ++j) {
-    const size_t at = keys.place(j);
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i)
-      if (i * 32 + lane < p.hd) s = fmaf(q[i], keys.key(at, i * 32 + lane), s);
-    s = warp_sum(s);
-    const float x = CAP ? ar_tanh(s * p.cap_pre) * p.scale_log2 : s * p.scale_log2;
-    const float top = x > m ? x : m, f = m == -INFINITY ? 0.f : ar_exp2(m - top), e = x == -INFINITY ? 0.f : ar_exp2(x - top);
-    m = top;
-    l = fmaf(l, f, e);
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i)
-      if (i * 32 + lane < p.hd) o[i] = fmaf(e, keys.value(at, i * 32 + lane), o[i] * f);
-  }
-  if (p.sink && m != -INFINITY) l += ar_exp2(p.sink[head] * 1.4426950408889634f - m);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int i = 0; i < HD / 32; ++i)
-    if (i * 32 + lane < p.hd) stf(p.out + size_t(row) * p.out_stride + size_t(head) * p.hd + i * 32 + lane, l == 0.f ? 0.f : o[i] * inv);
-}
 
 // 16 codes (elements 16 ch .. 16 ch + 15 of row r) as float16 into a 128-byte swizzled tile [HD/64][128 rows][64].  The lanes of a
 // row's second block write their halves the other way round, so that eight lanes meet in no bank.
@@ -508,6 +507,87 @@ struct ArSpan {
   }
 };
 
+// A row whose result is not finite, by a whole warp: if a value that it does not see, of the keys [from, first) and (last, to) that its
+// products had, is not finite, the row is attended again without the tensor cores: 32 keys at a time, a lane a key for the scores and
+// a lane two or four elements for the output.  That takes its time (32 rows behind 100,000 keys half a second), so the warp says
+// now and then that it is at work, and nobody's wait runs out meanwhile.
+template <int HD, bool CAP, bool PAGES>
+__device__ __forceinline__ void ar_again(const RowsParams& p, ArBeat* beat, int seq, int start, int head, int row, int first, int last, int from, int to) {
+  constexpr int N = HD / 32;
+  const int lane = threadIdx.x & 31, kvh = head / (p.nh / p.nkv), words = p.hd / 8;
+  const ArKeys<PAGES> keys{p, PAGES ? p.block_tables + size_t(seq) * p.max_blocks : nullptr, start, kvh};
+  bool sick = false;
+  for (int j = from + lane; j < to; j += 32) {
+    if (j >= first && j <= last) continue;
+    const size_t at = keys.place(j);
+    for (int c = 0; c < words; ++c) {
+      float x[8];
+      keys.value8(at, c, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sick |= !(fabsf(x[e]) <= 3.402823466e38f);
+    }
+  }
+  if (!__any_sync(0xffffffffu, sick)) return;
+  const uint4* const q = reinterpret_cast<const uint4*>(p.q + size_t(row) * p.q_stride + size_t(head) * p.hd);
+  float o[N], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = 0.f;
+#pragma unroll 1
+  for (int j0 = first; j0 <= last; j0 += 32) {
+    const int n = min(32, last - j0 + 1);
+    if (lane == 0) *beat = tc5::now_ns();
+    float x = -INFINITY;
+    size_t at = 0;
+    if (lane < n) {
+      at = keys.place(j0 + lane);
+      float s = 0.f;
+#pragma unroll 2
+      for (int c = 0; c < words; ++c) {
+        float k[8], w[8];
+        keys.key8(at, c, k);
+        keys.floats8(q[c], w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(w[e], k[e], s);
+      }
+      x = CAP ? ar_tanh(s * p.cap_pre) * p.scale_log2 : s * p.scale_log2;
+    }
+    const float top = fmaxf(m, warp_max(x)), f = m == -INFINITY ? 0.f : ar_exp2(m - top), e = x == -INFINITY ? 0.f : ar_exp2(x - top);
+    m = top;
+    l = fmaf(l, f, warp_sum(e));
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] *= f;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {                                  // (more at once take registers from the kernel around the call: 2 % of packed prompts)
+      float v[N];
+      keys.template value<N>(__shfl_sync(0xffffffffu, (unsigned long long)at, k), v);
+      const float w = __shfl_sync(0xffffffffu, e, k);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = fmaf(w, v[i], o[i]);
+    }
+  }
+  if (p.sink && m != -INFINITY) l += ar_exp2(p.sink[head] * 1.4426950408889634f - m);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (N * lane < p.hd) stf(p.out + size_t(row) * p.out_stride + size_t(head) * p.hd + N * lane + i, l == 0.f ? 0.f : o[i] * inv);
+}
+
+// The rows `odd` of the warp's 32 rows of group g.
+template <int HD, bool CAP, bool PAGES>
+__device__ __noinline__ void ar_redo(const RowsParams& p, ArBeat* beat, const ArItem& it, int g, uint32_t odd) {
+  const ArSpan w(p, it);
+  const int row0 = g * kArGroupRows + int(threadIdx.x >> 5 & 3) * 32;
+  // (the keys that the products of the group had: whole tiles, up to the last one's steps of 16 and the block's own)
+  const int from = PAGES ? w.lo : w.j0 * kArKeys, to = min(w.hi, ((g == 0 ? w.hi_first : w.hi) + 15) / 16 * 16);
+#pragma unroll 1
+  while (odd) {
+    const int row = row0 + __ffs(odd) - 1, pos = w.pos0 + row;
+    odd &= odd - 1;
+    ar_again<HD, CAP, PAGES>(p, beat, it.seq, it.q_start, it.head, it.q_start + it.q0 + row, first_visible(pos, p.window, 0), min(pos, w.hi - 1), from, to);
+    __syncwarp();
+  }
+}
+
 // Asks for the work of a block of the grid that has not begun, in its place (the answer in 16 bytes of shared memory, counted on `bar`).
 __device__ __forceinline__ void ar_ask_block(uint4* answer, uint64_t* bar) {
   tc5::mbar_expect_tx(bar, 16);
@@ -566,6 +646,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   __shared__ size_t group_at[2][2][PAGES ? kArKeys / 8 : 1];       // pages: where keys, and values, of a tile are, by eights
   __shared__ float value_base;                                     // log2 of the value scale that weights are relative to
   __shared__ volatile int abort_flag;
+  __shared__ ArBeat beat;
 
   int* const error = p.error;
   // Tiles and lengths may come from a kernel of the same step, so they are read behind the wait.  (Whoever leaves waits as
@@ -589,6 +670,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   if (threadIdx.x < 16) left[threadIdx.x >> 1][threadIdx.x & 1] = 0;
   if (threadIdx.x == 0) {
     abort_flag = 0;
+    beat = 0;
     items[0] = begin;
     tc5::mbar_init(&q_full, 1);
     tc5::mbar_init(&q_ready, 4 * SPLIT * (begin.rows > kArGroupRows ? 2 : 1));
@@ -626,7 +708,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     abort_flag = 1;
   };
   auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {  // the warp stays together whatever a lane saw
-    if (__all_sync(0xffffffffu, ar_wait(bar, parity))) return true;
+    if (__all_sync(0xffffffffu, ar_wait(bar, parity, &beat))) return true;
     if (!abort_flag && lane == 0) fail(code);                      // (the first to give up says so; the others' waits run out too)
     return false;
   };
@@ -730,7 +812,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const bool ends = n == w.n_tiles && tail % 16 != 0;
         if (lane == 0) {
           if (n == max(w.n_tiles - 3, 0)) ar_ask_block(&next_block, &next_told);        // (the later, the better blocks' ends fit)
-          ok = ar_wait(&kv_free[st], ((step >> 1) & 1) ^ 1);
+          ok = ar_wait(&kv_free[st], ((step >> 1) & 1) ^ 1, &beat);
           if (ok && n == 0) {                                      // (the work before has had its last scores one step ago)
             tc5::mbar_expect_tx(&q_full, w.groups * KB * kArTile);
             for (int g = 0; g < w.groups; ++g)
@@ -1029,17 +1111,8 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         if (ar_either<SPLIT>(pair, sick != 0.f)) {                          // (and every element of the rows is written)
           *mine_told = sick;
           ar_either<SPLIT>(pair, false);
-          // (the keys that the products of this row's group had: whole tiles, up to the last one's steps of 16 and the block's own)
-          uint32_t odd = half == 0 ? __ballot_sync(0xffffffffu, sick != 0.f || *other_told != 0.f) : 0u;
-          const ArSpan w(p, it);
-          const int from = PAGES ? w.lo : w.j0 * kArKeys, to = min(w.hi, ((g == 0 ? w.hi_first : w.hi) + 15) / 16 * 16);
-          while (odd) {
-            const int who = __ffs(odd) - 1;
-            odd &= odd - 1;
-            const int its = __shfl_sync(0xffffffffu, row, who);
-            ar_again<HD, CAP, PAGES>(p, it.seq, it.q_start, head, first_row + its, first_visible(w.pos0 + its, p.window, 0), min(w.pos0 + its, w.hi - 1), from, to);
-            __syncwarp();
-          }
+          const uint32_t odd = half == 0 ? __ballot_sync(0xffffffffu, sick != 0.f || *other_told != 0.f) : 0u;
+          if (odd) ar_redo<HD, CAP, PAGES>(p, &beat, it, g, odd);
         }
       }
       tc5::fence_before();
