@@ -21,8 +21,8 @@
 // each row, exact but for elements 2^-29 as large as the row's largest.  P is rounded to float16 (prompts: bfloat16).
 //
 // Values that are not finite and that some row of a tile does not see would come to it as zero times them.  Rows past the
-// last are zeros in shared memory; a row whose result is not finite looks whether an unseen value was the reason, and is then
-// attended once more without the tensor cores.
+// last are zeros in shared memory; a row whose result is not finite looks whether an unseen value was the reason, or (prompts)
+// whether sums relative to no maximum were too large for float32, and is then attended once more without the tensor cores.
 //
 // Prompts' blocks stay: three tiles before its end a block asks for another that has not begun and takes its work, so that Q, K and V come
 // while rows are written (16 ragged prompts 75 us in place of 104 without cap, asked for at a block's beginning 94).
@@ -507,27 +507,14 @@ struct ArSpan {
   }
 };
 
-// A row whose result is not finite, by a whole warp: if a value that it does not see, of the keys [from, first) and (last, to) that its
-// products had, is not finite, the row is attended again without the tensor cores: 32 keys at a time, a lane a key for the scores and
-// a lane two or four elements for the output.  That takes its time (32 rows behind 100,000 keys half a second), so the warp says
-// now and then that it is at work, and nobody's wait runs out meanwhile.
+// A row without the tensor cores, by a whole warp: 32 keys at a time, a lane a key for the scores and a lane two or four elements for the output,
+// which is kept as the mean that it is so far, so that it is finite where the values are.  That takes its time (32 rows behind 100,000 keys
+// half a second), so the warp says now and then that it is at work, and nobody's wait runs out meanwhile.
 template <int HD, bool CAP, bool PAGES>
-__device__ __forceinline__ void ar_again(const RowsParams& p, ArBeat* beat, int seq, int start, int head, int row, int first, int last, int from, int to) {
+__device__ __forceinline__ void ar_again(const RowsParams& p, ArBeat* beat, int seq, int start, int head, int row, int first, int last) {
   constexpr int N = HD / 32;
   const int lane = threadIdx.x & 31, kvh = head / (p.nh / p.nkv), words = p.hd / 8;
   const ArKeys<PAGES> keys{p, PAGES ? p.block_tables + size_t(seq) * p.max_blocks : nullptr, start, kvh};
-  bool sick = false;
-  for (int j = from + lane; j < to; j += 32) {
-    if (j >= first && j <= last) continue;
-    const size_t at = keys.place(j);
-    for (int c = 0; c < words; ++c) {
-      float x[8];
-      keys.value8(at, c, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sick |= !(fabsf(x[e]) <= 3.402823466e38f);
-    }
-  }
-  if (!__any_sync(0xffffffffu, sick)) return;
   const uint4* const q = reinterpret_cast<const uint4*>(p.q + size_t(row) * p.q_stride + size_t(head) * p.hd);
   float o[N], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -541,7 +528,7 @@ __device__ __forceinline__ void ar_again(const RowsParams& p, ArBeat* beat, int 
     if (lane < n) {
       at = keys.place(j0 + lane);
       float s = 0.f;
-#pragma unroll 2
+#pragma unroll 1
       for (int c = 0; c < words; ++c) {
         float k[8], w[8];
         keys.key8(at, c, k);
@@ -552,38 +539,70 @@ __device__ __forceinline__ void ar_again(const RowsParams& p, ArBeat* beat, int 
       x = CAP ? ar_tanh(s * p.cap_pre) * p.scale_log2 : s * p.scale_log2;
     }
     const float top = fmaxf(m, warp_max(x)), f = m == -INFINITY ? 0.f : ar_exp2(m - top), e = x == -INFINITY ? 0.f : ar_exp2(x - top);
+    const float before = m == -INFINITY ? 0.f : l * f, sum = before + warp_sum(e), per = sum == 0.f ? 0.f : 1.f / sum;
     m = top;
-    l = fmaf(l, f, warp_sum(e));
+    l = sum;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] *= f;
+    for (int i = 0; i < N; ++i) o[i] *= before * per;
 #pragma unroll 4
     for (int k = 0; k < n; ++k) {                                  // (more at once take registers from the kernel around the call: 2 % of packed prompts)
       float v[N];
       keys.template value<N>(__shfl_sync(0xffffffffu, (unsigned long long)at, k), v);
-      const float w = __shfl_sync(0xffffffffu, e, k);
+      const float w = __shfl_sync(0xffffffffu, e * per, k);
 #pragma unroll
       for (int i = 0; i < N; ++i) o[i] = fmaf(w, v[i], o[i]);
     }
   }
-  if (p.sink && m != -INFINITY) l += ar_exp2(p.sink[head] * 1.4426950408889634f - m);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float share = p.sink && m != -INFINITY ? l / (l + ar_exp2(p.sink[head] * 1.4426950408889634f - m)) : 1.f;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (N * lane < p.hd) stf(p.out + size_t(row) * p.out_stride + size_t(head) * p.hd + N * lane + i, l == 0.f ? 0.f : o[i] * inv);
+    if (N * lane < p.hd) stf(p.out + size_t(row) * p.out_stride + size_t(head) * p.hd + N * lane + i, l == 0.f ? 0.f : o[i] * share);
 }
 
-// The rows `odd` of the warp's 32 rows of group g.
+// The rows `odd` of the warp's 32 rows of group g, whose results are not finite.  Those are attended again that do not see a value that is
+// not finite but came beside (of the keys that the group's products had), and, where some value is large, those whose weights are numbers
+// (`counts`): their weights add up to 2^37 at most, so sums of values from 2^90 on may have left float32 although their mean does not.
+constexpr float kArLarge = 1.2379400392853803e27f;      // 2^90
 template <int HD, bool CAP, bool PAGES>
-__device__ __noinline__ void ar_redo(const RowsParams& p, ArBeat* beat, const ArItem& it, int g, uint32_t odd) {
+__device__ __noinline__ void ar_redo(const RowsParams& p, ArBeat* beat, const ArItem& it, int g, uint32_t odd, uint32_t counts) {
   const ArSpan w(p, it);
-  const int row0 = g * kArGroupRows + int(threadIdx.x >> 5 & 3) * 32;
-  // (the keys that the products of the group had: whole tiles, up to the last one's steps of 16 and the block's own)
+  const ArKeys<PAGES> keys{p, PAGES ? p.block_tables + size_t(it.seq) * p.max_blocks : nullptr, it.q_start, w.kvh};
+  const int lane = threadIdx.x & 31, row0 = g * kArGroupRows + int(threadIdx.x >> 5 & 3) * 32, pos = w.pos0 + row0 + lane;
+  const int first = first_visible(pos, p.window, 0), last = min(pos, w.hi - 1);
+  // (keys of whole tiles, up to the last one's steps of 16 and the block's own)
   const int from = PAGES ? w.lo : w.j0 * kArKeys, to = min(w.hi, ((g == 0 ? w.hi_first : w.hi) + 15) / 16 * 16);
+  const bool all = !PAGES && (odd & counts) != 0u;
+  const bool mine = odd >> lane & 1u;
+  const int seen_from = __reduce_max_sync(0xffffffffu, mine ? first : 0), seen_to = __reduce_min_sync(0xffffffffu, mine ? last : 0x7fffffff);
+  bool beside = false, large = false;
+#pragma unroll 1
+  for (int j0 = from; j0 < to; j0 += 32) {
+    if (!all && j0 >= seen_from && j0 + 31 <= seen_to) continue;   // (every row sees them)
+    if (lane == 0) *beat = tc5::now_ns();
+    bool bad = false;
+    if (j0 + lane < to) {
+      const size_t at = keys.place(j0 + lane);
+#pragma unroll 1
+      for (int c = 0; c < p.hd / 8; ++c) {
+        float x[8];
+        keys.value8(at, c, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool finite = fabsf(x[e]) <= 3.402823466e38f;
+          bad |= !finite;
+          large |= finite && fabsf(x[e]) >= kArLarge;
+        }
+      }
+    }
+    beside |= (__ballot_sync(0xffffffffu, bad) & ~ar_bits(first - j0, last + 1 - j0)) != 0u;
+  }
+  odd &= __ballot_sync(0xffffffffu, beside) | (all && __any_sync(0xffffffffu, large) ? counts : 0u);
 #pragma unroll 1
   while (odd) {
-    const int row = row0 + __ffs(odd) - 1, pos = w.pos0 + row;
+    const int who = __ffs(odd) - 1;
     odd &= odd - 1;
-    ar_again<HD, CAP, PAGES>(p, beat, it.seq, it.q_start, it.head, it.q_start + it.q0 + row, first_visible(pos, p.window, 0), min(pos, w.hi - 1), from, to);
+    ar_again<HD, CAP, PAGES>(p, beat, it.seq, it.q_start, it.head, it.q_start + it.q0 + row0 + who, __shfl_sync(0xffffffffu, first, who),
+                             __shfl_sync(0xffffffffu, last, who));
     __syncwarp();
   }
 }
@@ -1112,7 +1131,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           *mine_told = sick;
           ar_either<SPLIT>(pair, false);
           const uint32_t odd = half == 0 ? __ballot_sync(0xffffffffu, sick != 0.f || *other_told != 0.f) : 0u;
-          if (odd) ar_redo<HD, CAP, PAGES>(p, &beat, it, g, odd);
+          if (odd) ar_redo<HD, CAP, PAGES>(p, &beat, it, g, odd, __ballot_sync(0xffffffffu, l == l));
         }
       }
       tc5::fence_before();
