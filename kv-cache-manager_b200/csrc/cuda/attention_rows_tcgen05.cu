@@ -17,7 +17,8 @@
 // Pages: float16 operands.  Codes are exact in float16, so seven warps turn them into operands with one conversion for two; scales stay
 // out of the products: the key's enters the score's factor, the value's, a power of two, the probability's exponent
 // (2^(x - m) scale = 2^(x - m + log2 scale): weights in place of probabilities), one factor for eight keys, which lie in one page.
-// m is the reference of the weights, and sums take the weights' scales out again.  q enters as float16 times a power of two for
+// m is the reference of the weights, and sums take the weights' scales out again (rows of blocks whose values' scales are more than 2^100 apart,
+// which float32's exponents cannot hold that way, are attended once more without the tensor cores).  q enters as float16 times a power of two for
 // each row, exact but for elements 2^-29 as large as the row's largest.  P is rounded to float16 (prompts: bfloat16).
 //
 // Values that are not finite and that some row of a tile does not see would come to it as zero times them.  Rows past the
@@ -36,7 +37,8 @@
 // 5,000 keys 683 (740 TFLOP/s); 16 ragged prompts of some 600 rows, 16 heads, window, capped, sinks 104; five of 110 rows of heads of 64 17.
 //
 // Every wait for a barrier in memory is bounded (a second, in which no warp of the block has said that it is attending rows once more); one that
-// runs out sets the error word of the tcgen05 attention family (codes 33 and up) and ends the block.  Warps that wait for one another at named barriers, which have no limit, take every such step together whatever they saw.
+// runs out sets the error word of the tcgen05 attention family (codes 33 and up) and ends the block.  Warps that wait for one another at named
+// barriers, which have no limit, take every such step together whatever they saw.
 #include <cuda_fp16.h>
 
 #include "packed.cuh"
@@ -55,6 +57,7 @@ constexpr int kArStages = 2;                       // tiles of keys, and of valu
 constexpr int kArRing = 4;                         // tiles' scales
 constexpr int kArKeyWarps = 4, kArValueWarps = 3;  // pages: who turns codes into operands
 constexpr float kArMost = 4096.f;                  // pages: a row's sum of a tile's weights from which its maximum is renewed
+constexpr int kArFarApart = 100;                   // pages: exponents by which the scales of a block's values may differ
 constexpr float kArMostPrompt = 1048576.f, kArLeast = 9.094947e-13f;      // prompts: 2^20, and 2^-40
 // tensor memory: S of group g at column g * 128 (and P in its first 64 columns); O of group g at 256 + g * HD
 
@@ -560,8 +563,8 @@ __device__ __forceinline__ void ar_again(const RowsParams& p, ArBeat* beat, int 
 }
 
 // The rows `odd` of the warp's 32 rows of group g, whose results are not finite.  Those are attended again that do not see a value that is
-// not finite but came beside (of the keys that the group's products had), and, where some value is large, those whose weights are numbers
-// (`counts`): their weights add up to 2^37 at most, so sums of values from 2^90 on may have left float32 although their mean does not.
+// not finite but came beside (of the keys that the group's products had).  Pages: and those of `counts`, whose values' scales are too far
+// apart.  Prompts: and, where some value is large, those whose weights are numbers (`counts`): their weights add up to 2^37 at most, so sums of values from 2^90 on may have left float32 although their mean does not.
 constexpr float kArLarge = 1.2379400392853803e27f;      // 2^90
 template <int HD, bool CAP, bool PAGES>
 __device__ __noinline__ void ar_redo(const RowsParams& p, ArBeat* beat, const ArItem& it, int g, uint32_t odd, uint32_t counts) {
@@ -596,7 +599,7 @@ __device__ __noinline__ void ar_redo(const RowsParams& p, ArBeat* beat, const Ar
     }
     beside |= (__ballot_sync(0xffffffffu, bad) & ~ar_bits(first - j0, last + 1 - j0)) != 0u;
   }
-  odd &= __ballot_sync(0xffffffffu, beside) | (all && __any_sync(0xffffffffu, large) ? counts : 0u);
+  odd &= __ballot_sync(0xffffffffu, beside) | (PAGES || (all && __any_sync(0xffffffffu, large)) ? counts : 0u);
 #pragma unroll 1
   while (odd) {
     const int who = __ffs(odd) - 1;
@@ -664,6 +667,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   __shared__ int left[8][2];                                       // that a warp gave up
   __shared__ size_t group_at[2][2][PAGES ? kArKeys / 8 : 1];       // pages: where keys, and values, of a tile are, by eights
   __shared__ float value_base;                                     // log2 of the value scale that weights are relative to
+  __shared__ volatile int far_apart[2];                            // pages: that a group's value scales are further apart than sums of weights can hold
   __shared__ volatile int abort_flag;
   __shared__ ArBeat beat;
 
@@ -689,6 +693,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   if (threadIdx.x < 16) left[threadIdx.x >> 1][threadIdx.x & 1] = 0;
   if (threadIdx.x == 0) {
     abort_flag = 0;
+    far_apart[0] = far_apart[1] = 0;
     beat = 0;
     items[0] = begin;
     tc5::mbar_init(&q_full, 1);
@@ -922,6 +927,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     together();
     ask(0);
     float base = 0.f;
+    int least = 255, most = 0;                                     // exponents of the values' scales so far, in a lane's groups of eight
     bool there_is = true;                                          // room for the tile
     for (int n = 0; n < n_tiles; ++n) {
       // tile n of the keys is read in step n of the products, of the values in the one behind it
@@ -943,6 +949,19 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           s.value = there ? log_v - base : 0.f;
           s.out = there ? exp2f(base - log_v) : 0.f;
           scales[(n % kArRing) * (kArKeys / 8) + lane] = s;
+          if (there) {
+            const int e = int(__float_as_uint(scale.y) >> 23);
+            least = min(least, e);
+            most = max(most, e);
+          }
+        }
+        if (n == w.n_first - 1 || n == n_tiles - 1) {              // (ahead of the barrier that a group's last weights wait for)
+          least = __reduce_min_sync(0xffffffffu, least);
+          most = __reduce_max_sync(0xffffffffu, most);
+          if (lane == 0 && most - least > kArFarApart) {
+            if (n == w.n_first - 1) far_apart[0] = 1;
+            if (n == n_tiles - 1) far_apart[1] = 1;
+          }
         }
         __syncwarp();
         if (there_is && lane == 0) tc5::mbar_arrive(&sc_full[n % kArRing]);
@@ -1127,11 +1146,13 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
           }
         }
-        if (ar_either<SPLIT>(pair, sick != 0.f)) {                          // (and every element of the rows is written)
+        if (PAGES && far_apart[g]) {                                    // (a warp's rows are its own: nothing to tell)
+          ar_redo<HD, CAP, PAGES>(p, &beat, it, g, __ballot_sync(0xffffffffu, row < rows_here), ~0u);
+        } else if (ar_either<SPLIT>(pair, sick != 0.f)) {            // (and every element of the rows is written)
           *mine_told = sick;
           ar_either<SPLIT>(pair, false);
           const uint32_t odd = half == 0 ? __ballot_sync(0xffffffffu, sick != 0.f || *other_told != 0.f) : 0u;
-          if (odd) ar_redo<HD, CAP, PAGES>(p, &beat, it, g, odd, __ballot_sync(0xffffffffu, l == l));
+          if (odd) ar_redo<HD, CAP, PAGES>(p, &beat, it, g, odd, PAGES ? 0u : __ballot_sync(0xffffffffu, l == l));
         }
       }
       tc5::fence_before();
