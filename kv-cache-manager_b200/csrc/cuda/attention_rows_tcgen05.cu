@@ -79,19 +79,24 @@ struct RowsParams {
 
 namespace {
 
-typedef volatile unsigned long long ArBeat;        // when a warp of the block was last seen at work that may take longer than a wait's limit
+typedef volatile uint32_t ArBeat;                  // counts on while a warp of the block is at work that may take longer than a wait's limit
 
 // tc5::mbar_wait for waits of a microsecond: the thread sleeps in the instruction and does not take its scheduler's turns.
 __device__ __forceinline__ bool ar_wait(uint64_t* bar, uint32_t parity, const ArBeat* beat) {
-  unsigned long long start = 0;
+  uint32_t start = 0, seen = 0;
   for (;;) {
-    uint32_t done;
+    uint32_t done, now;
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n"
                  : "=r"(done) : "r"(tc5::s32(bar)), "r"(parity), "r"(100000u) : "memory");
     if (done) return true;
-    const unsigned long long now = tc5::now_ns();
-    if (start == 0) start = now;
-    else if (now - start > tc5::kWaitLimitNs && (long long)(now - *beat) > (long long)tc5::kWaitLimitNs) return false;
+    asm volatile("mov.u32 %0, %globaltimer_lo;\n" : "=r"(now));
+    if (start == 0) {
+      start = now | 1u;
+    } else if (int(now - start) > int(tc5::kWaitLimitNs)) {        // (start may be one ahead of now)
+      if (*beat == seen) return false;                             // nobody has been at work since it was looked at last
+      seen = *beat;
+      start = now | 1u;
+    }
   }
 }
 
@@ -525,7 +530,7 @@ __device__ __forceinline__ void ar_again(const RowsParams& p, ArBeat* beat, int 
 #pragma unroll 1
   for (int j0 = first; j0 <= last; j0 += 32) {
     const int n = min(32, last - j0 + 1);
-    if (lane == 0) *beat = tc5::now_ns();
+    if (lane == 0) *beat = *beat + 1;
     float x = -INFINITY;
     size_t at = 0;
     if (lane < n) {
@@ -581,7 +586,7 @@ __device__ __noinline__ void ar_redo(const RowsParams& p, ArBeat* beat, const Ar
 #pragma unroll 1
   for (int j0 = from; j0 < to; j0 += 32) {
     if (!all && j0 >= seen_from && j0 + 31 <= seen_to) continue;   // (every row sees them)
-    if (lane == 0) *beat = tc5::now_ns();
+    if (lane == 0) *beat = *beat + 1;
     bool bad = false;
     if (j0 + lane < to) {
       const size_t at = keys.place(j0 + lane);
