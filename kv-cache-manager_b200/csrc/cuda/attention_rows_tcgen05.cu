@@ -26,7 +26,7 @@
 // whether sums relative to no maximum were too large for float32, and is then attended once more without the tensor cores.
 //
 // Prompts' blocks stay: three tiles before its end a block asks for another that has not begun and takes its work, so that Q, K and V come
-// while rows are written (16 ragged prompts 75 us in place of 104 without cap, asked for at a block's beginning 94).
+// while rows are written (16 ragged prompts 78 us in place of 104 without cap, asked for at a block's beginning 94).
 //
 // What bounds it: a group's chain of softmax and products, of which two groups' overlap.  A tile of 256 x 128 takes some 3,200 cycles at
 // prompts of heads of 128, the products 2,048 of them, and the exponential units as many; the issuing warp's instructions between
@@ -34,7 +34,7 @@
 // four: 468 -> 444 us).  A product of 128 x 64 takes as long as one of 128 x 128, so smaller tiles that would
 // let S run ahead of the softmax lose (720 us for 8,192 rows against 640 at the time).  B200, 32 heads on 8 of 128:
 // a prompt of 8,192 rows 445 us (1,235 TFLOP/s; 520 after seconds of it, under the power cap), four portions of about 1,500 rows behind
-// 5,000 keys 683 (740 TFLOP/s); 16 ragged prompts of some 600 rows, 16 heads, window, capped, sinks 104; five of 110 rows of heads of 64 17.
+// 5,000 keys 683 (740 TFLOP/s); 16 ragged prompts of some 600 rows, 16 heads, window, capped, sinks 103; five of 110 rows of heads of 64 17.
 //
 // Every wait for a barrier in memory is bounded (a second, in which no warp of the block has said that it is attending rows once more); one that
 // runs out sets the error word of the tcgen05 attention family (codes 33 and up) and ends the block.  Warps that wait for one another at named

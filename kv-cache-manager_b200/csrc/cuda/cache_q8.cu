@@ -11,8 +11,8 @@
 // it finds the rows' maximum by shuffles, brings the page to its scale where that grows, and reads the rows a second time to write
 // them (out of the nearest cache; the first as many rows as a warp has lanes for stay in registers).  A lane has
 // two words of eight elements that turn with one another, so that angles are read once for both and nothing is exchanged.
-// What bounds it: a warp's chain (slots, scale, rows, rows again) at 64 registers a thread, some of them spilled, which let four blocks an
-// SM overlap.  B200, about 8,400 rows, 32 heads and 8 + 8 KV heads of 128: 70 us (29 at the rate of a copy; 139 with the rows of a page
+// What bounds it: a warp's chain (slots, scale, rows, rows again) at 64 registers a thread, which let four blocks an SM overlap but spill
+// 488 bytes a thread (668 read back) where windows are 8 or 16 rows, 344 (360) where they are one; float32 rows alike.  B200, about 8,400 rows, 32 heads and 8 + 8 KV heads of 128: 70 us (29 at the rate of a copy; 139 with the rows of a page
 // kept in 170 registers; four warps a run 96), read back 15; 64 rows 6.1 and 3.9.  All heads q 54 us, all KV heads 87, where copies take 35 and 27.
 // Windows: 900 rows 25 us in windows of 16, 21 of 8; 512 single rows 18 in windows of one.
 #include "packed.cuh"
